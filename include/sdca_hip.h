@@ -45,7 +45,12 @@ typedef enum sdca_status {
 typedef enum sdca_dtype {
   SDCA_F32 = 0,
   SDCA_F64 = 1,
-  SDCA_LONG_DOUBLE = 2 /* valid in the reference (mex_prox.cpp:195); not on the GPU */
+  SDCA_LONG_DOUBLE = 2, /* valid in the reference (mex_prox.cpp:195); not on the GPU */
+  /* The types below are those of the answering calls alone (sdca_quantize_i8,
+     sdca_scores_i8, sdca_sample). */
+  SDCA_F16 = 3,
+  SDCA_BF16 = 4,
+  SDCA_I8 = 5
 } sdca_dtype;
 
 /* Operators of the Matlab prox front end (mex_prox.cpp:145-172). */
@@ -401,6 +406,99 @@ int sdca_recompute_primal(sdca_dtype data, int64_t d, int64_t m, int64_t n,
 int sdca_scores(sdca_dtype data, int64_t d, int64_t m, int64_t n,
                 const void* X, const void* W, void* S,
                 unsigned flags, void* stream);
+
+/*
+ * Answering from a trained model.  The three calls below have no counterpart
+ * in the reference, which ends at the evaluation: they serve the scores of
+ * new examples in 8 bits and draw labels from them.  Arrays are column-major
+ * like the others, with a leading dimension of their own (at least the
+ * column's length, in elements): the distance from one column to the next.
+ * They take device pointers on `stream`, or with SDCA_HOST_PTR host arrays.
+ */
+
+/*
+ * Quantises the n columns of X (d x n, leading dimension ldx; data SDCA_F32,
+ * SDCA_F64, SDCA_F16 or SDCA_BF16) to 8-bit integers with a scale for each:
+ *   scales[i] = max_k |X_ki| (1 / 127),  Q_ki = X_ki / scales[i] to the
+ * nearest integer, halves to even, in 32-bit arithmetic (1 / 127 the float
+ * nearest to it, the product and the quotient rounded; doubles are rounded
+ * to float first).  A column of zeros has scale 0; a column that holds an
+ * infinity or a NaN has zeros and the scale NaN, so that every score of it
+ * is NaN.  Q: d x n with leading dimension ldq; bytes between d and ldq are
+ * not written.  A ldq that is a multiple of 16, and Q at such an address,
+ * lets sdca_scores_i8 read Q in place.
+ */
+int sdca_quantize_i8(sdca_dtype data, int64_t d, int64_t n, const void* X, int64_t ldx,
+                     int8_t* Q, int64_t ldq, float* scales, unsigned flags, void* stream);
+
+/*
+ * Scores from 8-bit weights: S = diag(sw) (W' X) diag(sx), the product in
+ * integers (sdca_scores for quantised operands).
+ *   X: d x n examples, leading dimension ldx.  data SDCA_I8 with sx their n
+ *      scales; or data SDCA_F32, SDCA_F64, SDCA_F16 or SDCA_BF16 with sx
+ *      NULL: quantised within the call as sdca_quantize_i8 does;
+ *   W: d x m weights in 8 bits, leading dimension ldw, sw their m scales;
+ *   S: m x n scores of type out (SDCA_F32, SDCA_F16 or SDCA_BF16), leading
+ *      dimension lds >= m.
+ * The sums are exact (32-bit integers: d is at most 131071); each score is
+ * float(sum) sx_i sw_j in 32-bit arithmetic, rounded to `out` at the end.
+ * W is read in place when its address and ldw are multiples of 16, and is
+ * copied to the stream's scratch in each call otherwise.
+ */
+int sdca_scores_i8(sdca_dtype data, sdca_dtype out, int64_t d, int64_t m, int64_t n,
+                   const void* X, int64_t ldx, const float* sx, const int8_t* W, int64_t ldw,
+                   const float* sw, void* S, int64_t lds, unsigned flags, void* stream);
+
+/* Settings of sdca_sample; the defaults cut nothing. */
+typedef struct sdca_sample_params {
+  double temperature; /* 1; 0: the largest score */
+  double top_p;       /* 1: off */
+  double min_p;       /* 0: off */
+  int64_t top_k;      /* 0: off */
+} sdca_sample_params;
+
+/* The same settings for each column apart: arrays of n values, or NULL where
+ * the params' value goes for all. */
+typedef struct sdca_sample_columns {
+  const float* temperature;
+  const float* top_p;
+  const float* min_p;
+  const int64_t* top_k;
+} sdca_sample_columns;
+
+/* Fills the defaults temperature=1, top_p=1, min_p=0, top_k=0. */
+void sdca_sample_params_default(sdca_sample_params* params);
+
+/*
+ * Draws a label for each of the n columns of scores S (m x n, leading
+ * dimension lds; data SDCA_F32, SDCA_F64, SDCA_F16 or SDCA_BF16, doubles
+ * rounded to float).  With M a column's largest score, the weights are
+ * w_i = exp((S_i - M) / temperature).  Of the labels by falling score (ties
+ * by rising index) the first top_k are kept, of these the shortest beginning
+ * whose weights sum to top_p of theirs (at least one), and of these the ones
+ * with w_i >= min_p.  labels[j] is the first label, by rising index, at
+ * which the sum of the kept weights exceeds u[j] times their total.
+ *   u: n random numbers in [0, 1);
+ *   params: NULL for the defaults; columns: NULL for none;
+ *   labels: n labels in [0, m); -1 for a column without one (all its scores
+ *           -infinity or NaN; a NaN counts as -infinity);
+ *   prob:   optional, n: the drawn label's share of the kept weights;
+ *   kept:   optional, n: how many labels of nonzero weight were kept.
+ * temperature 0 (or below the smallest normal float) draws the first of the
+ * largest scores, with prob = kept = 1.  The weights are 32-bit floats and
+ * their sums integers, so a label does not depend on launch shapes or on
+ * the column's neighbours.  Params, and host arrays of columns, outside
+ * temperature >= 0, 0 < top_p <= 1, 0 <= min_p <= 1, top_k >= 0 are
+ * SDCA_ERR_ARG_RANGE; device values are not read back by the host: a
+ * temperature that is negative or NaN draws the largest score, a top_k
+ * below 1 or above m, a top_p above 1 or NaN and a min_p below 0 or NaN cut
+ * nothing, a top_p of 0 or less keeps one label, a min_p above 1 the
+ * largest scores, and u is brought into [0, 1).
+ */
+int sdca_sample(sdca_dtype data, int64_t m, int64_t n, const void* S, int64_t lds,
+                const float* u, const sdca_sample_params* params,
+                const sdca_sample_columns* columns, int64_t* labels, float* prob,
+                int64_t* kept, unsigned flags, void* stream);
 
 /* Message of the last failure on this thread ("" if none). */
 const char* sdca_last_error(void);

@@ -21,6 +21,12 @@ operator table (src/matlab/mex_prox.cpp:145-172):
     prox_two_entropy(dim, p, A, alpha=1)
     lambert_w_exp(A)
 
+and the answers of a trained model, which the reference does not have:
+
+    quantize_i8(A)
+    scores_i8(X, W, w_scales)
+    sample(S, u, temperature=1, top_k=0, top_p=1, min_p=0)
+
 `A` holds n columns of length dim, contiguous (a C-contiguous (n, dim) array
 or tensor, i.e. the column-major dim x n matrix of the reference).  A torch
 CUDA tensor is processed in place on the device (stream-ordered on torch's
@@ -41,6 +47,7 @@ __all__ = [
     "prox_two_simplex_sort", "prox_two_entropy", "lambert_w_exp", "OPS", "F32", "F64",
     "OBJECTIVES", "objective", "scores", "eval_features", "eval_kernel", "eval_scores",
     "recompute_primal", "epoch_order", "epoch_features", "epoch_kernel", "BRANCHES",
+    "quantize_i8", "scores_i8", "sample",
 ]
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -98,6 +105,16 @@ class EvalRecord(ctypes.Structure):
                 ("dual_regularizer", ctypes.c_double), ("rank_loss", ctypes.c_double)]
 
 
+class SampleParams(ctypes.Structure):
+    _fields_ = [("temperature", ctypes.c_double), ("top_p", ctypes.c_double),
+                ("min_p", ctypes.c_double), ("top_k", ctypes.c_int64)]
+
+
+class SampleColumns(ctypes.Structure):
+    _fields_ = [("temperature", ctypes.c_void_p), ("top_p", ctypes.c_void_p),
+                ("min_p", ctypes.c_void_p), ("top_k", ctypes.c_void_p)]
+
+
 # Objectives of the evaluation pass, named after the reference's makers
 # (objective.h:55-160: make_objective_l2_hinge_topk, ...).
 OBJECTIVES = {
@@ -138,6 +155,12 @@ def library():
             ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int64,
             ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(ProxParams), ctypes.c_void_p,
             ctypes.c_void_p, ctypes.c_uint, ctypes.c_void_p]
+        i32, i64, ptr, u32 = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_uint
+        lib.sdca_quantize_i8.argtypes = [i32, i64, i64, ptr, i64, ptr, i64, ptr, u32, ptr]
+        lib.sdca_scores_i8.argtypes = [i32, i32, i64, i64, i64, ptr, i64, ptr, ptr, i64, ptr, ptr,
+                                       i64, u32, ptr]
+        lib.sdca_sample.argtypes = [i32, i64, i64, ptr, i64, ptr, ctypes.POINTER(SampleParams),
+                                    ctypes.POINTER(SampleColumns), ptr, ptr, ptr, u32, ptr]
         lib.sdca_last_error.restype = ctypes.c_char_p
         lib.sdca_abi_version.restype = ctypes.c_int
         _lib = lib
@@ -674,3 +697,224 @@ def eval_scores(objs, S, labels, A=None, offsets=None, primal_regularizer=0.0,
                                ctypes.c_uint(flags), stream))
     records = [{f: getattr(r, f) for f, _ in EvalRecord._fields_} for r in recs]
     return records, acc, pe
+
+
+# ---------------------------------------------------------------------------
+# Answering from a trained model: scores from 8-bit weights, and labels drawn
+# from scores.  Matrices may have rows further apart than their length (a
+# stride of 1 within a row); CUDA tensors run on torch's current stream,
+# numpy arrays go through the host-staging path.
+# ---------------------------------------------------------------------------
+F16, BF16, I8 = 3, 4, 5
+_answer_codes = None
+
+
+def _answer_dtype(x):
+    global _answer_codes
+    if _answer_codes is None:
+        _answer_codes = {np.dtype(np.float32): F32, np.dtype(np.float64): F64,
+                         np.dtype(np.float16): F16, np.dtype(np.int8): I8}
+        try:
+            import torch
+            _answer_codes.update({torch.float32: F32, torch.float64: F64, torch.float16: F16,
+                                  torch.bfloat16: BF16, torch.int8: I8})
+        except ImportError:
+            pass
+    return _answer_codes.get(x.dtype, -1)
+
+
+def _pitch(x, name, shape=None):
+    """The distance between the rows of the matrix x, in elements."""
+    if x.ndim != 2:
+        raise SdcaError(2, f"{name} must be 2-D (got {x.ndim} dimensions)")
+    n, d = x.shape
+    if shape is not None and (n, d) != shape:
+        raise SdcaError(2, f"{name} has shape {(n, d)}, expected {shape}")
+    if _is_torch(x):
+        step, one = x.stride()
+    else:
+        step, one = (s // x.itemsize for s in x.strides)
+        if not x.dtype.isnative or any(s % x.itemsize for s in x.strides):
+            raise SdcaError(2, f"{name}: unsupported layout")
+    if n <= 1:
+        step = d
+    if (one != 1 and d > 1) or step < d:
+        raise SdcaError(2, f"{name}: the values of a row must be neighbours, and rows apart")
+    return step
+
+
+def _values(x, name, n, dtype, like):
+    """Checks a vector of n values of the given element type beside `like`."""
+    if _is_torch(x) != _is_torch(like):
+        raise SdcaError(2, f"{name}: numpy arrays and torch tensors cannot be mixed in one call")
+    if x.dtype != dtype:
+        raise SdcaError(3, f"{name} has element type {x.dtype}, expected {dtype}")
+    if tuple(x.shape) != (n,):
+        raise SdcaError(2, f"{name} has shape {tuple(x.shape)}, expected {(n,)}")
+    if not (x.is_contiguous() if _is_torch(x) else x.flags.c_contiguous):
+        raise SdcaError(2, f"{name} must be contiguous")
+    if _is_torch(x) and x.device != like.device:
+        raise SdcaError(2, f"{name} is on {x.device}, expected {like.device}")
+    return x
+
+
+def _where(x, fn):
+    """(flags, stream) of a call on x; on another device than the current
+    one, torch's current stream there."""
+    if not _is_torch(x):
+        return HOST_PTR, None
+    if not x.is_cuda:
+        raise SdcaError(2, f"{fn} takes CUDA tensors or numpy arrays")
+    import torch
+    return 0, torch.cuda.current_stream(x.device).cuda_stream
+
+
+class _on:
+    """Makes a tensor's device the current one for a call, where it is not."""
+
+    def __init__(self, x):
+        self.guard = None
+        if _is_torch(x):
+            import torch
+            if x.device.index != torch.cuda.current_device():
+                self.guard = torch.cuda.device(x.device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *args):
+        if self.guard is not None:
+            self.guard.__exit__(*args)
+
+
+def _empty(shape, dtype, like):
+    """dtype by its numpy name."""
+    if _is_torch(like):
+        import torch
+        return torch.empty(shape, dtype=getattr(torch, dtype), device=like.device)
+    return np.empty(shape, dtype=dtype)
+
+
+def quantize_i8(A, out=None, scales=None):
+    """(Q, scales): the rows of A (float32, float64, float16 or bfloat16) as
+    8-bit integers with a float32 scale each, A[i] ~ Q[i] scales[i] with
+    scales[i] = max |A[i]| (1 / 127) (sdca_quantize_i8).  Without `out`, Q's rows
+    are a multiple of 16 bytes apart, which scores_i8 reads in place."""
+    lib = library()
+    data = _answer_dtype(A)
+    if data < 0 or data == I8:
+        raise SdcaError(3, f"unsupported element type {A.dtype}")
+    lda = _pitch(A, "A")
+    n, d = A.shape
+    flags, stream = _where(A, "quantize_i8")
+    like = out if out is not None else A
+    if _is_torch(like) != _is_torch(A) or (_is_torch(A) and like.device != A.device):
+        raise SdcaError(2, "out: expected the same kind and device as A")
+    Q = out if out is not None else _empty((n, (d + 15) // 16 * 16), "int8", A)[:, :d]
+    if _answer_dtype(Q) != I8:
+        raise SdcaError(3, f"out has element type {Q.dtype}, expected int8")
+    ldq = _pitch(Q, "out", (n, d))
+    s = scales if scales is not None else _empty((n,), "float32", A)
+    _values(s, "scales", n, _float32(A), A)
+    with _on(A):
+        check(lib.sdca_quantize_i8(data, d, n, _ptr(A), lda, _ptr(Q), ldq, _ptr(s), flags, stream))
+    return Q, s
+
+
+def _float32(like):
+    if _is_torch(like):
+        import torch
+        return torch.float32
+    return np.float32
+
+
+def scores_i8(X, W, w_scales, x_scales=None, out=None, dtype=None):
+    """S = X W^T with W in 8 bits (scores for a quantised model):
+    W (m, d) int8 with its m scales, as quantize_i8 gives them; X (n, d) int8
+    with x_scales, or float32, float64, float16 or bfloat16 without, which is
+    quantised row by row within the call.  S is (n, m) of `dtype` (float32 by
+    default, float16 or bfloat16; a dtype of torch or numpy) or of out's."""
+    lib = library()
+    data = _answer_dtype(X)
+    if data < 0:
+        raise SdcaError(3, f"unsupported element type {X.dtype}")
+    ldx = _pitch(X, "X")
+    n, d = X.shape
+    m = W.shape[0]
+    if _is_torch(W) != _is_torch(X) or (_is_torch(X) and W.device != X.device):
+        raise SdcaError(2, "W: expected the same kind and device as X")
+    if _answer_dtype(W) != I8:
+        raise SdcaError(3, f"W has element type {W.dtype}, expected int8")
+    ldw = _pitch(W, "W", (m, d))
+    f32 = _float32(X)
+    _values(w_scales, "w_scales", m, f32, X)
+    if (x_scales is None) == (data == I8):
+        raise SdcaError(1, "x_scales go with int8 examples, and with them only")
+    if x_scales is not None:
+        _values(x_scales, "x_scales", n, f32, X)
+    flags, stream = _where(X, "scores_i8")
+    if out is None:
+        if _is_torch(X):
+            import torch
+            out = torch.empty((n, m), dtype=dtype or f32, device=X.device)
+        else:
+            out = np.empty((n, m), dtype=dtype or f32)
+    elif _is_torch(out) != _is_torch(X) or (_is_torch(X) and out.device != X.device):
+        raise SdcaError(2, "out: expected the same kind and device as X")
+    code = _answer_dtype(out)
+    if code not in (F32, F16, BF16):
+        raise SdcaError(3, f"scores cannot be {out.dtype}")
+    lds = _pitch(out, "out", (n, m))
+    with _on(X):
+        check(lib.sdca_scores_i8(data, code, d, m, n, _ptr(X), ldx, _ptr(x_scales), _ptr(W), ldw,
+                                 _ptr(w_scales), _ptr(out), lds, flags, stream))
+    return out
+
+
+def _setting(v, name, n, kind, like):
+    """A setting's array of n values beside `like`, or None for a number."""
+    if not (_is_torch(v) or isinstance(v, (np.ndarray, list, tuple))):
+        return None
+    if _is_torch(like):
+        import torch
+        v = torch.as_tensor(v, dtype=getattr(torch, kind), device=like.device).contiguous()
+    elif _is_torch(v):
+        raise SdcaError(2, f"{name}: numpy arrays and torch tensors cannot be mixed in one call")
+    else:
+        v = np.ascontiguousarray(v, dtype=kind)
+    if tuple(v.shape) != (n,):
+        raise SdcaError(2, f"{name} has shape {tuple(v.shape)}, expected {(n,)}")
+    return v
+
+
+def sample(S, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, prob=False, kept=False):
+    """Draws a label for each row of the scores S (n, m) (float32, float64,
+    float16 or bfloat16) with the random numbers u (n float32 values in
+    [0, 1)): int64 labels, -1 for a row that has none (sdca_sample).  The
+    settings are numbers, or arrays of n values (float32; int64 for top_k).
+    With prob=True also the drawn labels' probabilities after the cuts, with
+    kept=True also the number of labels that the cuts left."""
+    lib = library()
+    data = _answer_dtype(S)
+    if data < 0 or data == I8:
+        raise SdcaError(3, f"unsupported element type {S.dtype}")
+    lds = _pitch(S, "S")
+    n, m = S.shape
+    flags, stream = _where(S, "sample")
+    _values(u, "u", n, _float32(S), S)
+    T = _setting(temperature, "temperature", n, "float32", S)
+    p = _setting(top_p, "top_p", n, "float32", S)
+    q = _setting(min_p, "min_p", n, "float32", S)
+    k = _setting(top_k, "top_k", n, "int64", S)
+    params = SampleParams(1.0 if T is not None else temperature, 1.0 if p is not None else top_p,
+                          0.0 if q is not None else min_p, 0 if k is not None else int(top_k))
+    columns = SampleColumns(_ptr(T), _ptr(p), _ptr(q), _ptr(k))
+    labels = _empty((n,), "int64", S)
+    pr = _empty((n,), "float32", S) if prob else None
+    kp = _empty((n,), "int64", S) if kept else None
+    with _on(S):
+        check(lib.sdca_sample(data, m, n, _ptr(S), lds, _ptr(u), params, columns, _ptr(labels),
+                              _ptr(pr), _ptr(kp), flags, stream))
+    res = (labels,) + ((pr,) if prob else ()) + ((kp,) if kept else ())
+    return res if len(res) > 1 else labels

@@ -20,6 +20,7 @@
 #include <vector>
 
 #include "../../include/sdca_hip.h"
+#include "answer_launch.hpp"
 #include "epoch_launch.hpp"
 #include "eval_launch.hpp"
 #include "prox_launch.hpp"
@@ -62,9 +63,9 @@ size_t dtype_size(int dt) { return dt == SDCA_F32 ? 4 : 8; }
 struct Workspace {
   // Slots: 0 deferred-column list, 1 scores, 2 evaluation scratch,
   // 3 transposes, 4 epoch, 5 the library GEMM's workspace, 6 the column
-  // slices of the prox beyond the LDS copy.
-  void* ptr[7] = {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
-  size_t cap[7] = {0, 0, 0, 0, 0, 0, 0};
+  // slices of the prox beyond the LDS copy, 7 quantised and repacked operands.
+  void* ptr[8] = {};
+  size_t cap[8] = {};
   // Pinned host block for the evaluation's results: copies into it are
   // asynchronous, so the call waits once for all of them.
   void* host = nullptr;
@@ -1153,6 +1154,331 @@ int sdca_epoch_kernel(const sdca_objective* obj, sdca_dtype data, sdca_dtype res
   g_last_error.clear();
   return epoch_common(obj, data, result, n, m, n, K, nullptr, A, labels, offsets, order, count,
                       nullptr, flags, stream_ptr, true);
+}
+
+}  // extern "C"
+
+namespace {
+
+bool is_float_type(int dt) {
+  return dt == SDCA_F32 || dt == SDCA_F64 || dt == SDCA_F16 || dt == SDCA_BF16;
+}
+
+size_t element_size(int dt) {
+  switch (dt) {
+    case SDCA_I8: return 1;
+    case SDCA_F16:
+    case SDCA_BF16: return 2;
+    default: return dtype_size(dt);
+  }
+}
+
+// Bytes from the first to behind the last element of `cols` columns.
+size_t span(int64_t rows, int64_t cols, int64_t ld, size_t es) {
+  return cols ? (static_cast<size_t>(cols - 1) * ld + rows) * es : 0;
+}
+
+int check_matrix(const char* name, int64_t rows, int64_t ld) {
+  if (ld < rows)
+    return fail(SDCA_ERR_ARG_RANGE, "%s: leading dimension %lld below %lld", name, (long long)ld,
+                (long long)rows);
+  if (ld > (int64_t(1) << 40))
+    return fail(SDCA_ERR_ARG_RANGE, "%s: leading dimension %lld is too large", name,
+                (long long)ld);
+  return SDCA_OK;
+}
+
+// A host array's device copy, or the pointer itself.
+template <class T>
+int staged(const T* p, size_t bytes, bool host, DeviceBuffer& buf, hipStream_t stream,
+           const T** out) {
+  *out = p;
+  if (!host || !p) return SDCA_OK;
+  const int rc = stage_in(p, bytes, buf, stream);
+  *out = static_cast<const T*>(buf.ptr);
+  return rc;
+}
+
+// A host result's device memory, or the pointer itself.
+template <class T>
+int staged_out(T* p, size_t bytes, bool host, DeviceBuffer& buf, T** out) {
+  *out = p;
+  if (!host || !p) return SDCA_OK;
+  SDCA_HIP_TRY(hipMalloc(&buf.ptr, bytes), "hipMalloc(staging)");
+  *out = static_cast<T*>(buf.ptr);
+  return SDCA_OK;
+}
+
+// Copies a device matrix into a host one, column by column where the columns
+// do not touch (what lies between them is the caller's).
+int fetch_columns(void* host, const void* dev, int64_t rows, int64_t cols, int64_t ld, size_t es,
+                  hipStream_t stream) {
+  if (cols == 1 || ld == rows)
+    SDCA_HIP_TRY(hipMemcpyAsync(host, dev, span(rows, cols, ld, es), hipMemcpyDeviceToHost, stream),
+                 "hipMemcpyAsync(D2H)");
+  else
+    SDCA_HIP_TRY(hipMemcpy2DAsync(host, ld * es, dev, ld * es, rows * es, cols,
+                                  hipMemcpyDeviceToHost, stream),
+                 "hipMemcpy2DAsync(D2H)");
+  return SDCA_OK;
+}
+
+int quantize_common(int data, int64_t d, int64_t n, const void* X, int64_t ldx, int8_t* Q,
+                    int64_t ldq, float* scales, unsigned flags, hipStream_t stream) {
+  if (!is_float_type(data))
+    return fail(SDCA_ERR_PRECISION, "quantize_i8 takes F32, F64, F16 or BF16 data (got %d)", data);
+  if (d < 1 || n < 0 || d > INT32_MAX / 2 || n > INT32_MAX)
+    return fail(SDCA_ERR_ARG_RANGE, "need d >= 1 and n >= 0 (got d %lld, n %lld)", (long long)d,
+                (long long)n);
+  int rc;
+  if ((rc = check_matrix("X", d, ldx)) || (rc = check_matrix("Q", d, ldq))) return rc;
+  if (n == 0) return SDCA_OK;
+  if (!X || !Q || !scales) return fail(SDCA_ERR_ARG_NULL, "X, Q and scales must not be NULL");
+  const bool host = (flags & SDCA_HOST_PTR) != 0;
+  DeviceBuffer dx, dq, ds;
+  sdca_gpu::QuantLaunch a;
+  a.data = data;
+  a.d = d;
+  a.n = n;
+  a.ldx = ldx;
+  a.ldq = ldq;
+  a.pad = d;
+  a.stream = stream;
+  if ((rc = staged(X, span(d, n, ldx, element_size(data)), host, dx, stream, &a.X)) ||
+      (rc = staged_out(Q, span(d, n, ldq, 1), host, dq, &a.Q)) ||
+      (rc = staged_out(scales, n * sizeof(float), host, ds, &a.scales)))
+    return rc;
+  SDCA_HIP_TRY(sdca_gpu::launch_quantize(a), "quantise kernel");
+  if (host) {
+    if ((rc = fetch_columns(Q, a.Q, d, n, ldq, 1, stream)) ||
+        (rc = fetch_columns(scales, a.scales, n, 1, n, sizeof(float), stream)))
+      return rc;
+    SDCA_HIP_TRY(hipStreamSynchronize(stream), "hipStreamSynchronize");
+  }
+  return SDCA_OK;
+}
+
+int scores_i8_common(int data, int out, int64_t d, int64_t m, int64_t n, const void* X,
+                     int64_t ldx, const float* sx, const int8_t* W, int64_t ldw, const float* sw,
+                     void* S, int64_t lds, unsigned flags, hipStream_t stream) {
+  using namespace sdca_gpu;
+  if (data != SDCA_I8 && !is_float_type(data))
+    return fail(SDCA_ERR_PRECISION, "scores_i8 takes I8, F32, F64, F16 or BF16 examples (got %d)",
+                data);
+  if (out != SDCA_F32 && out != SDCA_F16 && out != SDCA_BF16)
+    return fail(SDCA_ERR_PRECISION, "scores_i8 gives F32, F16 or BF16 scores (got %d)", out);
+  if (d < 1 || m < 1 || n < 0 || m > INT32_MAX / 2 || n > INT32_MAX / 2)
+    return fail(SDCA_ERR_ARG_RANGE, "need d, m >= 1 and n >= 0 (got d %lld, m %lld, n %lld)",
+                (long long)d, (long long)m, (long long)n);
+  if (d > 131071)  // 2^14 d stays below 2^31
+    return fail(SDCA_ERR_ARG_RANGE, "d is at most 131071: the sums are 32-bit integers (got %lld)",
+                (long long)d);
+  int rc;
+  if ((rc = check_matrix("X", d, ldx)) || (rc = check_matrix("W", d, ldw)) ||
+      (rc = check_matrix("S", m, lds)))
+    return rc;
+  if (n == 0) return SDCA_OK;
+  if (!X || !W || !sw || !S) return fail(SDCA_ERR_ARG_NULL, "X, W, sw and S must not be NULL");
+  if (data == SDCA_I8 ? !sx : !!sx)
+    return fail(SDCA_ERR_ARG_NULL, data == SDCA_I8
+                                       ? "8-bit examples need their scales sx"
+                                       : "float examples are quantised here: sx must be NULL");
+  const bool host = (flags & SDCA_HOST_PTR) != 0;
+  DeviceBuffer dx, dsx, dw, dsw, dS;
+  ScoresI8Launch a;
+  a.out = out;
+  a.d = d;
+  a.m = m;
+  a.n = n;
+  a.lds = lds;
+  a.stream = stream;
+  const void* x;
+  if ((rc = staged(X, span(d, n, ldx, element_size(data)), host, dx, stream, &x)) ||
+      (rc = staged(sx, n * sizeof(float), host, dsx, stream, &a.sx)) ||
+      (rc = staged(W, span(d, m, ldw, 1), host, dw, stream, &a.W)) ||
+      (rc = staged(sw, m * sizeof(float), host, dsw, stream, &a.sw)) ||
+      (rc = staged_out(S, span(m, n, lds, element_size(out)), host, dS, &a.S)))
+    return rc;
+  a.X = static_cast<const int8_t*>(x);
+  a.ldx = ldx;
+  a.ldw = ldw;
+
+  // X is read in place when its columns are whole tiles at aligned
+  // addresses, W when its columns are aligned; the kernels' offsets within a
+  // tile of columns are 32-bit.  What is not goes to scratch first.
+  const auto in_place = [](const int8_t* p, int64_t ld) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0 && ld <= (1 << 22);
+  };
+  const int64_t pad = (d + kI8TileK - 1) / kI8TileK * kI8TileK;
+  const bool own_x = data != SDCA_I8 || d != pad || !in_place(a.X, ldx);
+  const bool own_w = !in_place(a.W, ldw);
+  const size_t x_bytes = own_x ? static_cast<size_t>(n) * pad : 0;
+  const size_t s_bytes = data != SDCA_I8 ? (n * sizeof(float) + 255) / 256 * 256 : 0;
+  const size_t w_bytes = own_w ? static_cast<size_t>(m) * pad : 0;
+  if (x_bytes + s_bytes + w_bytes) {
+    void* ws = nullptr;
+    if ((rc = workspace(stream, 7, x_bytes + s_bytes + w_bytes, &ws))) return rc;
+    int8_t* wx = static_cast<int8_t*>(ws);
+    float* wsx = reinterpret_cast<float*>(wx + x_bytes + w_bytes);
+    int8_t* ww = wx + x_bytes;
+    if (data != SDCA_I8) {
+      QuantLaunch q;
+      q.data = data;
+      q.d = d;
+      q.n = n;
+      q.X = x;
+      q.ldx = ldx;
+      q.Q = wx;
+      q.ldq = q.pad = pad;
+      q.scales = wsx;
+      q.stream = stream;
+      SDCA_HIP_TRY(launch_quantize(q), "quantise kernel");
+      a.sx = wsx;
+    } else if (own_x) {
+      SDCA_HIP_TRY(launch_repack_i8(a.X, ldx, d, n, wx, pad, pad, stream), "repack kernel");
+    }
+    if (own_x) {
+      a.X = wx;
+      a.ldx = pad;
+    }
+    if (own_w) {
+      SDCA_HIP_TRY(launch_repack_i8(a.W, ldw, d, m, ww, pad, pad, stream), "repack kernel");
+      a.W = ww;
+      a.ldw = pad;
+    }
+  }
+  SDCA_HIP_TRY(launch_scores_i8(a), "8-bit score kernel");
+  if (host) {
+    if ((rc = fetch_columns(S, a.S, m, n, lds, element_size(out), stream))) return rc;
+    SDCA_HIP_TRY(hipStreamSynchronize(stream), "hipStreamSynchronize");
+  }
+  return SDCA_OK;
+}
+
+int check_sample_params(double temperature, double top_p, double min_p, int64_t top_k) {
+  if (!(temperature >= 0) || std::isinf(temperature))
+    return fail(SDCA_ERR_ARG_RANGE, "temperature must be >= 0 and finite (got %g)", temperature);
+  if (!(top_p > 0 && top_p <= 1))
+    return fail(SDCA_ERR_ARG_RANGE, "top_p must be in (0, 1] (got %g)", top_p);
+  if (!(min_p >= 0 && min_p <= 1))
+    return fail(SDCA_ERR_ARG_RANGE, "min_p must be in [0, 1] (got %g)", min_p);
+  if (top_k < 0)
+    return fail(SDCA_ERR_ARG_RANGE, "top_k must be >= 0 (got %lld)", (long long)top_k);
+  return SDCA_OK;
+}
+
+int sample_common(int data, int64_t m, int64_t n, const void* S, int64_t lds, const float* u,
+                  const sdca_sample_params* params, const sdca_sample_columns* columns,
+                  int64_t* labels, float* prob, int64_t* kept, unsigned flags,
+                  hipStream_t stream) {
+  if (!is_float_type(data))
+    return fail(SDCA_ERR_PRECISION, "sample takes F32, F64, F16 or BF16 scores (got %d)", data);
+  if (m < 1 || n < 0 || m > INT32_MAX / 2 || n > INT32_MAX / 2)
+    return fail(SDCA_ERR_ARG_RANGE, "need m >= 1 and n >= 0 (got m %lld, n %lld)", (long long)m,
+                (long long)n);
+  sdca_sample_params p;
+  if (params) p = *params;
+  else sdca_sample_params_default(&p);
+  sdca_sample_columns c = {nullptr, nullptr, nullptr, nullptr};
+  if (columns) c = *columns;
+  int rc;
+  if ((rc = check_sample_params(p.temperature, p.top_p, p.min_p, p.top_k)) ||
+      (rc = check_matrix("S", m, lds)))
+    return rc;
+  if (n == 0) return SDCA_OK;
+  if (!S || !u || !labels) return fail(SDCA_ERR_ARG_NULL, "S, u and labels must not be NULL");
+  const bool host = (flags & SDCA_HOST_PTR) != 0;
+  if (host)
+    for (int64_t j = 0; j < n; ++j) {
+      if ((rc = check_sample_params(c.temperature ? c.temperature[j] : p.temperature,
+                                    c.top_p ? c.top_p[j] : p.top_p,
+                                    c.min_p ? c.min_p[j] : p.min_p,
+                                    c.top_k ? c.top_k[j] : p.top_k)))
+        return rc;
+      if (!(u[j] >= 0 && u[j] < 1))
+        return fail(SDCA_ERR_ARG_RANGE, "u[%lld] = %g outside [0, 1)", (long long)j, u[j]);
+    }
+  DeviceBuffer dS, du, dt, dp, dq, dk, dl, dprob, dkept;
+  sdca_gpu::SampleLaunch a;
+  a.data = data;
+  a.m = m;
+  a.n = n;
+  a.lds = lds;
+  a.temperature.value = static_cast<float>(p.temperature);
+  a.top_p.value = static_cast<float>(p.top_p);
+  a.min_p.value = static_cast<float>(p.min_p);
+  a.top_k.value = p.top_k;
+  a.stream = stream;
+  if ((rc = staged(S, span(m, n, lds, element_size(data)), host, dS, stream, &a.S)) ||
+      (rc = staged(u, n * sizeof(float), host, du, stream, &a.u)) ||
+      (rc = staged(c.temperature, n * sizeof(float), host, dt, stream, &a.temperature.each)) ||
+      (rc = staged(c.top_p, n * sizeof(float), host, dp, stream, &a.top_p.each)) ||
+      (rc = staged(c.min_p, n * sizeof(float), host, dq, stream, &a.min_p.each)) ||
+      (rc = staged(c.top_k, n * sizeof(int64_t), host, dk, stream, &a.top_k.each)) ||
+      (rc = staged_out(labels, n * sizeof(int64_t), host, dl, &a.labels)) ||
+      (rc = staged_out(prob, n * sizeof(float), host, dprob, &a.prob)) ||
+      (rc = staged_out(kept, n * sizeof(int64_t), host, dkept, &a.kept)))
+    return rc;
+  SDCA_HIP_TRY(sdca_gpu::launch_sample(a), "sampling kernel");
+  if (host) {
+    if ((rc = fetch_columns(labels, a.labels, n, 1, n, sizeof(int64_t), stream)) ||
+        (prob && (rc = fetch_columns(prob, a.prob, n, 1, n, sizeof(float), stream))) ||
+        (kept && (rc = fetch_columns(kept, a.kept, n, 1, n, sizeof(int64_t), stream))))
+      return rc;
+    SDCA_HIP_TRY(hipStreamSynchronize(stream), "hipStreamSynchronize");
+  }
+  return SDCA_OK;
+}
+
+// Nothing is thrown through the C boundary (the workspace cache's map and
+// the messages can run out of memory).
+template <class F>
+int guarded(F f) {
+  try {
+    g_last_error.clear();
+    return f();
+  } catch (...) {
+    return SDCA_ERR_OUT_OF_MEMORY;
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int sdca_quantize_i8(sdca_dtype data, int64_t d, int64_t n, const void* X, int64_t ldx,
+                     int8_t* Q, int64_t ldq, float* scales, unsigned flags, void* stream) {
+  return guarded([&] {
+    return quantize_common(data, d, n, X, ldx, Q, ldq, scales, flags,
+                           static_cast<hipStream_t>(stream));
+  });
+}
+
+int sdca_scores_i8(sdca_dtype data, sdca_dtype out, int64_t d, int64_t m, int64_t n,
+                   const void* X, int64_t ldx, const float* sx, const int8_t* W, int64_t ldw,
+                   const float* sw, void* S, int64_t lds, unsigned flags, void* stream) {
+  return guarded([&] {
+    return scores_i8_common(data, out, d, m, n, X, ldx, sx, W, ldw, sw, S, lds, flags,
+                            static_cast<hipStream_t>(stream));
+  });
+}
+
+void sdca_sample_params_default(sdca_sample_params* p) {
+  if (!p) return;
+  p->temperature = 1;
+  p->top_p = 1;
+  p->min_p = 0;
+  p->top_k = 0;
+}
+
+int sdca_sample(sdca_dtype data, int64_t m, int64_t n, const void* S, int64_t lds,
+                const float* u, const sdca_sample_params* params,
+                const sdca_sample_columns* columns, int64_t* labels, float* prob,
+                int64_t* kept, unsigned flags, void* stream) {
+  return guarded([&] {
+    return sample_common(data, m, n, S, lds, u, params, columns, labels, prob, kept, flags,
+                         static_cast<hipStream_t>(stream));
+  });
 }
 
 }  // extern "C"
