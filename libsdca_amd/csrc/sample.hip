@@ -15,18 +15,26 @@
 // their order, so a drawn label depends neither on how a column is split
 // over threads nor on the order of atomics, and they are exact where sums of
 // 32-bit floats would lose the tail's small weights.
+//
+// A cut is found from a short list.  The lanes that share a column each hold
+// the largest of their part of it; an order statistic of those maxima is a
+// bound with a known number of scores at or above it, and not many more.
+// The scores above the bound are gathered with their indices and sorted;
+// the cuts are then prefixes of the sorted list.  Where the list does not
+// hold (very many equal scores, a nucleus of thousands) the cut comes from
+// a search over the whole column.  The draw itself goes by rising index: a
+// prefix sum over the kept labels.
 #include "answer_launch.hpp"
 #include "answer_types.hpp"
+#include "common.hpp"
 
 namespace sdca_gpu {
 namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kBlock = 1024;
-constexpr int kWaves = kBlock / 64;
-constexpr int kVec = 4;
 constexpr int kBins = 2048;
+constexpr u64 kOne52 = 0x4330000000000000ull;  // 2^52 as a double
 
 // A NaN counts as a label that cannot be drawn; -0 and 0 are one value.
 __device__ inline float score(float x) { return x == x ? x + 0.f : -INFINITY; }
@@ -39,73 +47,489 @@ __device__ inline unsigned key_of(float x) {
 __device__ inline float score_of(unsigned key) {
   return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
 }
+// Falling scores, ties by rising index, as falling integers (0: no label).
+__device__ inline u64 entry_of(float l, int index) {
+  return (static_cast<u64>(key_of(l)) << 32) | (0xffffffffu - static_cast<unsigned>(index));
+}
+__device__ inline int index_of(u64 entry) {
+  return static_cast<int>(0xffffffffu - static_cast<unsigned>(entry));
+}
 
 struct Weights {
-  float max, inv_t, scale;
+  float max, inv_t;
+  double scale;
   __device__ float of(float l) const { return l == max ? 1.f : expf((l - max) * inv_t); }
-  __device__ u64 fixed(float w) const { return static_cast<u64>(rintf(w * scale)); }
-};
-
-struct Shared {
-  u64 hist[kBins];
-  u64 wave[kWaves], wave2[kWaves], wave3[kWaves];
-  u64 found_above;
-  int found_bin;
-};
-
-__device__ inline u64 shfl_up64(u64 v, int d) {
-  const unsigned lo = __shfl_up(static_cast<unsigned>(v), d);
-  const unsigned hi = __shfl_up(static_cast<unsigned>(v >> 32), d);
-  return (static_cast<u64>(hi) << 32) | lo;
-}
-__device__ inline u64 shfl_xor64(u64 v, int d) {
-  const unsigned lo = __shfl_xor(static_cast<unsigned>(v), d);
-  const unsigned hi = __shfl_xor(static_cast<unsigned>(v >> 32), d);
-  return (static_cast<u64>(hi) << 32) | lo;
-}
-__device__ inline u64 wave_scan(u64 v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const u64 o = shfl_up64(v, d);
-    if (lane >= d) v += o;
+  // w 2^shift to the nearest integer, plus the pattern of 2^52: the sum
+  // w 2^shift + 2^52 has its integer part in the lowest bits.  Sums of
+  // these carry a known multiple of the pattern.
+  __device__ u64 raw(float w) const {
+    return static_cast<u64>(__double_as_longlong(__builtin_fma(static_cast<double>(w), scale, 4503599627370496.0)));
   }
+  __device__ u64 fixed(float w) const { return raw(w) - kOne52; }
+};
+
+// ---------------------------------------------------------------------------
+// Waves: 64-bit exchanges, scans and sorts.
+// ---------------------------------------------------------------------------
+template <int CTRL, int RM>
+__device__ inline u64 dpp64(u64 v) {
+  const unsigned lo = dpp_bits<CTRL, RM, false>(static_cast<int>(v));
+  const unsigned hi = dpp_bits<CTRL, RM, false>(static_cast<int>(v >> 32));
+  return (static_cast<u64>(hi) << 32) | lo;
+}
+// Inclusive sum over the lanes before: rows of 16 by shifts, then the last
+// lanes of rows 0 and 2 into 1 and 3, and of the first half into the second.
+__device__ inline u64 wave_scan(u64 v) {
+  v += dpp64<0x111, 0xF>(v);
+  v += dpp64<0x112, 0xF>(v);
+  v += dpp64<0x114, 0xF>(v);
+  v += dpp64<0x118, 0xF>(v);
+  v += dpp64<0x142, 0xA>(v);
+  v += dpp64<0x143, 0xC>(v);
   return v;
 }
-__device__ inline u64 wave_sum(u64 v) {
+__device__ inline int wave_scan(int v) {
+  v += dpp_bits<0x111, 0xF, false>(v);
+  v += dpp_bits<0x112, 0xF, false>(v);
+  v += dpp_bits<0x114, 0xF, false>(v);
+  v += dpp_bits<0x118, 0xF, false>(v);
+  v += dpp_bits<0x142, 0xA, false>(v);
+  v += dpp_bits<0x143, 0xC, false>(v);
+  return v;
+}
+__device__ inline u64 read_lane64(u64 v, int l) {
+  const unsigned lo = __builtin_amdgcn_readlane(static_cast<int>(v), l);
+  const unsigned hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), l);
+  return (static_cast<u64>(hi) << 32) | lo;
+}
+__device__ inline u64 wave_sum(u64 v) { return read_lane64(wave_scan(v), 63); }
+__device__ inline int wave_sum(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+
+template <int OFF, bool VALU>
+__device__ inline u64 xor_lane64(u64 v) {
+  const unsigned lo = xor_lane<OFF, VALU>(static_cast<int>(v));
+  const unsigned hi = xor_lane<OFF, VALU>(static_cast<int>(v >> 32));
+  return (static_cast<u64>(hi) << 32) | lo;
+}
+template <int OFF, bool VALU>
+__device__ inline u64 other(u64 v) { return xor_lane64<OFF, VALU>(v); }
+template <int OFF, bool VALU>
+__device__ inline float other(float v) { return xor_lane<OFF, VALU>(v); }
+
+template <bool VALU>
+__device__ inline float wave_max(float v) {
+  v = fmaxf(v, other<1, VALU>(v));
+  v = fmaxf(v, other<2, VALU>(v));
+  v = fmaxf(v, other<4, VALU>(v));
+  v = fmaxf(v, other<8, VALU>(v));
+  v = fmaxf(v, other<16, VALU>(v));
+  return fmaxf(v, other<32, VALU>(v));
+}
+
+// One step of a bitonic sort: the lane keeps the larger or the smaller of
+// its value and lane ^ STRIDE's.
+template <int STRIDE, bool VALU, class K>
+__device__ inline K sort_step(K v, bool falling) {
+  const K o = other<STRIDE, VALU>(v);
+  const bool larger = ((threadIdx.x & STRIDE) == 0) == falling;
+  return (o > v) == larger ? o : v;
+}
+template <int STRIDE, bool VALU, class K>
+__device__ inline K sort_merge(K v, bool falling) {
+  if constexpr (STRIDE >= 32) v = sort_step<32, VALU>(v, falling);
+  if constexpr (STRIDE >= 16) v = sort_step<16, VALU>(v, falling);
+  if constexpr (STRIDE >= 8) v = sort_step<8, VALU>(v, falling);
+  if constexpr (STRIDE >= 4) v = sort_step<4, VALU>(v, falling);
+  if constexpr (STRIDE >= 2) v = sort_step<2, VALU>(v, falling);
+  return sort_step<1, VALU>(v, falling);
+}
+// The wave's 64 values by lane, falling or rising.
+template <bool VALU, class K>
+__device__ inline K sort_wave(K v, bool falling) {
+  v = sort_merge<1, VALU>(v, (threadIdx.x & 2) == 0);
+  v = sort_merge<2, VALU>(v, (threadIdx.x & 4) == 0);
+  v = sort_merge<4, VALU>(v, (threadIdx.x & 8) == 0);
+  v = sort_merge<8, VALU>(v, (threadIdx.x & 16) == 0);
+  v = sort_merge<16, VALU>(v, (threadIdx.x & 32) == 0);
+  return sort_merge<32, VALU>(v, falling);
+}
+
+// ---------------------------------------------------------------------------
+// Settings and results of a column.
+// ---------------------------------------------------------------------------
+struct SampleArgs {
+  int m;
+  int64_t n, lds;
+  const float* u;
+  PerColumn<float> temperature, top_p, min_p;
+  PerColumn<int64_t> top_k;
+  int64_t* labels;
+  float* prob;
+  int64_t* kept;
+  double scale;
+};
+
+template <class T>
+__device__ inline T setting(const PerColumn<T>& c, int64_t col) {
+  return c.each ? c.each[col] : c.value;
+}
+
+struct Settings {
+  float t, p, q;
+  int k;  // 0: off
+  bool greedy, cut;
+  __device__ Settings(const SampleArgs& a, int64_t col) {
+    t = fminf(setting(a.temperature, col), 3.402823466e38f);
+    greedy = !(setting(a.temperature, col) >= 1.17549435e-38f);
+    p = setting(a.top_p, col);
+    p = p < 1.f ? fmaxf(p, 0.f) : 1.f;
+    q = setting(a.min_p, col);
+    q = q > 0.f ? fminf(q, 1.f) : 0.f;
+    const int64_t kk = setting(a.top_k, col);
+    k = kk > 0 && kk < a.m ? static_cast<int>(kk) : 0;
+    cut = k || p < 1.f;
+  }
+};
+
+__device__ inline void answer(const SampleArgs& a, int64_t col, int64_t label, float prob,
+                              int64_t kept) {
+  a.labels[col] = label;
+  if (a.prob) a.prob[col] = prob;
+  if (a.kept) a.kept[col] = kept;
+}
+
+// The shortest beginning with at least p of the mass, and at least one
+// label: the least integer sum that it reaches.
+__device__ inline u64 top_p_target(float p, u64 mass) {
+  const u64 t = static_cast<u64>(ceil(static_cast<double>(p) * static_cast<double>(mass)));
+  return t < 1 ? 1 : t > mass ? mass : t;
+}
+// The label is the first whose sum exceeds this.
+__device__ inline u64 draw_target(float u, u64 total) {
+  u = u > 0.f ? (u < 1.f ? u : 0.99999994f) : 0.f;
+  const u64 t = static_cast<u64>(static_cast<double>(u) * static_cast<double>(total));
+  return t < total ? t : total - 1;
+}
+__device__ inline float share(float w, double scale, u64 total) {
+  return static_cast<float>(static_cast<double>(w) * scale / static_cast<double>(total));
+}
+// Scores below this have weight 0: exp(-105) is below half the smallest
+// float.  (Rounded down, so that no score of nonzero weight is below.)
+__device__ inline float live_floor(float max, float t) {
+  const float f = max - 106.f * t;
+  return f == f ? f : -INFINITY;  // an infinite maximum
+}
+
+// ---------------------------------------------------------------------------
+// A column in a wave's registers: lane t holds the values 256 g + 4 t + e.
+// ---------------------------------------------------------------------------
+
+// The cut (tau, ties) by a search over the keys' bits, for a column whose
+// short list does not do: each step counts or sums what is at least a
+// trial key.
+template <int E>
+__device__ inline void wave_search(const float (&l)[E], const Weights& wt, const Settings& c,
+                                         unsigned* tau_out, int* ties_out) {
+  unsigned tau = 0;
+  int ties = 0;
+  if (c.k) {
+    for (int bit = 31; bit >= 0; --bit) {
+      const unsigned trial = tau | (1u << bit);
+      int count = 0;
 #pragma unroll
-  for (int d = 32; d; d >>= 1) v += shfl_xor64(v, d);
-  return v;
+      for (int e = 0; e < E; ++e) count += __popcll(__ballot(key_of(l[e]) >= trial));
+      if (count >= c.k) tau = trial;
+    }
+    int above = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) above += __popcll(__ballot(key_of(l[e]) > tau));
+    ties = c.k - above;
+  }
+  if (c.p < 1.f) {
+    const u64 f_tau = ties ? wt.fixed(wt.of(score_of(tau))) : 0;
+    u64 mass = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) mass += key_of(l[e]) > tau ? wt.fixed(wt.of(l[e])) : 0;
+    mass = wave_sum(mass) + ties * f_tau;
+    const u64 target = top_p_target(c.p, mass);
+    unsigned cut = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const unsigned trial = cut | (1u << bit);
+      u64 sum = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum += key_of(l[e]) >= trial ? wt.fixed(wt.of(l[e])) : 0;
+      if (wave_sum(sum) >= target) cut = trial;
+    }
+    u64 above = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) above += key_of(l[e]) > cut ? wt.fixed(wt.of(l[e])) : 0;
+    above = wave_sum(above);
+    const u64 f = wt.fixed(wt.of(score_of(cut)));
+    const u64 need = f ? (target - above + f - 1) / f : 1;
+    ties = cut == tau && ties && need > static_cast<u64>(ties) ? ties : static_cast<int>(need);
+    tau = cut;
+  }
+  *tau_out = tau;
+  *ties_out = ties;
 }
-__device__ inline u64 block_sum(u64 v, u64* part) {
-  v = wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-  __syncthreads();
+
+// The draw from a column in registers: the labels above tau and the first
+// `ties` at it, those with a weight of at least q.
+template <int E>
+__device__ inline void wave_draw(const float (&l)[E], const Weights& wt, const Settings& c,
+                                 const SampleArgs& a, int64_t col, unsigned tau, int ties) {
+  const int lane = threadIdx.x & 63;
+  const float w_tau = ties ? wt.of(score_of(tau)) : 0.f;
+  u64 mass = 0;
+  int count = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float w = wt.of(l[e]);
+    const bool in = (tau == 0 || key_of(l[e]) > tau) && w >= c.q && w > 0.f;
+    mass += in ? wt.fixed(w) : 0;
+    count += in;
+  }
+  const bool tied = ties && w_tau >= c.q && w_tau > 0.f;
+  int left = 0;  // of the ties
+  if (tied) {
+    int at = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) at += __popcll(__ballot(key_of(l[e]) == tau));
+    left = at < ties ? at : ties;
+  }
+  const u64 total = wave_sum(mass) + left * (tied ? wt.fixed(w_tau) : 0);
+  const int many = wave_sum(count) + left;
+  const u64 target = draw_target(a.u[col], total);
+  u64 base = 0;
+  bool done = false;
+#pragma unroll
+  for (int g = 0; g < E / 4; ++g) {
+    if (done) continue;
+    int own = 0;
+    if (tied) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) own += key_of(l[4 * g + e]) == tau;
+    }
+    const int before = tied ? wave_scan(own) - own : 0;
+    int rank = before;
+    u64 f[4];
+    float w[4];
+    u64 sum = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float v = l[4 * g + e];
+      w[e] = wt.of(v);
+      bool in = (tau == 0 || key_of(v) > tau);
+      if (tied && key_of(v) == tau) in = rank++ < left;
+      f[e] = in && w[e] >= c.q ? wt.fixed(w[e]) : 0;
+      sum += f[e];
+    }
+    const u64 incl = wave_scan(sum) + base;
+    const u64 passed = __ballot(incl > target);
+    if (passed) {
+      if (lane == __ffsll(passed) - 1) {
+        u64 s = incl - sum;
+        int pick = 3;
+        float wp = w[3];
+#pragma unroll
+        for (int e = 2; e >= 0; --e) {
+          u64 upto = s;
+#pragma unroll
+          for (int b = 0; b <= e; ++b) upto += f[b];
+          if (upto > target) {
+            pick = e;
+            wp = w[e];
+          }
+        }
+        answer(a, col, 256 * g + 4 * lane + pick, share(wp, wt.scale, total), many);
+      }
+      done = true;
+    }
+    base = read_lane64(incl, 63);
+    if (tied) {
+      const int used = __builtin_amdgcn_readlane(before + own, 63);
+      left = left > used ? left - used : 0;
+    }
+  }
+}
+
+template <class T, int E>
+__global__ __launch_bounds__(256) void sample_wave_kernel(const T* __restrict__ S, SampleArgs a) {
+  __shared__ u64 lists[4][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * 4 + wave;
+  if (col >= a.n) return;
+  const T* row = S + col * a.lds;
+
+  float l[E];
+  float most = -INFINITY;
+#pragma unroll
+  for (int g = 0; g < E / 4; ++g) {
+    float v[4];
+    load_vec<4>(row, 256 * g + 4 * lane, a.m, v, -INFINITY);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      l[4 * g + e] = score(v[e]);
+      most = fmaxf(most, l[4 * g + e]);
+    }
+  }
+  const Settings c(a, col);
+  Weights wt;
+  wt.max = wave_max<false>(most);
+  if (wt.max == -INFINITY) {
+    if (lane == 0) answer(a, col, -1, 0.f, 0);
+    return;
+  }
+  if (c.greedy) {
+#pragma unroll
+    for (int g = 0; g < E / 4; ++g) {
+      const bool here = l[4 * g] == wt.max || l[4 * g + 1] == wt.max || l[4 * g + 2] == wt.max ||
+                        l[4 * g + 3] == wt.max;
+      const u64 any = __ballot(here);
+      if (any) {
+        if (lane == __ffsll(any) - 1) {
+          const int e = l[4 * g] == wt.max ? 0 : l[4 * g + 1] == wt.max ? 1 : l[4 * g + 2] == wt.max ? 2 : 3;
+          answer(a, col, 256 * g + 4 * lane + e, 1.f, 1);
+        }
+        return;
+      }
+    }
+  }
+  wt.inv_t = 1.f / c.t;
+  wt.scale = a.scale;
+  if (!c.cut) {
+    wave_draw<E>(l, wt, c, a, col, 0, 0);
+    return;
+  }
+
+  // The bound: the k-th largest lane maximum, or for top-p alone the 32nd,
+  // which a list of 64 mostly holds (44 of 1000 scores on average).
+  const bool list_does = c.k <= 64;
+  const float floor_live = live_floor(wt.max, c.t);
+  int count = 65;
+  float bound = 0.f;
+  u64* list = lists[wave];
+  if (list_does) {
+    const float sorted = sort_wave<false>(most, true);
+    bound = read_lane(sorted, c.k ? c.k - 1 : 31);
+    const float from = fmaxf(bound, floor_live);
+    count = 0;
+#pragma unroll
+    for (int g = 0; g < E / 4; ++g) {
+      bool in[4];
+      u64 mask[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        in[e] = l[4 * g + e] >= from && l[4 * g + e] > -INFINITY;
+        mask[e] = __ballot(in[e]);
+      }
+      if ((mask[0] | mask[1] | mask[2] | mask[3]) == 0) continue;
+      int at = count;  // by rising index: the lanes before, then the lane's own before
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        at = __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask[e] >> 32),
+                                       __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask[e]), at));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (in[e] && at < 64) list[at] = entry_of(l[4 * g + e], 256 * g + 4 * lane + e);
+        at += in[e];
+        count += __popcll(mask[e]);
+      }
+    }
+  }
+  bool found = count <= 64;
+  if (found) {
+    wave_lds_sync();
+    const u64 mine = lane < count ? list[lane] : 0;
+    const u64 entry = sort_wave<false>(mine, true);
+    const float w = lane < count ? wt.of(score_of(static_cast<unsigned>(entry >> 32))) : 0.f;
+    const u64 f = lane < count ? wt.fixed(w) : 0;
+    const u64 incl = wave_scan(f);
+    const int first = c.k && c.k < count ? c.k : count;
+    bool keep = lane < first && w >= c.q && w > 0.f;
+    if (c.p < 1.f) {
+      const bool whole = bound <= floor_live;  // the list holds every label of nonzero weight
+      u64 mass;
+      if (c.k || whole) {
+        mass = read_lane64(incl, first - 1);
+      } else {
+        mass = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) mass += wt.raw(wt.of(l[e]));
+        mass = wave_sum(mass - E * kOne52);
+      }
+      const u64 target = top_p_target(c.p, mass);
+      keep = keep && incl - f < target;
+      found = c.k || whole || read_lane64(incl, 63) >= target;
+    }
+    if (found) {
+      const u64 kept = __ballot(keep);  // a prefix
+      const int many = ~kept ? __ffsll(~kept) - 1 : 64;
+      const u64 last = read_lane64(entry, many - 1);
+      const u64 total = read_lane64(incl, many - 1);
+      const float wm = wt.of(score_of(static_cast<unsigned>(mine >> 32)));
+      const u64 sum = wave_scan(mine >= last ? wt.fixed(wm) : 0);
+      const u64 passed = __ballot(sum > draw_target(a.u[col], total));
+      if (lane == __ffsll(passed) - 1)
+        answer(a, col, index_of(mine), share(wm, wt.scale, total), many);
+      return;
+    }
+  }
+  unsigned tau;
+  int ties;
+  wave_search<E>(l, wt, c, &tau, &ties);
+  wave_draw<E>(l, wt, c, a, col, tau, ties);
+}
+
+// ---------------------------------------------------------------------------
+// A column to a workgroup.
+// ---------------------------------------------------------------------------
+template <int THREADS>
+struct Shared {
+  static constexpr int kWaves = THREADS / 64;
+  union {
+    u64 hist[kBins];
+    struct {
+      u64 entry[THREADS];  // the short list, sorted; then by index
+      u64 swap[THREADS];
+    } list;
+  };
+  u64 sum[kWaves], sum2[kWaves], sum3[kWaves];
+  float value[kWaves], value2[kWaves];
+  int number[kWaves];
+  u64 found_above;
+  int found_bin, count;
+};
+
+template <int W>
+__device__ inline u64 total_of(const u64 (&part)[W]) {
   u64 s = 0;
-  for (int w = 0; w < kWaves; ++w) s += part[w];
+#pragma unroll
+  for (int w = 0; w < W; ++w) s += part[w];
   return s;
 }
 
-// f(score, index) over the row's entries from `begin` on, a stride of
+// f(score, index) over the entries [begin, end) of a row in memory, by
 // `threads` lanes.
 template <class T, class F>
-__device__ inline void each(const T* row, int64_t begin, int64_t end, int t, int threads, F f) {
-  for (int64_t at = begin + int64_t(t) * kVec; at < end; at += int64_t(threads) * kVec) {
-    float v[kVec];
-    load_vec<kVec>(row, at, end, v);
+__device__ inline void each_of(const T* row, int begin, int end, int t, int threads, F f) {
+  for (int64_t at = begin + int64_t(t) * 4; at < end; at += int64_t(threads) * 4) {
+    float v[4];
+    load_vec<4>(row, at, end, v);
 #pragma unroll
-    for (int e = 0; e < kVec; ++e)
-      if (at + e < end) f(score(v[e]), at + e);
+    for (int e = 0; e < 4; ++e)
+      if (at + e < end) f(score(v[e]), static_cast<int>(at) + e);
   }
 }
 
 // The key at which the running sum over falling keys, from `floor_key` up,
 // first reaches `target` (counts, or with MASS fixed weights), and the sum
 // above it: three digits of the key, a histogram each.
-template <bool MASS, class T>
-__device__ void descend(const T* row, int64_t m, const Weights& wt, unsigned floor_key, u64 target,
-                        Shared& s, unsigned* tau, u64* above) {
+template <bool MASS, int THREADS, class T>
+__device__ void descend(const T* row, int m, const Weights& wt, unsigned floor_key, u64 target,
+                        Shared<THREADS>& s, unsigned* tau, u64* above) {
+  constexpr int kOwn = kBins / THREADS;  // bins of a thread
   unsigned prefix = 0;
   u64 sum = 0;
   for (int level = 0; level < 3; ++level) {
@@ -113,30 +537,37 @@ __device__ void descend(const T* row, int64_t m, const Weights& wt, unsigned flo
     const int bits = level == 2 ? 10 : 11;
     const int bins = 1 << bits;
     __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kBlock) s.hist[i] = 0;
+    for (int i = threadIdx.x; i < kBins; i += THREADS) s.hist[i] = 0;
     if (threadIdx.x == 0) {
       s.found_bin = 0;
       s.found_above = sum;
     }
     __syncthreads();
-    each(row, 0, m, threadIdx.x, kBlock, [&](float l, int64_t) {
+    each_of(row, 0, m, threadIdx.x, THREADS, [&](float l, int) {
       const unsigned key = key_of(l);
       if (key < floor_key || (level && (key >> (shift + bits)) != prefix)) return;
       const u64 add = MASS ? wt.fixed(wt.of(l)) : 1;
       if (add) atomicAdd(&s.hist[(key >> shift) & (bins - 1)], add);
     });
     __syncthreads();
-    const int hi = bins - 1 - 2 * static_cast<int>(threadIdx.x);
-    const u64 a = hi >= 1 ? s.hist[hi] : 0, b = hi >= 1 ? s.hist[hi - 1] : 0;
-    u64 incl = wave_scan(a + b);
-    if ((threadIdx.x & 63) == 63) s.wave[threadIdx.x >> 6] = incl;
+    const int hi = bins - 1 - kOwn * static_cast<int>(threadIdx.x);
+    u64 own = 0;
+    for (int b = 0; b < kOwn; ++b) own += hi - b >= 0 ? s.hist[hi - b] : 0;
+    u64 before = wave_scan(own);
+    if ((threadIdx.x & 63) == 63) s.sum[threadIdx.x >> 6] = before;
     __syncthreads();
-    for (int w = 0; w < static_cast<int>(threadIdx.x >> 6); ++w) incl += s.wave[w];
-    const u64 before = sum + incl - a - b;
-    if (before < target && before + a + b >= target) {
-      const bool first = before + a >= target;
-      s.found_bin = first ? hi : hi - 1;
-      s.found_above = first ? before : before + a;
+    for (int w = 0; w < static_cast<int>(threadIdx.x >> 6); ++w) before += s.sum[w];
+    before += sum - own;
+    if (before < target && before + own >= target) {
+      for (int b = 0; b < kOwn; ++b) {
+        const u64 here = s.hist[hi - b];
+        if (before + here >= target) {
+          s.found_bin = hi - b;
+          s.found_above = before;
+          break;
+        }
+        before += here;
+      }
     }
     __syncthreads();
     prefix = (prefix << bits) | static_cast<unsigned>(s.found_bin);
@@ -146,83 +577,32 @@ __device__ void descend(const T* row, int64_t m, const Weights& wt, unsigned flo
   *above = sum;
 }
 
-template <class T>
-__device__ inline T setting(const PerColumn<T>& c, int64_t col) {
-  return c.each ? c.each[col] : c.value;
-}
-
-struct SampleArgs {
-  int64_t m, lds;
-  const float* u;
-  PerColumn<float> temperature, top_p, min_p;
-  PerColumn<int64_t> top_k;
-  int64_t* labels;
-  float* prob;
-  int64_t* kept;
-  float scale;
-};
-
-// A column per workgroup, read from memory on every pass.
-template <class T>
-__global__ __launch_bounds__(kBlock) void sample_column_kernel(const T* __restrict__ S,
-                                                               SampleArgs a) {
-  __shared__ Shared s;
-  const int64_t col = blockIdx.x, m = a.m;
-  const T* row = S + col * a.lds;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-
-  u64 best = 0;  // (key, falling index) of the first maximum
-  each(row, 0, m, threadIdx.x, kBlock, [&](float l, int64_t i) {
-    const u64 c = (static_cast<u64>(key_of(l)) << 32) | (0xffffffffu - static_cast<unsigned>(i));
-    best = c > best ? c : best;
-  });
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const u64 o = shfl_xor64(best, d);
-    best = o > best ? o : best;
-  }
-  if (lane == 0) s.wave[wave] = best;
-  __syncthreads();
-  for (int w = 0; w < kWaves; ++w) best = s.wave[w] > best ? s.wave[w] : best;
-
-  const float T_ = setting(a.temperature, col);
-  Weights wt;
-  wt.max = score_of(static_cast<unsigned>(best >> 32));
-  const bool greedy = !(T_ >= 1.17549435e-38f), none = wt.max == -INFINITY;
-  if (greedy || none) {
-    if (threadIdx.x == 0) {
-      a.labels[col] = none ? -1 : static_cast<int64_t>(0xffffffffu - static_cast<unsigned>(best));
-      if (a.prob) a.prob[col] = none ? 0.f : 1.f;
-      if (a.kept) a.kept[col] = none ? 0 : 1;
-    }
-    return;
-  }
-  wt.inv_t = 1.f / fminf(T_, 3.402823466e38f);
-  wt.scale = a.scale;
-  const float p = setting(a.top_p, col);
-  float q = setting(a.min_p, col);
-  q = q > 0.f ? fminf(q, 1.f) : 0.f;
-  const int64_t k = setting(a.top_k, col);
-
+// The cut by searches over the whole column, and the draw: for columns whose
+// short list does not do.
+template <int THREADS, class T>
+__device__ void search_and_draw(const T* row, const Weights& wt, const Settings& c,
+                                const SampleArgs& a, int64_t col, Shared<THREADS>& s) {
+  constexpr int kWaves = THREADS / 64;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = a.m;
   unsigned tau = 0;
   u64 ties = 0;  // labels at tau that are kept
-  if (k > 0 && k < m) {
+  if (c.k) {
     u64 above;
-    descend<false>(row, m, wt, 0, static_cast<u64>(k), s, &tau, &above);
-    ties = k - above;
+    descend<false>(row, m, wt, 0, static_cast<u64>(c.k), s, &tau, &above);
+    ties = c.k - above;
   }
-  if (p < 1.f) {
+  if (c.p < 1.f) {
     u64 mass = 0;
-    each(row, 0, m, threadIdx.x, kBlock, [&](float l, int64_t) {
+    each_of(row, 0, m, threadIdx.x, THREADS, [&](float l, int) {
       if (key_of(l) > tau) mass += wt.fixed(wt.of(l));
     });
-    mass = block_sum(mass, s.wave2);
+    mass = wave_sum(mass);
+    __syncthreads();
+    if (lane == 0) s.sum[wave] = mass;
+    __syncthreads();
+    mass = total_of(s.sum);
     if (ties) mass += ties * wt.fixed(wt.of(score_of(tau)));
-    // The shortest beginning with a sum of at least p mass, and of at least
-    // one label.
-    u64 target = static_cast<u64>(ceil(static_cast<double>(p) * static_cast<double>(mass)));
-    target = p > 0.f ? target : 1;
-    target = target < 1 ? 1 : target > mass ? mass : target;
+    const u64 target = top_p_target(c.p, mass);
     unsigned cut;
     u64 above;
     descend<true>(row, m, wt, tau, target, s, &cut, &above);
@@ -233,60 +613,51 @@ __global__ __launch_bounds__(kBlock) void sample_column_kernel(const T* __restri
     ties = need;
   }
 
-  // The draw.  The row is narrowed to the stretch that holds the label, a
-  // sixteenth at a time; the first narrowing also gives the total.
+  // The row is narrowed to the stretch that holds the label, a wave's share
+  // at a time; the first narrowing also gives the total.
   const float w_tau = ties ? wt.of(score_of(tau)) : 0.f;
-  const u64 f_tau = w_tau >= q ? wt.fixed(w_tau) : 0;
-  int64_t begin = 0, end = m;
-  u64 total = 0, target = 0, tie_base = 0, mass_base = 0;
+  const u64 f_tau = w_tau >= c.q ? wt.fixed(w_tau) : 0;
+  int begin = 0, end = m;
+  u64 total = 0, target = 0, tie_base = 0, mass_base = 0, many = 0;
   while (true) {
-    const int64_t part = ((end - begin + kWaves - 1) / kWaves + 63) / 64 * 64;
-    const int64_t b = begin + wave * part, e = b + part < end ? b + part : end;
-    u64 n_tie = 0, mass = 0, many = 0;
+    const int part = ((end - begin + kWaves - 1) / kWaves + 63) / 64 * 64;
+    const int b = begin + wave * part, e = b + part < end ? b + part : end;
+    u64 n_tie = 0, mass = 0, count = 0;
     if (b < e)
-      each(row, b, e, lane, 64, [&](float l, int64_t) {
+      each_of(row, b, e, lane, 64, [&](float l, int) {
         const unsigned key = key_of(l);
         const float w = wt.of(l);
-        if (key > tau && w >= q && w > 0.f) {
+        if (key > tau && w >= c.q && w > 0.f) {
           mass += wt.fixed(w);
-          ++many;
+          ++count;
         }
         n_tie += ties && key == tau;
       });
     n_tie = wave_sum(n_tie);
     mass = wave_sum(mass);
-    many = wave_sum(many);
+    count = wave_sum(count);
     __syncthreads();
     if (lane == 0) {
-      s.wave[wave] = n_tie;
-      s.wave2[wave] = mass;
-      s.wave3[wave] = many;
+      s.sum[wave] = n_tie;
+      s.sum2[wave] = mass;
+      s.sum3[wave] = count;
     }
     __syncthreads();
-    if (begin == 0 && end == m && total == 0) {
-      u64 all = 0, tied = 0, count = 0;
-      for (int w = 0; w < kWaves; ++w) {
-        all += s.wave2[w];
-        tied += s.wave[w];
-        count += s.wave3[w];
-      }
+    if (total == 0) {
+      u64 tied = total_of(s.sum);
       tied = tied < ties ? tied : ties;
-      total = all + tied * f_tau;
-      count += w_tau >= q && w_tau > 0.f ? tied : 0;
-      float u = a.u[col];
-      u = u > 0.f ? (u < 1.f ? u : 0.99999994f) : 0.f;
-      target = static_cast<u64>(static_cast<double>(u) * static_cast<double>(total));
-      target = target < total ? target : total - 1;
-      if (threadIdx.x == 0 && a.kept) a.kept[col] = static_cast<int64_t>(count);
+      total = total_of(s.sum2) + tied * f_tau;
+      many = total_of(s.sum3) + (w_tau >= c.q && w_tau > 0.f ? tied : 0);
+      target = draw_target(a.u[col], total);
     }
-    int64_t pick = begin;
+    int pick = begin;
     for (int w = 0; w < kWaves; ++w) {
       const u64 left = ties > tie_base ? ties - tie_base : 0;
-      const u64 t = s.wave[w] < left ? s.wave[w] : left;
-      const u64 here = s.wave2[w] + t * f_tau;
+      const u64 t = s.sum[w] < left ? s.sum[w] : left;
+      const u64 here = s.sum2[w] + t * f_tau;
       if (mass_base + here > target) break;
       mass_base += here;
-      tie_base += s.wave[w];
+      tie_base += s.sum[w];
       pick += part;
     }
     begin = pick;
@@ -299,22 +670,362 @@ __global__ __launch_bounds__(kBlock) void sample_column_kernel(const T* __restri
     const unsigned key = key_of(l);
     const float w = wt.of(l);
     const bool tied = in && ties && key == tau;
-    const u64 ranked = wave_scan(tied ? 1 : 0) + tie_base;
-    const bool keep = in && w >= q && (key > tau || (tied && ranked <= ties));
+    const u64 rank = wave_scan(tied ? u64(1) : u64(0)) + tie_base;
+    const bool keep = in && w >= c.q && (key > tau || (tied && rank <= ties));
     const u64 sum = wave_scan(keep ? wt.fixed(w) : 0) + mass_base;
     const u64 passed = __ballot(sum > target);
-    if (passed && lane == __ffsll(passed) - 1) {
-      a.labels[col] = begin + lane;
-      if (a.prob)
-        a.prob[col] = static_cast<float>(static_cast<double>(w) * wt.scale / static_cast<double>(total));
+    if (passed && lane == __ffsll(passed) - 1)
+      answer(a, col, begin + lane, share(w, wt.scale, total), static_cast<int64_t>(many));
+  }
+}
+
+// A workgroup's column in registers: wave w holds the stretch of 64 V G
+// scores from w 64 V G on, lane t of it the values V t .. V t + V - 1 of each
+// of G groups.  R: registers' worth of values of a lane; R = 0 reads them
+// from memory each time.
+template <class T, int THREADS, int R>
+struct Column {
+  static constexpr int V = sizeof(T) == 2 ? 8 : 4;
+  static constexpr int kGroups = R / V;
+  static constexpr bool kHalf = sizeof(T) == 2;
+  const T* row;
+  int m, groups, from;  // from: of this lane's first value
+  unsigned raw[kGroups ? kGroups * (kHalf ? V / 2 : V) : 1];
+
+  __device__ Column(const T* r, int m_) : row(r), m(m_) {
+    groups = (m + THREADS * V - 1) / (THREADS * V);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    from = wave * groups * 64 * V + (threadIdx.x & 63) * V;
+    if constexpr (R > 0) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        if (g >= groups) break;
+        T v[V];
+        const int at = from + g * 64 * V;
+        if (at + V <= m) {
+          __builtin_memcpy(v, row + at, sizeof(v));
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[e] = at + e < m ? row[at + e] : T(-INFINITY);
+        }
+        if constexpr (kHalf) {
+          __builtin_memcpy(&raw[g * V / 2], v, sizeof(v));
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) raw[g * V + e] = __float_as_uint(to_float(v[e]));
+        }
+      }
     }
   }
+  // Waves whose lanes all hold a score.
+  __device__ int full_waves() const {
+    const int stretch = groups * 64 * V;
+    return min(THREADS / 64, (m - 64 * V) / stretch + 1);
+  }
+  __device__ void group(int g, float (&l)[V]) const {
+    if constexpr (R > 0) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if constexpr (kHalf) {
+          const unsigned short b = static_cast<unsigned short>(raw[(g * V + e) / 2] >> (16 * (e & 1)));
+          T t;
+          __builtin_memcpy(&t, &b, 2);
+          l[e] = score(to_float(t));
+        } else {
+          l[e] = score(__uint_as_float(raw[g * V + e]));
+        }
+      }
+    } else {
+      load_vec<V>(row, int64_t(from) + int64_t(g) * 64 * V, m, l, -INFINITY);
+#pragma unroll
+      for (int e = 0; e < V; ++e) l[e] = score(l[e]);
+    }
+  }
+  // f(scores, index of the first) for each of the lane's groups, until it
+  // gives false (in all lanes of a wave alike).
+  template <class F>
+  __device__ void groups_until(F f) {
+    if constexpr (R > 0) {
+      // Each pass makes its own floats of the registers: kept from one pass
+      // to the next they would need twice the registers, and spill.
+#pragma unroll
+      for (unsigned& r : raw) asm volatile("" : "+v"(r));
+      bool go = true;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        if (g < groups && go) {
+          float l[V];
+          group(g, l);
+          go = f(l, from + g * 64 * V);
+        }
+      }
+    } else {
+      for (int g = 0; g < groups; ++g) {
+        float l[V];
+        group(g, l);
+        if (!f(l, from + g * 64 * V)) break;
+      }
+    }
+  }
+  template <class F>
+  __device__ void each(F f) {
+    groups_until([&](const float (&l)[V], int at) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) f(l[e], at + e);
+      return true;
+    });
+  }
+};
+
+// Sorts the first P (a power of two from 64 to THREADS) of the workgroup's
+// values, one a thread, falling.
+template <int THREADS>
+__device__ inline u64 sort_block(u64 v, int P, u64* swap) {
+  const int i = threadIdx.x;
+  v = sort_wave<true>(v, (i & 64) == 0 || P == 64);
+  for (int size = 128; size <= P; size <<= 1) {
+    const bool falling = (i & size) == 0 || size == P;
+    for (int stride = size >> 1; stride >= 64; stride >>= 1) {
+      __syncthreads();
+      if (i < P) swap[i] = v;
+      __syncthreads();
+      if (i < P) {
+        const u64 o = swap[i ^ stride];
+        const bool larger = ((i & stride) == 0) == falling;
+        v = (o > v) == larger ? o : v;
+      }
+    }
+    if (i < P) v = sort_merge<32, true>(v, falling);
+  }
+  return v;
+}
+
+// The inclusive sum over the workgroup's threads.
+template <int THREADS>
+__device__ inline u64 block_scan(u64 v, u64 (&part)[THREADS / 64], u64* total) {
+  v = wave_scan(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  u64 all = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    if (w == static_cast<int>(threadIdx.x >> 6)) before = all;
+    all += part[w];
+  }
+  *total = all;
+  return v + before;
+}
+
+template <class T, int THREADS, int R>
+__global__ __launch_bounds__(THREADS) void sample_block_kernel(const T* __restrict__ S,
+                                                               SampleArgs a) {
+  constexpr int kWaves = THREADS / 64;
+  __shared__ Shared<THREADS> s;
+  const int64_t col = blockIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const T* row = S + col * a.lds;
+  typedef Column<T, THREADS, R> Col;
+  Col column(row, a.m);
+  const Settings c(a, col);
+
+  float most = -INFINITY;
+  column.each([&](float l, int) { most = fmaxf(most, l); });
+  // Each wave's maximum, and its j-th largest lane maximum: at least j scores
+  // of each wave whose lanes all hold some reach the least of those.  For a
+  // top-k that is k of them; for a nucleus alone a hundred and more.
+  const int full = column.full_waves();
+  const int j = c.k ? (c.k + full - 1) / full : min(128 / full, 32);
+  const bool list_does = c.cut && j <= 40;
+  const float top = wave_max<true>(most);
+  float jth = -INFINITY;
+  if (list_does) jth = read_lane(sort_wave<true>(most, true), j - 1);
+  if (lane == 0) {
+    s.value[wave] = top;
+    s.value2[wave] = jth;
+  }
+  if (threadIdx.x == 0) s.count = 0;
+  __syncthreads();
+  float bound = s.value2[0];
+  Weights wt;
+  wt.max = s.value[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) {
+    wt.max = fmaxf(wt.max, s.value[w]);
+    bound = w < full ? fminf(bound, s.value2[w]) : bound;
+  }
+  if (wt.max == -INFINITY) {
+    if (threadIdx.x == 0) answer(a, col, -1, 0.f, 0);
+    return;
+  }
+  if (c.greedy) {
+    int best = a.m;
+    column.each([&](float l, int i) { best = l == wt.max && i < best ? i : best; });
+#pragma unroll
+    for (int d = 32; d; d >>= 1) best = min(best, __shfl_xor(best, d));
+    if (lane == 0) s.number[wave] = best;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 0; w < kWaves; ++w) best = min(best, s.number[w]);
+      answer(a, col, best, 1.f, 1);
+    }
+    return;
+  }
+  wt.inv_t = 1.f / c.t;
+  wt.scale = a.scale;
+
+  if (!c.cut) {
+    // Each wave's sum and count; then the wave whose stretch holds the label
+    // goes through it group by group.
+    u64 mass = 0;
+    int count = 0;
+    column.each([&](float l, int) {
+      const float w = wt.of(l);
+      const bool in = w >= c.q && w > 0.f;
+      mass += in ? wt.fixed(w) : 0;
+      count += in;
+    });
+    mass = wave_sum(mass);
+    count = wave_sum(count);
+    if (lane == 0) {
+      s.sum[wave] = mass;
+      s.number[wave] = count;
+    }
+    __syncthreads();
+    const u64 total = total_of(s.sum);
+    const u64 target = draw_target(a.u[col], total);
+    u64 base = 0;
+    for (int w = 0; w < wave; ++w) base += s.sum[w];
+    if (base > target || base + s.sum[wave] <= target) return;
+    int many = 0;
+    for (int w = 0; w < kWaves; ++w) many += s.number[w];
+    column.groups_until([&](const float (&l)[Col::V], int at) {
+      u64 f[Col::V], sum = 0;
+#pragma unroll
+      for (int e = 0; e < Col::V; ++e) {
+        const float w = wt.of(l[e]);
+        f[e] = w >= c.q ? wt.fixed(w) : 0;
+        sum += f[e];
+      }
+      const u64 incl = wave_scan(sum) + base;
+      const u64 passed = __ballot(incl > target);
+      base = read_lane64(incl, 63);
+      if (!passed) return true;
+      if (lane == __ffsll(passed) - 1) {
+        u64 upto = incl - sum;
+        int pick = -1;
+        float w = 0.f;
+#pragma unroll
+        for (int e = 0; e < Col::V; ++e) {
+          upto += f[e];
+          if (pick < 0 && upto > target) {
+            pick = at + e;
+            w = wt.of(l[e]);
+          }
+        }
+        answer(a, col, pick, share(w, wt.scale, total), many);
+      }
+      return false;
+    });
+    return;
+  }
+
+  const float floor_live = live_floor(wt.max, c.t);
+  const bool whole = bound <= floor_live;  // the list holds every label of nonzero weight
+  int count = THREADS + 1;
+  if (list_does) {
+    const float from = fmaxf(bound, floor_live);
+    column.each([&](float l, int i) {
+      const bool in = l >= from && l > -INFINITY;
+      const u64 mask = __ballot(in);
+      if (mask) {
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&s.count, __popcll(mask));
+        at = __builtin_amdgcn_readfirstlane(at);
+        at = __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask >> 32),
+                                       __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask), at));
+        if (in && at < THREADS) s.list.entry[at] = entry_of(l, i);
+      }
+    });
+    u64 mass = 0;
+    const bool sum_all = c.p < 1.f && !c.k && !whole;
+    if (sum_all) {
+      column.each([&](float l, int) { mass += wt.fixed(wt.of(l)); });
+      mass = wave_sum(mass);
+      if (lane == 0) s.sum3[wave] = mass;
+    }
+    __syncthreads();
+    count = s.count;
+    if (sum_all) mass = total_of(s.sum3);
+    if (count <= THREADS) {
+      int P = 64;
+      while (P < count) P <<= 1;
+      const int i = threadIdx.x;
+      const u64 entry = sort_block<THREADS>(i < count ? s.list.entry[i] : 0, P, s.list.swap);
+      const float w = i < count ? wt.of(score_of(static_cast<unsigned>(entry >> 32))) : 0.f;
+      const u64 f = i < count ? wt.fixed(w) : 0;
+      const int first = c.k && c.k < count ? c.k : count;
+      u64 all;
+      const u64 incl = block_scan<THREADS>(i < first ? f : 0, s.sum, &all);
+      bool keep = i < first && w >= c.q && w > 0.f, found = true;
+      if (c.p < 1.f) {
+        if (!sum_all) mass = all;
+        const u64 target = top_p_target(c.p, mass);
+        keep = keep && incl - f < target;
+        found = all >= target;
+      }
+      if (found) {
+        // The kept labels, a prefix of the list, by rising index: the
+        // complement of the index falls, with the weight's place behind it.
+        const u64 votes = __ballot(keep);
+        const int own = ~votes ? __ffsll(~votes) - 1 : 64;
+        if (lane == 0) s.number[wave] = own;
+        __syncthreads();
+        int many = 0;
+        for (int w2 = 0; w2 < kWaves; ++w2) {
+          many += s.number[w2];
+          if (s.number[w2] < 64) break;
+        }
+        s.list.swap[i] = entry;
+        __syncthreads();
+        int P2 = 64;
+        while (P2 < many) P2 <<= 1;
+        // index in the high half, rank in the low
+        u64 by = i < many ? (static_cast<u64>(static_cast<unsigned>(entry)) << 32) | static_cast<unsigned>(i) : 0;
+        by = sort_block<THREADS>(by, P2, s.list.entry);
+        float wk = 0.f;
+        if (i < many) wk = wt.of(score_of(static_cast<unsigned>(s.list.swap[static_cast<unsigned>(by)] >> 32)));
+        u64 total;
+        const u64 sum = block_scan<THREADS>(i < many ? wt.fixed(wk) : 0, s.sum2, &total);
+        const u64 target = draw_target(a.u[col], total);
+        const u64 own_f = i < many ? wt.fixed(wk) : 0;
+        if (sum > target && sum - own_f <= target && own_f)
+          answer(a, col, static_cast<int64_t>(0xffffffffu - static_cast<unsigned>(by >> 32)),
+                 share(wk, wt.scale, total), many);
+        return;
+      }
+    }
+  }
+  __syncthreads();
+  search_and_draw<THREADS>(row, wt, c, a, col, s);
+}
+
+template <class T, int THREADS, int R>
+void start_block(const SampleLaunch& l, const SampleArgs& a) {
+  sample_block_kernel<T, THREADS, R><<<static_cast<unsigned>(l.n), THREADS, 0, l.stream>>>(
+      static_cast<const T*>(l.S), a);
+}
+template <class T, int E>
+void start_wave(const SampleLaunch& l, const SampleArgs& a) {
+  sample_wave_kernel<T, E><<<static_cast<unsigned>((l.n + 3) / 4), 256, 0, l.stream>>>(
+      static_cast<const T*>(l.S), a);
 }
 
 template <class T>
 hipError_t sample(const SampleLaunch& l) {
   SampleArgs a;
-  a.m = l.m;
+  a.m = static_cast<int>(l.m);
+  a.n = l.n;
   a.lds = l.lds;
   a.u = l.u;
   a.temperature = l.temperature;
@@ -326,9 +1037,18 @@ hipError_t sample(const SampleLaunch& l) {
   a.kept = l.kept;
   int bits = 0;
   while ((int64_t(1) << bits) < l.m) ++bits;
-  a.scale = static_cast<float>(u64(1) << (62 - bits < 46 ? 62 - bits : 46));
-  sample_column_kernel<T><<<static_cast<unsigned>(l.n), kBlock, 0, l.stream>>>(
-      static_cast<const T*>(l.S), a);
+  a.scale = static_cast<double>(u64(1) << (62 - bits < 46 ? 62 - bits : 46));
+  // By the column's length: a wave up to 1024 scores, a workgroup that holds
+  // the column in registers above, and one that reads it again and again
+  // where the registers do not hold it.
+  if (l.m <= 256) start_wave<T, 4>(l, a);
+  else if (l.m <= 1024) start_wave<T, 16>(l, a);
+  else if (l.m <= 256 * 16) start_block<T, 256, 16>(l, a);
+  else if (l.m <= 1024 * 16) start_block<T, 1024, 16>(l, a);
+  else if (l.m <= 1024 * 32) start_block<T, 1024, 32>(l, a);
+  else if (l.m <= 1024 * 64) start_block<T, 1024, 64>(l, a);
+  else if (sizeof(T) == 2 && l.m <= 1024 * 128) start_block<T, 1024, sizeof(T) == 2 ? 128 : 64>(l, a);
+  else start_block<T, 1024, 0>(l, a);
   return hipGetLastError();
 }
 
