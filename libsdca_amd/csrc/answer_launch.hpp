@@ -66,8 +66,10 @@ struct SampleLaunch {
   int64_t* labels;
   float* prob;    // or NULL
   int64_t* kept;  // or NULL
+  void* work;     // sample_work_bytes of device memory
   hipStream_t stream;
 };
+size_t sample_work_bytes(int64_t m, int64_t n);
 hipError_t launch_sample(const SampleLaunch& a);
 
 }  // namespace sdca_gpu

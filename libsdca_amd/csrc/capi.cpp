@@ -63,9 +63,10 @@ size_t dtype_size(int dt) { return dt == SDCA_F32 ? 4 : 8; }
 struct Workspace {
   // Slots: 0 deferred-column list, 1 scores, 2 evaluation scratch,
   // 3 transposes, 4 epoch, 5 the library GEMM's workspace, 6 the column
-  // slices of the prox beyond the LDS copy, 7 quantised and repacked operands.
-  void* ptr[8] = {};
-  size_t cap[8] = {};
+  // slices of the prox beyond the LDS copy, 7 quantised and repacked operands,
+  // 8 the parts of columns that labels are drawn from.
+  void* ptr[9] = {};
+  size_t cap[9] = {};
   // Pinned host block for the evaluation's results: copies into it are
   // asynchronous, so the call waits once for all of them.
   void* host = nullptr;
@@ -1419,7 +1420,10 @@ int sample_common(int data, int64_t m, int64_t n, const void* S, int64_t lds, co
       (rc = staged_out(prob, n * sizeof(float), host, dprob, &a.prob)) ||
       (rc = staged_out(kept, n * sizeof(int64_t), host, dkept, &a.kept)))
     return rc;
-  SDCA_HIP_TRY(sdca_gpu::launch_sample(a), "sampling kernel");
+  a.work = nullptr;
+  const size_t work = sdca_gpu::sample_work_bytes(m, n);
+  if (work && (rc = workspace(stream, 8, work, &a.work))) return rc;
+  SDCA_HIP_TRY(sdca_gpu::launch_sample(a), "sampling kernels");
   if (host) {
     if ((rc = fetch_columns(labels, a.labels, n, 1, n, sizeof(int64_t), stream)) ||
         (prob && (rc = fetch_columns(prob, a.prob, n, 1, n, sizeof(float), stream))) ||

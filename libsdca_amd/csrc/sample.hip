@@ -36,12 +36,13 @@ typedef unsigned long long u64;
 constexpr int kBins = 2048;
 constexpr u64 kOne52 = 0x4330000000000000ull;  // 2^52 as a double
 
-// A NaN counts as a label that cannot be drawn; -0 and 0 are one value.
-__device__ inline float score(float x) { return x == x ? x + 0.f : -INFINITY; }
+// A NaN counts as a label that cannot be drawn (the larger of a NaN and a
+// number is the number).
+__device__ inline float score(float x) { return fmaxf(x, -INFINITY); }
 
-// Order-preserving integer of a score.
+// Order-preserving integer of a score; -0 and 0 are one value.
 __device__ inline unsigned key_of(float x) {
-  const unsigned b = __float_as_uint(x);
+  const unsigned b = __float_as_uint(x + 0.f);
   return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
 __device__ inline float score_of(unsigned key) {
@@ -58,7 +59,8 @@ __device__ inline int index_of(u64 entry) {
 struct Weights {
   float max, inv_t;
   double scale;
-  __device__ float of(float l) const { return l == max ? 1.f : expf((l - max) * inv_t); }
+  // (The smaller of NaN and 0 is 0: an infinite maximum has weight 1.)
+  __device__ float of(float l) const { return expf(fminf((l - max) * inv_t, 0.f)); }
   // w 2^shift to the nearest integer, plus the pattern of 2^52: the sum
   // w 2^shift + 2^52 has its integer part in the lowest bits.  Sums of
   // these carry a known multiple of the pattern.
@@ -483,20 +485,23 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const T* __restrict__ 
 }
 
 // ---------------------------------------------------------------------------
-// A column to a workgroup.
+// A column to a workgroup, and to several.
 // ---------------------------------------------------------------------------
+constexpr int kList = 1024;  // entries of a short list
+
 template <int THREADS>
 struct Shared {
   static constexpr int kWaves = THREADS / 64;
+  static constexpr int kEntries = THREADS < kList ? THREADS : kList;
   union {
     u64 hist[kBins];
     struct {
-      u64 entry[THREADS];  // the short list, sorted; then by index
+      u64 entry[kEntries];
       u64 swap[THREADS];
     } list;
   };
   u64 sum[kWaves], sum2[kWaves], sum3[kWaves];
-  float value[kWaves], value2[kWaves];
+  float value[kWaves], value2[kWaves], value3[kWaves];
   int number[kWaves];
   u64 found_above;
   int found_bin, count;
@@ -509,6 +514,28 @@ __device__ inline u64 total_of(const u64 (&part)[W]) {
   for (int w = 0; w < W; ++w) s += part[w];
   return s;
 }
+
+// A bound with `want` scores or more at or above it: of `units` waves that
+// each know their j-th largest lane maximum, r = three quarters reach the
+// r-th largest of these, which makes j r scores.  For a nucleus, whose size
+// is not known, j stops at half the lanes.
+struct Order {
+  int j, r;
+  __device__ Order(int units, int k, int nucleus) {
+    r = (3 * units + 3) / 4;
+    j = ((k ? k : nucleus) + r - 1) / r;
+    if (!k) j = min(j, 32);
+  }
+  __device__ bool fits() const { return j <= 40; }
+};
+// The r-th largest of the units' values (at most 64 units), in every wave.
+__device__ inline float unit_bound(const float* value, int units, int r) {
+  const int lane = threadIdx.x & 63;
+  return read_lane(sort_wave<true>(lane < units ? value[lane] : -INFINITY, true), r - 1);
+}
+// How many labels the list of a nucleus is made for: first a short one, and
+// a longer one where that holds too little.
+constexpr int kNucleus = 128, kNucleusLong = 320;
 
 // f(score, index) over the entries [begin, end) of a row in memory, by
 // `threads` lanes.
@@ -577,49 +604,23 @@ __device__ void descend(const T* row, int m, const Weights& wt, unsigned floor_k
   *above = sum;
 }
 
-// The cut by searches over the whole column, and the draw: for columns whose
-// short list does not do.
+// The draw within [begin, end) of a row: the labels above tau and the first
+// `ties` of the whole row at it, those with a weight of at least q.  The
+// stretch is narrowed to the one that holds the label, a wave's share at a
+// time.  total: of the whole row, with `base` before `begin`, and `many`
+// kept; or 0 where [begin, end) is the whole row, which gives them then.
 template <int THREADS, class T>
-__device__ void search_and_draw(const T* row, const Weights& wt, const Settings& c,
+__device__ void narrow_and_draw(const T* row, int begin, int end, u64 base, u64 total, u64 many,
+                                unsigned tau, u64 ties, const Weights& wt, const Settings& c,
                                 const SampleArgs& a, int64_t col, Shared<THREADS>& s) {
   constexpr int kWaves = THREADS / 64;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = a.m;
-  unsigned tau = 0;
-  u64 ties = 0;  // labels at tau that are kept
-  if (c.k) {
-    u64 above;
-    descend<false>(row, m, wt, 0, static_cast<u64>(c.k), s, &tau, &above);
-    ties = c.k - above;
-  }
-  if (c.p < 1.f) {
-    u64 mass = 0;
-    each_of(row, 0, m, threadIdx.x, THREADS, [&](float l, int) {
-      if (key_of(l) > tau) mass += wt.fixed(wt.of(l));
-    });
-    mass = wave_sum(mass);
-    __syncthreads();
-    if (lane == 0) s.sum[wave] = mass;
-    __syncthreads();
-    mass = total_of(s.sum);
-    if (ties) mass += ties * wt.fixed(wt.of(score_of(tau)));
-    const u64 target = top_p_target(c.p, mass);
-    unsigned cut;
-    u64 above;
-    descend<true>(row, m, wt, tau, target, s, &cut, &above);
-    const u64 w = wt.fixed(wt.of(score_of(cut)));
-    u64 need = w ? (target - above + w - 1) / w : 1;
-    if (cut == tau && ties && need > ties) need = ties;
-    tau = cut;
-    ties = need;
-  }
-
-  // The row is narrowed to the stretch that holds the label, a wave's share
-  // at a time; the first narrowing also gives the total.
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const float w_tau = ties ? wt.of(score_of(tau)) : 0.f;
   const u64 f_tau = w_tau >= c.q ? wt.fixed(w_tau) : 0;
-  int begin = 0, end = m;
-  u64 total = 0, target = 0, tie_base = 0, mass_base = 0, many = 0;
-  while (true) {
+  u64 target = total ? draw_target(a.u[col], total) : 0, tie_base = 0;
+  // Each step leaves a sixteenth (or 64 scores): the stretch is always down
+  // to 64 after eight steps, and the loop ends whatever the sums are.
+  for (int step = 0; step < 8; ++step) {
     const int part = ((end - begin + kWaves - 1) / kWaves + 63) / 64 * 64;
     const int b = begin + wave * part, e = b + part < end ? b + part : end;
     u64 n_tie = 0, mass = 0, count = 0;
@@ -655,14 +656,14 @@ __device__ void search_and_draw(const T* row, const Weights& wt, const Settings&
       const u64 left = ties > tie_base ? ties - tie_base : 0;
       const u64 t = s.sum[w] < left ? s.sum[w] : left;
       const u64 here = s.sum2[w] + t * f_tau;
-      if (mass_base + here > target) break;
-      mass_base += here;
+      if (base + here > target) break;
+      base += here;
       tie_base += s.sum[w];
       pick += part;
     }
     begin = pick;
     end = pick + part < end ? pick + part : end;
-    if (part == 64) break;
+    if (part <= 64) break;
   }
   if (wave == 0) {
     const bool in = begin + lane < end;
@@ -672,41 +673,80 @@ __device__ void search_and_draw(const T* row, const Weights& wt, const Settings&
     const bool tied = in && ties && key == tau;
     const u64 rank = wave_scan(tied ? u64(1) : u64(0)) + tie_base;
     const bool keep = in && w >= c.q && (key > tau || (tied && rank <= ties));
-    const u64 sum = wave_scan(keep ? wt.fixed(w) : 0) + mass_base;
+    const u64 sum = wave_scan(keep ? wt.fixed(w) : 0) + base;
     const u64 passed = __ballot(sum > target);
     if (passed && lane == __ffsll(passed) - 1)
       answer(a, col, begin + lane, share(w, wt.scale, total), static_cast<int64_t>(many));
   }
 }
 
-// A workgroup's column in registers: wave w holds the stretch of 64 V G
-// scores from w 64 V G on, lane t of it the values V t .. V t + V - 1 of each
-// of G groups.  R: registers' worth of values of a lane; R = 0 reads them
-// from memory each time.
+// The cut by searches over the whole column, and the draw: for columns whose
+// short list does not do.
+template <int THREADS, class T>
+__device__ void search_and_draw(const T* row, const Weights& wt, const Settings& c,
+                                const SampleArgs& a, int64_t col, Shared<THREADS>& s) {
+  unsigned tau = 0;
+  u64 ties = 0;  // labels at tau that are kept
+  if (c.k) {
+    u64 above;
+    descend<false>(row, a.m, wt, 0, static_cast<u64>(c.k), s, &tau, &above);
+    ties = c.k - above;
+  }
+  if (c.p < 1.f) {
+    u64 mass = 0;
+    each_of(row, 0, a.m, threadIdx.x, THREADS, [&](float l, int) {
+      if (key_of(l) > tau) mass += wt.fixed(wt.of(l));
+    });
+    mass = wave_sum(mass);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s.sum[threadIdx.x >> 6] = mass;
+    __syncthreads();
+    mass = total_of(s.sum);
+    if (ties) mass += ties * wt.fixed(wt.of(score_of(tau)));
+    const u64 target = top_p_target(c.p, mass);
+    unsigned cut;
+    u64 above;
+    descend<true>(row, a.m, wt, tau, target, s, &cut, &above);
+    const u64 w = wt.fixed(wt.of(score_of(cut)));
+    u64 need = w ? (target - above + w - 1) / w : 1;
+    if (cut == tau && ties && need > ties) need = ties;
+    tau = cut;
+    ties = need;
+  }
+  narrow_and_draw<THREADS>(row, 0, a.m, 0, 0, 0, tau, ties, wt, c, a, col, s);
+}
+
+// A stretch [begin, end) of a column, for the workgroup's waves: each has
+// the same number of groups of 64 V neighbouring scores, lane t the values
+// V t .. V t + V - 1 of each group.  R: a lane's scores that are kept in
+// registers; R = 0 reads them from memory each time, four groups at once.
 template <class T, int THREADS, int R>
 struct Column {
   static constexpr int V = sizeof(T) == 2 ? 8 : 4;
   static constexpr int kGroups = R / V;
   static constexpr bool kHalf = sizeof(T) == 2;
   const T* row;
-  int m, groups, from;  // from: of this lane's first value
+  int groups, from, end;  // from: this lane's first score; end: of the wave's
+  int length;
   unsigned raw[kGroups ? kGroups * (kHalf ? V / 2 : V) : 1];
 
-  __device__ Column(const T* r, int m_) : row(r), m(m_) {
-    groups = (m + THREADS * V - 1) / (THREADS * V);
+  __device__ Column(const T* r, int begin, int end_, int groups_)
+      : row(r), groups(groups_), length(end_ - begin) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    from = wave * groups * 64 * V + (threadIdx.x & 63) * V;
+    const int first = begin + wave * groups * 64 * V;
+    from = first + (threadIdx.x & 63) * V;
+    end = min(end_, first + groups * 64 * V);
     if constexpr (R > 0) {
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
         if (g >= groups) break;
         T v[V];
         const int at = from + g * 64 * V;
-        if (at + V <= m) {
+        if (at + V <= end) {
           __builtin_memcpy(v, row + at, sizeof(v));
         } else {
 #pragma unroll
-          for (int e = 0; e < V; ++e) v[e] = at + e < m ? row[at + e] : T(-INFINITY);
+          for (int e = 0; e < V; ++e) v[e] = at + e < end ? row[at + e] : T(-INFINITY);
         }
         if constexpr (kHalf) {
           __builtin_memcpy(&raw[g * V / 2], v, sizeof(v));
@@ -719,8 +759,7 @@ struct Column {
   }
   // Waves whose lanes all hold a score.
   __device__ int full_waves() const {
-    const int stretch = groups * 64 * V;
-    return min(THREADS / 64, (m - 64 * V) / stretch + 1);
+    return min(THREADS / 64, max(length - 64 * V, 0) / (groups * 64 * V) + 1);
   }
   __device__ void group(int g, float (&l)[V]) const {
     if constexpr (R > 0) {
@@ -736,7 +775,7 @@ struct Column {
         }
       }
     } else {
-      load_vec<V>(row, int64_t(from) + int64_t(g) * 64 * V, m, l, -INFINITY);
+      load_vec<V>(row, int64_t(from) + int64_t(g) * 64 * V, end, l, -INFINITY);
 #pragma unroll
       for (int e = 0; e < V; ++e) l[e] = score(l[e]);
     }
@@ -760,10 +799,15 @@ struct Column {
         }
       }
     } else {
-      for (int g = 0; g < groups; ++g) {
-        float l[V];
-        group(g, l);
-        if (!f(l, from + g * 64 * V)) break;
+      for (int g = 0; g < groups; g += 4) {
+        float l[4][V];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) group(g + b, l[b]);
+        bool go = true;
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          if (go) go = f(l[b], from + (g + b) * 64 * V);
+        if (!go) break;
       }
     }
   }
@@ -782,7 +826,7 @@ struct Column {
 template <int THREADS>
 __device__ inline u64 sort_block(u64 v, int P, u64* swap) {
   const int i = threadIdx.x;
-  v = sort_wave<true>(v, (i & 64) == 0 || P == 64);
+  if (i < P) v = sort_wave<true>(v, (i & 64) == 0 || P == 64);
   for (int size = 128; size <= P; size <<= 1) {
     const bool falling = (i & size) == 0 || size == P;
     for (int stride = size >> 1; stride >= 64; stride >>= 1) {
@@ -817,43 +861,91 @@ __device__ inline u64 block_scan(u64 v, u64 (&part)[THREADS / 64], u64* total) {
   return v + before;
 }
 
+// The cuts and the draw from a list of `count` (at most THREADS) entries,
+// thread i's in `entry`.  mass: of all labels, or 0 for that of the list
+// (after its top-k).  False, and nothing done, where the list holds less
+// than the nucleus.
+template <int THREADS>
+__device__ bool list_and_draw(u64 entry, int count, u64 mass, const Weights& wt,
+                              const Settings& c, const SampleArgs& a, int64_t col,
+                              Shared<THREADS>& s) {
+  constexpr int kWaves = THREADS / 64;
+  const int i = threadIdx.x, lane = i & 63, wave = i >> 6;
+  int P = 64;
+  while (P < count) P <<= 1;
+  entry = sort_block<THREADS>(entry, P, s.list.swap);
+  const float w = i < count ? wt.of(score_of(static_cast<unsigned>(entry >> 32))) : 0.f;
+  const u64 f = i < count ? wt.fixed(w) : 0;
+  const int first = c.k && c.k < count ? c.k : count;
+  u64 all;
+  const u64 incl = block_scan<THREADS>(i < first ? f : 0, s.sum, &all);
+  bool keep = i < first && w >= c.q && w > 0.f;
+  if (c.p < 1.f) {
+    const u64 target = top_p_target(c.p, mass ? mass : all);
+    if (all < target) return false;
+    keep = keep && incl - f < target;
+  }
+  // The kept labels are a prefix of the list; they are sorted again by index
+  // (its complement falls), each with its place in the list behind it.
+  const u64 votes = __ballot(keep);
+  const int own = ~votes ? __ffsll(~votes) - 1 : 64;
+  if (lane == 0) s.number[wave] = own;
+  s.list.swap[i] = entry;
+  __syncthreads();
+  int many = 0;
+  for (int v = 0; v < kWaves; ++v) {
+    many += s.number[v];
+    if (s.number[v] < 64) break;
+  }
+  int P2 = 64;
+  while (P2 < many) P2 <<= 1;
+  u64 by = i < many ? (static_cast<u64>(static_cast<unsigned>(entry)) << 32) | static_cast<unsigned>(i) : 0;
+  by = sort_block<THREADS>(by, P2, s.list.entry);
+  const float wk =
+      i < many ? wt.of(score_of(static_cast<unsigned>(s.list.swap[static_cast<unsigned>(by)] >> 32))) : 0.f;
+  const u64 fk = i < many ? wt.fixed(wk) : 0;
+  u64 total;
+  const u64 sum = block_scan<THREADS>(fk, s.sum2, &total);
+  const u64 target = draw_target(a.u[col], total);
+  if (sum > target && sum - fk <= target)
+    answer(a, col, index_of(by >> 32), share(wk, wt.scale, total), many);
+  return true;
+}
+
 template <class T, int THREADS, int R>
 __global__ __launch_bounds__(THREADS) void sample_block_kernel(const T* __restrict__ S,
                                                                SampleArgs a) {
   constexpr int kWaves = THREADS / 64;
+  constexpr int kEntries = Shared<THREADS>::kEntries;
   __shared__ Shared<THREADS> s;
   const int64_t col = blockIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const T* row = S + col * a.lds;
   typedef Column<T, THREADS, R> Col;
-  Col column(row, a.m);
+  Col column(row, 0, a.m, (a.m + THREADS * Col::V - 1) / (THREADS * Col::V));
   const Settings c(a, col);
 
   float most = -INFINITY;
   column.each([&](float l, int) { most = fmaxf(most, l); });
-  // Each wave's maximum, and its j-th largest lane maximum: at least j scores
-  // of each wave whose lanes all hold some reach the least of those.  For a
-  // top-k that is k of them; for a nucleus alone a hundred and more.
   const int full = column.full_waves();
-  const int j = c.k ? (c.k + full - 1) / full : min(128 / full, 32);
-  const bool list_does = c.cut && j <= 40;
+  const Order brief(full, c.k, kNucleus), longer(full, 0, kNucleusLong);
+  const bool list_does = c.cut && brief.fits();
+  const bool again = !c.k && THREADS >= kList && longer.j > brief.j;
   const float top = wave_max<true>(most);
-  float jth = -INFINITY;
-  if (list_does) jth = read_lane(sort_wave<true>(most, true), j - 1);
-  if (lane == 0) {
-    s.value[wave] = top;
-    s.value2[wave] = jth;
+  if (lane == 0) s.value[wave] = top;
+  if (list_does) {
+    const float sorted = sort_wave<true>(most, true);
+    const float x = read_lane(sorted, brief.j - 1), y = read_lane(sorted, again ? longer.j - 1 : 0);
+    if (lane == 0) {
+      s.value2[wave] = x;
+      s.value3[wave] = y;
+    }
   }
-  if (threadIdx.x == 0) s.count = 0;
   __syncthreads();
-  float bound = s.value2[0];
   Weights wt;
   wt.max = s.value[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) {
-    wt.max = fmaxf(wt.max, s.value[w]);
-    bound = w < full ? fminf(bound, s.value2[w]) : bound;
-  }
+  for (int w = 1; w < kWaves; ++w) wt.max = fmaxf(wt.max, s.value[w]);
   if (wt.max == -INFINITY) {
     if (threadIdx.x == 0) answer(a, col, -1, 0.f, 0);
     return;
@@ -931,83 +1023,241 @@ __global__ __launch_bounds__(THREADS) void sample_block_kernel(const T* __restri
   }
 
   const float floor_live = live_floor(wt.max, c.t);
-  const bool whole = bound <= floor_live;  // the list holds every label of nonzero weight
-  int count = THREADS + 1;
-  if (list_does) {
-    const float from = fmaxf(bound, floor_live);
-    column.each([&](float l, int i) {
-      const bool in = l >= from && l > -INFINITY;
-      const u64 mask = __ballot(in);
-      if (mask) {
-        int at = 0;
-        if (lane == 0) at = atomicAdd(&s.count, __popcll(mask));
-        at = __builtin_amdgcn_readfirstlane(at);
-        at = __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask >> 32),
-                                       __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask), at));
-        if (in && at < THREADS) s.list.entry[at] = entry_of(l, i);
-      }
-    });
-    u64 mass = 0;
+  u64 mass = 0;
+  for (int attempt = 0; list_does && attempt < (again ? 2 : 1); ++attempt) {
+    __syncthreads();
+    if (threadIdx.x == 0) s.count = 0;
+    const float bound = attempt ? unit_bound(s.value3, full, longer.r)
+                                : unit_bound(s.value2, full, brief.r);
+    // Whether the list holds every label of nonzero weight.
+    const bool whole = bound <= floor_live;
     const bool sum_all = c.p < 1.f && !c.k && !whole;
-    if (sum_all) {
-      column.each([&](float l, int) { mass += wt.fixed(wt.of(l)); });
+    const float from = whole ? floor_live : bound;
+    __syncthreads();
+    const auto push = [&](float l, int i) {
+      if (l >= from && l > -INFINITY) {
+        const int at = atomicAdd(&s.count, 1);
+        if (at < kEntries) s.list.entry[at] = entry_of(l, i);
+      }
+    };
+    if (sum_all && mass == 0) {
+      column.each([&](float l, int i) {
+        mass += wt.fixed(wt.of(l));
+        push(l, i);
+      });
       mass = wave_sum(mass);
       if (lane == 0) s.sum3[wave] = mass;
+    } else {
+      column.each(push);
     }
     __syncthreads();
-    count = s.count;
     if (sum_all) mass = total_of(s.sum3);
-    if (count <= THREADS) {
-      int P = 64;
-      while (P < count) P <<= 1;
-      const int i = threadIdx.x;
-      const u64 entry = sort_block<THREADS>(i < count ? s.list.entry[i] : 0, P, s.list.swap);
-      const float w = i < count ? wt.of(score_of(static_cast<unsigned>(entry >> 32))) : 0.f;
-      const u64 f = i < count ? wt.fixed(w) : 0;
-      const int first = c.k && c.k < count ? c.k : count;
-      u64 all;
-      const u64 incl = block_scan<THREADS>(i < first ? f : 0, s.sum, &all);
-      bool keep = i < first && w >= c.q && w > 0.f, found = true;
-      if (c.p < 1.f) {
-        if (!sum_all) mass = all;
-        const u64 target = top_p_target(c.p, mass);
-        keep = keep && incl - f < target;
-        found = all >= target;
-      }
-      if (found) {
-        // The kept labels, a prefix of the list, by rising index: the
-        // complement of the index falls, with the weight's place behind it.
-        const u64 votes = __ballot(keep);
-        const int own = ~votes ? __ffsll(~votes) - 1 : 64;
-        if (lane == 0) s.number[wave] = own;
-        __syncthreads();
-        int many = 0;
-        for (int w2 = 0; w2 < kWaves; ++w2) {
-          many += s.number[w2];
-          if (s.number[w2] < 64) break;
-        }
-        s.list.swap[i] = entry;
-        __syncthreads();
-        int P2 = 64;
-        while (P2 < many) P2 <<= 1;
-        // index in the high half, rank in the low
-        u64 by = i < many ? (static_cast<u64>(static_cast<unsigned>(entry)) << 32) | static_cast<unsigned>(i) : 0;
-        by = sort_block<THREADS>(by, P2, s.list.entry);
-        float wk = 0.f;
-        if (i < many) wk = wt.of(score_of(static_cast<unsigned>(s.list.swap[static_cast<unsigned>(by)] >> 32)));
-        u64 total;
-        const u64 sum = block_scan<THREADS>(i < many ? wt.fixed(wk) : 0, s.sum2, &total);
-        const u64 target = draw_target(a.u[col], total);
-        const u64 own_f = i < many ? wt.fixed(wk) : 0;
-        if (sum > target && sum - own_f <= target && own_f)
-          answer(a, col, static_cast<int64_t>(0xffffffffu - static_cast<unsigned>(by >> 32)),
-                 share(wk, wt.scale, total), many);
-        return;
-      }
-    }
+    const int count = s.count;
+    if (count > kEntries) break;
+    const u64 entry = static_cast<int>(threadIdx.x) < count ? s.list.entry[threadIdx.x] : 0;
+    if (list_and_draw<THREADS>(entry, count, sum_all ? mass : 0, wt, c, a, col, s)) return;
   }
   __syncthreads();
   search_and_draw<THREADS>(row, wt, c, a, col, s);
+}
+
+// ---------------------------------------------------------------------------
+// A column to several workgroups: with few columns one workgroup each leaves
+// most of the device idle.  Three kernels: the parts' maxima and order
+// statistics; then, with the column's maximum known, their sums and entries
+// of the list; then the draw.
+// ---------------------------------------------------------------------------
+constexpr int kPartThreads = 256, kPartWaves = kPartThreads / 64;
+constexpr int kMaxParts = 64 / kPartWaves;  // unit_bound takes 64 waves
+constexpr int kPartStep = 2048;             // parts are multiples of it: whole groups of any type
+
+struct PartsOf {  // one column's
+  u64 mass[kMaxParts];
+  float top[kMaxParts], jth[kMaxParts * kPartWaves];
+  int count[kMaxParts], first[kMaxParts];
+  int listed, unused;
+  u64 entry[kList];
+};
+
+struct PartArgs {
+  PartsOf* of;
+  int parts, part;  // how many, and the scores of each but the last
+};
+
+template <class T>
+__device__ inline Column<T, kPartThreads, 0> part_column(const T* row, int m, const PartArgs& p) {
+  typedef Column<T, kPartThreads, 0> Col;
+  const int begin = blockIdx.x * p.part;
+  return Col(row, begin, min(m, begin + p.part), p.part / (kPartThreads * Col::V));
+}
+// Waves of all parts whose lanes all hold a score.
+template <int V>
+__device__ inline int full_units(int m, const PartArgs& p) {
+  return min(p.parts * kPartWaves, max(m - 64 * V, 0) / (p.part / kPartWaves) + 1);
+}
+
+template <class T>
+__global__ __launch_bounds__(kPartThreads) void sample_parts_kernel(const T* __restrict__ S,
+                                                                    SampleArgs a, PartArgs p) {
+  __shared__ float tops[kPartWaves];
+  const int64_t col = blockIdx.y;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  PartsOf& of = p.of[col];
+  auto column = part_column(S + col * a.lds, a.m, p);
+  const Settings c(a, col);
+  float most = -INFINITY;
+  column.each([&](float l, int) { most = fmaxf(most, l); });
+  const float top = wave_max<true>(most);
+  if (lane == 0) tops[wave] = top;
+  const Order order(full_units<decltype(column)::V>(a.m, p), c.k, kNucleusLong);
+  if (c.cut && order.fits()) {
+    const float x = read_lane(sort_wave<true>(most, true), order.j - 1);
+    if (lane == 0) of.jth[blockIdx.x * kPartWaves + wave] = x;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float t = tops[0];
+    for (int w = 1; w < kPartWaves; ++w) t = fmaxf(t, tops[w]);
+    of.top[blockIdx.x] = t;
+    if (blockIdx.x == 0) of.listed = 0;
+  }
+}
+
+// What the second and third kernel know of a column.
+struct PartsKnown {
+  float max, bound, floor_live;
+  bool list_does, whole, sum_all;
+  __device__ PartsKnown(const PartsOf& of, const PartArgs& p, const Settings& c, int units) {
+    const int lane = threadIdx.x & 63;
+    max = wave_max<true>(lane < p.parts ? of.top[lane] : -INFINITY);
+    const Order order(units, c.k, kNucleusLong);
+    list_does = c.cut && !c.greedy && order.fits();
+    floor_live = live_floor(max, c.t);
+    bound = list_does ? unit_bound(of.jth, units, order.r) : 0.f;
+    whole = list_does && bound <= floor_live;
+    sum_all = list_does && c.p < 1.f && !c.k && !whole;
+  }
+};
+
+template <class T>
+__global__ __launch_bounds__(kPartThreads) void sample_lists_kernel(const T* __restrict__ S,
+                                                                    SampleArgs a, PartArgs p) {
+  __shared__ u64 sums[kPartWaves], entries[kList];
+  __shared__ int numbers[kPartWaves], counted, placed;
+  const int64_t col = blockIdx.y;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  PartsOf& of = p.of[col];
+  const Settings c(a, col);
+  auto column = part_column(S + col * a.lds, a.m, p);
+  const PartsKnown known(of, p, c, full_units<decltype(column)::V>(a.m, p));
+  if (known.max == -INFINITY || (c.cut && !known.list_does && !c.greedy)) return;
+  Weights wt;
+  wt.max = known.max;
+  wt.inv_t = 1.f / c.t;
+  wt.scale = a.scale;
+  if (threadIdx.x == 0) counted = 0;
+  __syncthreads();
+
+  const bool mine = of.top[blockIdx.x] == known.max;  // the column's maximum is in this part
+  u64 mass = 0;
+  int number = c.greedy ? a.m : 0;
+  const float from = known.whole ? known.floor_live : known.bound;
+  const auto push = [&](float l, int i) {
+    if (l >= from && l > -INFINITY) {
+      const int at = atomicAdd(&counted, 1);
+      if (at < kList) entries[at] = entry_of(l, i);
+    }
+  };
+  if (c.greedy) {
+    if (mine) column.each([&](float l, int i) { number = l == wt.max && i < number ? i : number; });
+#pragma unroll
+    for (int d = 32; d; d >>= 1) number = min(number, __shfl_xor(number, d));
+  } else if (!c.cut) {
+    column.each([&](float l, int) {
+      const float w = wt.of(l);
+      const bool in = w >= c.q && w > 0.f;
+      mass += in ? wt.fixed(w) : 0;
+      number += in;
+    });
+    number = wave_sum(number);
+  } else if (known.sum_all) {
+    column.each([&](float l, int i) {
+      mass += wt.fixed(wt.of(l));
+      push(l, i);
+    });
+  } else {
+    column.each(push);
+  }
+  mass = wave_sum(mass);
+  if (lane == 0) {
+    sums[wave] = mass;
+    numbers[wave] = number;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int n = numbers[0];
+    for (int w = 1; w < kPartWaves; ++w) n = c.greedy ? min(n, numbers[w]) : n + numbers[w];
+    of.mass[blockIdx.x] = total_of(sums);
+    (c.greedy ? of.first : of.count)[blockIdx.x] = n;
+    // The order of the parts' entries in the list does not matter: it is
+    // sorted.
+    placed = counted ? atomicAdd(&of.listed, counted) : 0;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < counted && i < kList; i += kPartThreads)
+    if (placed + i < kList) of.entry[placed + i] = entries[i];
+}
+
+template <class T>
+__global__ __launch_bounds__(kList) void sample_draw_kernel(const T* __restrict__ S, SampleArgs a,
+                                                            PartArgs p) {
+  __shared__ Shared<kList> s;
+  const int64_t col = blockIdx.x;
+  const T* row = S + col * a.lds;
+  const PartsOf& of = p.of[col];
+  const Settings c(a, col);
+  const PartsKnown known(of, p, c, full_units<Column<T, kPartThreads, 0>::V>(a.m, p));
+  if (known.max == -INFINITY) {
+    if (threadIdx.x == 0) answer(a, col, -1, 0.f, 0);
+    return;
+  }
+  if (c.greedy) {
+    if (threadIdx.x == 0) {
+      int best = a.m;
+      for (int i = 0; i < p.parts; ++i) best = min(best, of.first[i]);
+      answer(a, col, best, 1.f, 1);
+    }
+    return;
+  }
+  Weights wt;
+  wt.max = known.max;
+  wt.inv_t = 1.f / c.t;
+  wt.scale = a.scale;
+  if (!c.cut) {
+    u64 total = 0, base = 0;
+    int many = 0;
+    for (int i = 0; i < p.parts; ++i) {
+      total += of.mass[i];
+      many += of.count[i];
+    }
+    const u64 target = draw_target(a.u[col], total);
+    int i = 0;
+    for (; i < p.parts - 1 && base + of.mass[i] <= target; ++i) base += of.mass[i];
+    const int begin = i * p.part;
+    narrow_and_draw<kList>(row, begin, min(a.m, begin + p.part), base, total,
+                           static_cast<u64>(many), 0u, 0, wt, c, a, col, s);
+    return;
+  }
+  if (known.list_does && of.listed <= kList) {
+    u64 mass = 0;
+    if (known.sum_all)
+      for (int i = 0; i < p.parts; ++i) mass += of.mass[i];
+    const int count = of.listed;
+    const u64 entry = static_cast<int>(threadIdx.x) < count ? of.entry[threadIdx.x] : 0;
+    if (list_and_draw<kList>(entry, count, mass, wt, c, a, col, s)) return;
+  }
+  __syncthreads();
+  search_and_draw<kList>(row, wt, c, a, col, s);
 }
 
 template <class T, int THREADS, int R>
@@ -1020,6 +1270,25 @@ void start_wave(const SampleLaunch& l, const SampleArgs& a) {
   sample_wave_kernel<T, E><<<static_cast<unsigned>((l.n + 3) / 4), 256, 0, l.stream>>>(
       static_cast<const T*>(l.S), a);
 }
+
+template <class T>
+void start_parts(const SampleLaunch& l, const SampleArgs& a) {
+  PartArgs p;
+  p.of = static_cast<PartsOf*>(l.work);
+  p.part = (a.m / kMaxParts + kPartStep) / kPartStep * kPartStep;
+  p.parts = (a.m + p.part - 1) / p.part;
+  const T* S = static_cast<const T*>(l.S);
+  const dim3 grid(static_cast<unsigned>(p.parts), static_cast<unsigned>(l.n));
+  sample_parts_kernel<T><<<grid, kPartThreads, 0, l.stream>>>(S, a, p);
+  sample_lists_kernel<T><<<grid, kPartThreads, 0, l.stream>>>(S, a, p);
+  sample_draw_kernel<T><<<static_cast<unsigned>(l.n), kList, 0, l.stream>>>(S, a, p);
+}
+
+// Columns above 16384 scores go to several workgroups each where one apiece
+// leaves compute units idle.  Measured, one workgroup against several: top-k
+// of 32000 floats 22 against 16 us for one column, 26 against 19 for 64, 33
+// against 34 for 256; of 128000 25 against 18, 35 against 25, 51 against 56.
+bool in_parts(int64_t m, int64_t n) { return m > 16384 && n <= (m > 65536 ? 256 : 64); }
 
 template <class T>
 hipError_t sample(const SampleLaunch& l) {
@@ -1038,21 +1307,24 @@ hipError_t sample(const SampleLaunch& l) {
   int bits = 0;
   while ((int64_t(1) << bits) < l.m) ++bits;
   a.scale = static_cast<double>(u64(1) << (62 - bits < 46 ? 62 - bits : 46));
-  // By the column's length: a wave up to 1024 scores, a workgroup that holds
-  // the column in registers above, and one that reads it again and again
-  // where the registers do not hold it.
-  if (l.m <= 256) start_wave<T, 4>(l, a);
+  // Else by the column's length: a wave up to 1024 scores, a workgroup that
+  // holds the column in registers above, and one that reads it twice where
+  // the registers do not hold it.
+  if (in_parts(l.m, l.n)) start_parts<T>(l, a);
+  else if (l.m <= 256) start_wave<T, 4>(l, a);
   else if (l.m <= 1024) start_wave<T, 16>(l, a);
   else if (l.m <= 256 * 16) start_block<T, 256, 16>(l, a);
   else if (l.m <= 1024 * 16) start_block<T, 1024, 16>(l, a);
   else if (l.m <= 1024 * 32) start_block<T, 1024, 32>(l, a);
-  else if (l.m <= 1024 * 64) start_block<T, 1024, 64>(l, a);
-  else if (sizeof(T) == 2 && l.m <= 1024 * 128) start_block<T, 1024, sizeof(T) == 2 ? 128 : 64>(l, a);
   else start_block<T, 1024, 0>(l, a);
   return hipGetLastError();
 }
 
 }  // namespace
+
+size_t sample_work_bytes(int64_t m, int64_t n) {
+  return in_parts(m, n) ? static_cast<size_t>(n) * sizeof(PartsOf) : 0;
+}
 
 hipError_t launch_sample(const SampleLaunch& a) {
   switch (a.data) {
