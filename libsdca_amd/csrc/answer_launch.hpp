@@ -34,9 +34,12 @@ constexpr int64_t kI8TileK = 128;
 
 // S_ij = (sum_k X_ik W_jk) sx_i sw_j.
 struct ScoresI8Launch {
-  int out;  // SDCA_F32, F16, BF16
+  int data;  // X's type: SDCA_I8, or where scores_i8_few holds any of the quantiser's
+  int out;   // SDCA_F32, F16, BF16
   int64_t d, m, n;
-  const int8_t* X;  // n rows, pitch ldx, zeros from d up to a multiple of kI8TileK
+  // n rows, pitch ldx.  Int8 rows have zeros from d up to a multiple of
+  // kI8TileK and 16-byte addresses, but for scores_i8_few.
+  const void* X;
   int64_t ldx;
   const float* sx;
   const int8_t* W;  // m rows, pitch ldw
@@ -46,6 +49,8 @@ struct ScoresI8Launch {
   int64_t lds;
   hipStream_t stream;
 };
+// Whether X is taken as the caller has it, quantised on the way.
+bool scores_i8_few(int64_t n, int64_t d);
 hipError_t launch_scores_i8(const ScoresI8Launch& a);
 
 // One setting of the draw: a value for all columns, or one per column.

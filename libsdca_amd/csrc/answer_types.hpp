@@ -35,6 +35,38 @@ __device__ inline void load_vec(const T* row, int64_t at, int64_t len, float (&v
   }
 }
 
+// |x| as an integer: the order of the bit patterns is that of the values,
+// with infinity and the NaNs on top, so one integer maximum finds both the
+// largest magnitude and a non-finite value.
+__device__ inline unsigned magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// The scale of a column of that largest magnitude: max |x| (1 / 127).  A
+// column of zeros (or of values whose scale is no 32-bit number above zero)
+// gets 0 and zeros; one that holds an infinity or a NaN gets NaN and zeros,
+// so that every product with it is NaN.
+struct ColumnScale {
+  float scale;
+  bool some;  // whether any value is not quantised to zero
+  __device__ explicit ColumnScale(unsigned most) {
+    const bool finite = most < 0x7f800000u;
+    scale = finite ? __uint_as_float(most) * (1.f / 127.f) : __uint_as_float(0x7fc00000u);
+    some = finite && scale > 0.f;
+  }
+};
+
+// Eight values x / scale to the nearest integers, as bytes.  The quotient is
+// rounded to 32 bits first, halves go to even.  The clamp matters only where
+// the scale is so small that it has lost digits itself.
+__device__ inline void quantize8(const float (&v)[8], const ColumnScale& s, unsigned (&w)[2]) {
+  w[0] = w[1] = 0;
+  if (!s.some) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float q = rintf(v[e] / s.scale);
+    w[e / 4] |= (static_cast<int>(fminf(fmaxf(q, -127.f), 127.f)) & 0xffu) << (8 * (e % 4));
+  }
+}
+
 // Rounds to the output's type, to nearest, halves to even.
 template <class T> __device__ inline T from_float(float x);
 template <> __device__ inline float from_float<float>(float x) { return x; }

@@ -1293,28 +1293,28 @@ int scores_i8_common(int data, int out, int64_t d, int64_t m, int64_t n, const v
   a.n = n;
   a.lds = lds;
   a.stream = stream;
-  const void* x;
-  if ((rc = staged(X, span(d, n, ldx, element_size(data)), host, dx, stream, &x)) ||
+  if ((rc = staged(X, span(d, n, ldx, element_size(data)), host, dx, stream, &a.X)) ||
       (rc = staged(sx, n * sizeof(float), host, dsx, stream, &a.sx)) ||
       (rc = staged(W, span(d, m, ldw, 1), host, dw, stream, &a.W)) ||
       (rc = staged(sw, m * sizeof(float), host, dsw, stream, &a.sw)) ||
       (rc = staged_out(S, span(m, n, lds, element_size(out)), host, dS, &a.S)))
     return rc;
-  a.X = static_cast<const int8_t*>(x);
+  a.data = data;
   a.ldx = ldx;
   a.ldw = ldw;
 
-  // X is read in place when its columns are whole tiles at aligned
-  // addresses, W when its columns are aligned; the kernels' offsets within a
-  // tile of columns are 32-bit.  What is not goes to scratch first.
-  const auto in_place = [](const int8_t* p, int64_t ld) {
+  // W is read in place when its columns are aligned, and X when its columns
+  // are whole tiles besides, or few; the kernels' offsets within a tile of
+  // columns are 32-bit.  What is not goes to scratch first.
+  const auto in_place = [](const void* p, int64_t ld) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0 && ld <= (1 << 22);
   };
   const int64_t pad = (d + kI8TileK - 1) / kI8TileK * kI8TileK;
-  const bool own_x = data != SDCA_I8 || d != pad || !in_place(a.X, ldx);
+  const bool few = scores_i8_few(n, d);
+  const bool own_x = !few && (data != SDCA_I8 || d != pad || !in_place(a.X, ldx));
   const bool own_w = !in_place(a.W, ldw);
   const size_t x_bytes = own_x ? static_cast<size_t>(n) * pad : 0;
-  const size_t s_bytes = data != SDCA_I8 ? (n * sizeof(float) + 255) / 256 * 256 : 0;
+  const size_t s_bytes = own_x && data != SDCA_I8 ? (n * sizeof(float) + 255) / 256 * 256 : 0;
   const size_t w_bytes = own_w ? static_cast<size_t>(m) * pad : 0;
   if (x_bytes + s_bytes + w_bytes) {
     void* ws = nullptr;
@@ -1322,12 +1322,12 @@ int scores_i8_common(int data, int out, int64_t d, int64_t m, int64_t n, const v
     int8_t* wx = static_cast<int8_t*>(ws);
     float* wsx = reinterpret_cast<float*>(wx + x_bytes + w_bytes);
     int8_t* ww = wx + x_bytes;
-    if (data != SDCA_I8) {
+    if (own_x && data != SDCA_I8) {
       QuantLaunch q;
       q.data = data;
       q.d = d;
       q.n = n;
-      q.X = x;
+      q.X = a.X;
       q.ldx = ldx;
       q.Q = wx;
       q.ldq = q.pad = pad;
@@ -1336,11 +1336,12 @@ int scores_i8_common(int data, int out, int64_t d, int64_t m, int64_t n, const v
       SDCA_HIP_TRY(launch_quantize(q), "quantise kernel");
       a.sx = wsx;
     } else if (own_x) {
-      SDCA_HIP_TRY(launch_repack_i8(a.X, ldx, d, n, wx, pad, pad, stream), "repack kernel");
+      SDCA_HIP_TRY(launch_repack_i8(static_cast<const int8_t*>(a.X), ldx, d, n, wx, pad, pad, stream), "repack kernel");
     }
     if (own_x) {
       a.X = wx;
       a.ldx = pad;
+      a.data = SDCA_I8;
     }
     if (own_w) {
       SDCA_HIP_TRY(launch_repack_i8(a.W, ldw, d, m, ww, pad, pad, stream), "repack kernel");

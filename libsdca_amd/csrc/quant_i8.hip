@@ -10,24 +10,6 @@ namespace {
 
 constexpr int kVec = 8;  // values a lane takes at a time: 16 bytes of a 16-bit type, 8 of q
 
-// |x| as an integer: the order of the bit patterns is that of the values,
-// with infinity and the NaNs on top, so one integer maximum finds both the
-// largest magnitude and a non-finite value.
-__device__ inline unsigned magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-
-__device__ inline int quantized(float x, float s) {
-  // The quotient is rounded to 32 bits, then to the nearest integer, halves
-  // to even.  The clamp matters only where the scale is so small that it
-  // has lost digits itself.
-  const float q = rintf(x / s);
-  return static_cast<int>(fminf(fmaxf(q, -127.f), 127.f));
-}
-
-// s = max |x| (1 / 127), q = x / s to the nearest integer.  A column of zeros
-// (or of values whose scale is no 32-bit number above zero) gets s = 0 and
-// zeros; one that holds an infinity or a NaN gets s = NaN and zeros, so that
-// every product with it is NaN.
-//
 // TPC threads share a column and keep it in registers (G vectors of 8 values
 // each), so that it is read once; LOOP: a longer column is read twice.
 template <class T, int TPC, int G, bool LOOP>
@@ -68,10 +50,8 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ X, 
 #pragma unroll
     for (int w = 0; w < 4; ++w) most = part[w] > most ? part[w] : most;
   }
-  const bool finite = most < 0x7f800000u;
-  const float s = __uint_as_float(most) * (1.f / 127.f);
-  const bool some = finite && s > 0.f;
-  if (t == 0) scales[col] = finite ? s : __uint_as_float(0x7fc00000u);
+  const ColumnScale s(most);
+  if (t == 0) scales[col] = s.scale;
 
   for (int64_t sweep = 0; sweep < sweeps; ++sweep) {
 #pragma unroll
@@ -79,12 +59,8 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ X, 
       const int64_t at = (sweep * G + g) * TPC * kVec + int64_t(t) * kVec;
       if (LOOP) load_vec<kVec>(x, at, d, v[g]);
       if (at >= pad) continue;
-      unsigned w[2] = {0, 0};
-      if (some) {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e)
-          w[e / 4] |= (quantized(v[g][e], s) & 0xffu) << (8 * (e % 4));
-      }
+      unsigned w[2];
+      quantize8(v[g], s, w);
       if (at + kVec <= pad) {
         __builtin_memcpy(q + at, w, kVec);
       } else {

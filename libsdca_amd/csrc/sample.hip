@@ -785,10 +785,12 @@ struct Column {
   template <class F>
   __device__ void groups_until(F f) {
     if constexpr (R > 0) {
-      // Each pass makes its own floats of the registers: kept from one pass
-      // to the next they would need twice the registers, and spill.
+      // Each pass makes its own floats of the registers, and one group's work
+      // ends before the next one's begins: floats kept from one pass to the
+      // next, or indices, or many groups' exponentials in flight, spill.
 #pragma unroll
       for (unsigned& r : raw) asm volatile("" : "+v"(r));
+      asm volatile("" : "+v"(from));
       bool go = true;
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
@@ -797,6 +799,7 @@ struct Column {
           group(g, l);
           go = f(l, from + g * 64 * V);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     } else {
       for (int g = 0; g < groups; g += 4) {
@@ -805,8 +808,10 @@ struct Column {
         for (int b = 0; b < 4; ++b) group(g + b, l[b]);
         bool go = true;
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+        for (int b = 0; b < 4; ++b) {
           if (go) go = f(l[b], from + (g + b) * 64 * V);
+          __builtin_amdgcn_sched_barrier(0);
+        }
         if (!go) break;
       }
     }
@@ -1034,21 +1039,17 @@ __global__ __launch_bounds__(THREADS) void sample_block_kernel(const T* __restri
     const bool sum_all = c.p < 1.f && !c.k && !whole;
     const float from = whole ? floor_live : bound;
     __syncthreads();
-    const auto push = [&](float l, int i) {
+    const bool sum_now = sum_all && mass == 0;
+    column.each([&](float l, int i) {
+      if (sum_now) mass += wt.fixed(wt.of(l));
       if (l >= from && l > -INFINITY) {
         const int at = atomicAdd(&s.count, 1);
         if (at < kEntries) s.list.entry[at] = entry_of(l, i);
       }
-    };
-    if (sum_all && mass == 0) {
-      column.each([&](float l, int i) {
-        mass += wt.fixed(wt.of(l));
-        push(l, i);
-      });
+    });
+    if (sum_now) {
       mass = wave_sum(mass);
       if (lane == 0) s.sum3[wave] = mass;
-    } else {
-      column.each(push);
     }
     __syncthreads();
     if (sum_all) mass = total_of(s.sum3);

@@ -4,8 +4,11 @@
 // do not hang on the order of the terms; each score is rounded three times
 // in 32 bits (the sum, and the two scales' products) and once to the
 // output's type.
+#include <type_traits>
+
 #include "answer_launch.hpp"
 #include "answer_types.hpp"
+#include "common.hpp"
 
 namespace sdca_gpu {
 namespace {
@@ -13,6 +16,9 @@ namespace {
 typedef int v4i __attribute__((ext_vector_type(4)));
 
 constexpr int kTileK = static_cast<int>(kI8TileK);
+
+// An offset beyond any buffer (offsets in a buffer stay below 2^30 + 2^18).
+constexpr int kOutside = 0x7fffffff;
 
 // An operand's rows from `row` on as a buffer: loads beyond its last byte
 // give zeros.
@@ -34,109 +40,337 @@ __device__ inline void load_to_lds(__amdgpu_buffer_rsrc_t from, int8_t* dst, int
 #endif
 }
 
+// Blocks go round the eight XCDs in turn, and each XCD has its own L2: block
+// `id` takes a tile from its XCD's own eighth of the tiles, which run
+// through groups of eight rows of tiles, so that the tiles an XCD works on
+// together share their operands' rows.
+struct TileAt {
+  int n, m;
+};
+__device__ inline TileAt tile_of(int id, int tiles_n, int tiles_m) {
+  const int total = tiles_n * tiles_m, xcd = id & 7, per = total >> 3, more = total & 7;
+  const int at = xcd * per + min(xcd, more) + (id >> 3);
+  constexpr int kGroup = 8;
+  const int group = at / (kGroup * tiles_m);
+  const int high = min(kGroup, tiles_n - group * kGroup);
+  const int in = at - group * kGroup * tiles_m;
+  return {group * kGroup + in % high, in / high};
+}
+
 // A workgroup computes BN examples by BM classes; its WN x WM waves each a
 // (BN / WN) x (BM / WM) part in 16 x 16 x 64 matrix instructions.  Classes
-// are the instruction's rows and examples its columns, so a lane's four
-// results are neighbouring scores of one example.
+// are the instruction's rows and examples its columns; an instruction's rows
+// are classes 4 FM apart in fours, so that a lane ends with 4 FM neighbouring
+// scores of an example and stores them whole.
 //
-// K goes by in tiles of 128 bytes, two of them in LDS: while one is
-// multiplied, the other arrives by loads that write LDS directly.  A tile
-// row holds its eight 16-byte pieces in the order piece ^ (row % 8): the 16
-// rows that an instruction reads at one place then lie in different banks.
-template <class Out, int BN, int BM, int WN, int WM>
+// K goes by in tiles of 128 bytes, STAGES of them in LDS.  A tile row holds its
+// eight 16-byte pieces in the order piece ^ f(row): the rows that an
+// instruction reads at one place then lie in different banks.  Loads write
+// LDS directly, in the order of the lanes, so the lanes' addresses carry the
+// permutation.  While a half tile (64 bytes) is multiplied from registers,
+// the next half is read from LDS; between the halves of tile t is the one
+// barrier: behind it tile t + 1 has arrived, tile t is in registers, and the
+// loads of tile t + STAGES take its place.
+template <class Out, int BN, int BM, int WN, int WM, int STAGES>
 __global__ __launch_bounds__(64 * WN * WM) void scores_i8_kernel(
     const int8_t* __restrict__ X, int64_t ldx, const float* __restrict__ sx,
     const int8_t* __restrict__ W, int64_t ldw, const float* __restrict__ sw,
-    Out* __restrict__ S, int64_t lds, int d, int m, int n) {
+    Out* __restrict__ S, int64_t lds, int d, int m, int n, int tiles_n, int tiles_m) {
   constexpr int kWaves = WN * WM;
-  constexpr int kRows = BN + BM;                // tile rows, the examples' first
-  constexpr int kLoads = kRows / 8 / kWaves;    // of a wave: 8 rows each
+  constexpr int kRows = BN + BM;              // tile rows, the examples' first
+  constexpr int kLoads = kRows / 8 / kWaves;  // of a wave: 8 rows each
   constexpr int FN = BN / WN / 16, FM = BM / WM / 16;
   static_assert(kRows % (8 * kWaves) == 0 && BN % 8 == 0, "tile rows per wave");
-  __shared__ __align__(128) int8_t tile[2][kRows * kTileK];
+  __shared__ __align__(128) int8_t tile[STAGES][kRows * kTileK];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wn = wave % WN, wm = wave / WN;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.y) * BN;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.x) * BM;
+  const TileAt place = tile_of(blockIdx.x, tiles_n, tiles_m);
+  const int64_t n0 = static_cast<int64_t>(place.n) * BN;
+  const int64_t m0 = static_cast<int64_t>(place.m) * BM;
   const __amdgpu_buffer_rsrc_t xb = rows_buffer(X, ldx, n0, n, d);
   const __amdgpu_buffer_rsrc_t wb = rows_buffer(W, ldw, m0, m, d);
 
+  const auto order = [](int row) {
+    return row < BN ? row & 7 : (row & 3) | (((row - BN) / (4 * FM) & 1) << 2);
+  };
   int from[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
     const int row = (wave * kLoads + i) * 8 + lane / 8;
-    const int piece = (lane & 7) ^ (row & 7);
+    const int piece = (lane & 7) ^ order(row);
     from[i] = (row < BN ? row * static_cast<int>(ldx) : (row - BN) * static_cast<int>(ldw)) +
               piece * 16;
   }
-  auto fetch = [&](int k, int stage) {
+  const auto fetch = [&](int k, int stage) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int row = (wave * kLoads + i) * 8;
       load_to_lds(row < BN ? xb : wb, &tile[stage][row * kTileK], from[i] + k);
     }
   };
+  // The lane's first pieces in a tile; its other rows lie at fixed distances
+  // (they have the same f), and those of the second half tile at ^ 64.
+  const int row_a = BN + wm * (16 * FM) + ((lane & 15) >> 2) * (4 * FM) + (lane & 3);
+  const int row_b = wn * (16 * FN) + (lane & 15);
+  const int at_a = row_a * kTileK + ((lane / 16) ^ order(row_a)) * 16;
+  const int at_b = row_b * kTileK + ((lane / 16) ^ order(row_b)) * 16;
 
   v4i acc[FM][FN] = {};
-  const int tiles = (d + kTileK - 1) / kTileK;
-  fetch(0, 0);
-  for (int t = 0; t < tiles; ++t) {
-    __syncthreads();  // tile t has arrived, and tile t - 1 is no longer read
-    if (t + 1 < tiles) fetch((t + 1) * kTileK, (t + 1) & 1);
-    const int8_t* base = tile[t & 1];
+  v4i a[2][FM], b[2][FN];
+  const auto read = [&](int stage, int h) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int piece = k * 4 + lane / 16;
-      v4i a[FM], b[FN];
+    for (int i = 0; i < FM; ++i)
+      a[h][i] = *reinterpret_cast<const v4i*>(&tile[stage][(at_a ^ (h * 64)) + i * 4 * kTileK]);
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        const int row = BN + (wm * FM + i) * 16 + (lane & 15);
-        a[i] = *reinterpret_cast<const v4i*>(base + row * kTileK + ((piece ^ (row & 7)) * 16));
-      }
+    for (int j = 0; j < FN; ++j)
+      b[h][j] = *reinterpret_cast<const v4i*>(&tile[stage][(at_b ^ (h * 64)) + j * 16 * kTileK]);
+  };
+  const auto multiply = [&](int h) {
 #pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        const int row = (wn * FN + j) * 16 + (lane & 15);
-        b[j] = *reinterpret_cast<const v4i*>(base + row * kTileK + ((piece ^ (row & 7)) * 16));
-      }
+    for (int j = 0; j < FN; ++j)
 #pragma unroll
       for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i], b[j], acc[i][j], 0, 0, 0);
-    }
-  }
+        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[h][i], b[h][j], acc[i][j], 0, 0, 0);
+  };
 
+  // The wave's reads have ended and all but its last `kept` loads have
+  // arrived; then the same holds for the workgroup.
+  const auto meet = [](auto kept) {
+    constexpr int v = decltype(kept)::value;  // vmcnt in bits 0-3 and 14-15, lgkmcnt 0 in 8-11
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((v & 15) | ((v >> 4) << 14) | (7 << 4));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  constexpr std::integral_constant<int, (STAGES - 1) * kLoads> first_in;
+  constexpr std::integral_constant<int, (STAGES - 2) * kLoads> next_in;
+
+  // Tiles beyond the last are fetched from outside the buffers, which costs
+  // no memory access, and are not multiplied: a loop without cases keeps the
+  // products in one stream.
+  const int tiles = (d + kTileK - 1) / kTileK;
+#pragma unroll
+  for (int t = 0; t < STAGES; ++t) fetch(t < tiles ? t * kTileK : kOutside, t);
+  meet(first_in);
+  read(0, 0);
+  int stage = 0;
+  for (int t = 0; t < tiles; ++t) {
+    read(stage, 1);
+    __builtin_amdgcn_sched_barrier(0);  // first the reads, which the products cover
+    multiply(0);
+    meet(next_in);
+    fetch(t + STAGES < tiles ? (t + STAGES) * kTileK : kOutside, stage);
+    stage = stage + 1 < STAGES ? stage + 1 : 0;
+    read(stage, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(1);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // No load into LDS is left when the workgroup ends.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+  const int64_t at = m0 + wm * (16 * FM) + (lane / 16) * (4 * FM);
+  float scale[4 * FM];
+#pragma unroll
+  for (int e = 0; e < 4 * FM; ++e) scale[e] = sw[min(static_cast<int>(at) + e, m - 1)];
 #pragma unroll
   for (int j = 0; j < FN; ++j) {
     const int64_t row = n0 + (wn * FN + j) * 16 + (lane & 15);
     if (row >= n) continue;
     const float s = sx[row];
+    Out* out = S + row * lds + at;
+    Out v[4 * FM];
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const int64_t at = m0 + (wm * FM + i) * 16 + (lane / 16) * 4;
+    for (int e = 0; e < 4 * FM; ++e)
+      v[e] = from_float<Out>(static_cast<float>(acc[e / 4][j][e % 4]) * s * scale[e]);
+    if (at + 4 * FM <= m) {
+      __builtin_memcpy(out, v, sizeof(v));
+    } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (at + e < m)
-          S[row * lds + at + e] =
-              from_float<Out>(static_cast<float>(acc[i][j][e]) * s * sw[at + e]);
+      for (int e = 0; e < 4 * FM; ++e)
+        if (at + e < m) out[e] = v[e];
     }
   }
 }
 
+template <class Out, int BN, int BM, int WN, int WM, int STAGES>
+void start(const ScoresI8Launch& a) {
+  const int tiles_n = static_cast<int>((a.n + BN - 1) / BN);
+  const int tiles_m = static_cast<int>((a.m + BM - 1) / BM);
+  scores_i8_kernel<Out, BN, BM, WN, WM, STAGES>
+      <<<static_cast<unsigned>(tiles_n) * tiles_m, 64 * WN * WM, 0, a.stream>>>(
+          static_cast<const int8_t*>(a.X), a.ldx, a.sx, a.W, a.ldw, a.sw, static_cast<Out*>(a.S), a.lds,
+          static_cast<int>(a.d), static_cast<int>(a.m), static_cast<int>(a.n), tiles_n, tiles_m);
+}
+
+// ---------------------------------------------------------------------------
+// One or two examples: W goes by once, and that is what the time is.  Each
+// workgroup quantises the examples itself into LDS (which saves a launch
+// before it), and its waves take RW classes at a time, 16 neighbouring bytes
+// of a class to a lane, with four-byte dot products.  The examples' rows in
+// LDS are zero from d on, so what W holds there counts for nothing; a lane
+// whose 16 bytes all lie beyond d loads none.
+// ---------------------------------------------------------------------------
+constexpr int kFewThreads = 256;
+
+template <class T, class Out, int NX, int RW>
+__global__ __launch_bounds__(kFewThreads) void scores_i8_few_kernel(
+    const T* __restrict__ X, int64_t ldx, const float* __restrict__ sx,
+    const int8_t* __restrict__ W, int64_t ldw, const float* __restrict__ sw,
+    Out* __restrict__ S, int64_t lds, int d, int m, int rows) {
+  constexpr int kWaves = kFewThreads / 64, kChunk = 1024;
+  extern __shared__ __align__(16) int8_t few_x[];
+  __shared__ unsigned part[NX][kWaves];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int pad = (d + kChunk - 1) / kChunk * kChunk;
+  float scale[NX];
+  if constexpr (sizeof(T) == 1) {
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
+      const int8_t* x = reinterpret_cast<const int8_t*>(X) + i * ldx;
+      for (int at = threadIdx.x * 16; at < pad; at += kFewThreads * 16) {
+        int w[4] = {0, 0, 0, 0};
+        if (at + 16 <= d) {
+          __builtin_memcpy(w, x + at, 16);
+        } else {
+          for (int e = 0; at + e < d; ++e) w[e / 4] |= (x[at + e] & 0xff) << (8 * (e % 4));
+        }
+        __builtin_memcpy(few_x + i * pad + at, w, 16);
+      }
+      scale[i] = sx[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
+      unsigned most = 0;
+      for (int at = threadIdx.x * 8; at < d; at += kFewThreads * 8) {
+        float v[8];
+        load_vec<8>(X + i * ldx, at, d, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = max(most, magnitude(v[e]));
+      }
+#pragma unroll
+      for (int off = 32; off; off >>= 1) most = max(most, static_cast<unsigned>(__shfl_xor(most, off)));
+      if (lane == 0) part[i][wave] = most;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
+      unsigned most = part[i][0];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) most = max(most, part[i][w]);
+      const ColumnScale s(most);
+      scale[i] = s.scale;
+      for (int at = threadIdx.x * 8; at < pad; at += kFewThreads * 8) {
+        float v[8];
+        load_vec<8>(X + i * ldx, at, d, v);
+        unsigned w[2];
+        quantize8(v, s, w);
+        __builtin_memcpy(few_x + i * pad + at, w, 8);
+      }
+    }
+  }
+  __syncthreads();
+
+  const int first = blockIdx.x * rows, last = min(m, first + rows);
+  for (int r0 = first + wave * RW; r0 < last; r0 += kWaves * RW) {
+    const int8_t* row[RW];
+#pragma unroll
+    for (int r = 0; r < RW; ++r) row[r] = W + min(r0 + r, m - 1) * ldw + lane * 16;
+    int acc[RW][NX] = {};
+#pragma unroll 4
+    for (int at = 0; at < pad; at += kChunk) {
+      if (at + lane * 16 >= d) break;
+      v4i w[RW];
+#pragma unroll
+      for (int r = 0; r < RW; ++r) w[r] = *reinterpret_cast<const v4i*>(row[r] + at);
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        const v4i x = *reinterpret_cast<const v4i*>(few_x + i * pad + at + lane * 16);
+#pragma unroll
+        for (int r = 0; r < RW; ++r)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[r][i] = __builtin_amdgcn_sdot4(w[r][e], x[e], acc[r][i], false);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < RW; ++r)
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        const int sum = wave_total(acc[r][i]);
+        if (lane == 0 && r0 + r < last)
+          S[i * lds + r0 + r] = from_float<Out>(static_cast<float>(sum) * scale[i] * sw[r0 + r]);
+      }
+  }
+}
+
+template <class T, class Out, int NX, int RW>
+void start_few(const ScoresI8Launch& a) {
+  // About a thousand workgroups: four to a compute unit, which keeps enough
+  // loads in flight, and no more than that quantise the examples.
+  const int step = kFewThreads / 64 * RW;
+  const int64_t share = (a.m + 1023) / 1024;
+  const int rows = static_cast<int>((share + step - 1) / step * step);
+  const size_t bytes = static_cast<size_t>(NX) * ((a.d + 1023) / 1024 * 1024);
+  scores_i8_few_kernel<T, Out, NX, RW>
+      <<<static_cast<unsigned>((a.m + rows - 1) / rows), kFewThreads, bytes, a.stream>>>(
+          static_cast<const T*>(a.X), a.ldx, a.sx, a.W, a.ldw, a.sw, static_cast<Out*>(a.S), a.lds,
+          static_cast<int>(a.d), static_cast<int>(a.m), rows);
+}
+template <class T, class Out>
+void start_few(const ScoresI8Launch& a) {
+  // Four classes to a wave share the reads of the examples; where that
+  // leaves compute units without a workgroup, one class each.
+  if (a.m >= 8192) a.n == 1 ? start_few<T, Out, 1, 4>(a) : start_few<T, Out, 2, 4>(a);
+  else a.n == 1 ? start_few<T, Out, 1, 1>(a) : start_few<T, Out, 2, 1>(a);
+}
+
+// What a tile kernel takes for `tiles` of its tiles, in its time per tile of
+// K with one tile and with two tiles to a compute unit (256 of them).
+double tile_time(int64_t tiles, double one, double two) {
+  const int64_t rest = tiles % 512;
+  return static_cast<double>(tiles / 512) * two + (rest == 0 ? 0. : rest <= 256 ? one : two);
+}
+
 template <class Out>
 hipError_t scores(const ScoresI8Launch& a) {
-  constexpr int BN = 64, BM = 128;
-  const dim3 grid(static_cast<unsigned>((a.m + BM - 1) / BM),
-                  static_cast<unsigned>((a.n + BN - 1) / BN));
-  scores_i8_kernel<Out, BN, BM, 2, 2><<<grid, 256, 0, a.stream>>>(
-      a.X, a.ldx, a.sx, a.W, a.ldw, a.sw, static_cast<Out*>(a.S), a.lds, static_cast<int>(a.d),
-      static_cast<int>(a.m), static_cast<int>(a.n));
+  if (scores_i8_few(a.n, a.d)) {
+    switch (a.data) {
+      case SDCA_F32: start_few<float, Out>(a); break;
+      case SDCA_F64: start_few<double, Out>(a); break;
+      case SDCA_F16: start_few<__half, Out>(a); break;
+      case SDCA_BF16: start_few<__hip_bfloat16, Out>(a); break;
+      default: start_few<int8_t, Out>(a);
+    }
+    return hipGetLastError();
+  }
+  // The tile by its measured microseconds per 128 bytes of K: 256 x 256 does
+  // the most work per byte read, smaller ones fill the device with fewer
+  // scores.  (us by tile 256, 128, 64: 16384 x 8192, d 8192: 900, 1100, 1770;
+  // 20000 x 1000, d 4096: 132, 100, 150; 2048 x 2048, d 2048: 32, 15.6, 19;
+  // 128 x 8192, d 4096: 48, 25, 13.)
+  const auto tiles = [&](int64_t t) { return ((a.n + t - 1) / t) * ((a.m + t - 1) / t); };
+  const double t256 = tile_time(2 * tiles(256), 1.76, 1.76);
+  const double t128 = tile_time(tiles(128), 0.65, 1.07);
+  const double t64 = tile_time(tiles(64), 0.33, 0.43);
+  if (t256 <= t128 && t256 <= t64) start<Out, 256, 256, 2, 4, 2>(a);
+  else if (t128 <= t64) start<Out, 128, 128, 2, 4, 2>(a);
+  else start<Out, 64, 64, 2, 2, 4>(a);
   return hipGetLastError();
 }
 
 }  // namespace
+
+bool scores_i8_few(int64_t n, int64_t d) {
+  // By the examples' room in LDS; shorter rows of W leave most lanes without
+  // work, and the tile kernels do better.
+  return n <= 2 && d >= 512 && n * d <= 49152;
+}
 
 hipError_t launch_scores_i8(const ScoresI8Launch& a) {
   switch (a.out) {
