@@ -758,34 +758,34 @@ def _values(x, name, n, dtype, like):
     return x
 
 
-def _where(x, fn):
-    """(flags, stream) of a call on x; on another device than the current
-    one, torch's current stream there."""
+_raw_stream = None
+
+
+def _torch_stream(device):
+    """torch's current stream on a device, as the C ABI takes it."""
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        # The number alone; a Stream object takes longer to make than a
+        # small call to run.
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
+    return _raw_stream(device)
+
+
+def _answer(x, name, fn, *args):
+    """Calls fn(*args, flags, stream) for the tensor or array x: on torch's
+    current stream of its device, or with host arrays."""
     if not _is_torch(x):
-        return HOST_PTR, None
+        return check(fn(*args, HOST_PTR, None))
     if not x.is_cuda:
-        raise SdcaError(2, f"{fn} takes CUDA tensors or numpy arrays")
+        raise SdcaError(2, f"{name} takes CUDA tensors or numpy arrays")
     import torch
-    return 0, torch.cuda.current_stream(x.device).cuda_stream
-
-
-class _on:
-    """Makes a tensor's device the current one for a call, where it is not."""
-
-    def __init__(self, x):
-        self.guard = None
-        if _is_torch(x):
-            import torch
-            if x.device.index != torch.cuda.current_device():
-                self.guard = torch.cuda.device(x.device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *args):
-        if self.guard is not None:
-            self.guard.__exit__(*args)
+    device = x.get_device()
+    if device == torch.cuda.current_device():
+        return check(fn(*args, 0, _torch_stream(device)))
+    with torch.cuda.device(device):
+        return check(fn(*args, 0, _torch_stream(device)))
 
 
 def _empty(shape, dtype, like):
@@ -807,7 +807,6 @@ def quantize_i8(A, out=None, scales=None):
         raise SdcaError(3, f"unsupported element type {A.dtype}")
     lda = _pitch(A, "A")
     n, d = A.shape
-    flags, stream = _where(A, "quantize_i8")
     like = out if out is not None else A
     if _is_torch(like) != _is_torch(A) or (_is_torch(A) and like.device != A.device):
         raise SdcaError(2, "out: expected the same kind and device as A")
@@ -817,8 +816,7 @@ def quantize_i8(A, out=None, scales=None):
     ldq = _pitch(Q, "out", (n, d))
     s = scales if scales is not None else _empty((n,), "float32", A)
     _values(s, "scales", n, _float32(A), A)
-    with _on(A):
-        check(lib.sdca_quantize_i8(data, d, n, _ptr(A), lda, _ptr(Q), ldq, _ptr(s), flags, stream))
+    _answer(A, "quantize_i8", lib.sdca_quantize_i8, data, d, n, _ptr(A), lda, _ptr(Q), ldq, _ptr(s))
     return Q, s
 
 
@@ -853,7 +851,6 @@ def scores_i8(X, W, w_scales, x_scales=None, out=None, dtype=None):
         raise SdcaError(1, "x_scales go with int8 examples, and with them only")
     if x_scales is not None:
         _values(x_scales, "x_scales", n, f32, X)
-    flags, stream = _where(X, "scores_i8")
     if out is None:
         if _is_torch(X):
             import torch
@@ -866,15 +863,14 @@ def scores_i8(X, W, w_scales, x_scales=None, out=None, dtype=None):
     if code not in (F32, F16, BF16):
         raise SdcaError(3, f"scores cannot be {out.dtype}")
     lds = _pitch(out, "out", (n, m))
-    with _on(X):
-        check(lib.sdca_scores_i8(data, code, d, m, n, _ptr(X), ldx, _ptr(x_scales), _ptr(W), ldw,
-                                 _ptr(w_scales), _ptr(out), lds, flags, stream))
+    _answer(X, "scores_i8", lib.sdca_scores_i8, data, code, d, m, n, _ptr(X), ldx, _ptr(x_scales),
+            _ptr(W), ldw, _ptr(w_scales), _ptr(out), lds)
     return out
 
 
 def _setting(v, name, n, kind, like):
     """A setting's array of n values beside `like`, or None for a number."""
-    if not (_is_torch(v) or isinstance(v, (np.ndarray, list, tuple))):
+    if isinstance(v, (float, int)) or not (_is_torch(v) or isinstance(v, (np.ndarray, list, tuple))):
         return None
     if _is_torch(like):
         import torch
@@ -901,7 +897,6 @@ def sample(S, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, prob=False, kep
         raise SdcaError(3, f"unsupported element type {S.dtype}")
     lds = _pitch(S, "S")
     n, m = S.shape
-    flags, stream = _where(S, "sample")
     _values(u, "u", n, _float32(S), S)
     T = _setting(temperature, "temperature", n, "float32", S)
     p = _setting(top_p, "top_p", n, "float32", S)
@@ -913,8 +908,7 @@ def sample(S, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, prob=False, kep
     labels = _empty((n,), "int64", S)
     pr = _empty((n,), "float32", S) if prob else None
     kp = _empty((n,), "int64", S) if kept else None
-    with _on(S):
-        check(lib.sdca_sample(data, m, n, _ptr(S), lds, _ptr(u), params, columns, _ptr(labels),
-                              _ptr(pr), _ptr(kp), flags, stream))
+    _answer(S, "sample", lib.sdca_sample, data, m, n, _ptr(S), lds, _ptr(u), params, columns,
+            _ptr(labels), _ptr(pr), _ptr(kp))
     res = (labels,) + ((pr,) if prob else ()) + ((kp,) if kept else ())
     return res if len(res) > 1 else labels

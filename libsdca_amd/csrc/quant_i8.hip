@@ -82,7 +82,8 @@ template <class T>
 hipError_t quantize(const QuantLaunch& a) {
   // By the column's length alone: a wave for a short column, a workgroup
   // above, with as few registers as hold it.
-  if (a.pad <= 64 * 2 * kVec) start<T, 64, 2, false>(a);
+  if (a.pad <= 64 * kVec) start<T, 64, 1, false>(a);
+  else if (a.pad <= 64 * 2 * kVec) start<T, 64, 2, false>(a);
   else if (a.pad <= 256 * 2 * kVec) start<T, 256, 2, false>(a);
   else if (a.pad <= 256 * 6 * kVec) start<T, 256, 6, false>(a);
   else start<T, 256, 6, true>(a);

@@ -550,13 +550,45 @@ __device__ inline void each_of(const T* row, int begin, int end, int t, int thre
   }
 }
 
+// The bin at which the running sum over falling bins, `sum` before the
+// highest, first reaches `target`, and the sum above it: in s.found_bin and
+// s.found_above (the lowest bin where none does).
+template <int THREADS>
+__device__ void find_bin(int bins, u64 sum, u64 target, Shared<THREADS>& s) {
+  constexpr int kOwn = kBins / THREADS;  // bins of a thread
+  __syncthreads();
+  const int hi = bins - 1 - kOwn * static_cast<int>(threadIdx.x);
+  u64 own = 0;
+  for (int b = 0; b < kOwn; ++b) own += hi - b >= 0 ? s.hist[hi - b] : 0;
+  u64 before = wave_scan(own);
+  if ((threadIdx.x & 63) == 63) s.sum[threadIdx.x >> 6] = before;
+  if (threadIdx.x == 0) {
+    s.found_bin = 0;
+    s.found_above = sum;
+  }
+  __syncthreads();
+  for (int w = 0; w < static_cast<int>(threadIdx.x >> 6); ++w) before += s.sum[w];
+  before += sum - own;
+  if (before < target && before + own >= target) {
+    for (int b = 0; b < kOwn; ++b) {
+      const u64 here = s.hist[hi - b];
+      if (before + here >= target) {
+        s.found_bin = hi - b;
+        s.found_above = before;
+        break;
+      }
+      before += here;
+    }
+  }
+  __syncthreads();
+}
+
 // The key at which the running sum over falling keys, from `floor_key` up,
 // first reaches `target` (counts, or with MASS fixed weights), and the sum
 // above it: three digits of the key, a histogram each.
 template <bool MASS, int THREADS, class T>
 __device__ void descend(const T* row, int m, const Weights& wt, unsigned floor_key, u64 target,
                         Shared<THREADS>& s, unsigned* tau, u64* above) {
-  constexpr int kOwn = kBins / THREADS;  // bins of a thread
   unsigned prefix = 0;
   u64 sum = 0;
   for (int level = 0; level < 3; ++level) {
@@ -565,10 +597,6 @@ __device__ void descend(const T* row, int m, const Weights& wt, unsigned floor_k
     const int bins = 1 << bits;
     __syncthreads();
     for (int i = threadIdx.x; i < kBins; i += THREADS) s.hist[i] = 0;
-    if (threadIdx.x == 0) {
-      s.found_bin = 0;
-      s.found_above = sum;
-    }
     __syncthreads();
     each_of(row, 0, m, threadIdx.x, THREADS, [&](float l, int) {
       const unsigned key = key_of(l);
@@ -576,27 +604,7 @@ __device__ void descend(const T* row, int m, const Weights& wt, unsigned floor_k
       const u64 add = MASS ? wt.fixed(wt.of(l)) : 1;
       if (add) atomicAdd(&s.hist[(key >> shift) & (bins - 1)], add);
     });
-    __syncthreads();
-    const int hi = bins - 1 - kOwn * static_cast<int>(threadIdx.x);
-    u64 own = 0;
-    for (int b = 0; b < kOwn; ++b) own += hi - b >= 0 ? s.hist[hi - b] : 0;
-    u64 before = wave_scan(own);
-    if ((threadIdx.x & 63) == 63) s.sum[threadIdx.x >> 6] = before;
-    __syncthreads();
-    for (int w = 0; w < static_cast<int>(threadIdx.x >> 6); ++w) before += s.sum[w];
-    before += sum - own;
-    if (before < target && before + own >= target) {
-      for (int b = 0; b < kOwn; ++b) {
-        const u64 here = s.hist[hi - b];
-        if (before + here >= target) {
-          s.found_bin = hi - b;
-          s.found_above = before;
-          break;
-        }
-        before += here;
-      }
-    }
-    __syncthreads();
+    find_bin(bins, sum, target, s);
     prefix = (prefix << bits) | static_cast<unsigned>(s.found_bin);
     sum = s.found_above;
   }
@@ -607,17 +615,19 @@ __device__ void descend(const T* row, int m, const Weights& wt, unsigned floor_k
 // The draw within [begin, end) of a row: the labels above tau and the first
 // `ties` of the whole row at it, those with a weight of at least q.  The
 // stretch is narrowed to the one that holds the label, a wave's share at a
-// time.  total: of the whole row, with `base` before `begin`, and `many`
-// kept; or 0 where [begin, end) is the whole row, which gives them then.
+// time.  total: of the whole row, with `base` and `tie_base` ties before
+// `begin`, and `many` kept; or 0 where [begin, end) is the whole row, which
+// gives them then.
 template <int THREADS, class T>
-__device__ void narrow_and_draw(const T* row, int begin, int end, u64 base, u64 total, u64 many,
-                                unsigned tau, u64 ties, const Weights& wt, const Settings& c,
+__device__ void narrow_and_draw(const T* row, int begin, int end, u64 base, u64 tie_base,
+                                u64 total, u64 many, unsigned tau, u64 ties, const Weights& wt,
+                                const Settings& c,
                                 const SampleArgs& a, int64_t col, Shared<THREADS>& s) {
   constexpr int kWaves = THREADS / 64;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const float w_tau = ties ? wt.of(score_of(tau)) : 0.f;
   const u64 f_tau = w_tau >= c.q ? wt.fixed(w_tau) : 0;
-  u64 target = total ? draw_target(a.u[col], total) : 0, tie_base = 0;
+  u64 target = total ? draw_target(a.u[col], total) : 0;
   // Each step leaves a sixteenth (or 64 scores): the stretch is always down
   // to 64 after eight steps, and the loop ends whatever the sums are.
   for (int step = 0; step < 8; ++step) {
@@ -680,10 +690,158 @@ __device__ void narrow_and_draw(const T* row, int begin, int end, u64 base, u64 
   }
 }
 
-// The cut by searches over the whole column, and the draw: for columns whose
-// short list does not do.
+// Sorts the first P (a power of two from 64 to THREADS) of the workgroup's
+// values, one a thread, falling.
+template <int THREADS>
+__device__ inline u64 sort_block(u64 v, int P, u64* swap) {
+  const int i = threadIdx.x;
+  if (i < P) v = sort_wave<true>(v, (i & 64) == 0 || P == 64);
+  for (int size = 128; size <= P; size <<= 1) {
+    const bool falling = (i & size) == 0 || size == P;
+    for (int stride = size >> 1; stride >= 64; stride >>= 1) {
+      __syncthreads();
+      if (i < P) swap[i] = v;
+      __syncthreads();
+      if (i < P) {
+        const u64 o = swap[i ^ stride];
+        const bool larger = ((i & stride) == 0) == falling;
+        v = (o > v) == larger ? o : v;
+      }
+    }
+    if (i < P) v = sort_merge<32, true>(v, falling);
+  }
+  return v;
+}
+
+// The inclusive sum over the workgroup's threads.
+template <int THREADS>
+__device__ inline u64 block_scan(u64 v, u64 (&part)[THREADS / 64], u64* total) {
+  v = wave_scan(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  u64 all = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    if (w == static_cast<int>(threadIdx.x >> 6)) before = all;
+    all += part[w];
+  }
+  *total = all;
+  return v + before;
+}
+
+// The nucleus of a column with very many labels in it, in two passes over
+// the column: the mass in 2048 even steps of the score finds the step that
+// the target falls into; then the few labels of that step are gathered and
+// sorted, which gives the cut, while the labels above it are added up by
+// stretches of the column, which gives the draw its stretch.  Labels with
+// keys below floor_key are none.  False, and nothing done, where the step
+// holds more labels than the list.
 template <int THREADS, class T>
-__device__ void search_and_draw(const T* row, const Weights& wt, const Settings& c,
+__device__ bool nucleus_and_draw(const T* row, u64 mass, unsigned floor_key, const Weights& wt,
+                                 const Settings& c, const SampleArgs& a, int64_t col,
+                                 Shared<THREADS>& s) {
+  constexpr int kWaves = THREADS / 64, kEntries = Shared<THREADS>::kEntries;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const u64 target = top_p_target(c.p, mass);
+  // Labels of weights below e = (1 - p) mass / m sum to less than what the
+  // nucleus leaves out, so it has none of them.
+  const float rest = (1.f - c.p) * static_cast<float>(static_cast<double>(mass) / wt.scale) /
+                     static_cast<float>(a.m);
+  const float low = wt.max + (logf(rest) - 0.01f) / wt.inv_t - fabsf(wt.max) * 1e-5f;
+  const float per = static_cast<float>(kBins) / (wt.max - low);
+  if (!(per > 0.f && per < INFINITY && low > -INFINITY)) return false;
+  const auto step_of = [&](float l) {
+    return min(static_cast<int>((l - low) * per), kBins - 1);  // rises with l
+  };
+  for (int i = threadIdx.x; i < kBins; i += THREADS) s.hist[i] = 0;
+  __syncthreads();
+  each_of(row, 0, a.m, threadIdx.x, THREADS, [&](float l, int) {
+    if (l >= low && key_of(l) >= floor_key) atomicAdd(&s.hist[step_of(l)], wt.fixed(wt.of(l)));
+  });
+  find_bin(kBins, 0, target, s);
+  const int step = s.found_bin;
+  const u64 above = s.found_above;
+  __syncthreads();
+  if (threadIdx.x == 0) s.count = 0;
+  __syncthreads();
+
+  const int part = ((a.m + kWaves - 1) / kWaves + 63) / 64 * 64;
+  const int begin = wave * part, end = min(a.m, begin + part);
+  u64 sum = 0, many = 0;
+  if (begin < end)
+    each_of(row, begin, end, lane, 64, [&](float l, int i) {
+      if (!(l >= low)) return;
+      const int at_step = step_of(l);
+      if (at_step > step) {
+        const float w = wt.of(l);
+        if (w >= c.q) {
+          sum += wt.fixed(w);
+          ++many;
+        }
+      } else if (at_step == step && key_of(l) >= floor_key) {
+        const int at = atomicAdd(&s.count, 1);
+        if (at < kEntries) s.list.entry[at] = entry_of(l, i);
+      }
+    });
+  sum = wave_sum(sum);
+  many = wave_sum(many);
+  if (lane == 0) {
+    s.sum2[wave] = sum;
+    s.sum3[wave] = many;
+  }
+  __syncthreads();
+  const int count = s.count;
+  if (count > kEntries || count == 0) return false;
+  const int i = threadIdx.x;
+  int P = 64;
+  while (P < count) P <<= 1;
+  const u64 entry = sort_block<THREADS>(i < count ? s.list.entry[i] : 0, P, s.list.swap);
+  const float w = i < count ? wt.of(score_of(static_cast<unsigned>(entry >> 32))) : 0.f;
+  const u64 f = i < count ? wt.fixed(w) : 0;
+  u64 all;
+  const u64 incl = block_scan<THREADS>(f, s.sum, &all);
+  if (above + all < target) return false;
+  const bool in = i < count && above + incl - f < target;  // a prefix, not empty
+  const u64 votes = __ballot(in);
+  __syncthreads();
+  if (lane == 0) s.number[wave] = __popcll(votes);
+  s.list.swap[i] = entry;
+  __syncthreads();
+  int kept = 0;
+  for (int v = 0; v < kWaves; ++v) kept += s.number[v];
+  const unsigned tau = static_cast<unsigned>(s.list.swap[kept - 1] >> 32);
+  if (in && w >= c.q) {
+    atomicAdd(&s.sum2[index_of(entry) / part], f);
+    atomicAdd(&s.sum3[index_of(entry) / part], u64(1));
+  }
+  __syncthreads();
+  const u64 total = total_of(s.sum2), draw = draw_target(a.u[col], total);
+  many = total_of(s.sum3);
+  u64 base = 0;
+  int pick = 0;
+  for (; pick < kWaves - 1 && base + s.sum2[pick] <= draw; ++pick) base += s.sum2[pick];
+  // The ties that are kept, in all and before the stretch.
+  const u64 tied = __ballot(in && static_cast<unsigned>(entry >> 32) == tau);
+  const u64 early = __ballot(in && static_cast<unsigned>(entry >> 32) == tau && index_of(entry) < pick * part);
+  __syncthreads();
+  if (lane == 0) {
+    s.sum[wave] = __popcll(tied);
+    s.number[wave] = __popcll(early);
+  }
+  __syncthreads();
+  const u64 ties = total_of(s.sum);
+  u64 tie_base = 0;
+  for (int v = 0; v < kWaves; ++v) tie_base += s.number[v];
+  narrow_and_draw<THREADS>(row, pick * part, min(a.m, pick * part + part), base, tie_base, total,
+                           many, tau, ties, wt, c, a, col, s);
+  return true;
+}
+
+// The cut by searches over the whole column, and the draw: for columns whose
+// short list does not do.  mass: of all labels, where it is known.
+template <int THREADS, class T>
+__device__ void search_and_draw(const T* row, u64 mass, const Weights& wt, const Settings& c,
                                 const SampleArgs& a, int64_t col, Shared<THREADS>& s) {
   unsigned tau = 0;
   u64 ties = 0;  // labels at tau that are kept
@@ -693,16 +851,20 @@ __device__ void search_and_draw(const T* row, const Weights& wt, const Settings&
     ties = c.k - above;
   }
   if (c.p < 1.f) {
-    u64 mass = 0;
-    each_of(row, 0, a.m, threadIdx.x, THREADS, [&](float l, int) {
-      if (key_of(l) > tau) mass += wt.fixed(wt.of(l));
-    });
-    mass = wave_sum(mass);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) s.sum[threadIdx.x >> 6] = mass;
-    __syncthreads();
-    mass = total_of(s.sum);
-    if (ties) mass += ties * wt.fixed(wt.of(score_of(tau)));
+    if (c.k || mass == 0) {
+      mass = 0;
+      each_of(row, 0, a.m, threadIdx.x, THREADS, [&](float l, int) {
+        if (key_of(l) > tau) mass += wt.fixed(wt.of(l));
+      });
+      mass = wave_sum(mass);
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) s.sum[threadIdx.x >> 6] = mass;
+      __syncthreads();
+      mass = total_of(s.sum);
+      if (ties) mass += ties * wt.fixed(wt.of(score_of(tau)));
+      __syncthreads();
+    }
+    if (nucleus_and_draw<THREADS>(row, mass, tau, wt, c, a, col, s)) return;
     const u64 target = top_p_target(c.p, mass);
     unsigned cut;
     u64 above;
@@ -713,13 +875,13 @@ __device__ void search_and_draw(const T* row, const Weights& wt, const Settings&
     tau = cut;
     ties = need;
   }
-  narrow_and_draw<THREADS>(row, 0, a.m, 0, 0, 0, tau, ties, wt, c, a, col, s);
+  narrow_and_draw<THREADS>(row, 0, a.m, 0, 0, 0, 0, tau, ties, wt, c, a, col, s);
 }
 
 // A stretch [begin, end) of a column, for the workgroup's waves: each has
 // the same number of groups of 64 V neighbouring scores, lane t the values
 // V t .. V t + V - 1 of each group.  R: a lane's scores that are kept in
-// registers; R = 0 reads them from memory each time, four groups at once.
+// registers; R = 0 reads them from memory each time, 16 scores at once.
 template <class T, int THREADS, int R>
 struct Column {
   static constexpr int V = sizeof(T) == 2 ? 8 : 4;
@@ -802,13 +964,14 @@ struct Column {
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
-      for (int g = 0; g < groups; g += 4) {
-        float l[4][V];
+      constexpr int kBatch = 16 / V;
+      for (int g = 0; g < groups; g += kBatch) {
+        float l[kBatch][V];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) group(g + b, l[b]);
+        for (int b = 0; b < kBatch; ++b) group(g + b, l[b]);
         bool go = true;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
+        for (int b = 0; b < kBatch; ++b) {
           if (go) go = f(l[b], from + (g + b) * 64 * V);
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -826,44 +989,31 @@ struct Column {
   }
 };
 
-// Sorts the first P (a power of two from 64 to THREADS) of the workgroup's
-// values, one a thread, falling.
-template <int THREADS>
-__device__ inline u64 sort_block(u64 v, int P, u64* swap) {
-  const int i = threadIdx.x;
-  if (i < P) v = sort_wave<true>(v, (i & 64) == 0 || P == 64);
-  for (int size = 128; size <= P; size <<= 1) {
-    const bool falling = (i & size) == 0 || size == P;
-    for (int stride = size >> 1; stride >= 64; stride >>= 1) {
-      __syncthreads();
-      if (i < P) swap[i] = v;
-      __syncthreads();
-      if (i < P) {
-        const u64 o = swap[i ^ stride];
-        const bool larger = ((i & stride) == 0) == falling;
-        v = (o > v) == larger ? o : v;
-      }
-    }
-    if (i < P) v = sort_merge<32, true>(v, falling);
-  }
-  return v;
+// The fixed weights of a group of scores.
+template <int V>
+__device__ inline u64 mass_of(const Weights& wt, const float (&l)[V]) {
+  u64 sum = 0;
+#pragma unroll
+  for (int e = 0; e < V; ++e) sum += wt.raw(wt.of(l[e]));
+  return sum - V * kOne52;
 }
 
-// The inclusive sum over the workgroup's threads.
-template <int THREADS>
-__device__ inline u64 block_scan(u64 v, u64 (&part)[THREADS / 64], u64* total) {
-  v = wave_scan(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 63) part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  u64 all = 0, before = 0;
+// Appends the scores of a group that are at least `from` to a list in LDS
+// (it counts those beyond its room too).  Most groups have none.
+template <int V>
+__device__ inline void push_from(float from, const float (&l)[V], int at, u64* list, int room,
+                                 int* count) {
+  float most = l[0];
 #pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) {
-    if (w == static_cast<int>(threadIdx.x >> 6)) before = all;
-    all += part[w];
+  for (int e = 1; e < V; ++e) most = fmaxf(most, l[e]);
+  if (!(most >= from && most > -INFINITY)) return;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    if (l[e] >= from && l[e] > -INFINITY) {
+      const int i = atomicAdd(count, 1);
+      if (i < room) list[i] = entry_of(l[e], at + e);
+    }
   }
-  *total = all;
-  return v + before;
 }
 
 // The cuts and the draw from a list of `count` (at most THREADS) entries,
@@ -1040,12 +1190,10 @@ __global__ __launch_bounds__(THREADS) void sample_block_kernel(const T* __restri
     const float from = whole ? floor_live : bound;
     __syncthreads();
     const bool sum_now = sum_all && mass == 0;
-    column.each([&](float l, int i) {
-      if (sum_now) mass += wt.fixed(wt.of(l));
-      if (l >= from && l > -INFINITY) {
-        const int at = atomicAdd(&s.count, 1);
-        if (at < kEntries) s.list.entry[at] = entry_of(l, i);
-      }
+    column.groups_until([&](const float (&l)[Col::V], int at) {
+      if (sum_now) mass += mass_of(wt, l);
+      push_from(from, l, at, s.list.entry, kEntries, &s.count);
+      return true;
     });
     if (sum_now) {
       mass = wave_sum(mass);
@@ -1059,7 +1207,7 @@ __global__ __launch_bounds__(THREADS) void sample_block_kernel(const T* __restri
     if (list_and_draw<THREADS>(entry, count, sum_all ? mass : 0, wt, c, a, col, s)) return;
   }
   __syncthreads();
-  search_and_draw<THREADS>(row, wt, c, a, col, s);
+  search_and_draw<THREADS>(row, mass, wt, c, a, col, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -1163,12 +1311,6 @@ __global__ __launch_bounds__(kPartThreads) void sample_lists_kernel(const T* __r
   u64 mass = 0;
   int number = c.greedy ? a.m : 0;
   const float from = known.whole ? known.floor_live : known.bound;
-  const auto push = [&](float l, int i) {
-    if (l >= from && l > -INFINITY) {
-      const int at = atomicAdd(&counted, 1);
-      if (at < kList) entries[at] = entry_of(l, i);
-    }
-  };
   if (c.greedy) {
     if (mine) column.each([&](float l, int i) { number = l == wt.max && i < number ? i : number; });
 #pragma unroll
@@ -1181,13 +1323,12 @@ __global__ __launch_bounds__(kPartThreads) void sample_lists_kernel(const T* __r
       number += in;
     });
     number = wave_sum(number);
-  } else if (known.sum_all) {
-    column.each([&](float l, int i) {
-      mass += wt.fixed(wt.of(l));
-      push(l, i);
-    });
   } else {
-    column.each(push);
+    column.groups_until([&](const float (&l)[decltype(column)::V], int at) {
+      if (known.sum_all) mass += mass_of(wt, l);
+      push_from(from, l, at, entries, kList, &counted);
+      return true;
+    });
   }
   mass = wave_sum(mass);
   if (lane == 0) {
@@ -1245,20 +1386,20 @@ __global__ __launch_bounds__(kList) void sample_draw_kernel(const T* __restrict_
     int i = 0;
     for (; i < p.parts - 1 && base + of.mass[i] <= target; ++i) base += of.mass[i];
     const int begin = i * p.part;
-    narrow_and_draw<kList>(row, begin, min(a.m, begin + p.part), base, total,
+    narrow_and_draw<kList>(row, begin, min(a.m, begin + p.part), base, 0, total,
                            static_cast<u64>(many), 0u, 0, wt, c, a, col, s);
     return;
   }
+  u64 mass = 0;
+  if (known.sum_all)
+    for (int i = 0; i < p.parts; ++i) mass += of.mass[i];
   if (known.list_does && of.listed <= kList) {
-    u64 mass = 0;
-    if (known.sum_all)
-      for (int i = 0; i < p.parts; ++i) mass += of.mass[i];
     const int count = of.listed;
     const u64 entry = static_cast<int>(threadIdx.x) < count ? of.entry[threadIdx.x] : 0;
     if (list_and_draw<kList>(entry, count, mass, wt, c, a, col, s)) return;
   }
   __syncthreads();
-  search_and_draw<kList>(row, wt, c, a, col, s);
+  search_and_draw<kList>(row, mass, wt, c, a, col, s);
 }
 
 template <class T, int THREADS, int R>
