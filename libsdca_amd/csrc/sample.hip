@@ -495,6 +495,7 @@ struct Shared {
   static constexpr int kEntries = THREADS < kList ? THREADS : kList;
   union {
     u64 hist[kBins];
+    unsigned guide[kBins];
     struct {
       u64 entry[kEntries];
       u64 swap[THREADS];
@@ -541,11 +542,12 @@ constexpr int kNucleus = 128, kNucleusLong = 320;
 // `threads` lanes.
 template <class T, class F>
 __device__ inline void each_of(const T* row, int begin, int end, int t, int threads, F f) {
-  for (int64_t at = begin + int64_t(t) * 4; at < end; at += int64_t(threads) * 4) {
-    float v[4];
-    load_vec<4>(row, at, end, v);
+  constexpr int V = 8;
+  for (int64_t at = begin + int64_t(t) * V; at < end; at += int64_t(threads) * V) {
+    float v[V];
+    load_vec<V>(row, at, end, v);
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < V; ++e)
       if (at + e < end) f(score(v[e]), static_cast<int>(at) + e);
   }
 }
@@ -730,73 +732,80 @@ __device__ inline u64 block_scan(u64 v, u64 (&part)[THREADS / 64], u64* total) {
   return v + before;
 }
 
-// The nucleus of a column with very many labels in it, in two passes over
-// the column: the mass in 2048 even steps of the score finds the step that
-// the target falls into; then the few labels of that step are gathered and
-// sorted, which gives the cut, while the labels above it are added up by
-// stretches of the column, which gives the draw its stretch.  Labels with
-// keys below floor_key are none.  False, and nothing done, where the step
-// holds more labels than the list.
-template <int THREADS, class T>
-__device__ bool nucleus_and_draw(const T* row, u64 mass, unsigned floor_key, const Weights& wt,
-                                 const Settings& c, const SampleArgs& a, int64_t col,
-                                 Shared<THREADS>& s) {
-  constexpr int kWaves = THREADS / 64, kEntries = Shared<THREADS>::kEntries;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const u64 target = top_p_target(c.p, mass);
-  // Labels of weights below e = (1 - p) mass / m sum to less than what the
-  // nucleus leaves out, so it has none of them.
-  const float rest = (1.f - c.p) * static_cast<float>(static_cast<double>(mass) / wt.scale) /
-                     static_cast<float>(a.m);
-  const float low = wt.max + (logf(rest) - 0.01f) / wt.inv_t - fabsf(wt.max) * 1e-5f;
-  const float per = static_cast<float>(kBins) / (wt.max - low);
-  if (!(per > 0.f && per < INFINITY && low > -INFINITY)) return false;
-  const auto step_of = [&](float l) {
-    return min(static_cast<int>((l - low) * per), kBins - 1);  // rises with l
-  };
-  for (int i = threadIdx.x; i < kBins; i += THREADS) s.hist[i] = 0;
-  __syncthreads();
-  each_of(row, 0, a.m, threadIdx.x, THREADS, [&](float l, int) {
-    if (l >= low && key_of(l) >= floor_key) atomicAdd(&s.hist[step_of(l)], wt.fixed(wt.of(l)));
-  });
-  find_bin(kBins, 0, target, s);
-  const int step = s.found_bin;
-  const u64 above = s.found_above;
-  __syncthreads();
-  if (threadIdx.x == 0) s.count = 0;
-  __syncthreads();
-
-  const int part = ((a.m + kWaves - 1) / kWaves + 63) / 64 * 64;
-  const int begin = wave * part, end = min(a.m, begin + part);
-  u64 sum = 0, many = 0;
-  if (begin < end)
-    each_of(row, begin, end, lane, 64, [&](float l, int i) {
-      if (!(l >= low)) return;
-      const int at_step = step_of(l);
-      if (at_step > step) {
-        const float w = wt.of(l);
-        if (w >= c.q) {
-          sum += wt.fixed(w);
-          ++many;
-        }
-      } else if (at_step == step && key_of(l) >= floor_key) {
-        const int at = atomicAdd(&s.count, 1);
-        if (at < kEntries) s.list.entry[at] = entry_of(l, i);
-      }
-    });
-  sum = wave_sum(sum);
-  many = wave_sum(many);
-  if (lane == 0) {
-    s.sum2[wave] = sum;
-    s.sum3[wave] = many;
+// The nucleus of a column with very many labels in it takes two passes over
+// the column.  The first adds the mass up in 2048 even steps of the score,
+// which finds the step that the target falls into.  The second gathers the
+// few labels of that step, whose sorted list gives the cut, and adds up the
+// labels above it by stretches of the column, which gives the draw its
+// stretch.
+//
+// The first pass only guides: it takes hardware exponentials and sums of 32
+// bits, and the second one's exact sums check its step.
+struct NucleusSteps {
+  float low, per, rate, unit, max;
+  u64 target;
+  __device__ NucleusSteps(u64 mass, const Weights& wt, const Settings& c, int m) {
+    target = top_p_target(c.p, mass);
+    // Labels of weights below e = (1 - p) mass / m sum to less than what the
+    // nucleus leaves out, so it has none of them.
+    const float rest = (1.f - c.p) *
+                       static_cast<float>(static_cast<double>(mass) / wt.scale) /
+                       static_cast<float>(m);
+    low = wt.max + (logf(rest) - 0.01f) / wt.inv_t - fabsf(wt.max) * 1e-5f;
+    per = static_cast<float>(kBins) / (wt.max - low);
+    // Sums of at most 2^30, and a rounding up for each label besides.
+    unit = 1073741824.f * static_cast<float>(wt.scale / static_cast<double>(mass));
+    rate = wt.inv_t * 1.44269504f;
+    max = wt.max;
+    share = static_cast<u64>(static_cast<double>(target) / static_cast<double>(mass) * 1073741824.0);
   }
-  __syncthreads();
-  const int count = s.count;
-  if (count > kEntries || count == 0) return false;
-  const int i = threadIdx.x;
+  u64 share;  // the target as the guide has it
+  __device__ bool fit() const { return per > 0.f && per < INFINITY && low > -INFINITY; }
+  __device__ int of(float l) const {  // rises with l
+    return min(static_cast<int>((l - low) * per), kBins - 1);
+  }
+  __device__ unsigned weight(float l) const {
+    return static_cast<unsigned>(__builtin_amdgcn_exp2f((l - max) * rate) * unit + 0.5f);
+  }
+};
+
+// What the second pass finds in a lane's scores.
+struct NucleusSums {
+  u64 over = 0, sum = 0, many = 0;  // above the step; sum and many: those that min-p leaves
+  template <class F>
+  __device__ void add(const NucleusSteps& steps, int step, float l, const Weights& wt,
+                      const Settings& c, F in_step) {
+    if (!(l >= steps.low)) return;
+    const int at = steps.of(l);
+    if (at > step) {
+      const float w = wt.of(l);
+      const u64 f = wt.fixed(w);
+      over += f;
+      if (w >= c.q) {
+        sum += f;
+        ++many;
+      }
+    } else if (at == step) {
+      in_step();
+    }
+  }
+};
+
+// The cut and the draw behind the second pass.  entry: thread i's of the
+// `count` in the step; above: the mass above it; s.sum2 and s.sum3: the mass
+// and number of the labels above it that min-p leaves, for each of kWaves
+// stretches of `part` scores.  False, and nothing done, where the step was
+// not the right one.
+template <int THREADS, class T>
+__device__ bool finish_nucleus(const T* row, u64 entry, int count, u64 above, u64 target, int part,
+                               const Weights& wt, const Settings& c, const SampleArgs& a,
+                               int64_t col, Shared<THREADS>& s) {
+  constexpr int kWaves = THREADS / 64;
+  const int i = threadIdx.x, wave = i >> 6, lane = i & 63;
+  if (above >= target) return false;
   int P = 64;
   while (P < count) P <<= 1;
-  const u64 entry = sort_block<THREADS>(i < count ? s.list.entry[i] : 0, P, s.list.swap);
+  entry = sort_block<THREADS>(entry, P, s.list.swap);
   const float w = i < count ? wt.of(score_of(static_cast<unsigned>(entry >> 32))) : 0.f;
   const u64 f = i < count ? wt.fixed(w) : 0;
   u64 all;
@@ -816,14 +825,13 @@ __device__ bool nucleus_and_draw(const T* row, u64 mass, unsigned floor_key, con
     atomicAdd(&s.sum3[index_of(entry) / part], u64(1));
   }
   __syncthreads();
-  const u64 total = total_of(s.sum2), draw = draw_target(a.u[col], total);
-  many = total_of(s.sum3);
+  const u64 total = total_of(s.sum2), draw = draw_target(a.u[col], total), many = total_of(s.sum3);
   u64 base = 0;
   int pick = 0;
   for (; pick < kWaves - 1 && base + s.sum2[pick] <= draw; ++pick) base += s.sum2[pick];
   // The ties that are kept, in all and before the stretch.
-  const u64 tied = __ballot(in && static_cast<unsigned>(entry >> 32) == tau);
-  const u64 early = __ballot(in && static_cast<unsigned>(entry >> 32) == tau && index_of(entry) < pick * part);
+  const bool tie = in && static_cast<unsigned>(entry >> 32) == tau;
+  const u64 tied = __ballot(tie), early = __ballot(tie && index_of(entry) < pick * part);
   __syncthreads();
   if (lane == 0) {
     s.sum[wave] = __popcll(tied);
@@ -838,11 +846,68 @@ __device__ bool nucleus_and_draw(const T* row, u64 mass, unsigned floor_key, con
   return true;
 }
 
+// The nucleus by one workgroup, of the labels with keys from floor_key up.
+// False, and nothing done, where the step is not the right one or holds more
+// labels than the list.
+template <int THREADS, class T>
+__device__ bool nucleus_and_draw(const T* row, u64 mass, unsigned floor_key, const Weights& wt,
+                                 const Settings& c, const SampleArgs& a, int64_t col,
+                                 Shared<THREADS>& s) {
+  constexpr int kWaves = THREADS / 64, kEntries = Shared<THREADS>::kEntries;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const NucleusSteps steps(mass, wt, c, a.m);
+  if (!steps.fit()) return false;
+  for (int i = threadIdx.x; i < kBins; i += THREADS) s.guide[i] = 0;
+  __syncthreads();
+  each_of(row, 0, a.m, threadIdx.x, THREADS, [&](float l, int) {
+    if (l >= steps.low && key_of(l) >= floor_key) atomicAdd(&s.guide[steps.of(l)], steps.weight(l));
+  });
+  __syncthreads();
+  u64 own[kBins / THREADS];
+#pragma unroll
+  for (int b = 0; b < kBins / THREADS; ++b) own[b] = s.guide[threadIdx.x + b * THREADS];
+  __syncthreads();
+#pragma unroll
+  for (int b = 0; b < kBins / THREADS; ++b) s.hist[threadIdx.x + b * THREADS] = own[b];
+  find_bin(kBins, 0, steps.share, s);
+  const int step = s.found_bin;
+  __syncthreads();
+  if (threadIdx.x == 0) s.count = 0;
+  __syncthreads();
+
+  const int part = ((a.m + kWaves - 1) / kWaves + 63) / 64 * 64;
+  const int begin = wave * part, end = min(a.m, begin + part);
+  NucleusSums sums;
+  if (begin < end)
+    each_of(row, begin, end, lane, 64, [&](float l, int i) {
+      sums.add(steps, step, l, wt, c, [&] {
+        if (key_of(l) < floor_key) return;
+        const int at = atomicAdd(&s.count, 1);
+        if (at < kEntries) s.list.entry[at] = entry_of(l, i);
+      });
+    });
+  const u64 over = wave_sum(sums.over), sum = wave_sum(sums.sum), many = wave_sum(sums.many);
+  if (lane == 0) {
+    s.sum[wave] = over;
+    s.sum2[wave] = sum;
+    s.sum3[wave] = many;
+  }
+  __syncthreads();
+  const int count = s.count;
+  const u64 above = total_of(s.sum);
+  __syncthreads();
+  if (count > kEntries) return false;
+  const u64 entry = static_cast<int>(threadIdx.x) < count ? s.list.entry[threadIdx.x] : 0;
+  return finish_nucleus<THREADS>(row, entry, count, above, steps.target, part, wt, c, a, col, s);
+}
+
 // The cut by searches over the whole column, and the draw: for columns whose
-// short list does not do.  mass: of all labels, where it is known.
+// short list does not do.  mass: of all labels, where it is known; steps:
+// whether a nucleus is first searched in even steps.
 template <int THREADS, class T>
 __device__ void search_and_draw(const T* row, u64 mass, const Weights& wt, const Settings& c,
-                                const SampleArgs& a, int64_t col, Shared<THREADS>& s) {
+                                const SampleArgs& a, int64_t col, Shared<THREADS>& s,
+                                bool steps = true) {
   unsigned tau = 0;
   u64 ties = 0;  // labels at tau that are kept
   if (c.k) {
@@ -864,7 +929,7 @@ __device__ void search_and_draw(const T* row, u64 mass, const Weights& wt, const
       if (ties) mass += ties * wt.fixed(wt.of(score_of(tau)));
       __syncthreads();
     }
-    if (nucleus_and_draw<THREADS>(row, mass, tau, wt, c, a, col, s)) return;
+    if (steps && nucleus_and_draw<THREADS>(row, mass, tau, wt, c, a, col, s)) return;
     const u64 target = top_p_target(c.p, mass);
     unsigned cut;
     u64 above;
@@ -1067,8 +1132,9 @@ __device__ bool list_and_draw(u64 entry, int count, u64 mass, const Weights& wt,
   return true;
 }
 
+// (Four waves to a SIMD: they hide the loads and the exponentials' latencies.)
 template <class T, int THREADS, int R>
-__global__ __launch_bounds__(THREADS) void sample_block_kernel(const T* __restrict__ S,
+__global__ __launch_bounds__(THREADS, 4) void sample_block_kernel(const T* __restrict__ S,
                                                                SampleArgs a) {
   constexpr int kWaves = THREADS / 64;
   constexpr int kEntries = Shared<THREADS>::kEntries;
@@ -1214,7 +1280,10 @@ __global__ __launch_bounds__(THREADS) void sample_block_kernel(const T* __restri
 // A column to several workgroups: with few columns one workgroup each leaves
 // most of the device idle.  Three kernels: the parts' maxima and order
 // statistics; then, with the column's maximum known, their sums and entries
-// of the list; then the draw.
+// of the list; then the draw.  Where a nucleus can be larger than the list,
+// three more take the columns that the draw has left: the two passes, and
+// the draw behind them.  (For the others they end at once, at 2 us each; one
+// workgroup takes 50 us for the two passes over 10^5 scores.)
 // ---------------------------------------------------------------------------
 constexpr int kPartThreads = 256, kPartWaves = kPartThreads / 64;
 constexpr int kMaxParts = 64 / kPartWaves;  // unit_bound takes 64 waves
@@ -1224,13 +1293,25 @@ struct PartsOf {  // one column's
   u64 mass[kMaxParts];
   float top[kMaxParts], jth[kMaxParts * kPartWaves];
   int count[kMaxParts], first[kMaxParts];
-  int listed, unused;
+  int listed, gathered;
+  // Of a nucleus that the list does not hold: whether it is one, the guide
+  // to its step, and its sums by parts.
+  int large, unused;
+  NucleusSums sums[kMaxParts];
+  unsigned guide[kBins];
   u64 entry[kList];
+  __device__ u64 total(int parts) const {
+    u64 t = 0;
+    for (int i = 0; i < parts; ++i) t += mass[i];
+    return t;
+  }
 };
+static_assert(kMaxParts == kList / 64, "finish_nucleus takes the parts as the waves' stretches");
 
 struct PartArgs {
   PartsOf* of;
   int parts, part;  // how many, and the scores of each but the last
+  bool large;       // whether the kernels for large nuclei follow
 };
 
 template <class T>
@@ -1268,7 +1349,7 @@ __global__ __launch_bounds__(kPartThreads) void sample_parts_kernel(const T* __r
     float t = tops[0];
     for (int w = 1; w < kPartWaves; ++w) t = fmaxf(t, tops[w]);
     of.top[blockIdx.x] = t;
-    if (blockIdx.x == 0) of.listed = 0;
+    if (blockIdx.x == 0) of.listed = of.gathered = of.large = 0;
   }
 }
 
@@ -1287,6 +1368,16 @@ struct PartsKnown {
     sum_all = list_does && c.p < 1.f && !c.k && !whole;
   }
 };
+
+__device__ inline Weights weights_of(const PartsOf& of, const PartArgs& p, const Settings& c,
+                                     const SampleArgs& a) {
+  const int lane = threadIdx.x & 63;
+  Weights wt;
+  wt.max = wave_max<true>(lane < p.parts ? of.top[lane] : -INFINITY);
+  wt.inv_t = 1.f / c.t;
+  wt.scale = a.scale;
+  return wt;
+}
 
 template <class T>
 __global__ __launch_bounds__(kPartThreads) void sample_lists_kernel(const T* __restrict__ S,
@@ -1390,16 +1481,114 @@ __global__ __launch_bounds__(kList) void sample_draw_kernel(const T* __restrict_
                            static_cast<u64>(many), 0u, 0, wt, c, a, col, s);
     return;
   }
-  u64 mass = 0;
-  if (known.sum_all)
-    for (int i = 0; i < p.parts; ++i) mass += of.mass[i];
+  const u64 mass = known.sum_all ? of.total(p.parts) : 0;
   if (known.list_does && of.listed <= kList) {
     const int count = of.listed;
     const u64 entry = static_cast<int>(threadIdx.x) < count ? of.entry[threadIdx.x] : 0;
     if (list_and_draw<kList>(entry, count, mass, wt, c, a, col, s)) return;
   }
+  if (p.large && known.sum_all && NucleusSteps(mass, wt, c, a.m).fit()) {
+    for (int i = threadIdx.x; i < kBins; i += kList) p.of[col].guide[i] = 0;
+    if (threadIdx.x == 0) p.of[col].large = 1;
+    return;
+  }
   __syncthreads();
   search_and_draw<kList>(row, mass, wt, c, a, col, s);
+}
+
+template <class T>
+__global__ __launch_bounds__(kPartThreads) void sample_guide_kernel(const T* __restrict__ S,
+                                                                    SampleArgs a, PartArgs p) {
+  const int64_t col = blockIdx.y;
+  PartsOf& of = p.of[col];
+  if (!of.large) return;
+  __shared__ unsigned guide[kBins];
+  auto column = part_column(S + col * a.lds, a.m, p);
+  const Settings c(a, col);
+  const Weights wt = weights_of(of, p, c, a);
+  const NucleusSteps steps(of.total(p.parts), wt, c, a.m);
+  for (int i = threadIdx.x; i < kBins; i += kPartThreads) guide[i] = 0;
+  __syncthreads();
+  column.each([&](float l, int) {
+    if (l >= steps.low) atomicAdd(&guide[steps.of(l)], steps.weight(l));
+  });
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins; i += kPartThreads)
+    if (guide[i]) atomicAdd(&of.guide[i], guide[i]);
+}
+
+template <class T>
+__global__ __launch_bounds__(kPartThreads) void sample_gather_kernel(const T* __restrict__ S,
+                                                                     SampleArgs a, PartArgs p) {
+  const int64_t col = blockIdx.y;
+  PartsOf& of = p.of[col];
+  if (!of.large) return;
+  __shared__ Shared<kPartThreads> s;
+  __shared__ u64 entries[kList];
+  __shared__ int placed;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  auto column = part_column(S + col * a.lds, a.m, p);
+  const Settings c(a, col);
+  const Weights wt = weights_of(of, p, c, a);
+  const NucleusSteps steps(of.total(p.parts), wt, c, a.m);
+  for (int i = threadIdx.x; i < kBins; i += kPartThreads) s.hist[i] = of.guide[i];
+  if (threadIdx.x == 0) s.count = 0;
+  find_bin(kBins, 0, steps.share, s);
+  const int step = s.found_bin;
+  NucleusSums sums;
+  column.each([&](float l, int i) {
+    sums.add(steps, step, l, wt, c, [&] {
+      const int at = atomicAdd(&s.count, 1);
+      if (at < kList) entries[at] = entry_of(l, i);
+    });
+  });
+  const u64 over = wave_sum(sums.over), sum = wave_sum(sums.sum), many = wave_sum(sums.many);
+  __syncthreads();
+  if (lane == 0) {
+    s.sum[wave] = over;
+    s.sum2[wave] = sum;
+    s.sum3[wave] = many;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    NucleusSums& to = of.sums[blockIdx.x];
+    to.over = total_of(s.sum);
+    to.sum = total_of(s.sum2);
+    to.many = total_of(s.sum3);
+    placed = s.count ? atomicAdd(&of.gathered, s.count) : 0;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < s.count && i < kList; i += kPartThreads)
+    if (placed + i < kList) of.entry[placed + i] = entries[i];
+}
+
+template <class T>
+__global__ __launch_bounds__(kList) void sample_finish_kernel(const T* __restrict__ S,
+                                                              SampleArgs a, PartArgs p) {
+  const int64_t col = blockIdx.x;
+  const PartsOf& of = p.of[col];
+  if (!of.large) return;
+  __shared__ Shared<kList> s;
+  const T* row = S + col * a.lds;
+  const Settings c(a, col);
+  const Weights wt = weights_of(of, p, c, a);
+  const u64 mass = of.total(p.parts);
+  const int i = threadIdx.x, count = of.gathered;
+  if (count <= kList) {
+    u64 above = 0;
+    for (int v = 0; v < p.parts; ++v) above += of.sums[v].over;
+    if (i < kMaxParts) {
+      s.sum2[i] = i < p.parts ? of.sums[i].sum : 0;
+      s.sum3[i] = i < p.parts ? of.sums[i].many : 0;
+    }
+    __syncthreads();
+    const u64 entry = i < count ? of.entry[i] : 0;
+    if (finish_nucleus<kList>(row, entry, count, above, top_p_target(c.p, mass), p.part, wt, c, a,
+                              col, s))
+      return;
+  }
+  __syncthreads();
+  search_and_draw<kList>(row, mass, wt, c, a, col, s, false);
 }
 
 template <class T, int THREADS, int R>
@@ -1419,11 +1608,17 @@ void start_parts(const SampleLaunch& l, const SampleArgs& a) {
   p.of = static_cast<PartsOf*>(l.work);
   p.part = (a.m / kMaxParts + kPartStep) / kPartStep * kPartStep;
   p.parts = (a.m + p.part - 1) / p.part;
+  // A column with a top-k has its nucleus in the list, or none at all.
+  p.large = (a.top_k.each || a.top_k.value == 0) && (a.top_p.each || a.top_p.value < 1.f);
   const T* S = static_cast<const T*>(l.S);
   const dim3 grid(static_cast<unsigned>(p.parts), static_cast<unsigned>(l.n));
   sample_parts_kernel<T><<<grid, kPartThreads, 0, l.stream>>>(S, a, p);
   sample_lists_kernel<T><<<grid, kPartThreads, 0, l.stream>>>(S, a, p);
   sample_draw_kernel<T><<<static_cast<unsigned>(l.n), kList, 0, l.stream>>>(S, a, p);
+  if (!p.large) return;
+  sample_guide_kernel<T><<<grid, kPartThreads, 0, l.stream>>>(S, a, p);
+  sample_gather_kernel<T><<<grid, kPartThreads, 0, l.stream>>>(S, a, p);
+  sample_finish_kernel<T><<<static_cast<unsigned>(l.n), kList, 0, l.stream>>>(S, a, p);
 }
 
 // Columns above 16384 scores go to several workgroups each where one apiece
