@@ -294,6 +294,62 @@ inline std::vector<eval_record> evaluate_kernel(
 }
 
 // ---------------------------------------------------------------------------
+// Answering from a trained model (no counterpart in the reference): scores
+// from 8-bit weights and labels drawn from scores, on host arrays (for
+// device-resident data call the C ABI directly).  All matrices column-major.
+// ---------------------------------------------------------------------------
+
+// The columns of a d x n matrix in 8-bit integers, `ld` apart, and their
+// scales: column i is values[i ld ..] times scales[i].
+struct quantized {
+  std::int64_t d, n, ld;
+  std::vector<std::int8_t> values;
+  std::vector<float> scales;
+};
+
+template <typename Data>
+inline quantized quantize_i8(std::int64_t d, std::int64_t n, const Data* X) {
+  quantized q;
+  q.d = d;
+  q.n = n;
+  q.ld = (d + 15) / 16 * 16;
+  q.values.resize(static_cast<size_t>(q.ld) * static_cast<size_t>(n));
+  q.scales.resize(static_cast<size_t>(n));
+  detail::check(sdca_quantize_i8(detail::dtype<Data>::value, d, n, X, d, q.values.data(), q.ld,
+                                 q.scales.data(), SDCA_HOST_PTR, nullptr));
+  return q;
+}
+
+// The m x n scores of n examples (d x n, quantised within the call).
+template <typename Data>
+inline std::vector<float> scores_i8(std::int64_t n, const Data* X, const quantized& W) {
+  std::vector<float> S(static_cast<size_t>(W.n) * static_cast<size_t>(n));
+  detail::check(sdca_scores_i8(detail::dtype<Data>::value, SDCA_F32, W.d, W.n, n, X, W.d, nullptr,
+                               W.values.data(), W.ld, W.scales.data(), S.data(), W.n,
+                               SDCA_HOST_PTR, nullptr));
+  return S;
+}
+
+inline sdca_sample_params sample_params() {
+  sdca_sample_params p;
+  sdca_sample_params_default(&p);
+  return p;
+}
+
+// A label for each of the n columns of m scores, with n random numbers u in
+// [0, 1); prob (optional): their probabilities after the cuts.
+template <typename Data>
+inline std::vector<std::int64_t> sample(std::int64_t m, std::int64_t n, const Data* S,
+                                        const float* u,
+                                        const sdca_sample_params& params = sample_params(),
+                                        float* prob = nullptr) {
+  std::vector<std::int64_t> labels(static_cast<size_t>(n));
+  detail::check(sdca_sample(detail::dtype<Data>::value, m, n, S, m, u, &params, nullptr,
+                            labels.data(), prob, nullptr, SDCA_HOST_PTR, nullptr));
+  return labels;
+}
+
+// ---------------------------------------------------------------------------
 // evaluate_dataset with the reference's own signature (solver/eval.h:15-51):
 // the same template parameters and arguments, reading the reference's
 // solver_context (ctx.primal_variables, ctx.dual_variables,

@@ -87,3 +87,72 @@ def test_c_entries_refuse():
     assert lib.sdca_sample(0, 4, 2, at, 4, None, None, None, at, None, None, 1, None) == 1
     assert lib.sdca_sample(5, 4, 2, at, 4, at, None, None, at, None, None, 1, None) == 3
     assert lib.sdca_sample(0, 4, 0, None, 4, None, None, None, None, None, None, 1, None) == 0
+
+
+HPP_PROGRAM = r"""
+#include "sdca_hip.hpp"
+#include <cstdio>
+int main() {
+  const int d = 19, m = 7, n = 3;
+  std::vector<float> W(d * m), X(d * n), u(n, 0.5f), prob(n);
+  for (int i = 0; i < d * m; ++i) W[i] = static_cast<float>((i * 37) % 23 - 11);
+  for (int i = 0; i < d * n; ++i) X[i] = static_cast<float>((i * 29) % 17 - 8);
+  const sdca::hip::quantized q = sdca::hip::quantize_i8(d, m, W.data());
+  const std::vector<float> S = sdca::hip::scores_i8(n, X.data(), q);
+  sdca_sample_params p = sdca::hip::sample_params();
+  p.temperature = 100;
+  p.top_k = 3;
+  const std::vector<std::int64_t> label = sdca::hip::sample(m, n, S.data(), u.data(), p, prob.data());
+  for (int i = 0; i < n; ++i) std::printf("%d %.9g\n", static_cast<int>(label[i]), prob[i]);
+  for (float s : S) std::printf("%.9g\n", s);
+  p.top_p = 2;
+  try {
+    sdca::hip::sample(m, n, S.data(), u.data(), p);
+  } catch (const sdca::hip::error& e) {
+    std::printf("refused %d\n", e.status());
+  }
+  return 0;
+}
+"""
+
+
+def build_program(tmp_path):
+    import os
+    import shutil
+    import subprocess
+    import libsdca_amd as sd
+    if shutil.which("g++") is None:
+        pytest.skip("g++ not found")
+    src, exe = tmp_path / "answer.cpp", tmp_path / "answer"
+    src.write_text(HPP_PROGRAM)
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    libdir = os.path.dirname(sd.LIB_PATH)
+    out = subprocess.run(
+        ["g++", "-std=c++11", "-Wall", "-Werror", "-I", os.path.join(root, "include"), str(src), "-o", str(exe),
+         "-L", libdir, "-l:" + os.path.basename(sd.LIB_PATH), "-Wl,-rpath," + libdir, "-Wl,-rpath,/opt/rocm/lib",
+         "-Wl,--allow-shlib-undefined"], capture_output=True, text=True)
+    assert out.returncode == 0, out.stderr
+    return str(exe)
+
+
+def test_cpp_calls_compile(tmp_path):
+    build_program(tmp_path)
+
+
+@pytest.mark.gpu
+def test_cpp_calls_give_what_python_gives(cuda, tmp_path):
+    import subprocess
+    import libsdca_amd as sd
+    run = subprocess.run([build_program(tmp_path)], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0, run.stderr
+    lines = run.stdout.split("\n")
+    d, m, n = 19, 7, 3
+    W = ((np.arange(d * m) * 37) % 23 - 11).astype(np.float32).reshape(m, d)
+    X = ((np.arange(d * n) * 29) % 17 - 8).astype(np.float32).reshape(n, d)
+    S = sd.scores_i8(X, *sd.quantize_i8(W))
+    label, prob = sd.sample(S, np.full(n, 0.5, np.float32), temperature=100.0, top_k=3, prob=True)
+    got = [line.split() for line in lines[:n]]
+    assert [int(a) for a, _ in got] == label.tolist()
+    assert np.array_equal(np.array([b for _, b in got], np.float32), prob)
+    assert np.array_equal(np.array(lines[n:n + m * n], np.float32).reshape(n, m), S)
+    assert lines[n + m * n] == "refused 2"

@@ -79,6 +79,22 @@ def test_quantize_special_columns(cuda, d):
     assert bool(torch.isnan(s).all()) and bool((q == 0).all())
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_quantize_halves(cuda, kind):
+    """Values at and next to halves of a step, where the nearest integer
+    hangs on the last bit of the quotient."""
+    import torch
+    import libsdca_amd as sd
+    for top in (127.0, 1.0, 254.0, 96.0, 0.1875):
+        half = (torch.arange(-127, 127, device=cuda, dtype=torch.float64) + 0.5) * (top / 127)
+        row = torch.cat([torch.tensor([top], device=cuda, dtype=torch.float64), half, half * (1 + 2.0 ** -22),
+                         half * (1 - 2.0 ** -22), half * (1 + 2.0 ** -10)])
+        a = row.to(getattr(torch, kind)).repeat(3, 1)
+        q, s = sd.quantize_i8(a)
+        wq, ws = ref.quantized(_np(a))
+        assert np.array_equal(_np(s), ws) and np.array_equal(_np(q), wq), top
+
+
 # ---------------------------------------------------------------------------
 # scores_i8
 # ---------------------------------------------------------------------------
@@ -219,6 +235,28 @@ def test_sample_settings(cuda, kind, n, m):
         for got, want in zip(sd.sample(_spaced(S, m + 7), u, prob=True, kept=True, **kw), out):
             assert torch.equal(got, want)
         assert torch.equal(sd.sample(S, u, **kw), out[0])
+
+
+@pytest.mark.parametrize("kind,n,m", [("float32", 300, 70_001), ("float16", 300, 70_001), ("bfloat16", 90, 20_000),
+                                      ("float32", 70, 32_769), ("float64", 66, 17_000)])
+def test_sample_many_long_columns(cuda, kind, n, m):
+    """A workgroup to a column that its registers do not hold, or just hold;
+    nuclei of a few labels and of very many."""
+    import torch
+    import libsdca_amd as sd
+    g = _gen(cuda, n + m)
+    S = _logits(g, n, m, cuda, kind)
+    S[: n // 8] = S[: n // 8] / 8  # nearly even
+    for kw in (dict(temperature=0.8, top_k=50, top_p=0.9), dict(top_p=0.95), dict(temperature=1.5, top_p=0.97, min_p=1e-5),
+               dict(min_p=0.01), dict(top_k=900, top_p=0.99)):
+        print(kind, n, m, kw, flush=True)
+        u = torch.rand(n, generator=g, device=cuda)
+        out = sd.sample(S, u, prob=True, kept=True, **kw)
+        _check(S, u, out, **kw)
+        # a few of the columns alone go another way, to the same labels
+        few = sd.sample(S[:9], u[:9], prob=True, kept=True, **kw)
+        for a, b in zip(few, out):
+            assert torch.equal(a, b[:9])
 
 
 @pytest.mark.parametrize("n,m", [(300, 50), (200, 1000), (60, 5000), (12, 40_000)])
