@@ -36,6 +36,7 @@ raises.
 """
 import ctypes
 import os
+import sys
 
 import numpy as np
 
@@ -765,7 +766,7 @@ def _torch_stream(device):
     """torch's current stream on a device, as the C ABI takes it."""
     global _raw_stream
     if _raw_stream is None:
-        import torch
+        torch = sys.modules["torch"]
         # The number alone; a Stream object takes longer to make than a
         # small call to run.
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
@@ -780,7 +781,7 @@ def _answer(x, name, fn, *args):
         return check(fn(*args, HOST_PTR, None))
     if not x.is_cuda:
         raise SdcaError(2, f"{name} takes CUDA tensors or numpy arrays")
-    import torch
+    torch = sys.modules["torch"]
     device = x.get_device()
     if device == torch.cuda.current_device():
         return check(fn(*args, 0, _torch_stream(device)))
@@ -791,7 +792,7 @@ def _answer(x, name, fn, *args):
 def _empty(shape, dtype, like):
     """dtype by its numpy name."""
     if _is_torch(like):
-        import torch
+        torch = sys.modules["torch"]
         return torch.empty(shape, dtype=getattr(torch, dtype), device=like.device)
     return np.empty(shape, dtype=dtype)
 
@@ -822,8 +823,7 @@ def quantize_i8(A, out=None, scales=None):
 
 def _float32(like):
     if _is_torch(like):
-        import torch
-        return torch.float32
+        return sys.modules["torch"].float32
     return np.float32
 
 
@@ -853,8 +853,7 @@ def scores_i8(X, W, w_scales, x_scales=None, out=None, dtype=None):
         _values(x_scales, "x_scales", n, f32, X)
     if out is None:
         if _is_torch(X):
-            import torch
-            out = torch.empty((n, m), dtype=dtype or f32, device=X.device)
+            out = sys.modules["torch"].empty((n, m), dtype=dtype or f32, device=X.device)
         else:
             out = np.empty((n, m), dtype=dtype or f32)
     elif _is_torch(out) != _is_torch(X) or (_is_torch(X) and out.device != X.device):
@@ -873,7 +872,7 @@ def _setting(v, name, n, kind, like):
     if isinstance(v, (float, int)) or not (_is_torch(v) or isinstance(v, (np.ndarray, list, tuple))):
         return None
     if _is_torch(like):
-        import torch
+        torch = sys.modules["torch"]
         v = torch.as_tensor(v, dtype=getattr(torch, kind), device=like.device).contiguous()
     elif _is_torch(v):
         raise SdcaError(2, f"{name}: numpy arrays and torch tensors cannot be mixed in one call")

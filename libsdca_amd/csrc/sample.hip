@@ -1063,6 +1063,21 @@ __device__ inline u64 mass_of(const Weights& wt, const float (&l)[V]) {
   return sum - V * kOne52;
 }
 
+// The fixed weights of those of a group that min-p leaves, and their number.
+template <int V>
+__device__ inline void add_kept(const Weights& wt, float q, const float (&l)[V], u64* mass,
+                                int* count) {
+  u64 sum = 0;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    float w = wt.of(l[e]);
+    w = w >= q ? w : 0.f;
+    sum += wt.raw(w);
+    *count += w > 0.f;
+  }
+  *mass += sum - V * kOne52;
+}
+
 // Appends the scores of a group that are at least `from` to a list in LDS
 // (it counts those beyond its room too).  Most groups have none.
 template <int V>
@@ -1192,11 +1207,9 @@ __global__ __launch_bounds__(THREADS, 4) void sample_block_kernel(const T* __res
     // goes through it group by group.
     u64 mass = 0;
     int count = 0;
-    column.each([&](float l, int) {
-      const float w = wt.of(l);
-      const bool in = w >= c.q && w > 0.f;
-      mass += in ? wt.fixed(w) : 0;
-      count += in;
+    column.groups_until([&](const float (&l)[Col::V], int) {
+      add_kept(wt, c.q, l, &mass, &count);
+      return true;
     });
     mass = wave_sum(mass);
     count = wave_sum(count);
@@ -1357,6 +1370,7 @@ __global__ __launch_bounds__(kPartThreads) void sample_parts_kernel(const T* __r
 struct PartsKnown {
   float max, bound, floor_live;
   bool list_does, whole, sum_all;
+  PartsKnown() = default;
   __device__ PartsKnown(const PartsOf& of, const PartArgs& p, const Settings& c, int units) {
     const int lane = threadIdx.x & 63;
     max = wave_max<true>(lane < p.parts ? of.top[lane] : -INFINITY);
@@ -1389,14 +1403,19 @@ __global__ __launch_bounds__(kPartThreads) void sample_lists_kernel(const T* __r
   PartsOf& of = p.of[col];
   const Settings c(a, col);
   auto column = part_column(S + col * a.lds, a.m, p);
-  const PartsKnown known(of, p, c, full_units<decltype(column)::V>(a.m, p));
+  __shared__ PartsKnown shared_known;
+  if (wave == 0) {
+    const PartsKnown k(of, p, c, full_units<decltype(column)::V>(a.m, p));
+    if (lane == 0) shared_known = k;
+  }
+  if (threadIdx.x == 0) counted = 0;
+  __syncthreads();
+  const PartsKnown known = shared_known;
   if (known.max == -INFINITY || (c.cut && !known.list_does && !c.greedy)) return;
   Weights wt;
   wt.max = known.max;
   wt.inv_t = 1.f / c.t;
   wt.scale = a.scale;
-  if (threadIdx.x == 0) counted = 0;
-  __syncthreads();
 
   const bool mine = of.top[blockIdx.x] == known.max;  // the column's maximum is in this part
   u64 mass = 0;
@@ -1407,11 +1426,9 @@ __global__ __launch_bounds__(kPartThreads) void sample_lists_kernel(const T* __r
 #pragma unroll
     for (int d = 32; d; d >>= 1) number = min(number, __shfl_xor(number, d));
   } else if (!c.cut) {
-    column.each([&](float l, int) {
-      const float w = wt.of(l);
-      const bool in = w >= c.q && w > 0.f;
-      mass += in ? wt.fixed(w) : 0;
-      number += in;
+    column.groups_until([&](const float (&l)[decltype(column)::V], int) {
+      add_kept(wt, c.q, l, &mass, &number);
+      return true;
     });
     number = wave_sum(number);
   } else {
@@ -1621,11 +1638,12 @@ void start_parts(const SampleLaunch& l, const SampleArgs& a) {
   sample_finish_kernel<T><<<static_cast<unsigned>(l.n), kList, 0, l.stream>>>(S, a, p);
 }
 
-// Columns above 16384 scores go to several workgroups each where one apiece
-// leaves compute units idle.  Measured, one workgroup against several: top-k
-// of 32000 floats 22 against 16 us for one column, 26 against 19 for 64, 33
-// against 34 for 256; of 128000 25 against 18, 35 against 25, 51 against 56.
-bool in_parts(int64_t m, int64_t n) { return m > 16384 && n <= (m > 65536 ? 256 : 64); }
+// Columns that one workgroup's registers do not hold go to several workgroups
+// each where one apiece leaves compute units idle.  Measured, one workgroup
+// against several: a top-k of 65537 floats 20 against 17 us for one column,
+// 32 against 41 for 256; of 128000 25 against 18, 35 against 25 for 64, 51
+// against 56 for 256; of 32000 18 against 18 (and two launches less).
+bool in_parts(int64_t m, int64_t n) { return m > 32768 && n <= (m > 65536 ? 256 : 64); }
 
 template <class T>
 hipError_t sample(const SampleLaunch& l) {
