@@ -59,9 +59,11 @@ __device__ inline TileAt tile_of(int id, int tiles_n, int tiles_m) {
 
 // A workgroup computes BN examples by BM classes; its WN x WM waves each a
 // (BN / WN) x (BM / WM) part in 16 x 16 x 64 matrix instructions.  Classes
-// are the instruction's rows and examples its columns; an instruction's rows
-// are classes 4 FM apart in fours, so that a lane ends with 4 FM neighbouring
-// scores of an example and stores them whole.
+// are the instruction's rows and examples its columns, so a lane ends with
+// four neighbouring scores of an example (for a 16-bit type eight: two
+// instructions, Q = 2, take their classes in turn, four and four).  The wave
+// turns 16 examples at a time round in LDS, so that its stores take the
+// scores of an example in a row: 16 FM of them, at any address.
 //
 // K goes by in tiles of 128 bytes, STAGES of them in LDS.  A tile row holds its
 // eight 16-byte pieces in the order piece ^ f(row): the rows that an
@@ -80,7 +82,8 @@ __global__ __launch_bounds__(64 * WN * WM) void scores_i8_kernel(
   constexpr int kRows = BN + BM;              // tile rows, the examples' first
   constexpr int kLoads = kRows / 8 / kWaves;  // of a wave: 8 rows each
   constexpr int FN = BN / WN / 16, FM = BM / WM / 16;
-  static_assert(kRows % (8 * kWaves) == 0 && BN % 8 == 0, "tile rows per wave");
+  constexpr int Q = 4 / static_cast<int>(sizeof(Out));
+  static_assert(kRows % (8 * kWaves) == 0 && BN % 8 == 0 && FM % Q == 0, "tile rows per wave");
   __shared__ __align__(128) int8_t tile[STAGES][kRows * kTileK];
 
   const int lane = threadIdx.x & 63;
@@ -93,7 +96,7 @@ __global__ __launch_bounds__(64 * WN * WM) void scores_i8_kernel(
   const __amdgpu_buffer_rsrc_t wb = rows_buffer(W, ldw, m0, m, d);
 
   const auto order = [](int row) {
-    return row < BN ? row & 7 : (row & 3) | (((row - BN) / (4 * FM) & 1) << 2);
+    return row < BN || Q == 1 ? row & 7 : (row & 3) | ((row >> 3 & 1) << 2);
   };
   int from[kLoads];
 #pragma unroll
@@ -112,7 +115,7 @@ __global__ __launch_bounds__(64 * WN * WM) void scores_i8_kernel(
   };
   // The lane's first pieces in a tile; its other rows lie at fixed distances
   // (they have the same f), and those of the second half tile at ^ 64.
-  const int row_a = BN + wm * (16 * FM) + ((lane & 15) >> 2) * (4 * FM) + (lane & 3);
+  const int row_a = BN + wm * (16 * FM) + ((lane & 15) >> 2) * (4 * Q) + (lane & 3);
   const int row_b = wn * (16 * FN) + (lane & 15);
   const int at_a = row_a * kTileK + ((lane / 16) ^ order(row_a)) * 16;
   const int at_b = row_b * kTileK + ((lane / 16) ^ order(row_b)) * 16;
@@ -122,7 +125,7 @@ __global__ __launch_bounds__(64 * WN * WM) void scores_i8_kernel(
   const auto read = [&](int stage, int h) {
 #pragma unroll
     for (int i = 0; i < FM; ++i)
-      a[h][i] = *reinterpret_cast<const v4i*>(&tile[stage][(at_a ^ (h * 64)) + i * 4 * kTileK]);
+      a[h][i] = *reinterpret_cast<const v4i*>(&tile[stage][(at_a ^ (h * 64)) + (i / Q * 16 * Q + i % Q * 4) * kTileK]);
 #pragma unroll
     for (int j = 0; j < FN; ++j)
       b[h][j] = *reinterpret_cast<const v4i*>(&tile[stage][(at_b ^ (h * 64)) + j * 16 * kTileK]);
@@ -170,30 +173,50 @@ __global__ __launch_bounds__(64 * WN * WM) void scores_i8_kernel(
     multiply(1);
     __builtin_amdgcn_sched_barrier(0);
   }
-  // No load into LDS is left when the workgroup ends.
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();  // no load into LDS is left, and no read of it
 
-  const int64_t at = m0 + wm * (16 * FM) + (lane / 16) * (4 * FM);
-  float scale[4 * FM];
+  constexpr int kUnit = 16 / static_cast<int>(sizeof(Out));  // scores in 16 bytes
+  constexpr int kPitch = 16 * FM + kUnit;                    // other banks for each row
+  constexpr int kAcross = 16 * FM / kUnit;                   // lanes along an example
+  static_assert(kWaves * 16 * kPitch * sizeof(Out) <= sizeof(tile), "room to turn");
+  Out* turn = reinterpret_cast<Out*>(&tile[0][0]) + wave * 16 * kPitch;
+  const int first = static_cast<int>(m0) + wm * (16 * FM);
+  const int mine = lane / 16 * kUnit;  // this lane's first score of 16 Q
+  float scale[FM / Q][kUnit];
 #pragma unroll
-  for (int e = 0; e < 4 * FM; ++e) scale[e] = sw[min(static_cast<int>(at) + e, m - 1)];
+  for (int g = 0; g < FM / Q; ++g)
+#pragma unroll
+    for (int e = 0; e < kUnit; ++e) scale[g][e] = sw[min(first + g * 16 * Q + mine + e, m - 1)];
 #pragma unroll
   for (int j = 0; j < FN; ++j) {
-    const int64_t row = n0 + (wn * FN + j) * 16 + (lane & 15);
-    if (row >= n) continue;
-    const float s = sx[row];
-    Out* out = S + row * lds + at;
-    Out v[4 * FM];
+    const int64_t rows = n0 + (wn * FN + j) * 16;
+    const float s = sx[min(rows + (lane & 15), static_cast<int64_t>(n - 1))];
 #pragma unroll
-    for (int e = 0; e < 4 * FM; ++e)
-      v[e] = from_float<Out>(static_cast<float>(acc[e / 4][j][e % 4]) * s * scale[e]);
-    if (at + 4 * FM <= m) {
-      __builtin_memcpy(out, v, sizeof(v));
-    } else {
+    for (int g = 0; g < FM / Q; ++g) {
+      Out v[kUnit];
 #pragma unroll
-      for (int e = 0; e < 4 * FM; ++e)
-        if (at + e < m) out[e] = v[e];
+      for (int e = 0; e < kUnit; ++e)
+        v[e] = from_float<Out>(static_cast<float>(acc[g * Q + e / 4][j][e % 4]) * s * scale[g][e]);
+      __builtin_memcpy(__builtin_assume_aligned(turn + (lane & 15) * kPitch + g * 16 * Q + mine, 16),
+                       v, 16);
     }
+    wave_lds_sync();
+#pragma unroll
+    for (int r = 0; r < 16; r += 64 / kAcross) {
+      const int row = r + lane / kAcross, along = lane % kAcross * kUnit;
+      Out v[kUnit];
+      __builtin_memcpy(v, __builtin_assume_aligned(turn + row * kPitch + along, 16), 16);
+      if (rows + row >= n) continue;
+      Out* out = S + (rows + row) * lds + first + along;
+      if (first + along + kUnit <= m) {
+        __builtin_memcpy(out, v, 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kUnit; ++e)
+          if (first + along + e < m) out[e] = v[e];
+      }
+    }
+    wave_lds_sync();
   }
 }
 
