@@ -156,6 +156,38 @@ __device__ inline K sort_wave(K v, bool falling) {
   return sort_merge<32, VALU>(v, falling);
 }
 
+// 64 R values, the i-th in lane i % 64's v[i / 64], falling: within each
+// register as above, and between registers without an exchange.
+template <int SIZE, int STRIDE, int R, class K>
+__device__ inline void sort_registers(K (&v)[R]) {
+  if constexpr (STRIDE > 0) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (r & STRIDE) continue;
+      const K a = v[r], b = v[r + STRIDE];
+      const bool swap = (b > a) == ((r & SIZE) == 0);
+      v[r] = swap ? b : a;
+      v[r + STRIDE] = swap ? a : b;
+    }
+    sort_registers<SIZE, STRIDE / 2>(v);
+  }
+}
+template <bool VALU, int SIZE, int R, class K>
+__device__ inline void merge_registers(K (&v)[R]) {
+  if constexpr (SIZE <= R) {
+    sort_registers<SIZE, SIZE / 2>(v);
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r] = sort_merge<32, VALU>(v[r], (r & SIZE) == 0);
+    merge_registers<VALU, SIZE * 2>(v);
+  }
+}
+template <bool VALU, int R, class K>
+__device__ inline void sort_wave(K (&v)[R]) {
+#pragma unroll
+  for (int r = 0; r < R; ++r) v[r] = sort_wave<VALU>(v[r], (r & 1) == 0);
+  merge_registers<VALU, 2>(v);
+}
+
 // ---------------------------------------------------------------------------
 // Settings and results of a column.
 // ---------------------------------------------------------------------------
@@ -355,9 +387,81 @@ __device__ inline void wave_draw(const float (&l)[E], const Weights& wt, const S
   }
 }
 
+constexpr int kWaveList = 256;
+
+template <int E>
+__device__ inline int count_at_least(const float (&l)[E], float b) {
+  int n = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) n += __popcll(__ballot(l[e] >= b));
+  return n;
+}
+
+
+// The cuts and the draw from a list of `count` (at most 64 R) entries by
+// rising index.  mass: of all labels, or 0 for that of the list after its
+// top-k; the list holds the nucleus.
+template <int R>
+__device__ inline void wave_list_draw(const u64* list, int count, u64 mass, const Weights& wt,
+                                      const Settings& c, const SampleArgs& a, int64_t col) {
+  const int lane = threadIdx.x & 63;
+  u64 mine[R], entry[R], incl[R];
+  bool keep[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    mine[r] = 64 * r + lane < count ? list[64 * r + lane] : 0;
+    entry[r] = mine[r];
+  }
+  sort_wave<false>(entry);
+  const int first = c.k && c.k < count ? c.k : count;
+  u64 all = 0;
+  float w[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const bool in = 64 * r + lane < first;
+    w[r] = in ? wt.of(score_of(static_cast<unsigned>(entry[r] >> 32))) : 0.f;
+    incl[r] = wave_scan(in ? wt.fixed(w[r]) : 0) + all;
+    all = read_lane64(incl[r], 63);
+    keep[r] = w[r] >= c.q && w[r] > 0.f;
+  }
+  if (c.p < 1.f) {
+    const u64 target = top_p_target(c.p, mass ? mass : all);
+#pragma unroll
+    for (int r = 0; r < R; ++r) keep[r] = keep[r] && incl[r] - wt.fixed(w[r]) < target;
+  }
+  // The kept labels are a prefix; the last of them bounds them in the list by
+  // index.
+  int many = 0;
+  u64 last = 0, total = 0;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const u64 kept = __ballot(keep[r]);
+    const int n = many == 64 * r ? (~kept ? __ffsll(~kept) - 1 : 64) : 0;
+    if (n) {
+      last = read_lane64(entry[r], n - 1);
+      total = read_lane64(incl[r], n - 1);
+      many += n;
+    }
+  }
+  const u64 target = draw_target(a.u[col], total);
+  u64 base = 0;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float wm = wt.of(score_of(static_cast<unsigned>(mine[r] >> 32)));
+    const u64 sum = wave_scan(mine[r] >= last ? wt.fixed(wm) : 0) + base;
+    const u64 passed = __ballot(sum > target);
+    if (passed) {
+      if (lane == __ffsll(passed) - 1)
+        answer(a, col, index_of(mine[r]), share(wm, wt.scale, total), many);
+      return;
+    }
+    base = read_lane64(sum, 63);
+  }
+}
+
 template <class T, int E>
-__global__ __launch_bounds__(256) void sample_wave_kernel(const T* __restrict__ S, SampleArgs a) {
-  __shared__ u64 lists[4][64];
+__global__ __launch_bounds__(256, E <= 16 ? 5 : 3) void sample_wave_kernel(const T* __restrict__ S, SampleArgs a) {
+  __shared__ u64 lists[4][kWaveList];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t col = static_cast<int64_t>(blockIdx.x) * 4 + wave;
@@ -405,78 +509,87 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const T* __restrict__ 
     return;
   }
 
-  // The bound: the k-th largest lane maximum, or for top-p alone the 32nd,
-  // which a list of 64 mostly holds (44 of 1000 scores on average).
-  const bool list_does = c.k <= 64;
-  const float floor_live = live_floor(wt.max, c.t);
-  int count = 65;
-  float bound = 0.f;
-  u64* list = lists[wave];
-  if (list_does) {
-    const float sorted = sort_wave<false>(most, true);
-    bound = read_lane(sorted, c.k ? c.k - 1 : 31);
-    const float from = fmaxf(bound, floor_live);
-    count = 0;
+  // A bound with few enough scores at or above it for a list, and enough of
+  // them for the cut: `count` of them.
+  // (Scores of weight 0 need not be in it; nor are those at -infinity.)
+  const float floor_live = fmaxf(live_floor(wt.max, c.t), -3.402823466e38f);
+  const float sorted = sort_wave<false>(most, true);
+  float from = floor_live;
+  int count = 0;
+  u64 mass = 0;  // of all labels, where the list is not the whole of them
+  if (c.k) {
+    // The k-th largest lane maximum has k scores or more.  Where that is no
+    // bound, or one with too many, halving the keys' interval finds one.
+    if (c.k <= 64) from = fmaxf(read_lane(sorted, c.k - 1), floor_live);
+    count = count_at_least(l, from);
+    if (count > kWaveList && c.k <= kWaveList) {
+      unsigned low = key_of(from), high = key_of(wt.max) + 1;
+      while (count > kWaveList && high - low > 1) {
+        const unsigned mid = low + (high - low) / 2;
+        const int n = count_at_least(l, score_of(mid));
+        if (n < c.k) {
+          high = mid;
+        } else {
+          low = mid;
+          count = n;
+        }
+      }
+      from = score_of(low);
+    }
+  } else {
+    // A nucleus: bounds that leave some 44, 97 and 200 of 1000 scores, the
+    // first whose scores hold the mass.
+    float w[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      w[e] = wt.of(l[e]);
+      mass += wt.raw(w[e]);
+    }
+    mass = wave_sum(mass - E * kOne52);
+    const u64 target = top_p_target(c.p, mass);
+    for (int t = 0; t < 3; ++t) {
+      const float bound = read_lane(sorted, t == 0 ? 31 : t == 1 ? 49 : 61);
+      from = fmaxf(bound, floor_live);
+      u64 sum = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum += wt.raw(l[e] >= from ? w[e] : 0.f);
+      count = kWaveList + 1;
+      if (wave_sum(sum - E * kOne52) >= target) {
+        count = count_at_least(l, from);
+        break;
+      }
+    }
+  }
+  if (count <= kWaveList) {
+    u64* list = lists[wave];
+    int placed = 0;
 #pragma unroll
     for (int g = 0; g < E / 4; ++g) {
       bool in[4];
       u64 mask[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        in[e] = l[4 * g + e] >= from && l[4 * g + e] > -INFINITY;
+        in[e] = l[4 * g + e] >= from;
         mask[e] = __ballot(in[e]);
       }
       if ((mask[0] | mask[1] | mask[2] | mask[3]) == 0) continue;
-      int at = count;  // by rising index: the lanes before, then the lane's own before
+      int at = placed;  // by rising index: the lanes before, then the lane's own before
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         at = __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask[e] >> 32),
                                        __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask[e]), at));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (in[e] && at < 64) list[at] = entry_of(l[4 * g + e], 256 * g + 4 * lane + e);
+        if (in[e]) list[at] = entry_of(l[4 * g + e], 256 * g + 4 * lane + e);
         at += in[e];
-        count += __popcll(mask[e]);
+        placed += __popcll(mask[e]);
       }
     }
-  }
-  bool found = count <= 64;
-  if (found) {
     wave_lds_sync();
-    const u64 mine = lane < count ? list[lane] : 0;
-    const u64 entry = sort_wave<false>(mine, true);
-    const float w = lane < count ? wt.of(score_of(static_cast<unsigned>(entry >> 32))) : 0.f;
-    const u64 f = lane < count ? wt.fixed(w) : 0;
-    const u64 incl = wave_scan(f);
-    const int first = c.k && c.k < count ? c.k : count;
-    bool keep = lane < first && w >= c.q && w > 0.f;
-    if (c.p < 1.f) {
-      const bool whole = bound <= floor_live;  // the list holds every label of nonzero weight
-      u64 mass;
-      if (c.k || whole) {
-        mass = read_lane64(incl, first - 1);
-      } else {
-        mass = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) mass += wt.raw(wt.of(l[e]));
-        mass = wave_sum(mass - E * kOne52);
-      }
-      const u64 target = top_p_target(c.p, mass);
-      keep = keep && incl - f < target;
-      found = c.k || whole || read_lane64(incl, 63) >= target;
-    }
-    if (found) {
-      const u64 kept = __ballot(keep);  // a prefix
-      const int many = ~kept ? __ffsll(~kept) - 1 : 64;
-      const u64 last = read_lane64(entry, many - 1);
-      const u64 total = read_lane64(incl, many - 1);
-      const float wm = wt.of(score_of(static_cast<unsigned>(mine >> 32)));
-      const u64 sum = wave_scan(mine >= last ? wt.fixed(wm) : 0);
-      const u64 passed = __ballot(sum > draw_target(a.u[col], total));
-      if (lane == __ffsll(passed) - 1)
-        answer(a, col, index_of(mine), share(wm, wt.scale, total), many);
-      return;
-    }
+    if (count <= 64) wave_list_draw<1>(list, count, mass, wt, c, a, col);
+    else if (count <= 128) wave_list_draw<2>(list, count, mass, wt, c, a, col);
+    else wave_list_draw<4>(list, count, mass, wt, c, a, col);
+    return;
   }
   unsigned tau;
   int ties;
@@ -1669,6 +1782,7 @@ hipError_t sample(const SampleLaunch& l) {
   if (in_parts(l.m, l.n)) start_parts<T>(l, a);
   else if (l.m <= 256) start_wave<T, 4>(l, a);
   else if (l.m <= 1024) start_wave<T, 16>(l, a);
+  else if (l.m <= 2048) start_wave<T, 32>(l, a);
   else if (l.m <= 256 * 16) start_block<T, 256, 16>(l, a);
   else if (l.m <= 1024 * 16) start_block<T, 1024, 16>(l, a);
   else start_block<T, 1024, 0>(l, a);
