@@ -34,11 +34,11 @@ constexpr int64_t kI8TileK = 128;
 
 // S_ij = (sum_k X_ik W_jk) sx_i sw_j.
 struct ScoresI8Launch {
-  int data;  // X's type: SDCA_I8, or where scores_i8_few holds any of the quantiser's
+  int data;  // X's type: SDCA_I8, or where scores_i8_quantises holds any of the quantiser's
   int out;   // SDCA_F32, F16, BF16
   int64_t d, m, n;
   // n rows, pitch ldx.  Int8 rows have zeros from d up to a multiple of
-  // kI8TileK and 16-byte addresses, but for scores_i8_few.
+  // kI8TileK and 16-byte addresses, but where scores_i8_quantises holds.
   const void* X;
   int64_t ldx;
   const float* sx;
@@ -50,7 +50,7 @@ struct ScoresI8Launch {
   hipStream_t stream;
 };
 // Whether X is taken as the caller has it, quantised on the way.
-bool scores_i8_few(int64_t n, int64_t d);
+bool scores_i8_quantises(int data, int64_t d, int64_t m, int64_t n);
 hipError_t launch_scores_i8(const ScoresI8Launch& a);
 
 // One setting of the draw: a value for all columns, or one per column.

@@ -35,6 +35,31 @@ __device__ inline void load_vec(const T* row, int64_t at, int64_t len, float (&v
   }
 }
 
+// Eight values of a column of d for its quantiser: those from `at` on, or the
+// last eight where the column ends before at + 8: one load whatever d (20011
+// columns of 513 half-precision values 12 us, with a load for each value of
+// the end 13.5).
+template <class T>
+__device__ inline void load_column(const T* x, int64_t at, int64_t d, T (&raw)[8]) {
+  if (d >= 8) {
+    __builtin_memcpy(raw, x + (at + 8 <= d ? at : d - 8), sizeof(raw));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) raw[e] = at + e < d ? x[at + e] : T(0.f);
+  }
+}
+
+// The bytes that load_column's values at `at` were quantised to, from `at` on,
+// zeros from d on.
+__device__ inline void end_column(int64_t at, int64_t d, unsigned (&w)[2]) {
+  if (d < 8 || at + 8 <= d) return;
+  const int64_t more = at + 8 - d;  // bytes of values before `at`, or beyond d
+  uint64_t b;
+  __builtin_memcpy(&b, w, 8);
+  b = more < 8 ? b >> (8 * more) : 0;
+  __builtin_memcpy(w, &b, 8);
+}
+
 // |x| as an integer: the order of the bit patterns is that of the values,
 // with infinity and the NaNs on top, so one integer maximum finds both the
 // largest magnitude and a non-finite value.

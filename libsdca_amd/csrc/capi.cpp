@@ -1304,14 +1304,13 @@ int scores_i8_common(int data, int out, int64_t d, int64_t m, int64_t n, const v
   a.ldw = ldw;
 
   // W is read in place when its columns are aligned, and X when its columns
-  // are whole tiles besides, or few; the kernels' offsets within a tile of
+  // are whole tiles besides, or quantised by the kernel; the kernels' offsets within a tile of
   // columns are 32-bit.  What is not goes to scratch first.
   const auto in_place = [](const void* p, int64_t ld) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0 && ld <= (1 << 22);
   };
   const int64_t pad = (d + kI8TileK - 1) / kI8TileK * kI8TileK;
-  const bool few = scores_i8_few(n, d);
-  const bool own_x = !few && (data != SDCA_I8 || d != pad || !in_place(a.X, ldx));
+  const bool own_x = !scores_i8_quantises(data, d, m, n) && (data != SDCA_I8 || d != pad || !in_place(a.X, ldx));
   const bool own_w = !in_place(a.W, ldw);
   const size_t x_bytes = own_x ? static_cast<size_t>(n) * pad : 0;
   const size_t s_bytes = own_x && data != SDCA_I8 ? (n * sizeof(float) + 255) / 256 * 256 : 0;

@@ -10,6 +10,14 @@ namespace {
 
 constexpr int kVec = 8;  // values a lane takes at a time: 16 bytes of a 16-bit type, 8 of q
 
+template <class T>
+__device__ inline void load_values(const T* x, int64_t at, int64_t d, float (&v)[kVec]) {
+  T raw[kVec];
+  load_column(x, at, d, raw);
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) v[e] = to_float(raw[e]);
+}
+
 // TPC threads share a column and keep it in registers (G vectors of 8 values
 // each), so that it is read once; LOOP: a longer column is read twice.
 template <class T, int TPC, int G, bool LOOP>
@@ -21,7 +29,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ X, 
   __shared__ unsigned part[4];
   const int t = threadIdx.x % TPC;
   const int64_t col = static_cast<int64_t>(blockIdx.x) * kColumns + threadIdx.x / TPC;
-  if (TPC == 64 && col >= n) return;  // a whole wave, and no barrier below
+  if (TPC <= 64 && col >= n) return;  // whole columns, and no barrier below
   const T* x = X + col * ldx;
   int8_t* q = Q + col * ldq;
 
@@ -31,7 +39,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ X, 
   for (int64_t sweep = 0; sweep < sweeps; ++sweep) {
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      load_vec<kVec>(x, (sweep * G + g) * TPC * kVec + int64_t(t) * kVec, d, v[g]);
+      load_values(x, (sweep * G + g) * TPC * kVec + int64_t(t) * kVec, d, v[g]);
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
         const unsigned b = magnitude(v[g][e]);
@@ -40,7 +48,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ X, 
     }
   }
 #pragma unroll
-  for (int off = 32; off; off >>= 1) {
+  for (int off = TPC < 64 ? TPC / 2 : 32; off; off >>= 1) {
     const unsigned o = __shfl_xor(most, off);
     most = o > most ? o : most;
   }
@@ -57,10 +65,11 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ X, 
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       const int64_t at = (sweep * G + g) * TPC * kVec + int64_t(t) * kVec;
-      if (LOOP) load_vec<kVec>(x, at, d, v[g]);
+      if (LOOP) load_values(x, at, d, v[g]);
       if (at >= pad) continue;
       unsigned w[2];
       quantize8(v[g], s, w);
+      end_column(at, d, w);
       if (at + kVec <= pad) {
         __builtin_memcpy(q + at, w, kVec);
       } else {
@@ -80,10 +89,14 @@ void start(const QuantLaunch& a) {
 
 template <class T>
 hipError_t quantize(const QuantLaunch& a) {
-  // By the column's length alone: a wave for a short column, a workgroup
-  // above, with as few registers as hold it.
-  if (a.pad <= 64 * kVec) start<T, 64, 1, false>(a);
-  else if (a.pad <= 64 * 2 * kVec) start<T, 64, 2, false>(a);
+  // By the column's length alone: part of a wave for a short column, so that
+  // a wave has some KiB to read (200000 columns of 128 floats took 69 us with
+  // a wave each, 21 with a quarter; of 512 half-precision values 81 and 51),
+  // a workgroup above, with as few registers as hold it.
+  if (a.pad <= 16 * kVec) start<T, 16, 1, false>(a);
+  else if (a.pad <= 16 * 2 * kVec) start<T, 16, 2, false>(a);
+  else if (a.pad <= 16 * 4 * kVec) start<T, 16, 4, false>(a);
+  else if (a.pad <= 32 * 4 * kVec) start<T, 32, 4, false>(a);
   else if (a.pad <= 256 * 2 * kVec) start<T, 256, 2, false>(a);
   else if (a.pad <= 256 * 6 * kVec) start<T, 256, 6, false>(a);
   else start<T, 256, 6, true>(a);

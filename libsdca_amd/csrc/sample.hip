@@ -460,7 +460,8 @@ __device__ inline void wave_list_draw(const u64* list, int count, u64 mass, cons
 }
 
 template <class T, int E>
-__global__ __launch_bounds__(256, E <= 16 ? 5 : 3) void sample_wave_kernel(const T* __restrict__ S, SampleArgs a) {
+__global__ __launch_bounds__(256, E <= 16 ? 5 : 3) void sample_wave_kernel(
+    const T* __restrict__ S, SampleArgs a) {
   __shared__ u64 lists[4][kWaveList];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1775,10 +1776,12 @@ hipError_t sample(const SampleLaunch& l) {
   int bits = 0;
   while ((int64_t(1) << bits) < l.m) ++bits;
   a.scale = static_cast<double>(u64(1) << (62 - bits < 46 ? 62 - bits : 46));
-  // Else by the column's length: a wave up to 1024 scores, a workgroup that
-  // holds the column in registers above, 16 scores to a thread, and one that
-  // reads it twice from there on.  (32 to a thread spill: a top-k of 32000
-  // floats took 18 us, against 14 read twice; 12000 take 11 held, 12 read.)
+  // Else by the column's length: a wave up to 2048 scores (8000 columns of
+  // 2000: 31 us with a top-k, 110 by a workgroup; one column 7.4 and 9.3), a
+  // workgroup that holds the column in registers above, 16 scores to a
+  // thread, and one that reads it twice from there on.  (32 to a thread spill:
+  // a top-k of 32000 floats took 18 us, against 14 read twice; 12000 take 11
+  // held, 12 read.)
   if (in_parts(l.m, l.n)) start_parts<T>(l, a);
   else if (l.m <= 256) start_wave<T, 4>(l, a);
   else if (l.m <= 1024) start_wave<T, 16>(l, a);

@@ -57,6 +57,63 @@ __device__ inline TileAt tile_of(int id, int tiles_n, int tiles_m) {
   return {group * kGroup + in % high, in / high};
 }
 
+// A wave's scores to memory: 16 examples at a time are turned round in LDS,
+// so that stores take the scores of an example in a row, 16 FM of them, at
+// any address.  acc[i][j] holds four neighbouring scores of a lane's example;
+// for a 16-bit type two of them (Q) take their classes in turn, four and four.
+template <class Out, int FM>
+struct Turned {
+  static constexpr int Q = 4 / static_cast<int>(sizeof(Out));
+  static constexpr int kUnit = 16 / static_cast<int>(sizeof(Out));  // scores in 16 bytes
+  static constexpr int kPitch = 16 * FM + kUnit;                    // other banks for each row
+  static constexpr int kAcross = 16 * FM / kUnit;                   // lanes along an example
+  static constexpr int kSize = 16 * kPitch;
+  static_assert(FM % Q == 0, "whole units");
+
+  // x_scale(row) is the scale of example rows + row.
+  template <int FN, class XScale>
+  static __device__ inline void store(const v4i (&acc)[FM][FN], Out* turn, XScale x_scale,
+                                      const float* sw, Out* S, int64_t lds, int64_t rows,
+                                      int first, int m, int64_t n, int lane) {
+    const int mine = lane / 16 * kUnit;  // this lane's first score of 16 Q
+    float scale[FM / Q][kUnit];
+#pragma unroll
+    for (int g = 0; g < FM / Q; ++g)
+#pragma unroll
+      for (int e = 0; e < kUnit; ++e) scale[g][e] = sw[min(first + g * 16 * Q + mine + e, m - 1)];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const float s = x_scale(j * 16 + (lane & 15));
+#pragma unroll
+      for (int g = 0; g < FM / Q; ++g) {
+        Out v[kUnit];
+#pragma unroll
+        for (int e = 0; e < kUnit; ++e)
+          v[e] = from_float<Out>(static_cast<float>(acc[g * Q + e / 4][j][e % 4]) * s * scale[g][e]);
+        __builtin_memcpy(__builtin_assume_aligned(turn + (lane & 15) * kPitch + g * 16 * Q + mine, 16),
+                         v, 16);
+      }
+      wave_lds_sync();
+#pragma unroll
+      for (int r = 0; r < 16; r += 64 / kAcross) {
+        const int row = r + lane / kAcross, along = lane % kAcross * kUnit;
+        Out v[kUnit];
+        __builtin_memcpy(v, __builtin_assume_aligned(turn + row * kPitch + along, 16), 16);
+        if (rows + j * 16 + row >= n) continue;
+        Out* out = S + (rows + j * 16 + row) * lds + first + along;
+        if (first + along + kUnit <= m) {
+          __builtin_memcpy(out, v, 16);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kUnit; ++e)
+            if (first + along + e < m) out[e] = v[e];
+        }
+      }
+      wave_lds_sync();
+    }
+  }
+};
+
 // A workgroup computes BN examples by BM classes; its WN x WM waves each a
 // (BN / WN) x (BM / WM) part in 16 x 16 x 64 matrix instructions.  Classes
 // are the instruction's rows and examples its columns, so a lane ends with
@@ -175,49 +232,12 @@ __global__ __launch_bounds__(64 * WN * WM) void scores_i8_kernel(
   }
   __syncthreads();  // no load into LDS is left, and no read of it
 
-  constexpr int kUnit = 16 / static_cast<int>(sizeof(Out));  // scores in 16 bytes
-  constexpr int kPitch = 16 * FM + kUnit;                    // other banks for each row
-  constexpr int kAcross = 16 * FM / kUnit;                   // lanes along an example
-  static_assert(kWaves * 16 * kPitch * sizeof(Out) <= sizeof(tile), "room to turn");
-  Out* turn = reinterpret_cast<Out*>(&tile[0][0]) + wave * 16 * kPitch;
-  const int first = static_cast<int>(m0) + wm * (16 * FM);
-  const int mine = lane / 16 * kUnit;  // this lane's first score of 16 Q
-  float scale[FM / Q][kUnit];
-#pragma unroll
-  for (int g = 0; g < FM / Q; ++g)
-#pragma unroll
-    for (int e = 0; e < kUnit; ++e) scale[g][e] = sw[min(first + g * 16 * Q + mine + e, m - 1)];
-#pragma unroll
-  for (int j = 0; j < FN; ++j) {
-    const int64_t rows = n0 + (wn * FN + j) * 16;
-    const float s = sx[min(rows + (lane & 15), static_cast<int64_t>(n - 1))];
-#pragma unroll
-    for (int g = 0; g < FM / Q; ++g) {
-      Out v[kUnit];
-#pragma unroll
-      for (int e = 0; e < kUnit; ++e)
-        v[e] = from_float<Out>(static_cast<float>(acc[g * Q + e / 4][j][e % 4]) * s * scale[g][e]);
-      __builtin_memcpy(__builtin_assume_aligned(turn + (lane & 15) * kPitch + g * 16 * Q + mine, 16),
-                       v, 16);
-    }
-    wave_lds_sync();
-#pragma unroll
-    for (int r = 0; r < 16; r += 64 / kAcross) {
-      const int row = r + lane / kAcross, along = lane % kAcross * kUnit;
-      Out v[kUnit];
-      __builtin_memcpy(v, __builtin_assume_aligned(turn + row * kPitch + along, 16), 16);
-      if (rows + row >= n) continue;
-      Out* out = S + (rows + row) * lds + first + along;
-      if (first + along + kUnit <= m) {
-        __builtin_memcpy(out, v, 16);
-      } else {
-#pragma unroll
-        for (int e = 0; e < kUnit; ++e)
-          if (first + along + e < m) out[e] = v[e];
-      }
-    }
-    wave_lds_sync();
-  }
+  using Turn = Turned<Out, FM>;
+  static_assert(kWaves * Turn::kSize * sizeof(Out) <= sizeof(tile), "room to turn");
+  const int64_t rows = n0 + wn * FN * 16;
+  Turn::store(acc, reinterpret_cast<Out*>(&tile[0][0]) + wave * Turn::kSize,
+              [&](int row) { return sx[min(rows + row, static_cast<int64_t>(n - 1))]; }, sw, S, lds,
+              rows, static_cast<int>(m0) + wm * (16 * FM), m, n, lane);
 }
 
 template <class Out, int BN, int BM, int WN, int WM, int STAGES>
@@ -353,12 +373,163 @@ void start_few(const ScoresI8Launch& a) {
   else a.n == 1 ? start_few<T, Out, 1, 1>(a) : start_few<T, Out, 2, 1>(a);
 }
 
+// ---------------------------------------------------------------------------
+// Few classes: a workgroup takes 32 examples with all the classes.  It
+// quantises the examples into LDS, so their 8-bit form never goes to memory
+// and there is one launch; then each wave takes 32 classes at a time, whose
+// bytes go from W (which stays in the caches) to registers without a barrier,
+// the next four steps of K while these four are multiplied.  The examples'
+// rows in LDS are zero from d on, and 16 bytes longer than whole steps, so
+// that the rows an instruction reads at one place lie in different banks.
+// ---------------------------------------------------------------------------
+constexpr int kStrip = 32, kStripStep = 64, kStripWaves = 8;
+
+__device__ inline v4i load_buffer(__amdgpu_buffer_rsrc_t from, int offset) {
+  return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(from, offset, 0, 0));
+}
+
+__host__ __device__ inline int strip_pitch(int d) {
+  return (d + kStripStep - 1) / kStripStep * kStripStep + 16;
+}
+
+// G: vectors of eight values that a lane holds of an example.
+template <class T, class Out, int G>
+__global__ __launch_bounds__(64 * kStripWaves, 6) void scores_i8_strip_kernel(
+    const T* __restrict__ X, int64_t ldx, const int8_t* __restrict__ W, int64_t ldw,
+    const float* __restrict__ sw, Out* __restrict__ S, int64_t lds, int d, int m, int n) {
+  constexpr int Q = 4 / static_cast<int>(sizeof(Out));
+  constexpr int FM = 2, FN = kStrip / 16, kAhead = 2;
+  constexpr int kMine = kStrip / kStripWaves;        // a wave's examples,
+  constexpr int kOnce = (sizeof(T) == 8 ? 2 : 4) / G;  // so many at once
+  static_assert(kMine % kOnce == 0, "whole rounds");
+  extern __shared__ __align__(16) int8_t strip[];
+  __shared__ __align__(16) Out turned[kStripWaves][Turned<Out, FM>::kSize];
+  __shared__ float scales[kStrip];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kStrip;
+  const int pitch = strip_pitch(d), steps = (d + kStripStep - 1) / kStripStep;
+  const __amdgpu_buffer_rsrc_t wb = rows_buffer(W, ldw, 0, m, d);
+
+  int from[FM];
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int row = ((lane & 15) >> 2) * (4 * Q) + (lane & 3) + i / Q * 16 * Q + i % Q * 4;
+    from[i] = row * static_cast<int>(ldw) + lane / 16 * 16;
+  }
+  v4i next[kAhead][FM];
+  const auto fetch = [&](int class0, int step0) {
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s)
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+        next[s][i] = load_buffer(wb, class0 < m && step0 + s < steps
+                                         ? from[i] + class0 * static_cast<int>(ldw) +
+                                               (step0 + s) * kStripStep
+                                         : kOutside);
+  };
+#pragma unroll
+  for (int r0 = 0; r0 < kMine; r0 += kOnce) {
+    T raw[kOnce][G][8];
+    unsigned most[kOnce] = {};
+#pragma unroll
+    for (int r = 0; r < kOnce; ++r) {
+      const int64_t row = n0 + wave * kMine + r0 + r;
+      const T* x = X + (row < n ? row : n - 1) * ldx;
+#pragma unroll
+      for (int g = 0; g < G; ++g) load_column(x, (g * 64 + lane) * 8, d, raw[r][g]);
+    }
+#pragma unroll
+    for (int r = 0; r < kOnce; ++r)
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most[r] = max(most[r], magnitude(to_float(raw[r][g][e])));
+#pragma unroll
+    for (int off = 32; off; off >>= 1)
+#pragma unroll
+      for (int r = 0; r < kOnce; ++r)
+        most[r] = max(most[r], static_cast<unsigned>(__shfl_xor(most[r], off)));
+#pragma unroll
+    for (int r = 0; r < kOnce; ++r) {
+      const ColumnScale s(most[r]);
+      const int at_row = wave * kMine + r0 + r;
+      if (lane == 0) scales[at_row] = s.scale;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const int at = (g * 64 + lane) * 8;
+        // Converted again: held as floats since the maximum they spill.
+        unsigned words[2 * sizeof(T)];
+        __builtin_memcpy(words, raw[r][g], sizeof(words));
+#pragma unroll
+        for (unsigned& word : words) asm volatile("" : "+v"(word));
+        __builtin_memcpy(raw[r][g], words, sizeof(words));
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = to_float(raw[r][g][e]);
+        unsigned w[2];
+        quantize8(v, s, w);
+        end_column(at, d, w);
+        if (at < steps * kStripStep) __builtin_memcpy(strip + at_row * pitch + at, w, 8);
+      }
+    }
+  }
+  fetch(wave * 16 * FM, 0);
+  __syncthreads();
+
+  const int8_t* mine = strip + (lane & 15) * pitch + lane / 16 * 16;
+  for (int class0 = wave * 16 * FM; class0 < m; class0 += kStripWaves * 16 * FM) {
+    v4i acc[FM][FN] = {};
+    for (int step0 = 0; step0 < steps; step0 += kAhead) {
+      v4i a[kAhead][FM];
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s)
+#pragma unroll
+        for (int i = 0; i < FM; ++i) a[s][i] = next[s][i];
+      const bool more = step0 + kAhead < steps;
+      fetch(more ? class0 : class0 + kStripWaves * 16 * FM, more ? step0 + kAhead : 0);
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        if (step0 + s >= steps) break;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          const v4i b = *reinterpret_cast<const v4i*>(mine + j * 16 * pitch + (step0 + s) * kStripStep);
+#pragma unroll
+          for (int i = 0; i < FM; ++i)
+            acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[s][i], b, acc[i][j], 0, 0, 0);
+        }
+      }
+    }
+    Turned<Out, FM>::store(acc, turned[wave], [&](int row) { return scales[row]; }, sw, S, lds, n0,
+                           class0, m, n, lane);
+  }
+}
+
+template <class T, class Out, int G>
+void start_strip(const ScoresI8Launch& a) {
+  scores_i8_strip_kernel<T, Out, G>
+      <<<static_cast<unsigned>((a.n + kStrip - 1) / kStrip), 64 * kStripWaves,
+         kStrip * static_cast<size_t>(strip_pitch(static_cast<int>(a.d))), a.stream>>>(
+          static_cast<const T*>(a.X), a.ldx, a.W, a.ldw, a.sw, static_cast<Out*>(a.S), a.lds,
+          static_cast<int>(a.d), static_cast<int>(a.m), static_cast<int>(a.n));
+}
+template <class T, class Out>
+void start_strip(const ScoresI8Launch& a) {
+  if (a.d <= 512) start_strip<T, Out, 1>(a);
+  else start_strip<T, Out, 2>(a);
+}
+
 // What a tile kernel takes for `tiles` of its tiles, in its time per tile of
 // K with one tile and with two tiles to a compute unit (256 of them).
 double tile_time(int64_t tiles, double one, double two) {
   const int64_t rest = tiles % 512;
   return static_cast<double>(tiles / 512) * two + (rest == 0 ? 0. : rest <= 256 ? one : two);
 }
+
+// By the examples' room in LDS; shorter rows of W leave most lanes without
+// work, and the other kernels do better.
+bool scores_i8_few(int64_t n, int64_t d) { return n <= 2 && d >= 512 && n * d <= 49152; }
 
 template <class Out>
 hipError_t scores(const ScoresI8Launch& a) {
@@ -371,6 +542,12 @@ hipError_t scores(const ScoresI8Launch& a) {
       default: start_few<int8_t, Out>(a);
     }
     return hipGetLastError();
+  }
+  switch (a.data) {
+    case SDCA_F32: start_strip<float, Out>(a); return hipGetLastError();
+    case SDCA_F64: start_strip<double, Out>(a); return hipGetLastError();
+    case SDCA_F16: start_strip<__half, Out>(a); return hipGetLastError();
+    case SDCA_BF16: start_strip<__hip_bfloat16, Out>(a); return hipGetLastError();
   }
   // The tile by its measured microseconds per 128 bytes of K: 256 x 256 does
   // the most work per byte read, smaller ones fill the device with fewer
@@ -389,10 +566,16 @@ hipError_t scores(const ScoresI8Launch& a) {
 
 }  // namespace
 
-bool scores_i8_few(int64_t n, int64_t d) {
-  // By the examples' room in LDS; shorter rows of W leave most lanes without
-  // work, and the tile kernels do better.
-  return n <= 2 && d >= 512 && n * d <= 49152;
+bool scores_i8_quantises(int data, int64_t d, int64_t m, int64_t n) {
+  if (scores_i8_few(n, d)) return true;
+  // The strip kernel reads all of W for every 32 examples, so W is to be
+  // small, and one workgroup does all there is to do for them, which pays
+  // while there are few rounds of workgroups.  (us with half-precision
+  // examples, against the quantiser and the product one after the other,
+  // without the second launch's 2 us: 20011 x 513, m 137: 19.0, 25.0; 20000 x
+  // 128, m 128: 10.1, 12.3; m 256: 13.2, 14.6; 100 x 512, m 128: 6.6, 8.9; but
+  // 20000 x 1024, m 256: 37, 28; 200000 x 256, m 128: 71, 60.)
+  return data != SDCA_I8 && n <= 65536 && m <= 256 && d <= 1024 && m * d <= 98304;
 }
 
 hipError_t launch_scores_i8(const ScoresI8Launch& a) {

@@ -162,6 +162,60 @@ def test_scores_of_float_examples(cuda, kind, n, m, d):
         assert bool(((S.double() - full).abs() <= bound * 1.0001 + 1e-30).all())
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("out", ["float32", "float16", "bfloat16"])
+def test_scores_few_classes(cuda, kind, out):
+    """Few classes, at the ends of the kernels' units of d, m and n: equal to
+    the scores of the examples quantised beforehand, whose kernel is another;
+    also from rows apart, with values between that are not to be read, and
+    into rows apart, whose values between stay."""
+    import torch
+    import libsdca_amd as sd
+    dt, odt = getattr(torch, kind), getattr(torch, out)
+    for i, d in enumerate((1, 7, 8, 9, 15, 63, 64, 65, 127, 200, 511, 512, 513, 520, 767, 1017, 1024, 1025)):
+        for m in (1, 15, 32, 33, 96, 137, 256, 257):
+            n = (1, 3, 31, 32, 33, 100)[(i + m) % 6]
+            print(kind, out, n, m, d, flush=True)
+            g = _gen(cuda, n * m + d)
+            X = torch.randn((n, d), generator=g, device=cuda).to(dt)
+            X[n // 2] = 0
+            if n > 3:
+                X[n - 1, d - 1] = float("-inf")
+                X[1, : d // 2] = 0
+            W, sw = sd.quantize_i8(torch.randn((m, d), generator=g, device=cuda))
+            q, s = sd.quantize_i8(X)
+            want = torch.nan_to_num(sd.scores_i8(q, W, sw, x_scales=s, dtype=odt), nan=-3.0)
+            got = torch.nan_to_num(sd.scores_i8(X, W, sw, dtype=odt), nan=-3.0)
+            assert torch.equal(got, want)
+            wide = torch.full((n, d + 5), float("nan"), dtype=dt, device=cuda)
+            wide[:, 1:d + 1] = X
+            spare = torch.full((m, (d + 15) // 16 * 16 + 16), 99, dtype=torch.int8, device=cuda)
+            spare[:, :d] = W
+            S = torch.full((n, m + 3), -7, dtype=odt, device=cuda)
+            sd.scores_i8(wide[:, 1:d + 1], spare[:, :d], sw, out=S[:, :m])
+            assert torch.equal(torch.nan_to_num(S[:, :m], nan=-3.0), want)
+            assert bool((S[:, m:] == -7).all())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_quantize_ends_of_columns(cuda, kind):
+    """Every end of a column within a lane's eight values, from rows apart and
+    into rows apart."""
+    import torch
+    import libsdca_amd as sd
+    for d in [*range(1, 27), *range(126, 139), 255, 257, 511, 515, 1021, 1030, 2047, 4099]:
+        n = 9
+        g = _gen(cuda, d)
+        wide = torch.full((n, d + 3), float("nan"), dtype=getattr(torch, kind), device=cuda)
+        wide[:, 2:d + 2] = torch.randn((n, d), generator=g, device=cuda).to(wide.dtype)
+        X = wide[:, 2:d + 2]
+        Q = torch.full((n, d + 9), 77, dtype=torch.int8, device=cuda)
+        q, s = sd.quantize_i8(X, out=Q[:, :d])
+        want_q, want_s = ref.quantized(_np(X.contiguous()))
+        assert np.array_equal(_np(q), want_q) and np.array_equal(_np(s), want_s), d
+        assert bool((Q[:, d:] == 77).all()), d
+
+
 def test_scores_extreme_sums(cuda):
     """The largest d, every product at its extreme: sums next to 2^31."""
     import torch
