@@ -905,6 +905,16 @@ struct NucleusSums {
   }
 };
 
+// The first of `parts` (at most 64; lane i has the mass of part i) at which
+// the sum passes the target, else the last, and the sum of those before it.
+__device__ inline int part_of(u64 mass, int parts, u64 target, u64* before) {
+  const u64 incl = wave_scan(mass);
+  const u64 passed = __ballot(incl > target);
+  const int part = passed ? min(__ffsll(passed), parts) - 1 : parts - 1;
+  *before = read_lane64(incl - mass, part);
+  return part;
+}
+
 // The cut and the draw behind the second pass.  entry: thread i's of the
 // `count` in the step; above: the mass above it; s.sum2 and s.sum3: the mass
 // and number of the labels above it that min-p leaves, for each of kWaves
@@ -940,9 +950,8 @@ __device__ bool finish_nucleus(const T* row, u64 entry, int count, u64 above, u6
   }
   __syncthreads();
   const u64 total = total_of(s.sum2), draw = draw_target(a.u[col], total), many = total_of(s.sum3);
-  u64 base = 0;
-  int pick = 0;
-  for (; pick < kWaves - 1 && base + s.sum2[pick] <= draw; ++pick) base += s.sum2[pick];
+  u64 base;
+  const int pick = part_of(lane < kWaves ? s.sum2[lane] : 0, kWaves, draw, &base);
   // The ties that are kept, in all and before the stretch.
   const bool tie = in && static_cast<unsigned>(entry >> 32) == tau;
   const u64 tied = __ballot(tie), early = __ballot(tie && index_of(entry) < pick * part);
@@ -1220,10 +1229,18 @@ __device__ bool list_and_draw(u64 entry, int count, u64 mass, const Weights& wt,
                               Shared<THREADS>& s) {
   constexpr int kWaves = THREADS / 64;
   const int i = threadIdx.x, lane = i & 63, wave = i >> 6;
+  const auto weight = [&] {
+    return i < count ? wt.of(score_of(static_cast<unsigned>(entry >> 32))) : 0.f;
+  };
+  if (mass && !c.k) {  // before the sort, which a nucleus of thousands need not wait for
+    u64 held;
+    block_scan<THREADS>(i < count ? wt.fixed(weight()) : 0, s.sum, &held);
+    if (held < top_p_target(c.p, mass)) return false;
+  }
   int P = 64;
   while (P < count) P <<= 1;
   entry = sort_block<THREADS>(entry, P, s.list.swap);
-  const float w = i < count ? wt.of(score_of(static_cast<unsigned>(entry >> 32))) : 0.f;
+  const float w = weight();
   const u64 f = i < count ? wt.fixed(w) : 0;
   const int first = c.k && c.k < count ? c.k : count;
   u64 all;
@@ -1427,10 +1444,10 @@ struct PartsOf {  // one column's
   NucleusSums sums[kMaxParts];
   unsigned guide[kBins];
   u64 entry[kList];
+  // (A part to a lane: one after the other the loads of 16 parts took 2 us.)
   __device__ u64 total(int parts) const {
-    u64 t = 0;
-    for (int i = 0; i < parts; ++i) t += mass[i];
-    return t;
+    const int lane = threadIdx.x & 63;
+    return wave_sum(lane < parts ? mass[lane] : 0);
   }
 };
 static_assert(kMaxParts == kList / 64, "finish_nucleus takes the parts as the waves' stretches");
@@ -1598,16 +1615,11 @@ __global__ __launch_bounds__(kList) void sample_draw_kernel(const T* __restrict_
   wt.inv_t = 1.f / c.t;
   wt.scale = a.scale;
   if (!c.cut) {
-    u64 total = 0, base = 0;
-    int many = 0;
-    for (int i = 0; i < p.parts; ++i) {
-      total += of.mass[i];
-      many += of.count[i];
-    }
-    const u64 target = draw_target(a.u[col], total);
-    int i = 0;
-    for (; i < p.parts - 1 && base + of.mass[i] <= target; ++i) base += of.mass[i];
-    const int begin = i * p.part;
+    const int lane = threadIdx.x & 63;
+    const u64 mass = lane < p.parts ? of.mass[lane] : 0, total = wave_sum(mass);
+    const int many = wave_sum(lane < p.parts ? of.count[lane] : 0);
+    u64 base;
+    const int begin = p.part * part_of(mass, p.parts, draw_target(a.u[col], total), &base);
     narrow_and_draw<kList>(row, begin, min(a.m, begin + p.part), base, 0, total,
                            static_cast<u64>(many), 0u, 0, wt, c, a, col, s);
     return;
@@ -1706,8 +1718,8 @@ __global__ __launch_bounds__(kList) void sample_finish_kernel(const T* __restric
   const u64 mass = of.total(p.parts);
   const int i = threadIdx.x, count = of.gathered;
   if (count <= kList) {
-    u64 above = 0;
-    for (int v = 0; v < p.parts; ++v) above += of.sums[v].over;
+    const int lane = threadIdx.x & 63;
+    const u64 above = wave_sum(lane < p.parts ? of.sums[lane].over : 0);
     if (i < kMaxParts) {
       s.sum2[i] = i < p.parts ? of.sums[i].sum : 0;
       s.sum3[i] = i < p.parts ? of.sums[i].many : 0;

@@ -551,9 +551,10 @@ hipError_t scores(const ScoresI8Launch& a) {
   }
   // The tile by its measured microseconds per 128 bytes of K: 256 x 256 does
   // the most work per byte read, smaller ones fill the device with fewer
-  // scores.  (us by tile 256, 128, 64: 16384 x 8192, d 8192: 900, 1100, 1770;
-  // 20000 x 1000, d 4096: 132, 100, 150; 2048 x 2048, d 2048: 32, 15.6, 19;
-  // 128 x 8192, d 4096: 48, 25, 13.)
+  // scores.  (us by tile 256, 128, 64: 16384 x 8192, d 8192: 880, 1030, 1620;
+  // 1024 x 14336, d 4096: 63, 70, 109; 20000 x 1000, d 4096: 118, 98, 145; 2048
+  // x 2048, d 2048: 31, 15.6, 19; 512 x 4096, d 4096: 50, 23, 17; 128 x 8192,
+  // d 4096: 48, 24, 11.5.)
   const auto tiles = [&](int64_t t) { return ((a.n + t - 1) / t) * ((a.m + t - 1) / t); };
   const double t256 = tile_time(2 * tiles(256), 1.76, 1.76);
   const double t128 = tile_time(tiles(128), 0.65, 1.07);
