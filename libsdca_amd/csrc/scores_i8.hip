@@ -527,6 +527,64 @@ double tile_time(int64_t tiles, double one, double two) {
   return static_cast<double>(tiles / 512) * two + (rest == 0 ? 0. : rest <= 256 ? one : two);
 }
 
+// The tile by its measured microseconds per 128 bytes of K: 256 x 256 does
+// the most work per byte read, smaller ones fill the device with fewer
+// scores.  (us by tile 256, 128, 64: 16384 x 8192, d 8192: 880, 1030, 1620;
+// 1024 x 14336, d 4096: 63, 70, 109; 20000 x 1000, d 4096: 118, 98, 145; 2048
+// x 2048, d 2048: 31, 15.6, 19; 512 x 4096, d 4096: 50, 23, 17; 128 x 8192,
+// d 4096: 48, 24, 11.5.)
+struct TilePlan {
+  double us;
+  int tile;
+};
+inline TilePlan plan_tiles(int64_t n, int64_t m, int64_t d) {
+  const auto tiles = [&](int64_t t) { return ((n + t - 1) / t) * ((m + t - 1) / t); };
+  const double steps = static_cast<double>((d + kTileK - 1) / kTileK);
+  const double t256 = steps * tile_time(2 * tiles(256), 1.76, 1.76);
+  const double t128 = steps * tile_time(tiles(128), 0.65, 1.07);
+  const double t64 = steps * tile_time(tiles(64), 0.33, 0.43);
+  if (t256 <= t128 && t256 <= t64) return {t256, 256};
+  return t128 <= t64 ? TilePlan{t128, 128} : TilePlan{t64, 64};
+}
+
+template <class Out>
+void start_tile(const ScoresI8Launch& a, int tile) {
+  if (tile == 256) start<Out, 256, 256, 2, 4, 2>(a);
+  else if (tile == 128) start<Out, 128, 128, 2, 4, 2>(a);
+  else start<Out, 64, 64, 2, 2, 4>(a);
+}
+
+// Tiles of 256 come in rounds of 256, one to a compute unit.  What the last
+// whole round leaves of the examples goes to a launch of its own where that,
+// by the tile that suits it, takes less than another round: kSecond us are
+// the launch's own, with its first loads and last stores.  (us in one launch
+// and in two: 17000 x 1024, d 8192: 161, 128; 16640 x 1000, d 4096: 88, 76;
+// 200000 x 256, d 4096: 270, 245; 9000 x 8192, d 8192: 521, 503; but 20000 x
+// 1000, d 2048: 59, 63.)
+constexpr double kSecond = 6.5;
+template <class Out>
+void start_tiles(const ScoresI8Launch& a) {
+  const TilePlan all = plan_tiles(a.n, a.m, a.d);
+  const int64_t across = (a.m + 255) / 256, rounds = (a.n + 255) / 256 * across / 256;
+  const int64_t head = rounds * 256 / across * 256;
+  if (head > 0 && head < a.n) {
+    const double first = static_cast<double>(rounds * ((a.d + kTileK - 1) / kTileK)) * 1.76;
+    const TilePlan rest = plan_tiles(a.n - head, a.m, a.d);
+    if (first + kSecond + rest.us < all.us) {
+      ScoresI8Launch part = a;
+      part.n = head;
+      start_tile<Out>(part, 256);
+      part.n = a.n - head;
+      part.X = static_cast<const int8_t*>(a.X) + head * a.ldx;
+      part.sx = a.sx + head;
+      part.S = static_cast<Out*>(a.S) + head * a.lds;
+      start_tile<Out>(part, rest.tile);
+      return;
+    }
+  }
+  start_tile<Out>(a, all.tile);
+}
+
 // By the examples' room in LDS; shorter rows of W leave most lanes without
 // work, and the other kernels do better.
 bool scores_i8_few(int64_t n, int64_t d) { return n <= 2 && d >= 512 && n * d <= 49152; }
@@ -549,19 +607,7 @@ hipError_t scores(const ScoresI8Launch& a) {
     case SDCA_F16: start_strip<__half, Out>(a); return hipGetLastError();
     case SDCA_BF16: start_strip<__hip_bfloat16, Out>(a); return hipGetLastError();
   }
-  // The tile by its measured microseconds per 128 bytes of K: 256 x 256 does
-  // the most work per byte read, smaller ones fill the device with fewer
-  // scores.  (us by tile 256, 128, 64: 16384 x 8192, d 8192: 880, 1030, 1620;
-  // 1024 x 14336, d 4096: 63, 70, 109; 20000 x 1000, d 4096: 118, 98, 145; 2048
-  // x 2048, d 2048: 31, 15.6, 19; 512 x 4096, d 4096: 50, 23, 17; 128 x 8192,
-  // d 4096: 48, 24, 11.5.)
-  const auto tiles = [&](int64_t t) { return ((a.n + t - 1) / t) * ((a.m + t - 1) / t); };
-  const double t256 = tile_time(2 * tiles(256), 1.76, 1.76);
-  const double t128 = tile_time(tiles(128), 0.65, 1.07);
-  const double t64 = tile_time(tiles(64), 0.33, 0.43);
-  if (t256 <= t128 && t256 <= t64) start<Out, 256, 256, 2, 4, 2>(a);
-  else if (t128 <= t64) start<Out, 128, 128, 2, 4, 2>(a);
-  else start<Out, 64, 64, 2, 2, 4>(a);
+  start_tiles<Out>(a);
   return hipGetLastError();
 }
 

@@ -216,6 +216,26 @@ def test_quantize_ends_of_columns(cuda, kind):
         assert bool((Q[:, d:] == 77).all()), d
 
 
+@pytest.mark.parametrize("n,m,d,out", [(17_000, 1000, 4096, "float32"), (9000, 8192, 1030, "bfloat16"),
+                                       (50_001, 1000, 768, "float16")])
+def test_scores_in_two_launches(cuda, n, m, d, out):
+    """More examples than whole rounds of the largest tiles: what is left is a
+    launch of its own.  The rows next to every multiple of 256 are checked,
+    and no row is left out."""
+    import torch
+    import libsdca_amd as sd
+    print(n, m, d, out, flush=True)
+    X, sx, W, sw = _operands(cuda, n, m, d, n + d)
+    if out == "float16":
+        sw = sw / 1000  # within the type's range
+    S = torch.full((n, m + 5), float("nan"), dtype=getattr(torch, out), device=cuda)
+    sd.scores_i8(X, W, sw, x_scales=sx, out=S[:, :m])
+    assert not bool(torch.isnan(S[:, :m]).any()) and bool(torch.isnan(S[:, m:]).all())
+    rows = sorted({r for t in range(0, n, 256) for r in (t - 1, t) if r >= 0} | {n - 1})
+    cols = sorted({*range(0, m, 61), m - 1})
+    ref.check_scores(_np(S[rows][:, cols].contiguous()), _np(X[rows]), _np(sx[rows]), _np(W[cols]), _np(sw[cols]), out)
+
+
 def test_scores_extreme_sums(cuda):
     """The largest d, every product at its extreme: sums next to 2^31."""
     import torch
