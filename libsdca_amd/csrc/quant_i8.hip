@@ -3,6 +3,7 @@
 #include <hip/hip_fp16.h>
 
 #include "answer_launch.hpp"
+#include "answer_limits.hpp"
 #include "answer_types.hpp"
 
 namespace sdca_gpu {
@@ -82,9 +83,13 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ X, 
 
 template <class T, int TPC, int G, bool LOOP>
 void start(const QuantLaunch& a) {
-  const int64_t blocks = (a.n + 256 / TPC - 1) / (256 / TPC);
-  quantize_kernel<T, TPC, G, LOOP><<<static_cast<unsigned>(blocks), 256, 0, a.stream>>>(
-      static_cast<const T*>(a.X), a.ldx, a.d, a.n, a.Q, a.ldq, a.pad, a.scales);
+  constexpr int64_t kColumns = 256 / TPC;
+  each_slice(a.n, kColumns, 256, [&](int64_t first, int64_t n) {
+    quantize_kernel<T, TPC, G, LOOP>
+        <<<static_cast<unsigned>((n + kColumns - 1) / kColumns), 256, 0, a.stream>>>(
+            static_cast<const T*>(a.X) + first * a.ldx, a.ldx, a.d, n, a.Q + first * a.ldq, a.ldq,
+            a.pad, a.scales + first);
+  });
 }
 
 template <class T>

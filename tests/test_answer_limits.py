@@ -1,0 +1,80 @@
+"""The answering calls at the limits of a dispatch and of their own: columns
+beyond one grid's threads, offsets at the ends of a buffer."""
+import os
+import shutil
+import subprocess
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "libsdca_amd", "csrc")
+
+
+def _run_host(tmp_path, body, *flags):
+    """Compiles and runs a program on the host-only header of the limits."""
+    if shutil.which("g++") is None:
+        pytest.skip("g++ not found")
+    src, exe = tmp_path / "limits.cpp", tmp_path / "limits"
+    src.write_text(f'#include "answer_limits.hpp"\n#include <cstdio>\n#include <initializer_list>\nusing namespace sdca_gpu;\nint main() {{\n{body}\n}}\n')
+    out = subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", *flags, "-I", CSRC, str(src), "-o", str(exe)],
+                         capture_output=True, text=True)
+    assert out.returncode == 0, out.stderr
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0, run.stdout + run.stderr
+    return run.stdout
+
+
+def test_slices_cover_and_fit_a_dispatch(tmp_path):
+    """Slices follow one another to the end, and each is a grid of fewer than
+    2^32 threads."""
+    out = _run_host(tmp_path, r"""
+  const int64_t many[] = {0, 1, 5, 1 << 21, (1 << 22) + 3, (1 << 24) + 3, (int64_t(1) << 30) - 1, INT32_MAX};
+  for (int64_t n : many)
+    for (int threads : {64, 256, 512, 1024})
+      for (int64_t per : {1, 4, 16, 64, 256}) {
+        int64_t next = 0;
+        each_slice(n, per, threads, [&](int64_t first, int64_t count) {
+          const int64_t blocks = (count + per - 1) / per;
+          if (first != next || count < 1 || blocks * threads >= int64_t(1) << 32 || first % per) std::printf("bad\n");
+          next = first + count;
+        });
+        if (next != n) std::printf("left out\n");
+      }
+""")
+    assert out == ""
+
+
+def _room(cuda, gib):
+    import torch
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info(cuda)[0] < gib * 2 ** 30:
+        pytest.skip(f"needs {gib} GiB of device memory")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,d", [(2 ** 28 + 5, 2), (2 ** 24 + 3, 1025)])
+def test_quantize_more_columns_than_a_dispatch(cuda, n, d):
+    """Sixteen threads to a column and a workgroup to a column, beyond 2^32
+    threads.  Every column is of ones but the ones around the places where a
+    grid could end, which are compared with the same columns alone."""
+    import torch
+    import libsdca_amd as sd
+    _room(cuda, 70)
+    print(n, d, flush=True)
+    A = torch.ones((n, d), dtype=torch.float16, device=cuda)
+    edge = torch.tensor(sorted({r for e in range(20, 29) for r in range(2 ** e - 2, 2 ** e + 2) if r < n} | {0, n - 2, n - 1}),
+                        device=cuda)
+    g = torch.Generator(device=cuda)
+    g.manual_seed(d)
+    some = torch.randn((len(edge), d), generator=g, device=cuda).half()
+    A[edge] = some
+    Q = torch.zeros((n, d), dtype=torch.int8, device=cuda)
+    s = torch.full((n,), -1.0, device=cuda)
+    sd.quantize_i8(A, out=Q, scales=s)
+    want_q, want_s = sd.quantize_i8(some)
+    assert torch.equal(Q[edge], want_q) and torch.equal(s[edge], want_s)
+    rest = torch.ones(n, dtype=torch.bool, device=cuda)
+    rest[edge] = False
+    one = sd.quantize_i8(A[3:4])[1]
+    assert bool(((s == one) | ~rest).all())
+    for i in range(0, n, 1 << 22):
+        assert bool(((Q[i:i + (1 << 22)] == 127).all(dim=1) | ~rest[i:i + (1 << 22)]).all()), i
