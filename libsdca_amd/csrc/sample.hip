@@ -25,6 +25,7 @@
 // a search over the whole column.  The draw itself goes by rising index: a
 // prefix sum over the kept labels.
 #include "answer_launch.hpp"
+#include "answer_limits.hpp"
 #include "answer_types.hpp"
 #include "common.hpp"
 
@@ -1734,15 +1735,37 @@ __global__ __launch_bounds__(kList) void sample_finish_kernel(const T* __restric
   search_and_draw<kList>(row, mass, wt, c, a, col, s, false);
 }
 
+// The arguments of the n columns from `first` on.
+SampleArgs columns_of(const SampleArgs& a, int64_t first, int64_t n) {
+  SampleArgs part = a;
+  const auto from = [&](auto& p) {
+    if (p) p += first;
+  };
+  part.n = n;
+  from(part.u);
+  from(part.temperature.each);
+  from(part.top_p.each);
+  from(part.min_p.each);
+  from(part.top_k.each);
+  from(part.labels);
+  from(part.prob);
+  from(part.kept);
+  return part;
+}
+
 template <class T, int THREADS, int R>
 void start_block(const SampleLaunch& l, const SampleArgs& a) {
-  sample_block_kernel<T, THREADS, R><<<static_cast<unsigned>(l.n), THREADS, 0, l.stream>>>(
-      static_cast<const T*>(l.S), a);
+  each_slice(l.n, 1, THREADS, [&](int64_t first, int64_t n) {
+    sample_block_kernel<T, THREADS, R><<<static_cast<unsigned>(n), THREADS, 0, l.stream>>>(
+        static_cast<const T*>(l.S) + first * l.lds, columns_of(a, first, n));
+  });
 }
 template <class T, int E>
 void start_wave(const SampleLaunch& l, const SampleArgs& a) {
-  sample_wave_kernel<T, E><<<static_cast<unsigned>((l.n + 3) / 4), 256, 0, l.stream>>>(
-      static_cast<const T*>(l.S), a);
+  each_slice(l.n, 4, 256, [&](int64_t first, int64_t n) {
+    sample_wave_kernel<T, E><<<static_cast<unsigned>((n + 3) / 4), 256, 0, l.stream>>>(
+        static_cast<const T*>(l.S) + first * l.lds, columns_of(a, first, n));
+  });
 }
 
 template <class T>

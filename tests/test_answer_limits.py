@@ -78,3 +78,35 @@ def test_quantize_more_columns_than_a_dispatch(cuda, n, d):
     assert bool(((s == one) | ~rest).all())
     for i in range(0, n, 1 << 22):
         assert bool(((Q[i:i + (1 << 22)] == 127).all(dim=1) | ~rest[i:i + (1 << 22)]).all()), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,m", [(2 ** 26 + 5, 10), (2 ** 24 + 3, 2049), (2 ** 22 + 3, 4097)])
+def test_sample_more_columns_than_a_dispatch(cuda, n, m):
+    """A wave, four waves and sixteen waves to a column, beyond 2^32 threads.
+    Every column has one label that can be drawn but the ones around the
+    places where a grid could end, which are compared with the same columns
+    alone, settings of their own included."""
+    import torch
+    import libsdca_amd as sd
+    _room(cuda, 80)
+    print(n, m, flush=True)
+    g = torch.Generator(device=cuda)
+    g.manual_seed(m)
+    S = torch.full((n, m), -30000.0, dtype=torch.float16, device=cuda)
+    at = torch.randint(0, m, (n,), generator=g, device=cuda)
+    S.scatter_(1, at[:, None], 1.0)
+    edge = torch.tensor(sorted({r for e in range(20, 27) for r in range(2 ** e - 5, 2 ** e + 5) if r < n} | {0, n - 2, n - 1}),
+                        device=cuda)
+    S[edge] = torch.randn((len(edge), m), generator=g, device=cuda).half()
+    u = torch.rand(n, generator=g, device=cuda)
+    kw = dict(temperature=0.5 + torch.rand(n, generator=g, device=cuda), top_p=0.5 + 0.5 * torch.rand(n, generator=g, device=cuda),
+              min_p=0.1 * torch.rand(n, generator=g, device=cuda), top_k=torch.randint(0, 9, (n,), generator=g, device=cuda))
+    label, prob, kept = sd.sample(S, u, prob=True, kept=True, **kw)
+    want = sd.sample(S[edge], u[edge], prob=True, kept=True, **{name: v[edge] for name, v in kw.items()})
+    for a, b in zip((label, prob, kept), want):
+        assert torch.equal(a[edge], b)
+    rest = torch.ones(n, dtype=torch.bool, device=cuda)
+    rest[edge] = False
+    assert bool(((label == at) | ~rest).all())
+    assert bool((((prob == 1) & (kept == 1)) | ~rest).all())
