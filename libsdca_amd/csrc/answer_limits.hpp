@@ -14,9 +14,9 @@ namespace sdca_gpu {
 constexpr int64_t kDispatchThreads = int64_t(1) << 31;
 
 // f(first, count) for slices that make up [0, n) in their order, each of no
-// more than one dispatch takes in workgroups of `threads`, `per` to a workgroup.
+// more than one dispatch takes at `threads` threads for `per` of them.
 template <class F>
-void each_slice(int64_t n, int64_t per, int threads, F f) {
+void each_slice(int64_t n, int64_t per, int64_t threads, F f) {
   const int64_t most = kDispatchThreads / threads * per;
   for (int64_t first = 0; first < n; first += most)
     f(first, n - first < most ? n - first : most);

@@ -7,6 +7,7 @@
 #include <type_traits>
 
 #include "answer_launch.hpp"
+#include "answer_limits.hpp"
 #include "answer_types.hpp"
 #include "common.hpp"
 
@@ -242,12 +243,18 @@ __global__ __launch_bounds__(64 * WN * WM) void scores_i8_kernel(
 
 template <class Out, int BN, int BM, int WN, int WM, int STAGES>
 void start(const ScoresI8Launch& a) {
-  const int tiles_n = static_cast<int>((a.n + BN - 1) / BN);
-  const int tiles_m = static_cast<int>((a.m + BM - 1) / BM);
-  scores_i8_kernel<Out, BN, BM, WN, WM, STAGES>
-      <<<static_cast<unsigned>(tiles_n) * tiles_m, 64 * WN * WM, 0, a.stream>>>(
-          static_cast<const int8_t*>(a.X), a.ldx, a.sx, a.W, a.ldw, a.sw, static_cast<Out*>(a.S), a.lds,
-          static_cast<int>(a.d), static_cast<int>(a.m), static_cast<int>(a.n), tiles_n, tiles_m);
+  constexpr int kThreads = 64 * WN * WM;
+  each_slice(a.m, BM, kThreads, [&](int64_t m0, int64_t m) {
+    const int tiles_m = static_cast<int>((m + BM - 1) / BM);
+    each_slice(a.n, BN, static_cast<int64_t>(kThreads) * tiles_m, [&](int64_t n0, int64_t n) {
+      const int tiles_n = static_cast<int>((n + BN - 1) / BN);
+      scores_i8_kernel<Out, BN, BM, WN, WM, STAGES>
+          <<<static_cast<unsigned>(tiles_n) * tiles_m, kThreads, 0, a.stream>>>(
+              static_cast<const int8_t*>(a.X) + n0 * a.ldx, a.ldx, a.sx + n0, a.W + m0 * a.ldw, a.ldw,
+              a.sw + m0, static_cast<Out*>(a.S) + n0 * a.lds + m0, a.lds, static_cast<int>(a.d),
+              static_cast<int>(m), static_cast<int>(n), tiles_n, tiles_m);
+    });
+  });
 }
 
 // ---------------------------------------------------------------------------

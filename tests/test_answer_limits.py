@@ -110,3 +110,32 @@ def test_sample_more_columns_than_a_dispatch(cuda, n, m):
     rest[edge] = False
     assert bool(((label == at) | ~rest).all())
     assert bool((((prob == 1) & (kept == 1)) | ~rest).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,m,d", [(3, 2 ** 30 - 1, 16), (2 ** 29 + 70, 3, 128)])
+def test_scores_more_tiles_than_a_dispatch(cuda, n, m, d):
+    """Tiles of one side beyond a dispatch's threads: each score equal to the
+    integers' sum times its scales."""
+    import torch
+    import libsdca_amd as sd
+    _room(cuda, 100)
+    print(n, m, d, flush=True)
+    g = torch.Generator(device=cuda)
+    g.manual_seed(d)
+    long = torch.empty((max(n, m), d), dtype=torch.int8, device=cuda)
+    for part in long.split(1 << 26):
+        part.random_(-127, 128, generator=g)
+    short = torch.randint(-127, 128, (min(n, m), d), generator=g, device=cuda, dtype=torch.int8)
+    scale = 0.01 + torch.rand(max(n, m), generator=g, device=cuda)
+    own = 0.01 + torch.rand(min(n, m), generator=g, device=cuda)
+    X, sx, W, sw = (short, own, long, scale) if n < m else (long, scale, short, own)
+    S = torch.full((n, m), float("nan"), dtype=torch.bfloat16, device=cuda)
+    sd.scores_i8(X, W, sw, x_scales=sx, out=S)
+    step = 1 << 24
+    for i in range(0, max(n, m), step):
+        x, s = (X, sx) if n < m else (X[i:i + step], sx[i:i + step])
+        w, t = (W[i:i + step], sw[i:i + step]) if n < m else (W, sw)
+        sums = x.float() @ w.float().T  # whole numbers below 2^24
+        want = (sums * s[:, None] * t).to(torch.bfloat16)
+        assert torch.equal(S[:, i:i + step] if n < m else S[i:i + step], want), i
