@@ -22,6 +22,18 @@ void each_slice(int64_t n, int64_t per, int64_t threads, F f) {
     f(first, n - first < most ? n - first : most);
 }
 
+// Offsets of the 8-bit product's loads into a buffer that holds rows of an
+// operand.  A row's own offset is below kI8MostOffset: a tile's 256 rows, and
+// up to 32 beyond the last class, of at most kI8MaxPitch, and K up to 131071.
+// A buffer has at most 2^31 - 1 bytes, so kOutside added to any row's offset
+// lies beyond it, where loads give zeros.  (Unsigned: the sum may pass 2^31,
+// which a signed one must not.)
+constexpr int64_t kI8MaxPitch = int64_t(1) << 22;
+constexpr uint32_t kI8MostOffset = 288 * kI8MaxPitch + (1 << 17);
+constexpr uint32_t kOutside = 0x7fffffffu;
+constexpr uint32_t i8_offset(uint32_t row, uint32_t k) { return row + k; }
+static_assert(i8_offset(kI8MostOffset, kOutside) >= kOutside, "outside of any buffer");
+
 }  // namespace sdca_gpu
 
 #endif  // SDCA_HIP_ANSWER_LIMITS_HPP

@@ -21,6 +21,7 @@
 
 #include "../../include/sdca_hip.h"
 #include "answer_launch.hpp"
+#include "answer_limits.hpp"
 #include "epoch_launch.hpp"
 #include "eval_launch.hpp"
 #include "prox_launch.hpp"
@@ -1307,7 +1308,7 @@ int scores_i8_common(int data, int out, int64_t d, int64_t m, int64_t n, const v
   // are whole tiles besides, or quantised by the kernel; the kernels' offsets within a tile of
   // columns are 32-bit.  What is not goes to scratch first.
   const auto in_place = [](const void* p, int64_t ld) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0 && ld <= (1 << 22);
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0 && ld <= sdca_gpu::kI8MaxPitch;
   };
   const int64_t pad = (d + kI8TileK - 1) / kI8TileK * kI8TileK;
   const bool own_x = !scores_i8_quantises(data, d, m, n) && (data != SDCA_I8 || d != pad || !in_place(a.X, ldx));

@@ -18,9 +18,6 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 
 constexpr int kTileK = static_cast<int>(kI8TileK);
 
-// An offset beyond any buffer (offsets in a buffer stay below 2^30 + 2^18).
-constexpr int kOutside = 0x7fffffff;
-
 // An operand's rows from `row` on as a buffer: loads beyond its last byte
 // give zeros.
 __device__ inline __amdgpu_buffer_rsrc_t rows_buffer(const int8_t* base, int64_t ld, int64_t row,
@@ -34,7 +31,7 @@ __device__ inline __amdgpu_buffer_rsrc_t rows_buffer(const int8_t* base, int64_t
 
 // 16 bytes of each lane from `offset` in the buffer to LDS: lane i's go to
 // dst + 16 i.  (The host pass does not know the builtin's width.)
-__device__ inline void load_to_lds(__amdgpu_buffer_rsrc_t from, int8_t* dst, int offset) {
+__device__ inline void load_to_lds(__amdgpu_buffer_rsrc_t from, int8_t* dst, uint32_t offset) {
 #ifdef __HIP_DEVICE_COMPILE__
   __builtin_amdgcn_raw_ptr_buffer_load_lds(
       from, (__attribute__((address_space(3))) void*)(dst), 16, offset, 0, 0, 0);
@@ -156,7 +153,7 @@ __global__ __launch_bounds__(64 * WN * WM) void scores_i8_kernel(
   const auto order = [](int row) {
     return row < BN || Q == 1 ? row & 7 : (row & 3) | ((row >> 3 & 1) << 2);
   };
-  int from[kLoads];
+  uint32_t from[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
     const int row = (wave * kLoads + i) * 8 + lane / 8;
@@ -164,11 +161,11 @@ __global__ __launch_bounds__(64 * WN * WM) void scores_i8_kernel(
     from[i] = (row < BN ? row * static_cast<int>(ldx) : (row - BN) * static_cast<int>(ldw)) +
               piece * 16;
   }
-  const auto fetch = [&](int k, int stage) {
+  const auto fetch = [&](uint32_t k, int stage) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int row = (wave * kLoads + i) * 8;
-      load_to_lds(row < BN ? xb : wb, &tile[stage][row * kTileK], from[i] + k);
+      load_to_lds(row < BN ? xb : wb, &tile[stage][row * kTileK], i8_offset(from[i], k));
     }
   };
   // The lane's first pieces in a tile; its other rows lie at fixed distances
@@ -215,7 +212,7 @@ __global__ __launch_bounds__(64 * WN * WM) void scores_i8_kernel(
   // products in one stream.
   const int tiles = (d + kTileK - 1) / kTileK;
 #pragma unroll
-  for (int t = 0; t < STAGES; ++t) fetch(t < tiles ? t * kTileK : kOutside, t);
+  for (int t = 0; t < STAGES; ++t) fetch(t < tiles ? static_cast<uint32_t>(t) * kTileK : kOutside, t);
   meet(first_in);
   read(0, 0);
   int stage = 0;
@@ -224,7 +221,7 @@ __global__ __launch_bounds__(64 * WN * WM) void scores_i8_kernel(
     __builtin_amdgcn_sched_barrier(0);  // first the reads, which the products cover
     multiply(0);
     meet(next_in);
-    fetch(t + STAGES < tiles ? (t + STAGES) * kTileK : kOutside, stage);
+    fetch(t + STAGES < tiles ? static_cast<uint32_t>(t + STAGES) * kTileK : kOutside, stage);
     stage = stage + 1 < STAGES ? stage + 1 : 0;
     read(stage, 0);
     __builtin_amdgcn_sched_barrier(0);
@@ -391,7 +388,7 @@ void start_few(const ScoresI8Launch& a) {
 // ---------------------------------------------------------------------------
 constexpr int kStrip = 32, kStripStep = 64, kStripWaves = 8;
 
-__device__ inline v4i load_buffer(__amdgpu_buffer_rsrc_t from, int offset) {
+__device__ inline v4i load_buffer(__amdgpu_buffer_rsrc_t from, uint32_t offset) {
   return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(from, offset, 0, 0));
 }
 
@@ -419,7 +416,7 @@ __global__ __launch_bounds__(64 * kStripWaves, 6) void scores_i8_strip_kernel(
   const int pitch = strip_pitch(d), steps = (d + kStripStep - 1) / kStripStep;
   const __amdgpu_buffer_rsrc_t wb = rows_buffer(W, ldw, 0, m, d);
 
-  int from[FM];
+  uint32_t from[FM];
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const int row = ((lane & 15) >> 2) * (4 * Q) + (lane & 3) + i / Q * 16 * Q + i % Q * 4;
@@ -431,10 +428,11 @@ __global__ __launch_bounds__(64 * kStripWaves, 6) void scores_i8_strip_kernel(
     for (int s = 0; s < kAhead; ++s)
 #pragma unroll
       for (int i = 0; i < FM; ++i)
-        next[s][i] = load_buffer(wb, class0 < m && step0 + s < steps
-                                         ? from[i] + class0 * static_cast<int>(ldw) +
-                                               (step0 + s) * kStripStep
-                                         : kOutside);
+        next[s][i] = load_buffer(
+            wb, class0 < m && step0 + s < steps
+                    ? i8_offset(from[i], static_cast<uint32_t>(class0 * static_cast<int>(ldw) +
+                                                               (step0 + s) * kStripStep))
+                    : kOutside);
   };
 #pragma unroll
   for (int r0 = 0; r0 < kMine; r0 += kOnce) {

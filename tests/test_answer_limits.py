@@ -139,3 +139,17 @@ def test_scores_more_tiles_than_a_dispatch(cuda, n, m, d):
         sums = x.float() @ w.float().T  # whole numbers below 2^24
         want = (sums * s[:, None] * t).to(torch.bfloat16)
         assert torch.equal(S[:, i:i + step] if n < m else S[i:i + step], want), i
+
+
+def test_offsets_outside_stay_outside(tmp_path):
+    """The product's loads of tiles that are not there: whatever row's offset
+    the one outside is added to, the sum is defined and beyond any buffer."""
+    out = _run_host(tmp_path, r"""
+  for (int64_t pitch : {int64_t(16), int64_t(4096), int64_t(1) << 20, kI8MaxPitch})
+    for (int row = 0; row < 256; ++row) {
+      const auto from = i8_offset(static_cast<uint32_t>(row * pitch), 7 * 16);
+      const auto at = i8_offset(from, kOutside);
+      if (int64_t(at) != row * pitch + 7 * 16 + int64_t(kOutside) || from > kI8MostOffset) std::printf("%d %lld\n", row, (long long)pitch);
+    }
+""", "-fsanitize=undefined", "-fno-sanitize-recover=all")
+    assert out == ""
