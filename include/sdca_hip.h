@@ -487,7 +487,11 @@ void sdca_sample_params_default(sdca_sample_params* params);
  * temperature 0 (or below the smallest normal float) draws the first of the
  * largest scores, with prob = kept = 1.  The weights are 32-bit floats and
  * their sums integers, so a label does not depend on launch shapes or on
- * the column's neighbours.  Params, and host arrays of columns, outside
+ * the column's neighbours.  m is at most 8388608 (2^23): the sums count in
+ * units of 2^-46, or of m / 2^62 where that is more (m to the next power of
+ * two), so they are off by up to m / 2 units, 2^-29 of the largest weight at
+ * m = 131072 and 2^-17 at the most; a label of less than half a unit counts
+ * as kept but is not drawn.  Params, and host arrays of columns, outside
  * temperature >= 0, 0 < top_p <= 1, 0 <= min_p <= 1, top_k >= 0 are
  * SDCA_ERR_ARG_RANGE; device values are not read back by the host: a
  * temperature that is negative or NaN draws the largest score, a top_k

@@ -888,6 +888,7 @@ def sample(S, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, prob=False, kep
     float16 or bfloat16) with the random numbers u (n float32 values in
     [0, 1)): int64 labels, -1 for a row that has none (sdca_sample).  The
     settings are numbers, or arrays of n values (float32; int64 for top_k).
+    A row has at most 2^23 scores.
     With prob=True also the drawn labels' probabilities after the cuts, with
     kept=True also the number of labels that the cuts left."""
     lib = library()

@@ -60,6 +60,13 @@ struct PerColumn {
   const T* each;  // device, or NULL
 };
 
+// Labels of a column at most.  Weights are added up in units of 2^-shift with
+// m 2^shift <= 2^62, and each is off by half a unit at most, so a sum is off by
+// m 2^-(shift + 1): here 2^-17 of the largest weight, which is less than the
+// weights' own rounding can make of it.  The error grows with the square of m
+// (2^-7 at 2^28 labels).
+constexpr int64_t kSampleMostLabels = int64_t(1) << 23;
+
 struct SampleLaunch {
   int data;  // SDCA_F32, F64, F16, BF16
   int64_t m, n;

@@ -1375,9 +1375,12 @@ int sample_common(int data, int64_t m, int64_t n, const void* S, int64_t lds, co
                   hipStream_t stream) {
   if (!is_float_type(data))
     return fail(SDCA_ERR_PRECISION, "sample takes F32, F64, F16 or BF16 scores (got %d)", data);
-  if (m < 1 || n < 0 || m > INT32_MAX / 2 || n > INT32_MAX / 2)
+  if (m < 1 || n < 0 || n > INT32_MAX / 2)
     return fail(SDCA_ERR_ARG_RANGE, "need m >= 1 and n >= 0 (got m %lld, n %lld)", (long long)m,
                 (long long)n);
+  if (m > sdca_gpu::kSampleMostLabels)
+    return fail(SDCA_ERR_ARG_RANGE, "m is at most %lld: the sums' units are sized by it (got %lld)",
+                (long long)sdca_gpu::kSampleMostLabels, (long long)m);
   sdca_sample_params p;
   if (params) p = *params;
   else sdca_sample_params_default(&p);

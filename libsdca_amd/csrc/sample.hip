@@ -13,8 +13,10 @@
 // taken in integers, w 2^shift rounded to the nearest with the shift as
 // large as m of them allow (2^45 at m = 131072): integer sums do not hang on
 // their order, so a drawn label depends neither on how a column is split
-// over threads nor on the order of atomics, and they are exact where sums of
-// 32-bit floats would lose the tail's small weights.
+// over threads nor on the order of atomics, and they keep small weights that
+// sums of 32-bit floats would lose.  What a unit cannot hold they lose too:
+// m / 2 units at most in all, 2^-29 of the largest weight at m = 131072 and
+// 2^-17 at kSampleMostLabels, where the entry point ends.
 //
 // A cut is found from a short list.  The lanes that share a column each hold
 // the largest of their part of it; an order statistic of those maxima is a

@@ -153,3 +153,42 @@ def test_offsets_outside_stay_outside(tmp_path):
     }
 """, "-fsanitize=undefined", "-fno-sanitize-recover=all")
     assert out == ""
+
+
+def test_sample_refuses_columns_beyond_its_sums():
+    """Beyond 2^23 labels the sums' units would be too coarse."""
+    import ctypes
+    import libsdca_amd as sd
+    lib = sd.library()
+    at = ctypes.c_void_p(16)  # never read
+    for m in (2 ** 23 + 1, 2 ** 28, 2 ** 30 - 1):
+        assert lib.sdca_sample(0, m, 0, at, m, at, None, None, at, None, None, 0, None) == 2
+        assert b"8388608" in lib.sdca_last_error()
+    assert lib.sdca_sample(0, 2 ** 23, 0, at, 2 ** 23, at, None, None, at, None, None, 0, None) == 0
+
+
+@pytest.mark.gpu
+def test_sample_longest_columns(cuda):
+    """2^23 labels, the tail's weights just below and just above half a unit
+    of the sums (2^-40): all of it is lost or counted twice, 2^-17 of the
+    largest weight, within what the weights' own rounding allows."""
+    import numpy as np
+    import torch
+    import libsdca_amd as sd
+    from tests import answer_oracle as ref
+    m = 2 ** 23
+    g = torch.Generator(device=cuda)
+    g.manual_seed(3)
+    S = torch.empty((4, m), device=cuda)
+    S[0] = float(np.log(0.97 * 2.0 ** -40))
+    S[1] = float(np.log(1.03 * 2.0 ** -40))
+    S[2:] = torch.randn((2, m), generator=g, device=cuda)
+    S[:2, m // 3] = 0
+    for u, kw in (([0.5, 0.5, 0.5, 0.9], dict()), ([0.999999, 0.999999, 0.1, 0.3], dict(top_p=0.9)),
+                  ([0.2, 0.99999, 0.7, 0.999], dict(temperature=1.5, top_k=500, min_p=1e-3))):
+        print(kw, flush=True)
+        u = torch.tensor(u, device=cuda)
+        label, prob, kept = sd.sample(S, u, prob=True, kept=True, **kw)
+        full = dict(dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0), **kw)
+        ref.check_sample(S.cpu().numpy(), u.cpu().numpy(), *(np.float32(v) for v in full.values()),
+                         label.cpu().numpy(), prob.cpu().numpy(), kept.cpu().numpy())
