@@ -744,6 +744,13 @@ def _pitch(x, name, shape=None):
     return step
 
 
+def _written(x, name):
+    """The library writes through a raw pointer, so an array that numpy holds
+    read-only (a view of bytes, of a file mapped for reading) is refused."""
+    if not _is_torch(x) and not x.flags.writeable:
+        raise SdcaError(2, f"{name} is read-only")
+
+
 def _values(x, name, n, dtype, like):
     """Checks a vector of n values of the given element type beside `like`."""
     if _is_torch(x) != _is_torch(like):
@@ -815,8 +822,10 @@ def quantize_i8(A, out=None, scales=None):
     if _answer_dtype(Q) != I8:
         raise SdcaError(3, f"out has element type {Q.dtype}, expected int8")
     ldq = _pitch(Q, "out", (n, d))
+    _written(Q, "out")
     s = scales if scales is not None else _empty((n,), "float32", A)
     _values(s, "scales", n, _float32(A), A)
+    _written(s, "scales")
     _answer(A, "quantize_i8", lib.sdca_quantize_i8, data, d, n, _ptr(A), lda, _ptr(Q), ldq, _ptr(s))
     return Q, s
 
@@ -862,6 +871,7 @@ def scores_i8(X, W, w_scales, x_scales=None, out=None, dtype=None):
     if code not in (F32, F16, BF16):
         raise SdcaError(3, f"scores cannot be {out.dtype}")
     lds = _pitch(out, "out", (n, m))
+    _written(out, "out")
     _answer(X, "scores_i8", lib.sdca_scores_i8, data, code, d, m, n, _ptr(X), ldx, _ptr(x_scales),
             _ptr(W), ldw, _ptr(w_scales), _ptr(out), lds)
     return out

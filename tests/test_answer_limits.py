@@ -192,3 +192,17 @@ def test_sample_longest_columns(cuda):
         full = dict(dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0), **kw)
         ref.check_sample(S.cpu().numpy(), u.cpu().numpy(), *(np.float32(v) for v in full.values()),
                          label.cpu().numpy(), prob.cpu().numpy(), kept.cpu().numpy())
+
+
+def test_read_only_results_are_refused():
+    import numpy as np
+    import libsdca_amd as sd
+    A = np.ones((3, 8), np.float32)
+    W, w = np.ones((5, 8), np.int8), np.ones(5, np.float32)
+    held = lambda shape, dtype: np.frombuffer(bytes(int(np.prod(shape)) * np.dtype(dtype).itemsize), dtype).reshape(shape)  # noqa: E731
+    for fn, args, kw in ((sd.quantize_i8, (A,), dict(out=held((3, 8), np.int8))),
+                         (sd.quantize_i8, (A,), dict(scales=held((3,), np.float32))),
+                         (sd.scores_i8, (A, W, w), dict(out=held((3, 5), np.float32)))):
+        with pytest.raises(sd.SdcaError) as e:
+            fn(*args, **kw)
+        assert e.value.status == 2 and "read-only" in str(e.value)
