@@ -422,11 +422,14 @@ int sdca_scores(sdca_dtype data, int64_t d, int64_t m, int64_t n,
  *   scales[i] = max_k |X_ki| (1 / 127),  Q_ki = X_ki / scales[i] to the
  * nearest integer, halves to even, in 32-bit arithmetic (1 / 127 the float
  * nearest to it, the product and the quotient rounded; doubles are rounded
- * to float first).  A column of zeros has scale 0; a column that holds an
+ * to float first), and at most 127 in magnitude (a scale among the smallest
+ * floats has lost digits itself).  A column of zeros, or of values too small
+ * for a scale above zero, has scale 0 and zeros; a column that holds an
  * infinity or a NaN has zeros and the scale NaN, so that every score of it
- * is NaN.  Q: d x n with leading dimension ldq; bytes between d and ldq are
- * not written.  A ldq that is a multiple of 16, and Q at such an address,
- * lets sdca_scores_i8 read Q in place.
+ * is NaN.  d is at most 2^30 - 1, n at most 2^31 - 1.  Q: d x n with leading
+ * dimension ldq; bytes between d and ldq are not written.  A ldq that is a
+ * multiple of 16, and Q at such an address, lets sdca_scores_i8 read Q in
+ * place.
  */
 int sdca_quantize_i8(sdca_dtype data, int64_t d, int64_t n, const void* X, int64_t ldx,
                      int8_t* Q, int64_t ldq, float* scales, unsigned flags, void* stream);
@@ -440,10 +443,11 @@ int sdca_quantize_i8(sdca_dtype data, int64_t d, int64_t n, const void* X, int64
  *   W: d x m weights in 8 bits, leading dimension ldw, sw their m scales;
  *   S: m x n scores of type out (SDCA_F32, SDCA_F16 or SDCA_BF16), leading
  *      dimension lds >= m.
- * The sums are exact (32-bit integers: d is at most 131071); each score is
- * float(sum) sx_i sw_j in 32-bit arithmetic, rounded to `out` at the end.
- * W is read in place when its address and ldw are multiples of 16, and is
- * copied to the stream's scratch in each call otherwise.
+ * The sums are exact (32-bit integers: d is at most 131071; m and n are at
+ * most 2^30 - 1); each score is float(sum) sx_i sw_j in 32-bit arithmetic,
+ * rounded to `out` at the end.  W is read in place when its address and ldw
+ * are multiples of 16 (and ldw at most 2^22), and is copied to the stream's
+ * scratch in each call otherwise.
  */
 int sdca_scores_i8(sdca_dtype data, sdca_dtype out, int64_t d, int64_t m, int64_t n,
                    const void* X, int64_t ldx, const float* sx, const int8_t* W, int64_t ldw,

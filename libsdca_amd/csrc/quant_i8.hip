@@ -96,8 +96,11 @@ template <class T>
 hipError_t quantize(const QuantLaunch& a) {
   // By the column's length alone: part of a wave for a short column, so that
   // a wave has some KiB to read (200000 columns of 128 floats took 69 us with
-  // a wave each, 21 with a quarter; of 512 half-precision values 81 and 51),
-  // a workgroup above, with as few registers as hold it.
+  // a wave each, 21 with a quarter, both from the last-level cache; 30 from
+  // memory, at 4.3 TB/s; of 512 half-precision values 81 and 51), a workgroup
+  // above, with as few registers as hold it (20000 columns of 4096 floats 72 us,
+  // 5.7 TB/s).  Columns beyond the registers are read twice (4000 of 40000
+  // floats 273 us; 16 of 100000, which leave most of the device idle, 34).
   if (a.pad <= 16 * kVec) start<T, 16, 1, false>(a);
   else if (a.pad <= 16 * 2 * kVec) start<T, 16, 2, false>(a);
   else if (a.pad <= 16 * 4 * kVec) start<T, 16, 4, false>(a);

@@ -747,8 +747,11 @@ __device__ void narrow_and_draw(const T* row, int begin, int end, u64 base, u64 
   const float w_tau = ties ? wt.of(score_of(tau)) : 0.f;
   const u64 f_tau = w_tau >= c.q ? wt.fixed(w_tau) : 0;
   u64 target = total ? draw_target(a.u[col], total) : 0;
-  // Each step leaves a sixteenth (or 64 scores): the stretch is always down
-  // to 64 after eight steps, and the loop ends whatever the sums are.
+  // The sums below are those that the caller's total is made of (the same
+  // weights under the same cuts, as integers), so one stretch passes the
+  // target at each step.  Each step leaves a sixteenth, or a quarter with four
+  // waves, or 64 scores: the stretch is down to 64 after eight steps, and the
+  // loop ends whatever the sums are.
   for (int step = 0; step < 8; ++step) {
     const int part = ((end - begin + kWaves - 1) / kWaves + 63) / 64 * 64;
     const int b = begin + wave * part, e = b + part < end ? b + part : end;
@@ -1790,10 +1793,27 @@ void start_parts(const SampleLaunch& l, const SampleArgs& a) {
 }
 
 // Columns that one workgroup's registers do not hold go to several workgroups
-// each where one apiece leaves compute units idle.  Measured, one workgroup
-// against several: a top-k of 65537 floats 20 against 17 us for one column,
-// 32 against 41 for 256; of 128000 25 against 18, 35 against 25 for 64, 51
-// against 56 for 256; of 32000 18 against 18 (and two launches less).
+// each where one apiece leaves compute units idle.  Measured in us, one
+// workgroup / several, for n columns of m scores:
+//
+//             m        n = 16     64       128      256      512
+//   top-k 5   40000 f32  15/18    16/18    17/21    21/31    39/50
+//             65537 f32  18/17    21/20    23/25    29/39    61/71
+//            128000 f32  22/19    32/24    36/34    51/60   100/109
+//            128000 f16  20/18    22/21    24/26    29/40    58/75
+//   top-p .95 40000 f32  25/29    37/39    28/36    47/58    77/89
+//             65537 f32  32/31    83/62    84/71    90/88   133/137
+//            128000 f32  68/42   130/69   134/83   146/117  249/189
+//            128000 f16  69/39   126/65   128/76   131/100  221/163
+//   uncut     40000 f32  20/17    21/20    22/24    26/34    47/58
+//             65537 f32  29/19    33/24    34/32    40/47    81/86
+//            128000 f32  45/21    54/29    58/40    71/68   135/122
+//            128000 f16  42/19    44/26    45/35    50/52   100/99
+//
+// The limits on n are the nucleus's, which differs most and which settings of
+// each column's own may hold.  They cost a top-k or an uncut draw of 128 to
+// 256 columns up to 11 us (20/31 for 256 of 65537 f16), and a nucleus of
+// more than 256 columns of 128000 the 60 us that several would save.
 bool in_parts(int64_t m, int64_t n) { return m > 32768 && n <= (m > 65536 ? 256 : 64); }
 
 template <class T>
@@ -1816,7 +1836,9 @@ hipError_t sample(const SampleLaunch& l) {
   // Else by the column's length: a wave up to 2048 scores (8000 columns of
   // 2000: 31 us with a top-k, 110 by a workgroup; one column 7.4 and 9.3), a
   // workgroup that holds the column in registers above, 16 scores to a
-  // thread, and one that reads it twice from there on.  (32 to a thread spill:
+  // thread (with four waves the arguments and settings lie in 224 to 260 bytes
+  // of scratch, read again for each group), and one that reads it twice from
+  // there on.  (32 to a thread spill:
   // a top-k of 32000 floats took 18 us, against 14 read twice; 12000 take 11
   // held, 12 read.)
   if (in_parts(l.m, l.n)) start_parts<T>(l, a);
