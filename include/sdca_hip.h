@@ -408,9 +408,9 @@ int sdca_scores(sdca_dtype data, int64_t d, int64_t m, int64_t n,
                 unsigned flags, void* stream);
 
 /*
- * Answering from a trained model.  The three calls below have no counterpart
- * in the reference, which ends at the evaluation: they serve the scores of
- * new examples in 8 bits and draw labels from them.  Arrays are column-major
+ * Answering from a trained model.  The calls below have no counterpart in the
+ * reference, which ends at the evaluation: they serve the scores of new
+ * examples in 8 bits, draw labels from them and say how probable labels are.  Arrays are column-major
  * like the others, with a leading dimension of their own (at least the
  * column's length, in elements): the distance from one column to the next.
  * They take device pointers on `stream`, or with SDCA_HOST_PTR host arrays.
@@ -507,6 +507,56 @@ int sdca_sample(sdca_dtype data, int64_t m, int64_t n, const void* S, int64_t ld
                 const float* u, const sdca_sample_params* params,
                 const sdca_sample_columns* columns, int64_t* labels, float* prob,
                 int64_t* kept, unsigned flags, void* stream);
+
+/*
+ * Log-probabilities of given labels: with M the largest of a column's m scores
+ * (m x n, leading dimension lds; data SDCA_F32, SDCA_F16 or SDCA_BF16), the
+ * weights w_i = exp((S_i - M) / temperature) as sdca_sample has them before
+ * its cuts (1 where S_i = M, so infinite scores share), Z their sum and
+ * p_i = w_i / Z:
+ *   labels: n labels in [0, m), or -1 for a column that asks for none;
+ *   logp:      optional, n: log p of the label (0 for -1);
+ *   entropy:   optional, n: - sum p_i log p_i;
+ *   stats:     optional, 3 n: M, log Z and the entropy of each column, for
+ *              sdca_log_probs_grad;
+ *   top_logp, top_index: optional, top n each, column after column: the `top`
+ *              largest scores' log-probabilities and places, falling, ties by
+ *              rising index; -infinity and -1 beyond the scores above
+ *              -infinity.  top is at most 64; 0 for none.
+ * All in 32 bits.  A column whose scores are all -infinity has log-
+ * probabilities of -infinity, log Z = -infinity and entropy 0; one that holds
+ * a NaN has NaN for all of them.  A label that is none of [-1, m) is
+ * SDCA_ERR_LABELS in host arrays; in device memory its logp is NaN.
+ * temperature is at least 2^-126 and finite; m is at most 2^30 - 1.
+ *   work: device memory of at least sdca_log_probs_work bytes, 16-byte
+ *      aligned, or NULL: the library's scratch of the stream, which a capture
+ *      cannot grow and all graphs captured on the stream share.
+ */
+size_t sdca_log_probs_work(sdca_dtype data, int64_t m, int64_t n, int64_t top);
+int sdca_log_probs(sdca_dtype data, int64_t m, int64_t n, const void* S, int64_t lds,
+                   const int64_t* labels, double temperature, int64_t top, float* logp,
+                   float* entropy, float* stats, float* top_logp, int64_t* top_index, void* work,
+                   unsigned flags, void* stream);
+
+/*
+ * The scores' gradient where g (n) is that of the labels' log-probabilities
+ * and h (n, or NULL for 0) that of the entropies:
+ *   D_ij = (g_j ([i = label_j] - p_ij) - h_j p_ij (log p_ij + entropy_j)) / temperature
+ * in 32 bits, rounded to data's type once.  S, labels, temperature, work: as
+ * sdca_log_probs.  A column of label -1 takes part through h alone; one
+ * without a score above -infinity has zeros; one that holds a NaN, or has a
+ * label outside [-1, m), NaN.
+ *   stats: 3 n as sdca_log_probs gave them for the same S and temperature, or
+ *      NULL: computed here;
+ *   D: m x n of data's type, leading dimension ldd; may be S itself with the
+ *      same leading dimension, and must not overlap it otherwise;
+ *   logp: optional, n: the labels' log-probabilities.
+ */
+size_t sdca_log_probs_grad_work(sdca_dtype data, int64_t m, int64_t n, const float* stats);
+int sdca_log_probs_grad(sdca_dtype data, int64_t m, int64_t n, const void* S, int64_t lds,
+                        const int64_t* labels, const float* g, const float* h,
+                        const float* stats, double temperature, void* D, int64_t ldd,
+                        float* logp, void* work, unsigned flags, void* stream);
 
 /* Message of the last failure on this thread ("" if none). */
 const char* sdca_last_error(void);

@@ -26,6 +26,8 @@ and the answers of a trained model, which the reference does not have:
     quantize_i8(A)
     scores_i8(X, W, w_scales)
     sample(S, u, temperature=1, top_k=0, top_p=1, min_p=0)
+    log_probs(S, labels, temperature=1, top=0)
+    log_probs_grad(S, labels, g)
 
 `A` holds n columns of length dim, contiguous (a C-contiguous (n, dim) array
 or tensor, i.e. the column-major dim x n matrix of the reference).  A torch
@@ -48,7 +50,7 @@ __all__ = [
     "prox_two_simplex_sort", "prox_two_entropy", "lambert_w_exp", "OPS", "F32", "F64",
     "OBJECTIVES", "objective", "scores", "eval_features", "eval_kernel", "eval_scores",
     "recompute_primal", "epoch_order", "epoch_features", "epoch_kernel", "BRANCHES",
-    "quantize_i8", "scores_i8", "sample",
+    "quantize_i8", "scores_i8", "sample", "log_probs", "log_probs_grad",
 ]
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -162,6 +164,13 @@ def library():
                                        i64, u32, ptr]
         lib.sdca_sample.argtypes = [i32, i64, i64, ptr, i64, ptr, ctypes.POINTER(SampleParams),
                                     ctypes.POINTER(SampleColumns), ptr, ptr, ptr, u32, ptr]
+        f64, size = ctypes.c_double, ctypes.c_size_t
+        lib.sdca_log_probs_work.argtypes, lib.sdca_log_probs_work.restype = [i32, i64, i64, i64], size
+        lib.sdca_log_probs.argtypes = [i32, i64, i64, ptr, i64, ptr, f64, i64, ptr, ptr, ptr, ptr, ptr,
+                                       ptr, u32, ptr]
+        lib.sdca_log_probs_grad_work.argtypes, lib.sdca_log_probs_grad_work.restype = [i32, i64, i64, ptr], size
+        lib.sdca_log_probs_grad.argtypes = [i32, i64, i64, ptr, i64, ptr, ptr, ptr, ptr, f64, ptr, i64,
+                                            ptr, ptr, u32, ptr]
         lib.sdca_last_error.restype = ctypes.c_char_p
         lib.sdca_abi_version.restype = ctypes.c_int
         _lib = lib
@@ -922,3 +931,91 @@ def sample(S, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, prob=False, kep
             _ptr(labels), _ptr(pr), _ptr(kp))
     res = (labels,) + ((pr,) if prob else ()) + ((kp,) if kept else ())
     return res if len(res) > 1 else labels
+
+
+def _scratch(x, size, *args):
+    """Device scratch of size(*args) bytes for a call on the tensor x, from
+    torch's allocator (a captured call's then belongs to its graph); None for
+    numpy arrays, whose calls use the library's own."""
+    if not _is_torch(x):
+        return None
+    n = size(*args)
+    return sys.modules["torch"].empty(n, dtype=sys.modules["torch"].uint8, device=x.device) if n else None
+
+
+def _label_values(labels, n, like):
+    return _values(labels, "labels", n, sys.modules["torch"].int64 if _is_torch(like) else np.int64, like)
+
+
+def _score_type(S):
+    data = _answer_dtype(S)
+    if data not in (F32, F16, BF16):
+        raise SdcaError(3, f"unsupported element type {S.dtype}")
+    return data
+
+
+def log_probs(S, labels, temperature=1.0, top=0, entropy=False, stats=False):
+    """The log-probability of a given label for each row of the scores S (n, m)
+    (float32, float16 or bfloat16): float32, 0 for a label of -1, which asks for
+    none (sdca_log_probs).  labels: n int64 in [-1, m).
+    With entropy=True also the rows' entropies (n,), with stats=True also what
+    log_probs_grad takes of them (n, 3): the largest score, the logarithm of the
+    sum of the weights relative to it and the entropy; with top > 0 also the
+    log-probabilities and the indices (int64) of each row's `top` largest
+    scores, (n, top) each, ties by rising index, -inf and -1 where a row has
+    fewer scores above -inf.  top is at most 64."""
+    lib = library()
+    data = _score_type(S)
+    lds = _pitch(S, "S")
+    n, m = S.shape
+    _label_values(labels, n, S)
+    top = int(top)
+    logp = _empty((n,), "float32", S)
+    ent = _empty((n,), "float32", S) if entropy else None
+    st = _empty((n, 3), "float32", S) if stats else None
+    best = _empty((n, max(top, 0)), "float32", S) if top else None
+    at = _empty((n, max(top, 0)), "int64", S) if top else None
+    work = _scratch(S, lib.sdca_log_probs_work, data, m, n, top)
+    _answer(S, "log_probs", lib.sdca_log_probs, data, m, n, _ptr(S), lds, _ptr(labels), temperature, top,
+            _ptr(logp), _ptr(ent), _ptr(st), _ptr(best), _ptr(at), _ptr(work))
+    res = (logp,) + ((ent,) if entropy else ()) + ((st,) if stats else ()) + ((best, at) if top else ())
+    return res if len(res) > 1 else logp
+
+
+def log_probs_grad(S, labels, g, g_entropy=None, stats=None, temperature=1.0, out=None, logp=False):
+    """The gradient of the scores S where g (n float32) is that of the labels'
+    log-probabilities and g_entropy, if given, that of the rows' entropies
+    (sdca_log_probs_grad): a matrix of S's type, or `out`, which may be S.
+    A row of label -1 has none from g.  stats: what log_probs(stats=True) gave
+    for the same S and temperature; without, they are computed here.  With
+    logp=True also the labels' log-probabilities."""
+    lib = library()
+    data = _score_type(S)
+    lds = _pitch(S, "S")
+    n, m = S.shape
+    f32 = _float32(S)
+    _label_values(labels, n, S)
+    _values(g, "g", n, f32, S)
+    if g_entropy is not None:
+        _values(g_entropy, "g_entropy", n, f32, S)
+    if stats is not None:
+        if len(stats.shape) != 2:
+            raise SdcaError(2, f"stats has shape {tuple(stats.shape)}, expected {(n, 3)}")
+        _values(stats.reshape(-1), "stats", 3 * n, f32, S)
+        if tuple(stats.shape) != (n, 3) or not (
+                stats.is_contiguous() if _is_torch(stats) else stats.flags.c_contiguous):
+            raise SdcaError(2, f"stats must be a contiguous {(n, 3)} matrix")
+    if out is None:
+        out = sys.modules["torch"].empty((n, m), dtype=S.dtype, device=S.device) if _is_torch(S) else \
+            np.empty((n, m), dtype=S.dtype)
+    elif _is_torch(out) != _is_torch(S) or (_is_torch(S) and out.device != S.device):
+        raise SdcaError(2, "out: expected the same kind and device as S")
+    if out.dtype != S.dtype:
+        raise SdcaError(3, f"out has element type {out.dtype}, expected {S.dtype}")
+    ldd = _pitch(out, "out", (n, m))
+    _written(out, "out")
+    lp = _empty((n,), "float32", S) if logp else None
+    work = _scratch(S, lib.sdca_log_probs_grad_work, data, m, n, _ptr(stats))
+    _answer(S, "log_probs_grad", lib.sdca_log_probs_grad, data, m, n, _ptr(S), lds, _ptr(labels), _ptr(g),
+            _ptr(g_entropy), _ptr(stats), temperature, _ptr(out), ldd, _ptr(lp), _ptr(work))
+    return (out, lp) if logp else out

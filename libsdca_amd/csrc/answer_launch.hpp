@@ -1,6 +1,6 @@
 // Host-side launch interface of the kernels that answer from a trained model
-// (internal): the 8-bit quantiser, the 8-bit score product and the draw of a
-// label from scores.
+// (internal): the 8-bit quantiser, the 8-bit score product, the draw of a
+// label from scores, and labels' log-probabilities with their gradient.
 #ifndef SDCA_HIP_ANSWER_LAUNCH_HPP
 #define SDCA_HIP_ANSWER_LAUNCH_HPP
 
@@ -83,6 +83,44 @@ struct SampleLaunch {
 };
 size_t sample_work_bytes(int64_t m, int64_t n);
 hipError_t launch_sample(const SampleLaunch& a);
+
+// Alternatives of a column at most: a wave's sorted list has one to a lane.
+constexpr int64_t kMostTop = 64;
+
+struct LogProbsLaunch {
+  int data;  // SDCA_F32, F16, BF16
+  int64_t m, n;
+  const void* S;
+  int64_t lds;
+  const int64_t* labels;
+  float inv_t;
+  int top;
+  // Results, each or NULL: n, n, 3 n, top n, top n values.
+  float *logp, *entropy, *stats, *top_logp;
+  int64_t* top_index;
+  void* work;  // log_probs_work_bytes of device memory
+  hipStream_t stream;
+};
+size_t log_probs_work_bytes(int data, int64_t m, int64_t n, int top);
+hipError_t launch_log_probs(const LogProbsLaunch& a);
+
+struct LogProbsGradLaunch {
+  int data;  // SDCA_F32, F16, BF16
+  int64_t m, n;
+  const void* S;
+  int64_t lds;
+  const int64_t* labels;
+  const float *g, *h;  // n; h or NULL
+  const float* stats;  // 3 n, or NULL
+  float inv_t;
+  void* D;  // S's type; may be S
+  int64_t ldd;
+  float* logp;  // n, or NULL
+  void* work;   // log_probs_grad_work_bytes of device memory
+  hipStream_t stream;
+};
+size_t log_probs_grad_work_bytes(int data, int64_t m, int64_t n, bool stats);
+hipError_t launch_log_probs_grad(const LogProbsGradLaunch& a);
 
 }  // namespace sdca_gpu
 

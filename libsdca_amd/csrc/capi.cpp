@@ -65,9 +65,10 @@ struct Workspace {
   // Slots: 0 deferred-column list, 1 scores, 2 evaluation scratch,
   // 3 transposes, 4 epoch, 5 the library GEMM's workspace, 6 the column
   // slices of the prox beyond the LDS copy, 7 quantised and repacked operands,
-  // 8 the parts of columns that labels are drawn from.
-  void* ptr[9] = {};
-  size_t cap[9] = {};
+  // 8 the parts of columns that labels are drawn from, 9 the scratch of calls
+  // whose caller brings none.
+  void* ptr[10] = {};
+  size_t cap[10] = {};
   // Pinned host block for the evaluation's results: copies into it are
   // asynchronous, so the call waits once for all of them.
   void* host = nullptr;
@@ -1438,6 +1439,131 @@ int sample_common(int data, int64_t m, int64_t n, const void* S, int64_t lds, co
   return SDCA_OK;
 }
 
+// The types of the scores that log-probabilities and gradients are taken of.
+bool is_score_type(int dt) { return dt == SDCA_F32 || dt == SDCA_F16 || dt == SDCA_BF16; }
+
+// A call's scratch: the caller's memory, or the stream's.
+int scratch(void* given, size_t bytes, hipStream_t stream, void** out) {
+  *out = given;
+  if (!bytes || given) return SDCA_OK;
+  return workspace(stream, 9, bytes, out);
+}
+
+int check_log_probs(const char* name, int data, int64_t m, int64_t n, int64_t lds,
+                    double temperature) {
+  if (!is_score_type(data))
+    return fail(SDCA_ERR_PRECISION, "%s takes F32, F16 or BF16 scores (got %d)", name, data);
+  if (m < 1 || n < 0 || m > INT32_MAX / 2 || n > INT32_MAX / 2)
+    return fail(SDCA_ERR_ARG_RANGE, "need m >= 1 and n >= 0 (got m %lld, n %lld)", (long long)m,
+                (long long)n);
+  // (Below the smallest normal float its reciprocal can be infinite.)
+  if (!(temperature >= 1.17549435e-38 && temperature <= 3.4028234e38))
+    return fail(SDCA_ERR_ARG_RANGE, "temperature must be above 0 and finite in 32 bits (got %g)",
+                temperature);
+  return check_matrix("S", m, lds);
+}
+
+int check_labels(const int64_t* labels, int64_t m, int64_t n) {
+  for (int64_t j = 0; j < n; ++j)
+    if (labels[j] < -1 || labels[j] >= m)
+      return fail(SDCA_ERR_LABELS, "labels[%lld] = %lld outside [-1, %lld)", (long long)j,
+                  (long long)labels[j], (long long)m);
+  return SDCA_OK;
+}
+
+int log_probs_common(int data, int64_t m, int64_t n, const void* S, int64_t lds,
+                     const int64_t* labels, double temperature, int64_t top, float* logp,
+                     float* entropy, float* stats, float* top_logp, int64_t* top_index, void* work,
+                     unsigned flags, hipStream_t stream) {
+  using namespace sdca_gpu;
+  int rc;
+  if ((rc = check_log_probs("log_probs", data, m, n, lds, temperature))) return rc;
+  if (top < 0 || top > kMostTop)
+    return fail(SDCA_ERR_ARG_RANGE, "top must be in [0, %lld] (got %lld)", (long long)kMostTop,
+                (long long)top);
+  if (n == 0) return SDCA_OK;
+  if (!S || (logp && !labels)) return fail(SDCA_ERR_ARG_NULL, "S and labels must not be NULL");
+  const bool host = (flags & SDCA_HOST_PTR) != 0;
+  if (host && logp && (rc = check_labels(labels, m, n))) return rc;
+  if (host) work = nullptr;
+  if (!top) top_logp = nullptr, top_index = nullptr;
+  DeviceBuffer dS, dl, dp, de, ds, dt, di;
+  LogProbsLaunch a;
+  a.data = data;
+  a.m = m;
+  a.n = n;
+  a.lds = lds;
+  a.inv_t = 1.f / static_cast<float>(temperature);
+  a.top = top_logp || top_index ? static_cast<int>(top) : 0;
+  a.stream = stream;
+  if ((rc = staged(S, span(m, n, lds, element_size(data)), host, dS, stream, &a.S)) ||
+      (rc = staged(labels, n * sizeof(int64_t), host, dl, stream, &a.labels)) ||
+      (rc = staged_out(logp, n * sizeof(float), host, dp, &a.logp)) ||
+      (rc = staged_out(entropy, n * sizeof(float), host, de, &a.entropy)) ||
+      (rc = staged_out(stats, 3 * n * sizeof(float), host, ds, &a.stats)) ||
+      (rc = staged_out(top_logp, top * n * sizeof(float), host, dt, &a.top_logp)) ||
+      (rc = staged_out(top_index, top * n * sizeof(int64_t), host, di, &a.top_index)) ||
+      (rc = scratch(work, log_probs_work_bytes(data, m, n, a.top), stream, &a.work)))
+    return rc;
+  SDCA_HIP_TRY(launch_log_probs(a), "log-probability kernels");
+  if (host) {
+    if ((logp && (rc = fetch_columns(logp, a.logp, n, 1, n, sizeof(float), stream))) ||
+        (entropy && (rc = fetch_columns(entropy, a.entropy, n, 1, n, sizeof(float), stream))) ||
+        (stats && (rc = fetch_columns(stats, a.stats, 3 * n, 1, 3 * n, sizeof(float), stream))) ||
+        (top_logp && (rc = fetch_columns(top_logp, a.top_logp, top * n, 1, top * n, sizeof(float), stream))) ||
+        (top_index && (rc = fetch_columns(top_index, a.top_index, top * n, 1, top * n, sizeof(int64_t), stream))))
+      return rc;
+    SDCA_HIP_TRY(hipStreamSynchronize(stream), "hipStreamSynchronize");
+  }
+  return SDCA_OK;
+}
+
+int log_probs_grad_common(int data, int64_t m, int64_t n, const void* S, int64_t lds,
+                          const int64_t* labels, const float* g, const float* h,
+                          const float* stats, double temperature, void* D, int64_t ldd,
+                          float* logp, void* work, unsigned flags, hipStream_t stream) {
+  using namespace sdca_gpu;
+  int rc;
+  if ((rc = check_log_probs("log_probs_grad", data, m, n, lds, temperature)) ||
+      (rc = check_matrix("D", m, ldd)))
+    return rc;
+  if (n == 0) return SDCA_OK;
+  if (!S || !labels || !g || !D)
+    return fail(SDCA_ERR_ARG_NULL, "S, labels, g and D must not be NULL");
+  if (S == D && lds != ldd && n > 1)
+    return fail(SDCA_ERR_ARG_RANGE, "D in S's place needs S's leading dimension (%lld and %lld)",
+                (long long)ldd, (long long)lds);
+  const bool host = (flags & SDCA_HOST_PTR) != 0;
+  if (host && (rc = check_labels(labels, m, n))) return rc;
+  if (host) work = nullptr;
+  DeviceBuffer dS, dl, dg, dh, ds, dD, dp;
+  LogProbsGradLaunch a;
+  a.data = data;
+  a.m = m;
+  a.n = n;
+  a.lds = lds;
+  a.ldd = ldd;
+  a.inv_t = 1.f / static_cast<float>(temperature);
+  a.stream = stream;
+  if ((rc = staged(S, span(m, n, lds, element_size(data)), host, dS, stream, &a.S)) ||
+      (rc = staged(labels, n * sizeof(int64_t), host, dl, stream, &a.labels)) ||
+      (rc = staged(g, n * sizeof(float), host, dg, stream, &a.g)) ||
+      (rc = staged(h, n * sizeof(float), host, dh, stream, &a.h)) ||
+      (rc = staged(stats, 3 * n * sizeof(float), host, ds, stream, &a.stats)) ||
+      (rc = staged_out(D, span(m, n, ldd, element_size(data)), host, dD, &a.D)) ||
+      (rc = staged_out(logp, n * sizeof(float), host, dp, &a.logp)) ||
+      (rc = scratch(work, log_probs_grad_work_bytes(data, m, n, stats != nullptr), stream, &a.work)))
+    return rc;
+  SDCA_HIP_TRY(launch_log_probs_grad(a), "log-probability gradient kernels");
+  if (host) {
+    if ((rc = fetch_columns(D, a.D, m, n, ldd, element_size(data), stream)) ||
+        (logp && (rc = fetch_columns(logp, a.logp, n, 1, n, sizeof(float), stream))))
+      return rc;
+    SDCA_HIP_TRY(hipStreamSynchronize(stream), "hipStreamSynchronize");
+  }
+  return SDCA_OK;
+}
+
 // Nothing is thrown through the C boundary (the workspace cache's map and
 // the messages can run out of memory).
 template <class F>
@@ -1486,6 +1612,36 @@ int sdca_sample(sdca_dtype data, int64_t m, int64_t n, const void* S, int64_t ld
   return guarded([&] {
     return sample_common(data, m, n, S, lds, u, params, columns, labels, prob, kept, flags,
                          static_cast<hipStream_t>(stream));
+  });
+}
+
+size_t sdca_log_probs_work(sdca_dtype data, int64_t m, int64_t n, int64_t top) {
+  if (m < 1 || n < 1 || top < 0 || top > sdca_gpu::kMostTop) return 0;
+  return sdca_gpu::log_probs_work_bytes(data, m, n, static_cast<int>(top));
+}
+
+int sdca_log_probs(sdca_dtype data, int64_t m, int64_t n, const void* S, int64_t lds,
+                   const int64_t* labels, double temperature, int64_t top, float* logp,
+                   float* entropy, float* stats, float* top_logp, int64_t* top_index, void* work,
+                   unsigned flags, void* stream) {
+  return guarded([&] {
+    return log_probs_common(data, m, n, S, lds, labels, temperature, top, logp, entropy, stats,
+                            top_logp, top_index, work, flags, static_cast<hipStream_t>(stream));
+  });
+}
+
+size_t sdca_log_probs_grad_work(sdca_dtype data, int64_t m, int64_t n, const float* stats) {
+  if (m < 1 || n < 1) return 0;
+  return sdca_gpu::log_probs_grad_work_bytes(data, m, n, stats != nullptr);
+}
+
+int sdca_log_probs_grad(sdca_dtype data, int64_t m, int64_t n, const void* S, int64_t lds,
+                        const int64_t* labels, const float* g, const float* h,
+                        const float* stats, double temperature, void* D, int64_t ldd,
+                        float* logp, void* work, unsigned flags, void* stream) {
+  return guarded([&] {
+    return log_probs_grad_common(data, m, n, S, lds, labels, g, h, stats, temperature, D, ldd,
+                                 logp, work, flags, static_cast<hipStream_t>(stream));
   });
 }
 

@@ -1,0 +1,673 @@
+// Log-probabilities of given labels, and their gradient.
+//
+// For a column of m scores s with the largest M and a temperature T, the
+// weights are w_j = exp((s_j - M) / T) (1 where s_j = M), Z their sum and
+// p_j = w_j / Z the probabilities; a label's log-probability is log p_label,
+// the entropy H = log Z - sum w_j log w_j / Z, and with a gradient g of the
+// log-probability and h of the entropy the scores' gradient is
+//   d_j = (g ([j = label] - p_j) - h p_j (log p_j + H)) / T.
+//
+// A column goes by once: each lane keeps a running maximum with Z and
+// sum w log w relative to it, and brings them to a larger maximum when one
+// comes.  Exponents are in base 2, relative to a reference rather than to
+// the maximum itself: with c = log2(e) / T and ref = M c rounded and held
+// within +-1e30, e_j = fma(s_j, c, -ref) is one instruction, and the same
+// reference in every term cancels in the differences that are the results.
+// Masked scores at the type's lowest value or -infinity then have weight 0
+// beside any ordinary score.  A column whose M c is beyond 1e30 (scores near
+// the largest float, +infinity, or nothing but lowest values) is gone through
+// a second time with exponents from s_j - M.
+#include "answer_launch.hpp"
+#include "answer_limits.hpp"
+#include "answer_types.hpp"
+#include "answer_wave.hpp"
+#include "common.hpp"
+
+namespace sdca_gpu {
+namespace {
+
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+constexpr float kFar = 1e30f;
+constexpr float kLowest = -3.402823466e38f;
+// Exponents below this have weight 0, and 0 times this is 0.
+constexpr float kGone = -200.f;
+
+__device__ inline float exp2_of(float e) { return __builtin_amdgcn_exp2f(e); }
+__device__ inline float ref_of(float max, float c) { return fminf(fmaxf(max * c, -kFar), kFar); }
+
+template <bool VALU>
+__device__ inline float wave_largest(float v) {
+  v = fmaxf(v, other<1, VALU>(v));
+  v = fmaxf(v, other<2, VALU>(v));
+  v = fmaxf(v, other<4, VALU>(v));
+  v = fmaxf(v, other<8, VALU>(v));
+  v = fmaxf(v, other<16, VALU>(v));
+  return fmaxf(v, other<32, VALU>(v));
+}
+
+// The weights of some scores: their largest, and the sums of 2^e and e 2^e
+// with exponents relative to ref_of(max).  (A NaN among the scores makes the
+// sums NaN and leaves max.)
+struct Mass {
+  float max = -INFINITY, sum = 0.f, weighted = 0.f;
+
+  __device__ void rise(float to, float c) {  // to a larger or equal maximum
+    const float by = ref_of(max, c) - ref_of(to, c), f = exp2_of(by);
+    weighted = f * fmaf(fmaxf(by, kGone), sum, weighted);
+    sum *= f;
+    max = to;
+  }
+  // All lanes' together, in every lane.
+  __device__ void over_wave(float c) {
+    rise(wave_largest<true>(max), c);
+    sum = wave_total(sum);
+    weighted = wave_total(weighted);
+  }
+};
+
+// ---------------------------------------------------------------------------
+// The best of a column: a wave's 64 entries (score, index) by lane, falling.
+// Candidates, which are scores of at least `bound`, gather in LDS; 64 of
+// them are sorted and merged into the list.
+// ---------------------------------------------------------------------------
+struct Best {
+  u64 list = 0;
+  float bound = kLowest;  // a score below it, or -infinity or NaN, is none
+  int waiting = 0;
+
+  __device__ void merge_sorted(u64 rising) {
+    list = rising > list ? rising : list;
+    list = sort_merge<32, true>(list, true);
+  }
+  __device__ void merge(u64 some, int top) {
+    merge_sorted(sort_wave<true>(some, false));
+    const u64 last = read_lane64(list, top - 1);
+    if (last) bound = fmaxf(bound, score_of(static_cast<unsigned>(last >> 32)));
+  }
+  __device__ void take(float s, int index, bool candidate, u64* room, int top) {
+    const u64 mask = __ballot(candidate);
+    if (!mask) return;
+    const int lane = threadIdx.x & 63;
+    if (candidate) {
+      const int before = __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask >> 32),
+                                                   __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask), 0));
+      room[waiting + before] = entry_of(s, index);
+    }
+    waiting += __popcll(mask);
+    wave_lds_sync();
+    if (waiting < 64) return;
+    const u64 first = room[lane], rest = room[64 + lane];
+    wave_lds_sync();
+    room[lane] = rest;
+    wave_lds_sync();
+    waiting -= 64;
+    merge(first, top);
+  }
+  // Behind scores of lower index than all that follow: of those, ones equal
+  // to the last of a full list come after it.
+  __device__ void pass(int top) {
+    const u64 last = read_lane64(list, top - 1);
+    if (!last) return;
+    const unsigned key = static_cast<unsigned>(last >> 32);
+    if (score_of(key) == bound) bound = score_of(key + 1);
+  }
+  __device__ void finish(u64* room, int top) {
+    if (!waiting) return;
+    const int lane = threadIdx.x & 63;
+    merge(lane < waiting ? room[lane] : 0, top);
+    waiting = 0;
+  }
+};
+
+struct LogProbsArgs {
+  int m;
+  int64_t n, lds;
+  const int64_t* labels;
+  float inv_t;
+  int top;
+  float *logp, *entropy, *stats, *top_logp;
+  int64_t* top_index;
+  // Columns in parts: `length` scores each, their masses and best.
+  int parts, length;
+  Mass* masses;
+  u64* lists;
+};
+
+// A column's results, by one wave.
+template <class T>
+__device__ void finish(const T* row, int64_t col, Mass mass, u64 list, const LogProbsArgs& a) {
+  const int lane = threadIdx.x & 63;
+  const float c = a.inv_t * kLog2e, max = mass.max, ref = ref_of(max, c);
+  const bool near = fabsf(max * c) <= kFar;
+  const auto exponent = [&](float s) { return near ? fmaf(s, c, -ref) : fminf(s - max, 0.f) * c; };
+  if (!near && max > -INFINITY) {
+    float sum = 0.f, weighted = 0.f;
+    bool bad = false;
+    for (int64_t i = lane; i < a.m; i += 64) {
+      const float s = to_float(row[i]), e = exponent(s), w = exp2_of(e);
+      bad |= s != s;
+      sum += w;
+      weighted = fmaf(w, fmaxf(e, kGone), weighted);
+    }
+    mass.sum = __ballot(bad) ? NAN : wave_total(sum);
+    mass.weighted = wave_total(weighted);
+  }
+  const bool none = max == -INFINITY && mass.sum == 0.f;
+  const float log_sum = log2f(mass.sum);
+  float entropy = none ? 0.f : (log_sum - mass.weighted / mass.sum) * kLn2;
+  if (entropy < 0.f) entropy = 0.f;
+  const auto logp = [&](float s) { return none ? -INFINITY : (exponent(s) - log_sum) * kLn2; };
+  if (lane == 0) {
+    if (a.logp) {
+      const int64_t label = a.labels[col];
+      a.logp[col] = label == -1 ? 0.f : label < 0 || label >= a.m ? NAN : logp(to_float(row[label]));
+    }
+    if (a.entropy) a.entropy[col] = entropy;
+    if (a.stats) {
+      float* out = a.stats + 3 * col;
+      out[0] = max;
+      // The sum relative to the maximum, not to the reference.
+      out[1] = none ? -INFINITY : (log_sum - exponent(max)) * kLn2;
+      out[2] = entropy;
+    }
+  }
+  if (lane < a.top) {
+    const float s = score_of(static_cast<unsigned>(list >> 32));
+    if (a.top_logp) a.top_logp[col * a.top + lane] = list ? logp(s) : -INFINITY;
+    if (a.top_index) a.top_index[col * a.top + lane] = list ? index_of(list) : -1;
+  }
+}
+
+// The masses of WAVES waves, and their best, in the first.
+template <int WAVES, bool TOP>
+__device__ inline void join_waves(Mass& mass, u64& list, u64 (*room)[128], float c, int wave) {
+  __shared__ float of_wave[WAVES][3];
+  const int lane = threadIdx.x & 63;
+  if (lane == 0) {
+    of_wave[wave][0] = mass.max;
+    of_wave[wave][1] = mass.sum;
+    of_wave[wave][2] = mass.weighted;
+  }
+#pragma unroll
+  for (int s = 1; s < WAVES; s *= 2) {
+    if (TOP && (wave & (2 * s - 1)) == s) room[wave][lane] = list;
+    if (TOP || s == 1) __syncthreads();
+    if (TOP && (wave & (2 * s - 1)) == 0) {
+      Best b;
+      b.list = list;
+      b.merge_sorted(room[wave + s][63 - lane]);
+      list = b.list;
+    }
+  }
+  if (wave == 0) {
+    mass = Mass();
+    if (lane < WAVES) {
+      mass.max = of_wave[lane][0];
+      mass.sum = of_wave[lane][1];
+      mass.weighted = of_wave[lane][2];
+    }
+    mass.over_wave(c);
+  }
+}
+
+// WAVES waves to a column, or to a part of it; with one wave, four columns to
+// a workgroup.  A wave takes 64 kLoads vectors of 16 bytes at a time.
+template <class T, int WAVES, bool TOP>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void log_probs_kernel(
+    const T* __restrict__ S, LogProbsArgs a) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T)), kLoads = 4, kStep = 64 * V * kLoads;
+  constexpr int kColumns = WAVES == 1 ? 4 : 1;
+  __shared__ u64 room[TOP ? kColumns * WAVES : 1][128];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * kColumns + (WAVES == 1 ? wave : 0);
+  if (WAVES == 1 && col >= a.n) return;  // whole waves, and no barrier below
+  const T* row = S + col * a.lds;
+  const float c = a.inv_t * kLog2e;
+  const int first = blockIdx.y * a.length, end = min(a.m, first + a.length);
+
+  Mass mass;
+  Best best;
+  bool started = false;
+  for (int64_t at = first + (WAVES == 1 ? 0 : wave) * kStep; at < end; at += WAVES * kStep) {
+    float v[kLoads][V];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) load_vec<V>(row, at + (u * 64 + lane) * V, end, v[u], -INFINITY);
+    float most = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) most = fmaxf(most, v[u][e]);
+    if (most > mass.max) mass.rise(most, c);
+    const float ref = ref_of(mass.max, c);
+    float sum = 0.f, weighted = 0.f;
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float x = fmaf(v[u][e], c, -ref), w = exp2_of(x);
+        sum += w;
+        weighted = fmaf(w, fmaxf(x, kGone), weighted);
+      }
+    mass.sum += sum;
+    mass.weighted += weighted;
+    if constexpr (TOP) {
+      if (!started) {
+        // `top` lanes have a score of at least this.
+        best.bound = fmaxf(read_lane(sort_wave<true>(most, true), a.top - 1), kLowest);
+        started = true;
+      }
+      if (__ballot(most >= best.bound)) {
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            best.take(v[u][e], static_cast<int>(at) + (u * 64 + lane) * V + e, v[u][e] >= best.bound,
+                      room[wave], a.top);
+        best.pass(a.top);
+      }
+    }
+  }
+  if constexpr (TOP) best.finish(room[wave], a.top);
+  mass.over_wave(c);
+  if constexpr (WAVES > 1) {
+    join_waves<WAVES, TOP>(mass, best.list, room, c, wave);
+    if (wave) return;
+  }
+  if (a.parts == 1) {
+    finish(row, col, mass, best.list, a);
+  } else {
+    const int64_t part = col * a.parts + blockIdx.y;
+    if (lane == 0) a.masses[part] = mass;
+    if (TOP && lane < a.top) a.lists[part * a.top + lane] = best.list;
+  }
+}
+
+// A column from its parts (64 of them at most).
+constexpr int kJoinWaves = 4;
+template <class T, bool TOP>
+__global__ __launch_bounds__(64 * kJoinWaves) void log_probs_join_kernel(const T* __restrict__ S,
+                                                                         LogProbsArgs a) {
+  __shared__ u64 room[TOP ? kJoinWaves : 1][128];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t col = blockIdx.x;
+  const float c = a.inv_t * kLog2e;
+  Mass mass;
+  const int mine = wave + lane * kJoinWaves;
+  if (mine < a.parts) mass = a.masses[col * a.parts + mine];
+  mass.over_wave(c);
+  Best best;
+  if constexpr (TOP) {
+    for (int p = wave; p < a.parts; p += kJoinWaves)
+      best.merge_sorted(63 - lane < a.top ? a.lists[(col * a.parts + p) * a.top + 63 - lane] : 0);
+  }
+  join_waves<kJoinWaves, TOP>(mass, best.list, room, c, wave);
+  if (wave == 0) finish(S + col * a.lds, col, mass, best.list, a);
+}
+
+// How a launch takes the columns: waves to a part, parts to a column.
+struct LogProbsPlan {
+  int waves, parts, length;
+};
+LogProbsPlan plan_log_probs(int64_t m, int64_t n) {
+  const auto split = [&](int64_t parts) {
+    const int64_t length = ((m + parts - 1) / parts + 2047) / 2048 * 2048;
+    return LogProbsPlan{4, static_cast<int>((m + length - 1) / length), static_cast<int>(length)};
+  };
+  if (m <= 2048) return {1, 1, static_cast<int>(m)};
+  if (n < 256 && m > 32768) {
+    const int64_t parts = (1024 + n - 1) / n, most = (m + 8191) / 8192;
+    return split(parts < most ? (parts < 64 ? parts : 64) : (most < 64 ? most : 64));
+  }
+  if (n < 512) return {16, 1, static_cast<int>(m)};
+  return {4, 1, static_cast<int>(m)};
+}
+
+template <class T, int WAVES, bool TOP>
+void start(const LogProbsLaunch& l, LogProbsArgs a) {
+  constexpr int64_t kColumns = WAVES == 1 ? 4 : 1;
+  constexpr int kThreads = WAVES == 1 ? 256 : 64 * WAVES;
+  const int64_t n = a.n;
+  each_slice(n, kColumns, static_cast<int64_t>(kThreads) * a.parts, [&](int64_t first, int64_t count) {
+    LogProbsArgs s = a;
+    s.n = count;
+    s.labels = a.labels + first;
+    if (a.logp) s.logp = a.logp + first;
+    if (a.entropy) s.entropy = a.entropy + first;
+    if (a.stats) s.stats = a.stats + 3 * first;
+    if (a.top_logp) s.top_logp = a.top_logp + first * a.top;
+    if (a.top_index) s.top_index = a.top_index + first * a.top;
+    s.masses = a.masses + first * a.parts;
+    s.lists = a.lists + first * a.parts * a.top;
+    const T* S = static_cast<const T*>(l.S) + first * a.lds;
+    log_probs_kernel<T, WAVES, TOP>
+        <<<dim3(static_cast<unsigned>((count + kColumns - 1) / kColumns), a.parts), kThreads, 0, l.stream>>>(S, s);
+    if (a.parts > 1)
+      log_probs_join_kernel<T, TOP><<<static_cast<unsigned>(count), 64 * kJoinWaves, 0, l.stream>>>(S, s);
+  });
+}
+
+template <class T, bool TOP>
+void log_probs(const LogProbsLaunch& l) {
+  const LogProbsPlan plan = plan_log_probs(l.m, l.n);
+  LogProbsArgs a = {};
+  a.m = static_cast<int>(l.m);
+  a.n = l.n;
+  a.lds = l.lds;
+  a.labels = l.labels;
+  a.inv_t = l.inv_t;
+  a.top = l.top;
+  a.logp = l.logp;
+  a.entropy = l.entropy;
+  a.stats = l.stats;
+  a.top_logp = l.top_logp;
+  a.top_index = l.top_index;
+  a.parts = plan.parts;
+  a.length = plan.length;
+  a.masses = static_cast<Mass*>(l.work);
+  a.lists = reinterpret_cast<u64*>(static_cast<char*>(l.work) +
+                                   (plan.parts > 1 ? (l.n * plan.parts * sizeof(Mass) + 15) / 16 * 16 : 0));
+  switch (plan.waves) {
+    case 1: return start<T, 1, TOP>(l, a);
+    case 4: return start<T, 4, TOP>(l, a);
+    default: return start<T, 16, TOP>(l, a);
+  }
+}
+
+template <class T>
+hipError_t log_probs(const LogProbsLaunch& l) {
+  l.top ? log_probs<T, true>(l) : log_probs<T, false>(l);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// The gradient.
+// ---------------------------------------------------------------------------
+struct GradArgs {
+  int m;
+  int64_t n, lds, ldd;
+  const int64_t* labels;
+  const float *g, *h, *stats;
+  float inv_t;
+  float* logp;
+};
+
+// A column's own numbers.  `g` and `h` are the gradients over T.
+struct GradColumn {
+  float max, log2_sum, entropy, g, h;
+  int label;
+  bool none;
+  __device__ GradColumn(const GradArgs& a, int64_t col) {
+    const int64_t l = a.labels[col];
+    label = l >= 0 && l < a.m ? static_cast<int>(l) : -1;
+    g = l == -1 ? 0.f : label < 0 ? NAN : a.g[col] * a.inv_t;
+    h = a.h ? a.h[col] * a.inv_t : 0.f;
+    if (a.logp && label < 0 && threadIdx.x % 64 == 0) a.logp[col] = l == -1 ? 0.f : NAN;
+  }
+  // log2 p -> the gradient of a score that is not the label's.
+  __device__ float of(float e) const {
+    const float p = exp2_of(e);
+    return none ? (g != g ? g : 0.f) : -p * fmaf(h, fmaf(fmaxf(e, kGone), kLn2, entropy), g);
+  }
+};
+
+template <class T, int V>
+__device__ inline void store_vec(T* row, int64_t at, int64_t len, const T (&v)[V]) {
+  if (at + V <= len) {
+    __builtin_memcpy(row + at, v, sizeof(v));
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (at + e < len) row[at + e] = v[e];
+  }
+}
+
+// V scores of a column to their gradients; the lane that has the label's
+// writes its log-probability.  (S and D may be one matrix: a lane has read
+// what it writes.)
+template <class T, int V, class Exponent>
+__device__ inline void grad_vec(const float (&s)[V], int at, const GradColumn& c, Exponent exponent,
+                                float* logp, T (&d)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) d[e] = from_float<T>(c.of(exponent(s[e])));
+  if (c.label >= at && c.label < at + V) {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (c.label == at + e) {
+        const float x = exponent(s[e]);
+        if (!c.none) d[e] = from_float<T>(c.of(x) + c.g);
+        if (logp) *logp = c.none ? -INFINITY : x * kLn2;
+      }
+  }
+}
+
+// From the columns' statistics.  A workgroup takes 256 kLoads vectors of a
+// column (ROWS = 1), or each of its waves a column of its own.
+template <class T, int ROWS>
+__global__ __launch_bounds__(256) void log_probs_grad_kernel(const T* S, T* D, GradArgs a) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T)), kLoads = 4, kLanes = 256 / ROWS;
+  const int lane = threadIdx.x % kLanes;
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / kLanes;
+  if (col >= a.n) return;
+  GradColumn c(a, col);
+  const float* stats = a.stats + 3 * col;
+  c.max = stats[0];
+  c.log2_sum = stats[1] * kLog2e;
+  c.entropy = stats[2];
+  c.none = c.max == -INFINITY && c.log2_sum == -INFINITY;
+  const float by = a.inv_t * kLog2e;
+  const auto exponent = [&](float s) { return fmaf(fminf(s - c.max, 0.f), by, -c.log2_sum); };
+  const T* s = S + col * a.lds;
+  T* d = D + col * a.ldd;
+  for (int64_t at0 = static_cast<int64_t>(blockIdx.y) * kLanes * V * kLoads; at0 < a.m;
+       at0 += static_cast<int64_t>(gridDim.y) * kLanes * V * kLoads) {
+    float v[kLoads][V];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) load_vec<V>(s, at0 + (u * kLanes + lane) * V, a.m, v[u], -INFINITY);
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int64_t at = at0 + (u * kLanes + lane) * V;
+      if (at >= a.m) break;
+      T out[V];
+      grad_vec<T, V>(v[u], static_cast<int>(at), c, exponent, a.logp ? a.logp + col : nullptr, out);
+      store_vec(d, at, a.m, out);
+    }
+  }
+}
+
+// The whole column in registers: its statistics and then its gradient from
+// one reading.  WAVES waves to a column (with one, four columns to a
+// workgroup), NV vectors to a lane.
+template <class T, int WAVES, int NV>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void log_probs_grad_whole_kernel(
+    const T* S, T* D, GradArgs a) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T)), kLanes = 64 * WAVES;
+  constexpr int kColumns = WAVES == 1 ? 4 : 1;
+  __shared__ float part[3][WAVES];
+  const int lane = threadIdx.x % kLanes;
+  const int wave = __builtin_amdgcn_readfirstlane(lane >> 6);
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * kColumns + threadIdx.x / kLanes;
+  if (WAVES == 1 && col >= a.n) return;
+  const T* s = S + col * a.lds;
+  T raw[NV][V];
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    const int64_t at = static_cast<int64_t>(u * kLanes + lane) * V;
+    if (at + V <= a.m) {
+      __builtin_memcpy(raw[u], s + at, 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) raw[u][e] = at + e < a.m ? s[at + e] : from_float<T>(-INFINITY);
+    }
+  }
+  GradColumn c(a, col);
+  float max = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < NV; ++u)
+#pragma unroll
+    for (int e = 0; e < V; ++e) max = fmaxf(max, to_float(raw[u][e]));
+  max = wave_largest<true>(max);
+  if constexpr (WAVES > 1) {
+    if ((threadIdx.x & 63) == 0) part[0][wave] = max;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) max = fmaxf(max, part[0][w]);
+  }
+  const float by = a.inv_t * kLog2e, ref = ref_of(max, by);
+  float sum = 0.f, weighted = 0.f;
+  const auto add = [&](auto exponent) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float x = exponent(to_float(raw[u][e])), w = exp2_of(x);
+        sum += w;
+        weighted = fmaf(w, fmaxf(x, kGone), weighted);
+      }
+  };
+  const bool near = fabsf(max * by) <= kFar || max == -INFINITY;
+  if (near) {
+    add([&](float x) { return fmaf(x, by, -ref); });
+  } else {
+    // (NaN keeps its NaN: the smaller of it and 0 would be 0.)
+    add([&](float x) { return x != x ? x : fminf(x - max, 0.f) * by; });
+  }
+  sum = wave_total(sum);
+  weighted = wave_total(weighted);
+  if constexpr (WAVES > 1) {
+    if ((threadIdx.x & 63) == 0) part[1][wave] = sum, part[2][wave] = weighted;
+    __syncthreads();
+    sum = weighted = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) sum += part[1][w], weighted += part[2][w];
+  }
+  c.max = max;
+  c.none = max == -INFINITY && sum == 0.f;
+  c.log2_sum = log2f(sum);
+  c.entropy = (c.log2_sum - weighted / sum) * kLn2;
+  if (c.entropy < 0.f) c.entropy = 0.f;
+  T* d = D + col * a.ldd;
+  const auto write = [&](auto exponent) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int64_t at = static_cast<int64_t>(u * kLanes + lane) * V;
+      if (at >= a.m) break;
+      float v[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = to_float(raw[u][e]);
+      T out[V];
+      grad_vec<T, V>(v, static_cast<int>(at), c, exponent, a.logp ? a.logp + col : nullptr, out);
+      store_vec(d, at, a.m, out);
+    }
+  };
+  if (near) write([&](float x) { return fmaf(x, by, -ref) - c.log2_sum; });
+  else write([&](float x) { return fmaf(fminf(x - max, 0.f), by, -c.log2_sum); });
+}
+
+// Columns that the whole-column kernel holds.
+template <class T>
+constexpr int64_t whole_most() { return 64 * 16 * 8 * 16 / static_cast<int64_t>(sizeof(T)); }
+
+template <class T>
+GradArgs args_of(const LogProbsGradLaunch& l, int64_t first, int64_t count) {
+  GradArgs a;
+  a.m = static_cast<int>(l.m);
+  a.n = count;
+  a.lds = l.lds;
+  a.ldd = l.ldd;
+  a.labels = l.labels + first;
+  a.g = l.g + first;
+  a.h = l.h ? l.h + first : nullptr;
+  a.stats = l.stats ? l.stats + 3 * first : nullptr;
+  a.inv_t = l.inv_t;
+  a.logp = l.logp ? l.logp + first : nullptr;
+  return a;
+}
+
+template <class T, int WAVES, int NV>
+void start_whole(const LogProbsGradLaunch& l) {
+  constexpr int64_t kColumns = WAVES == 1 ? 4 : 1;
+  constexpr int kThreads = WAVES == 1 ? 256 : 64 * WAVES;
+  each_slice(l.n, kColumns, kThreads, [&](int64_t first, int64_t count) {
+    log_probs_grad_whole_kernel<T, WAVES, NV>
+        <<<static_cast<unsigned>((count + kColumns - 1) / kColumns), kThreads, 0, l.stream>>>(
+            static_cast<const T*>(l.S) + first * l.lds, static_cast<T*>(l.D) + first * l.ldd,
+            args_of<T>(l, first, count));
+  });
+}
+
+template <class T, int ROWS>
+void start_grad(const LogProbsGradLaunch& l) {
+  constexpr int64_t kEach = 256 / ROWS * (16 / sizeof(T)) * 4;
+  const int64_t parts = ROWS > 1 ? 1 : (l.m + kEach - 1) / kEach;
+  const unsigned across = static_cast<unsigned>(parts < 1024 ? parts : 1024);
+  each_slice(l.n, ROWS, 256 * static_cast<int64_t>(across), [&](int64_t first, int64_t count) {
+    log_probs_grad_kernel<T, ROWS>
+        <<<dim3(static_cast<unsigned>((count + ROWS - 1) / ROWS), across), 256, 0, l.stream>>>(
+            static_cast<const T*>(l.S) + first * l.lds, static_cast<T*>(l.D) + first * l.ldd,
+            args_of<T>(l, first, count));
+  });
+}
+
+template <class T>
+hipError_t log_probs_grad(LogProbsGradLaunch l) {
+  constexpr int64_t V = 16 / sizeof(T);
+  if (!l.stats) {
+    if (l.m <= 64 * V) return start_whole<T, 1, 1>(l), hipGetLastError();
+    if (l.m <= 64 * V * 4) return start_whole<T, 1, 4>(l), hipGetLastError();
+    if (l.m <= 256 * V * 4) return start_whole<T, 4, 4>(l), hipGetLastError();
+    if (l.m <= 256 * V * 8) return start_whole<T, 4, 8>(l), hipGetLastError();
+    if (l.m <= 1024 * V * 4) return start_whole<T, 16, 4>(l), hipGetLastError();
+    if (l.m <= whole_most<T>()) return start_whole<T, 16, 8>(l), hipGetLastError();
+    LogProbsLaunch s = {};
+    s.data = l.data;
+    s.m = l.m;
+    s.n = l.n;
+    s.S = l.S;
+    s.lds = l.lds;
+    s.labels = l.labels;
+    s.inv_t = l.inv_t;
+    s.stats = static_cast<float*>(l.work);
+    s.work = static_cast<char*>(l.work) + (3 * l.n * sizeof(float) + 15) / 16 * 16;
+    s.stream = l.stream;
+    l.stats = s.stats;
+    const hipError_t e = launch_log_probs(s);
+    if (e != hipSuccess) return e;
+  }
+  if (l.m <= 64 * V * 4) start_grad<T, 4>(l);
+  else start_grad<T, 1>(l);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+size_t log_probs_work_bytes(int, int64_t m, int64_t n, int top) {
+  const LogProbsPlan plan = plan_log_probs(m, n);
+  if (plan.parts == 1) return 0;
+  return (static_cast<size_t>(n) * plan.parts * sizeof(Mass) + 15) / 16 * 16 +
+         static_cast<size_t>(n) * plan.parts * top * sizeof(u64);
+}
+
+hipError_t launch_log_probs(const LogProbsLaunch& l) {
+  switch (l.data) {
+    case SDCA_F32: return log_probs<float>(l);
+    case SDCA_F16: return log_probs<__half>(l);
+    default: return log_probs<__hip_bfloat16>(l);
+  }
+}
+
+size_t log_probs_grad_work_bytes(int data, int64_t m, int64_t n, bool stats) {
+  if (stats || m <= (data == SDCA_F32 ? whole_most<float>() : whole_most<__half>())) return 0;
+  return (3 * static_cast<size_t>(n) * sizeof(float) + 15) / 16 * 16 + log_probs_work_bytes(data, m, n, 0);
+}
+
+hipError_t launch_log_probs_grad(const LogProbsGradLaunch& l) {
+  switch (l.data) {
+    case SDCA_F32: return log_probs_grad<float>(l);
+    case SDCA_F16: return log_probs_grad<__half>(l);
+    default: return log_probs_grad<__hip_bfloat16>(l);
+  }
+}
+
+}  // namespace sdca_gpu
