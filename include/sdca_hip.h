@@ -558,6 +558,61 @@ int sdca_log_probs_grad(sdca_dtype data, int64_t m, int64_t n, const void* S, in
                         const float* stats, double temperature, void* D, int64_t ldd,
                         float* logp, void* work, unsigned flags, void* stream);
 
+/*
+ * Low-rank adapters of one weight matrix: example i's scores get
+ * scale_a B_a (A_a x_i), a = index[i].
+ *   count (1..65535) adapters of `rank` (1..128);
+ *   A: count times a d x rank matrix, B: count times a rank x m one, column-
+ *      major, contiguous and one behind the other, in the examples' type;
+ *   index: n adapters in [0, count), or -1 for an example without one.
+ *      Another one is SDCA_ERR_ARG_RANGE in host arrays; in device memory it
+ *      gives the example NaN scores, and no part in a gradient;
+ *   scale: count values, or NULL: `factor` for all adapters.
+ */
+typedef struct sdca_adapters {
+  int64_t count, rank;
+  const void* A;
+  const void* B;
+  const int64_t* index;
+  const float* scale;
+  double factor;
+} sdca_adapters;
+
+/*
+ * Scores from shared 8-bit weights with an adapter for each example:
+ *   S_i = sdca_scores_i8's for float examples + scale_a B_a (A_a x_i),
+ * the second part of x_i itself, not of its 8-bit form, in 32 bits; the two
+ * are added in 32 bits and rounded to `out` once.  data, and the adapters'
+ * type: SDCA_F32, SDCA_F16 or SDCA_BF16; the other arguments and their limits
+ * as in sdca_scores_i8.  An example's scores depend on its own adapter alone.
+ *   work: device memory of at least sdca_scores_adapted_work bytes, 256-byte
+ *      aligned, or NULL: the stream's scratch, as in sdca_log_probs.
+ */
+size_t sdca_scores_adapted_work(sdca_dtype data, int64_t d, int64_t m, int64_t n,
+                                const int8_t* W, int64_t ldw, int64_t rank);
+int sdca_scores_adapted(sdca_dtype data, sdca_dtype out, int64_t d, int64_t m, int64_t n,
+                        const void* X, int64_t ldx, const int8_t* W, int64_t ldw, const float* sw,
+                        const sdca_adapters* adapters, void* S, int64_t lds, void* work,
+                        unsigned flags, void* stream);
+
+/*
+ * The adapters' gradients where G (m x n, leading dimension ldg; grad
+ * SDCA_F32, SDCA_F16 or SDCA_BF16) is that of such scores: with the sums over
+ * the examples i of adapter a
+ *   dA_a = scale_a sum x_i (B_a' g_i)',   dB_a = scale_a sum (A_a x_i) g_i',
+ * laid out as A and B, in 32-bit floats whatever the types (zeros for an
+ * adapter without examples).  The sums' order depends on the sizes and the
+ * index alone.  The examples are data and the weights fixed: neither has a
+ * gradient.  d and m are at most 2^30 - 1.
+ *   work: as above, sdca_scores_adapted_grad_work bytes.
+ */
+size_t sdca_scores_adapted_grad_work(sdca_dtype data, sdca_dtype grad, int64_t d, int64_t m,
+                                     int64_t n, int64_t count, int64_t rank);
+int sdca_scores_adapted_grad(sdca_dtype data, sdca_dtype grad, int64_t d, int64_t m, int64_t n,
+                             const void* G, int64_t ldg, const void* X, int64_t ldx,
+                             const sdca_adapters* adapters, float* dA, float* dB, void* work,
+                             unsigned flags, void* stream);
+
 /* Message of the last failure on this thread ("" if none). */
 const char* sdca_last_error(void);
 

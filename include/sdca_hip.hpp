@@ -25,6 +25,7 @@
 #include <stdexcept>
 #include <string>
 #include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "sdca_hip.h"
@@ -347,6 +348,60 @@ inline std::vector<std::int64_t> sample(std::int64_t m, std::int64_t n, const Da
   detail::check(sdca_sample(detail::dtype<Data>::value, m, n, S, m, u, &params, nullptr,
                             labels.data(), prob, nullptr, SDCA_HOST_PTR, nullptr));
   return labels;
+}
+
+// The log-probabilities of n labels (-1: none) in n columns of m scores, and
+// optionally the columns' entropies (n) and statistics (3 n).
+template <typename Data>
+inline std::vector<float> log_probs(std::int64_t m, std::int64_t n, const Data* S,
+                                    const std::int64_t* labels, double temperature = 1,
+                                    float* entropy = nullptr, float* stats = nullptr) {
+  std::vector<float> logp(static_cast<size_t>(n));
+  detail::check(sdca_log_probs(detail::dtype<Data>::value, m, n, S, m, labels, temperature, 0,
+                               logp.data(), entropy, stats, nullptr, nullptr, nullptr,
+                               SDCA_HOST_PTR, nullptr));
+  return logp;
+}
+
+// The scores' gradient (m x n) from that of the log-probabilities, g, and of
+// the entropies, h (optional).
+template <typename Data>
+inline std::vector<Data> log_probs_grad(std::int64_t m, std::int64_t n, const Data* S,
+                                        const std::int64_t* labels, const float* g,
+                                        const float* h = nullptr, double temperature = 1) {
+  std::vector<Data> D(static_cast<size_t>(m) * static_cast<size_t>(n));
+  detail::check(sdca_log_probs_grad(detail::dtype<Data>::value, m, n, S, m, labels, g, h, nullptr,
+                                    temperature, D.data(), m, nullptr, nullptr, SDCA_HOST_PTR,
+                                    nullptr));
+  return D;
+}
+
+// The m x n scores of n examples with a low-rank adapter for each (the
+// adapters' A, B of Data, on the host).
+template <typename Data>
+inline std::vector<float> scores_adapted(std::int64_t n, const Data* X, const quantized& W,
+                                         const sdca_adapters& adapters) {
+  std::vector<float> S(static_cast<size_t>(W.n) * static_cast<size_t>(n));
+  detail::check(sdca_scores_adapted(detail::dtype<Data>::value, SDCA_F32, W.d, W.n, n, X, W.d,
+                                    W.values.data(), W.ld, W.scales.data(), &adapters, S.data(),
+                                    W.n, nullptr, SDCA_HOST_PTR, nullptr));
+  return S;
+}
+
+// The gradients of the adapters' A and B (the first and the second) from that
+// of such scores, G (m x n).
+template <typename Data>
+inline std::pair<std::vector<float>, std::vector<float>> scores_adapted_grad(
+    std::int64_t d, std::int64_t m, std::int64_t n, const Data* G, const Data* X,
+    const sdca_adapters& adapters) {
+  const size_t rows = static_cast<size_t>(adapters.count) * static_cast<size_t>(adapters.rank);
+  std::pair<std::vector<float>, std::vector<float>> r;
+  r.first.resize(rows * static_cast<size_t>(d));
+  r.second.resize(rows * static_cast<size_t>(m));
+  detail::check(sdca_scores_adapted_grad(detail::dtype<Data>::value, detail::dtype<Data>::value, d,
+                                         m, n, G, m, X, d, &adapters, r.first.data(),
+                                         r.second.data(), nullptr, SDCA_HOST_PTR, nullptr));
+  return r;
 }
 
 // ---------------------------------------------------------------------------

@@ -28,6 +28,8 @@ and the answers of a trained model, which the reference does not have:
     sample(S, u, temperature=1, top_k=0, top_p=1, min_p=0)
     log_probs(S, labels, temperature=1, top=0)
     log_probs_grad(S, labels, g)
+    scores_adapted(X, W, w_scales, A, B, index, scale=1)
+    scores_adapted_grad(G, X, A, B, index, scale=1)
 
 `A` holds n columns of length dim, contiguous (a C-contiguous (n, dim) array
 or tensor, i.e. the column-major dim x n matrix of the reference).  A torch
@@ -51,6 +53,7 @@ __all__ = [
     "OBJECTIVES", "objective", "scores", "eval_features", "eval_kernel", "eval_scores",
     "recompute_primal", "epoch_order", "epoch_features", "epoch_kernel", "BRANCHES",
     "quantize_i8", "scores_i8", "sample", "log_probs", "log_probs_grad",
+    "scores_adapted", "scores_adapted_grad",
 ]
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -118,6 +121,12 @@ class SampleColumns(ctypes.Structure):
                 ("min_p", ctypes.c_void_p), ("top_k", ctypes.c_void_p)]
 
 
+class Adapters(ctypes.Structure):
+    _fields_ = [("count", ctypes.c_int64), ("rank", ctypes.c_int64), ("A", ctypes.c_void_p),
+                ("B", ctypes.c_void_p), ("index", ctypes.c_void_p), ("scale", ctypes.c_void_p),
+                ("factor", ctypes.c_double)]
+
+
 # Objectives of the evaluation pass, named after the reference's makers
 # (objective.h:55-160: make_objective_l2_hinge_topk, ...).
 OBJECTIVES = {
@@ -171,6 +180,15 @@ def library():
         lib.sdca_log_probs_grad_work.argtypes, lib.sdca_log_probs_grad_work.restype = [i32, i64, i64, ptr], size
         lib.sdca_log_probs_grad.argtypes = [i32, i64, i64, ptr, i64, ptr, ptr, ptr, ptr, f64, ptr, i64,
                                             ptr, ptr, u32, ptr]
+        ads = ctypes.POINTER(Adapters)
+        lib.sdca_scores_adapted_work.argtypes = [i32, i64, i64, i64, ptr, i64, i64]
+        lib.sdca_scores_adapted_work.restype = size
+        lib.sdca_scores_adapted.argtypes = [i32, i32, i64, i64, i64, ptr, i64, ptr, i64, ptr, ads, ptr, i64,
+                                            ptr, u32, ptr]
+        lib.sdca_scores_adapted_grad_work.argtypes = [i32, i32, i64, i64, i64, i64, i64]
+        lib.sdca_scores_adapted_grad_work.restype = size
+        lib.sdca_scores_adapted_grad.argtypes = [i32, i32, i64, i64, i64, ptr, i64, ptr, i64, ads, ptr, ptr,
+                                                 ptr, u32, ptr]
         lib.sdca_last_error.restype = ctypes.c_char_p
         lib.sdca_abi_version.restype = ctypes.c_int
         _lib = lib
@@ -1019,3 +1037,93 @@ def log_probs_grad(S, labels, g, g_entropy=None, stats=None, temperature=1.0, ou
     _answer(S, "log_probs_grad", lib.sdca_log_probs_grad, data, m, n, _ptr(S), lds, _ptr(labels), _ptr(g),
             _ptr(g_entropy), _ptr(stats), temperature, _ptr(out), ldd, _ptr(lp), _ptr(work))
     return (out, lp) if logp else out
+
+
+def _stack(x, name, shape, like):
+    """Checks the matrices of all adapters, one behind the other."""
+    if _is_torch(x) != _is_torch(like) or (_is_torch(x) and x.device != like.device):
+        raise SdcaError(2, f"{name}: expected the same kind and device as X")
+    if x.dtype != like.dtype:
+        raise SdcaError(3, f"{name} has element type {x.dtype}, expected {like.dtype}")
+    if tuple(x.shape) != shape:
+        raise SdcaError(2, f"{name} has shape {tuple(x.shape)}, expected {shape}")
+    if not (x.is_contiguous() if _is_torch(x) else x.flags.c_contiguous):
+        raise SdcaError(2, f"{name} must be contiguous")
+
+
+def _adapters(X, A, B, index, scale, m):
+    """(the call's argument, what has to live as long) for the adapters A
+    (count, rank, d), B (count, m, rank)."""
+    n, d = X.shape
+    if len(A.shape) != 3:
+        raise SdcaError(2, f"A must be 3-D (got {len(A.shape)} dimensions)")
+    count, rank = int(A.shape[0]), int(A.shape[1])
+    _stack(A, "A", (count, rank, d), X)
+    _stack(B, "B", (count, m, rank), X)
+    _values(index, "index", n, sys.modules["torch"].int64 if _is_torch(X) else np.int64, X)
+    each = _setting(scale, "scale", count, "float32", X)
+    return Adapters(count, rank, _ptr(A), _ptr(B), _ptr(index), _ptr(each),
+                    1.0 if each is not None else scale), each
+
+
+def scores_adapted(X, W, w_scales, A, B, index, scale=1.0, out=None, dtype=None):
+    """S = scores_i8(X, W, w_scales) + scale[a] (X A[a]^T) B[a]^T with an adapter
+    a = index[i] for each row of X, -1 for none (sdca_scores_adapted): the
+    scores of many requests, each with a low-rank correction of the shared 8-bit
+    weights.  X (n, d) float32, float16 or bfloat16; A (count, rank, d) and
+    B (count, m, rank) contiguous and of X's type, rank at most 128; index n
+    int64; scale a number or count values.  S as scores_i8 gives it."""
+    lib = library()
+    data = _score_type(X)
+    ldx = _pitch(X, "X")
+    n, d = X.shape
+    if _is_torch(W) != _is_torch(X) or (_is_torch(X) and W.device != X.device):
+        raise SdcaError(2, "W: expected the same kind and device as X")
+    if _answer_dtype(W) != I8:
+        raise SdcaError(3, f"W has element type {W.dtype}, expected int8")
+    m = W.shape[0]
+    ldw = _pitch(W, "W", (m, d))
+    f32 = _float32(X)
+    _values(w_scales, "w_scales", m, f32, X)
+    adapters, each = _adapters(X, A, B, index, scale, m)
+    if out is None:
+        if _is_torch(X):
+            out = sys.modules["torch"].empty((n, m), dtype=dtype or f32, device=X.device)
+        else:
+            out = np.empty((n, m), dtype=dtype or f32)
+    elif _is_torch(out) != _is_torch(X) or (_is_torch(X) and out.device != X.device):
+        raise SdcaError(2, "out: expected the same kind and device as X")
+    code = _answer_dtype(out)
+    if code not in (F32, F16, BF16):
+        raise SdcaError(3, f"scores cannot be {out.dtype}")
+    lds = _pitch(out, "out", (n, m))
+    _written(out, "out")
+    work = _scratch(X, lib.sdca_scores_adapted_work, data, d, m, n, _ptr(W), ldw, adapters.rank)
+    _answer(X, "scores_adapted", lib.sdca_scores_adapted, data, code, d, m, n, _ptr(X), ldx, _ptr(W), ldw,
+            _ptr(w_scales), adapters, _ptr(out), lds, _ptr(work))
+    return out
+
+
+def scores_adapted_grad(G, X, A, B, index, scale=1.0):
+    """(dA, dB): the gradients of the adapters where G (n, m) (float32, float16
+    or bfloat16) is that of scores_adapted's scores, float32, laid out as A and
+    B (sdca_scores_adapted_grad); zeros for an adapter that no row has.  The
+    examples and the shared weights are fixed and have none."""
+    lib = library()
+    data = _score_type(X)
+    ldx = _pitch(X, "X")
+    n, d = X.shape
+    if _is_torch(G) != _is_torch(X) or (_is_torch(X) and G.device != X.device):
+        raise SdcaError(2, "G: expected the same kind and device as X")
+    grad = _score_type(G)
+    if G.ndim != 2:
+        raise SdcaError(2, f"G must be 2-D (got {G.ndim} dimensions)")
+    m = G.shape[1]
+    ldg = _pitch(G, "G", (n, m))
+    adapters, each = _adapters(X, A, B, index, scale, m)
+    dA = _empty(tuple(A.shape), "float32", X)
+    dB = _empty(tuple(B.shape), "float32", X)
+    work = _scratch(X, lib.sdca_scores_adapted_grad_work, data, grad, d, m, n, adapters.count, adapters.rank)
+    _answer(X, "scores_adapted_grad", lib.sdca_scores_adapted_grad, data, grad, d, m, n, _ptr(G), ldg, _ptr(X),
+            ldx, adapters, _ptr(dA), _ptr(dB), _ptr(work))
+    return dA, dB

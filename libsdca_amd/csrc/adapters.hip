@@ -1,0 +1,468 @@
+// What low-rank adapters need besides the score product: the examples' terms
+// T_i = scale_a X_i A_a', and the adapters' gradients.  With G the scores'
+// gradient and U_i = scale_a G_i B_a (a product of the same form as T),
+//   dB_a = sum over the rows i of a of G_i (x) T_i,
+//   dA_a = sum over the rows i of a of U_i (x) X_i,
+// in 32 bits throughout.  The rows are brought into the order of their
+// adapters first (positions, not data), and each adapter's into segments;
+// sums over several segments are joined in the segments' order, so that
+// results do not change from run to run.
+#include <algorithm>
+
+#include "answer_launch.hpp"
+#include "answer_limits.hpp"
+#include "answer_types.hpp"
+#include "common.hpp"
+
+namespace sdca_gpu {
+namespace {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+// ---------------------------------------------------------------------------
+// Terms.
+// ---------------------------------------------------------------------------
+struct TermsArgs {
+  int64_t ldx, lda;  // lda: from one adapter's A to the next one's
+  int wide, rank, pitch, count;
+  const int64_t* index;
+  PerColumn<float> scale;
+  float* terms;
+};
+
+// A workgroup takes eight of the adapter's rows for one example.
+template <class TX, class TA>
+__global__ __launch_bounds__(256) void terms_row_kernel(const TX* __restrict__ X,
+                                                        const TA* __restrict__ A, TermsArgs a) {
+  __shared__ float part[4][8];
+  const int64_t row = blockIdx.x;
+  const int64_t id = a.index[row];
+  if (id < 0 || id >= a.count) return;
+  const int k0 = blockIdx.y * 8;
+  const TX* x = X + row * a.ldx;
+  const TA* w = A + id * a.lda + static_cast<int64_t>(k0) * a.wide;
+  float acc[8] = {};
+  for (int at = threadIdx.x * 8; at < a.wide; at += 256 * 8) {
+    float v[8];
+    load_vec<8>(x, at, a.wide, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k0 + k >= a.rank) break;
+      float u[8];
+      load_vec<8>(w + static_cast<int64_t>(k) * a.wide, at, a.wide, u);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[k] = fmaf(v[e], u[e], acc[k]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) acc[k] = wave_total(acc[k]);
+  if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) part[threadIdx.x >> 6][k] = acc[k];
+  }
+  __syncthreads();
+  if (threadIdx.x < 8) {
+    const int k = threadIdx.x;
+    const float sum = part[0][k] + part[1][k] + part[2][k] + part[3][k];
+    const float scale = a.scale.each ? a.scale.each[id] : a.scale.value;
+    a.terms[row * a.pitch + k0 + k] = k0 + k < a.rank ? sum * scale : 0.f;
+  }
+}
+
+template <class TX, class TA>
+hipError_t terms(const TermsLaunch& l) {
+  const Adapters& ad = *l.adapters;
+  TermsArgs a;
+  a.ldx = l.ldx;
+  a.lda = ad.rank * l.wide;
+  a.wide = static_cast<int>(l.wide);
+  a.rank = static_cast<int>(ad.rank);
+  a.pitch = static_cast<int>(terms_pitch(ad.rank));
+  a.count = static_cast<int>(ad.count);
+  a.scale = ad.scale;
+  const int64_t groups = a.pitch / 8;
+  each_slice(l.n, 1, 256 * groups, [&](int64_t first, int64_t count) {
+    a.index = ad.index + first;
+    a.terms = l.terms + first * a.pitch;
+    terms_row_kernel<TX, TA><<<dim3(static_cast<unsigned>(count), static_cast<unsigned>(groups)), 256, 0, l.stream>>>(
+        static_cast<const TX*>(l.X) + first * l.ldx, static_cast<const TA*>(l.A), a);
+  });
+  return hipGetLastError();
+}
+template <class TX>
+hipError_t terms(const TermsLaunch& l) {
+  switch (l.adapters->data) {
+    case SDCA_F32: return terms<TX, float>(l);
+    case SDCA_F16: return terms<TX, __half>(l);
+    default: return terms<TX, __hip_bfloat16>(l);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The rows by adapter, and segments of at most `length` of them.
+// ---------------------------------------------------------------------------
+struct Segment {
+  int adapter, first, rows, slot;  // slot: where the partial sums go; -1: the result itself
+};
+// Segment numbers need no sum over the adapters before: with `before` rows of
+// those, adapter a's begin at before / length + a, and there are
+// ceil(rows / length) <= (before + rows) / length - before / length + 1.  In
+// the same way the slots of adapters of several segments begin at
+// 2 before / length.  Numbers that are not taken have no rows.
+struct Segments {
+  int length;
+  Segment* table;
+  __host__ __device__ int64_t first(int64_t before, int64_t a) const { return before / length + a; }
+  __host__ __device__ int64_t slot(int64_t before) const { return 2 * before / length; }
+};
+
+struct GroupArgs {
+  const int64_t* index;
+  int n, count;
+  int* order;    // rows by adapter, rising within each
+  int2* spans;   // an adapter's first place in `order`, and its number of rows
+  Segments by[2];
+};
+
+// A workgroup finds the places of one adapter's rows: its waves each count
+// their part of the index, then write.
+__global__ __launch_bounds__(1024) void group_kernel(GroupArgs a) {
+  constexpr int kWaves = 16;
+  __shared__ int less_of[kWaves], equal_of[kWaves];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t me = blockIdx.x;
+  const int64_t share = ((static_cast<int64_t>(a.n) + kWaves - 1) / kWaves + 63) / 64 * 64;
+  const int64_t begin = min(static_cast<int64_t>(a.n), wave * share);
+  const int64_t end = min(static_cast<int64_t>(a.n), begin + share);
+  int less = 0, equal = 0;
+#pragma unroll 4
+  for (int64_t i = begin + lane; i < end + lane; i += 64) {
+    const int64_t id = i < end ? a.index[i] : -1;
+    less += id >= 0 && id < me;
+    equal += id == me;
+  }
+  less = wave_total(less);
+  equal = wave_total(equal);
+  if (lane == 0) less_of[wave] = less, equal_of[wave] = equal;
+  __syncthreads();
+  int before = 0, rows = 0, place = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    before += less_of[w];
+    if (w < wave) place += equal_of[w];
+    rows += equal_of[w];
+  }
+  place += before;
+  if (equal) {
+    for (int64_t i = begin + lane; i < end + lane; i += 64) {
+      const bool mine = i < end && a.index[i] == me;
+      const unsigned long long mask = __ballot(mine);
+      if (mine)
+        a.order[place + __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask >> 32),
+                                                  __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask), 0))] =
+            static_cast<int>(i);
+      place += __popcll(mask);
+    }
+  }
+  if (threadIdx.x == 0) a.spans[me] = make_int2(before, rows);
+  const bool last = me == a.count - 1;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const Segments& s = a.by[t];
+    const int64_t first = s.first(before, me);
+    const int64_t behind = last ? s.first(a.n, a.count) : s.first(before + rows, me + 1);
+    for (int64_t i = first + threadIdx.x; i < behind; i += 1024) {
+      const int64_t done = (i - first) * s.length;
+      Segment g;
+      g.adapter = static_cast<int>(me);
+      g.first = before + static_cast<int>(min(done, static_cast<int64_t>(rows)));
+      g.rows = static_cast<int>(max(int64_t(0), min(static_cast<int64_t>(s.length), rows - done)));
+      g.slot = rows > s.length ? static_cast<int>(s.slot(before) + i - first) : -1;
+      s.table[i] = g;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// B (m x rank for each adapter) with its classes in a row.
+// ---------------------------------------------------------------------------
+template <class T>
+__global__ __launch_bounds__(256) void turn_kernel(const T* __restrict__ B, int m, int rank,
+                                                   T* __restrict__ Bt, int64_t first) {
+  constexpr int kClasses = 64;
+  __shared__ T tile[kClasses * (kMostRank + 1)];
+  const int64_t blocks = (m + kClasses - 1) / kClasses;
+  const int64_t id = first + blockIdx.x, a = id / blocks, c0 = id % blocks * kClasses;
+  const int classes = static_cast<int>(min(static_cast<int64_t>(kClasses), m - c0));
+  const T* b = B + (a * m + c0) * rank;
+  for (int i = threadIdx.x; i < classes * rank; i += 256) tile[i / rank * (rank + 1) + i % rank] = b[i];
+  __syncthreads();
+  const int c = threadIdx.x % kClasses;
+  if (c >= classes) return;
+  for (int k = threadIdx.x / kClasses; k < rank; k += 256 / kClasses)
+    Bt[(a * rank + k) * m + c0 + c] = tile[c * (rank + 1) + k];
+}
+
+// ---------------------------------------------------------------------------
+// Sums over rows: out[c][k] or out[k][c] = sum_i Z_ic V_ik for the rows of a
+// segment, by 16 x 16 x 4 products in 32 bits.  A lane loads 16 bytes of a
+// row, V neighbouring values, four rows at a time; value e of all lanes makes
+// an operand, 16 columns V apart by four rows, without a turn through LDS.
+// A wave has 16 V columns and 16 RF ranks.
+// ---------------------------------------------------------------------------
+struct SumArgs {
+  int64_t ldz;
+  int wide, rank, pitch;
+  const float* terms;
+  const int* order;
+  const Segment* segments;
+  int64_t blocks, first;  // of columns; the launch's first workgroup
+  float *out, *partial;
+};
+
+template <class T, int RF, bool RANKS_FIRST>
+__global__ __launch_bounds__(256) void sum_kernel(const T* __restrict__ Z, SumArgs a) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T)), kSteps = 4;
+  const int lane = threadIdx.x & 63, low = lane & 15, high = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t id = a.first + blockIdx.x;
+  const Segment seg = a.segments[id / a.blocks];
+  const int64_t c0 = (id % a.blocks * 4 + wave) * (16 * V);
+  if (!seg.rows || c0 >= a.wide) return;
+  const int rank0 = blockIdx.y * 16 * RF;
+  const int64_t c = c0 + low * V;
+  const int* order = a.order + seg.first;
+  v4f acc[V][RF] = {};
+  for (int p0 = 0; p0 < seg.rows; p0 += 4 * kSteps) {
+    float z[kSteps][V], t[kSteps][RF];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int p = p0 + 4 * s + high;
+      const bool in = p < seg.rows;
+      const int64_t row = order[in ? p : 0];
+      load_vec<V>(Z + row * a.ldz, c, in ? a.wide : 0, z[s]);
+#pragma unroll
+      for (int f = 0; f < RF; ++f) {
+        const int k = rank0 + f * 16 + low;
+        t[s][f] = in && k < a.pitch ? a.terms[row * a.pitch + k] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+#pragma unroll
+        for (int f = 0; f < RF; ++f)
+          acc[e][f] = RANKS_FIRST ? __builtin_amdgcn_mfma_f32_16x16x4f32(t[s][f], z[s][e], acc[e][f], 0, 0, 0)
+                                  : __builtin_amdgcn_mfma_f32_16x16x4f32(z[s][e], t[s][f], acc[e][f], 0, 0, 0);
+  }
+  const int64_t size = static_cast<int64_t>(a.rank) * a.wide;
+  float* out = seg.slot < 0 ? a.out + seg.adapter * size : a.partial + seg.slot * size;
+#pragma unroll
+  for (int f = 0; f < RF; ++f)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if constexpr (RANKS_FIRST) {
+        const int k = rank0 + f * 16 + high * 4 + x;
+        if (k >= a.rank) continue;
+        float v[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = acc[e][f][x];
+        float* to = out + static_cast<int64_t>(k) * a.wide;
+        if (c + V <= a.wide) {
+          __builtin_memcpy(to + c, v, sizeof(v));
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (c + e < a.wide) to[c + e] = v[e];
+        }
+      } else {
+        const int k = rank0 + f * 16 + low;
+        const int64_t at = c0 + V * (high * 4 + x);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (k < a.rank && at + e < a.wide) out[(at + e) * a.rank + k] = acc[e][f][x];
+      }
+    }
+}
+
+// Adapters of several segments from their partial sums; zeros for those
+// without rows.
+__global__ __launch_bounds__(256) void join_kernel(const int2* __restrict__ spans, Segments s,
+                                                   int64_t size, const float* __restrict__ partial,
+                                                   float* __restrict__ out) {
+  const int64_t a = blockIdx.y;
+  const int2 span = spans[a];
+  if (span.y && span.y <= s.length) return;
+  const int parts = (span.y + s.length - 1) / s.length;
+  const float* from = partial + s.slot(span.x) * size;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < size;
+       i += static_cast<int64_t>(gridDim.x) * 256) {
+    float sum = 0.f;
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) sum += from[p * size + i];
+    out[a * size + i] = sum;
+  }
+}
+
+// Rows of a segment, so that the columns' workgroups times the segments come
+// to about 512, two waves to a SIMD: more parts cost the joining of their sums.
+int segment_length(int es, int64_t wide, int64_t n) {
+  const int64_t columns = 4 * 16 * (16 / es), blocks = (wide + columns - 1) / columns;
+  const int64_t parts = std::max<int64_t>(1, 512 / blocks);
+  const int64_t length = ((n + parts - 1) / parts + 15) / 16 * 16;
+  return static_cast<int>(std::max<int64_t>(length, 64));
+}
+
+template <class T, int RF, bool RANKS_FIRST>
+void start_sums(const T* Z, SumArgs a, int64_t segments, hipStream_t stream) {
+  constexpr int64_t kColumns = 4 * 16 * (16 / sizeof(T));
+  a.blocks = (a.wide + kColumns - 1) / kColumns;
+  const unsigned ranks = (a.rank + 16 * RF - 1) / (16 * RF);
+  each_slice(segments * a.blocks, 1, 256 * static_cast<int64_t>(ranks), [&](int64_t first, int64_t count) {
+    a.first = first;
+    sum_kernel<T, RF, RANKS_FIRST><<<dim3(static_cast<unsigned>(count), ranks), 256, 0, stream>>>(Z, a);
+  });
+}
+
+struct GradPlan {
+  int length[2];  // of segments: dB's, dA's
+  int64_t segments[2];
+  size_t order, spans, table[2], turned, terms[2], partial, end;
+};
+GradPlan plan_grad(int grad, int data, int64_t d, int64_t m, int64_t n, int64_t count, int64_t rank) {
+  GradPlan p;
+  size_t at = 0;
+  const auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  const auto es = [](int type) { return type == SDCA_F32 ? 4 : 2; };
+  p.length[0] = segment_length(es(grad), m, n);
+  p.length[1] = segment_length(es(data), d, n);
+  p.order = take(n * sizeof(int));
+  p.spans = take(count * sizeof(int2));
+  size_t partial = 0;
+  for (int t = 0; t < 2; ++t) {
+    const Segments s = {p.length[t], nullptr};
+    p.segments[t] = s.first(n, count);
+    p.table[t] = take(p.segments[t] * sizeof(Segment));
+    if (n > p.length[t])
+      partial = std::max(partial, static_cast<size_t>(s.slot(n) + 1) * rank * (t ? d : m) * sizeof(float));
+    p.terms[t] = take(static_cast<size_t>(n) * terms_pitch(rank) * sizeof(float));
+  }
+  p.turned = take(static_cast<size_t>(count) * m * rank * es(data));
+  p.partial = take(partial);
+  p.end = at;
+  return p;
+}
+
+template <class T>
+void sums(const void* Z, int64_t ldz, int64_t wide, bool ranks_first, const GradPlan& p, int t,
+          const float* terms, float* out, const AdaptedGradLaunch& l) {
+  char* work = static_cast<char*>(l.work);
+  SumArgs a;
+  a.ldz = ldz;
+  a.wide = static_cast<int>(wide);
+  a.rank = static_cast<int>(l.adapters.rank);
+  a.pitch = static_cast<int>(terms_pitch(a.rank));
+  a.terms = terms;
+  a.order = reinterpret_cast<const int*>(work + p.order);
+  a.segments = reinterpret_cast<const Segment*>(work + p.table[t]);
+  a.out = out;
+  a.partial = reinterpret_cast<float*>(work + p.partial);
+  const T* z = static_cast<const T*>(Z);
+  const int frags = a.rank <= 16 ? 1 : a.rank <= 32 ? 2 : 4;
+  if (ranks_first) {
+    if (frags == 1) start_sums<T, 1, true>(z, a, p.segments[t], l.stream);
+    else if (frags == 2) start_sums<T, 2, true>(z, a, p.segments[t], l.stream);
+    else start_sums<T, 4, true>(z, a, p.segments[t], l.stream);
+  } else {
+    if (frags == 1) start_sums<T, 1, false>(z, a, p.segments[t], l.stream);
+    else if (frags == 2) start_sums<T, 2, false>(z, a, p.segments[t], l.stream);
+    else start_sums<T, 4, false>(z, a, p.segments[t], l.stream);
+  }
+  const int64_t size = wide * a.rank, blocks = std::min<int64_t>((size + 255) / 256, 4096);
+  const Segments s = {p.length[t], nullptr};
+  join_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(l.adapters.count)), 256, 0, l.stream>>>(
+      reinterpret_cast<const int2*>(work + p.spans), s, size, a.partial, out);
+}
+void sums(int type, const void* Z, int64_t ldz, int64_t wide, bool ranks_first, const GradPlan& p,
+          int t, const float* terms, float* out, const AdaptedGradLaunch& l) {
+  switch (type) {
+    case SDCA_F32: return sums<float>(Z, ldz, wide, ranks_first, p, t, terms, out, l);
+    case SDCA_F16: return sums<__half>(Z, ldz, wide, ranks_first, p, t, terms, out, l);
+    default: return sums<__hip_bfloat16>(Z, ldz, wide, ranks_first, p, t, terms, out, l);
+  }
+}
+
+template <class T>
+void turn(const AdaptedGradLaunch& l, void* Bt) {
+  const int64_t blocks = (l.m + 63) / 64;
+  each_slice(blocks * l.adapters.count, 1, 256, [&](int64_t first, int64_t count) {
+    turn_kernel<T><<<static_cast<unsigned>(count), 256, 0, l.stream>>>(
+        static_cast<const T*>(l.adapters.B), static_cast<int>(l.m), static_cast<int>(l.adapters.rank),
+        static_cast<T*>(Bt), first);
+  });
+}
+
+}  // namespace
+
+hipError_t launch_terms(const TermsLaunch& l) {
+  switch (l.data) {
+    case SDCA_F32: return terms<float>(l);
+    case SDCA_F16: return terms<__half>(l);
+    default: return terms<__hip_bfloat16>(l);
+  }
+}
+
+size_t adapted_grad_work_bytes(int grad, int data, int64_t d, int64_t m, int64_t n, int64_t count,
+                               int64_t rank) {
+  return plan_grad(grad, data, d, m, n, count, rank).end;
+}
+
+hipError_t launch_adapted_grad(const AdaptedGradLaunch& l) {
+  const Adapters& ad = l.adapters;
+  const GradPlan p = plan_grad(l.grad, ad.data, l.d, l.m, l.n, ad.count, ad.rank);
+  char* work = static_cast<char*>(l.work);
+  GroupArgs g;
+  g.index = ad.index;
+  g.n = static_cast<int>(l.n);
+  g.count = static_cast<int>(ad.count);
+  g.order = reinterpret_cast<int*>(work + p.order);
+  g.spans = reinterpret_cast<int2*>(work + p.spans);
+  for (int t = 0; t < 2; ++t) g.by[t] = Segments{p.length[t], reinterpret_cast<Segment*>(work + p.table[t])};
+  group_kernel<<<static_cast<unsigned>(ad.count), 1024, 0, l.stream>>>(g);
+  void* Bt = work + p.turned;
+  if (ad.data == SDCA_F32) turn<float>(l, Bt);
+  else turn<__half>(l, Bt);  // (two bytes either way)
+  float *T = reinterpret_cast<float*>(work + p.terms[0]), *U = reinterpret_cast<float*>(work + p.terms[1]);
+  TermsLaunch t;
+  t.adapters = &ad;
+  t.n = l.n;
+  t.order = g.order;
+  t.ordered = nullptr;
+  t.stream = l.stream;
+  t.data = ad.data;
+  t.wide = l.d;
+  t.X = l.X;
+  t.ldx = l.ldx;
+  t.A = ad.A;
+  t.terms = T;
+  hipError_t e = launch_terms(t);
+  if (e != hipSuccess) return e;
+  t.data = l.grad;
+  t.wide = l.m;
+  t.X = l.G;
+  t.ldx = l.ldg;
+  t.A = Bt;
+  t.terms = U;
+  if ((e = launch_terms(t)) != hipSuccess) return e;
+  sums(l.grad, l.G, l.ldg, l.m, false, p, 0, T, l.dB, l);
+  sums(ad.data, l.X, l.ldx, l.d, true, p, 1, U, l.dA, l);
+  return hipGetLastError();
+}
+
+}  // namespace sdca_gpu

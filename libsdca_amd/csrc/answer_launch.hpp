@@ -122,6 +122,59 @@ struct LogProbsGradLaunch {
 size_t log_probs_grad_work_bytes(int data, int64_t m, int64_t n, bool stats);
 hipError_t launch_log_probs_grad(const LogProbsGradLaunch& a);
 
+// Low-rank adapters: matrices of an example's adapter a = index[i], in the
+// examples' type.  -1: none; another index outside [0, count): NaN scores.
+struct Adapters {
+  int data;  // SDCA_F32, F16, BF16
+  int64_t count, rank;
+  const void* A;  // count x rank rows of d values
+  const void* B;  // count x m rows of `rank` values
+  const int64_t* index;
+  PerColumn<float> scale;
+};
+constexpr int64_t kMostRank = 128, kMostAdapters = 65535;
+// Rows of terms: rank values of an example, zeros up to whole 16.
+constexpr int64_t terms_pitch(int64_t rank) { return (rank + 15) / 16 * 16; }
+
+// terms[i] = scale_a X_i A_a' for the n rows of X (`wide` values of type
+// `data`, pitch ldx) with A_a's `rank` rows of `wide` values, adapters
+// count apart; rows without an adapter are left as they are.
+struct TermsLaunch {
+  int data;
+  int64_t wide, n;
+  const void* X;
+  int64_t ldx;
+  const Adapters* adapters;
+  const void* A;
+  // The rows in the order of their adapters, as `group` leaves it (NULL: as
+  // they come), and their number.
+  const int* order;
+  const int* ordered;
+  float* terms;
+  hipStream_t stream;
+};
+hipError_t launch_terms(const TermsLaunch& a);
+
+// launch_scores_i8 with adapters: terms are the examples' (of X_i itself, not
+// of its 8-bit form).
+hipError_t launch_scores_adapted(const ScoresI8Launch& a, const Adapters& adapters,
+                                 const float* terms);
+
+struct AdaptedGradLaunch {
+  int grad;  // G's type
+  int64_t d, m, n;
+  const void* G;
+  int64_t ldg;
+  const void* X;
+  int64_t ldx;
+  Adapters adapters;
+  float *dA, *dB;
+  void* work;  // adapted_grad_work_bytes of device memory
+  hipStream_t stream;
+};
+size_t adapted_grad_work_bytes(int grad, int data, int64_t d, int64_t m, int64_t n, int64_t count, int64_t rank);
+hipError_t launch_adapted_grad(const AdaptedGradLaunch& a);
+
 }  // namespace sdca_gpu
 
 #endif  // SDCA_HIP_ANSWER_LAUNCH_HPP

@@ -1564,6 +1564,212 @@ int log_probs_grad_common(int data, int64_t m, int64_t n, const void* S, int64_t
   return SDCA_OK;
 }
 
+int check_adapters(const char* name, int data, const sdca_adapters* ad) {
+  if (!is_score_type(data))
+    return fail(SDCA_ERR_PRECISION, "%s takes F32, F16 or BF16 examples (got %d)", name, data);
+  if (!ad) return fail(SDCA_ERR_ARG_NULL, "adapters must not be NULL");
+  if (ad->count < 1 || ad->count > sdca_gpu::kMostAdapters)
+    return fail(SDCA_ERR_ARG_RANGE, "the number of adapters must be in [1, %lld] (got %lld)",
+                (long long)sdca_gpu::kMostAdapters, (long long)ad->count);
+  if (ad->rank < 1 || ad->rank > sdca_gpu::kMostRank)
+    return fail(SDCA_ERR_ARG_RANGE, "the adapters' rank must be in [1, %lld] (got %lld)",
+                (long long)sdca_gpu::kMostRank, (long long)ad->rank);
+  if (!ad->scale && !(std::abs(ad->factor) <= 3.4028234e38))
+    return fail(SDCA_ERR_ARG_RANGE, "the adapters' scale must be finite in 32 bits (got %g)",
+                ad->factor);
+  return SDCA_OK;
+}
+
+// What check_adapters leaves to be checked behind the sizes.
+int check_adapter_arrays(int64_t n, bool host, const sdca_adapters& ad) {
+  if (!ad.A || !ad.B || (n && !ad.index))
+    return fail(SDCA_ERR_ARG_NULL, "the adapters' A, B and index must not be NULL");
+  if (host)
+    for (int64_t i = 0; i < n; ++i)
+      if (ad.index[i] < -1 || ad.index[i] >= ad.count)
+        return fail(SDCA_ERR_ARG_RANGE, "index[%lld] = %lld outside [-1, %lld)", (long long)i,
+                    (long long)ad.index[i], (long long)ad.count);
+  return SDCA_OK;
+}
+
+// The adapters on the device.
+struct StagedAdapters {
+  DeviceBuffer a, b, index, scale;
+  int stage(int data, int64_t d, int64_t m, int64_t n, const sdca_adapters& ad, bool host,
+            hipStream_t stream, sdca_gpu::Adapters* out) {
+    const size_t es = element_size(data), rows = static_cast<size_t>(ad.count) * ad.rank;
+    out->data = data;
+    out->count = ad.count;
+    out->rank = ad.rank;
+    out->scale.value = static_cast<float>(ad.scale ? 1. : ad.factor);
+    int rc;
+    if ((rc = staged(ad.A, rows * d * es, host, a, stream, &out->A)) ||
+        (rc = staged(ad.B, rows * m * es, host, b, stream, &out->B)) ||
+        (rc = staged(ad.index, n * sizeof(int64_t), host, index, stream, &out->index)) ||
+        (rc = staged(ad.scale, ad.count * sizeof(float), host, scale, stream, &out->scale.each)))
+      return rc;
+    return SDCA_OK;
+  }
+};
+
+// The scratch of the 8-bit product with adapters: the 8-bit examples, W where
+// it is not read in place, the examples' scales, their terms.
+struct AdaptedPlan {
+  int64_t pad;
+  bool own_x, own_w;
+  size_t w, scales, terms, end;
+};
+AdaptedPlan plan_adapted(int data, int64_t d, int64_t m, int64_t n, const void* W, int64_t ldw,
+                         int64_t rank) {
+  using namespace sdca_gpu;
+  const auto whole = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
+  AdaptedPlan p;
+  p.pad = (d + kI8TileK - 1) / kI8TileK * kI8TileK;
+  p.own_x = !scores_i8_quantises(data, d, m, n);
+  p.own_w = reinterpret_cast<uintptr_t>(W) % 16 != 0 || ldw % 16 != 0 || ldw > kI8MaxPitch;
+  p.w = p.own_x ? whole(static_cast<size_t>(n) * p.pad) : 0;
+  p.scales = p.w + (p.own_w ? whole(static_cast<size_t>(m) * p.pad) : 0);
+  p.terms = p.scales + (p.own_x ? whole(n * sizeof(float)) : 0);
+  p.end = p.terms + whole(static_cast<size_t>(n) * terms_pitch(rank) * sizeof(float));
+  return p;
+}
+
+int scores_adapted_common(int data, int out, int64_t d, int64_t m, int64_t n, const void* X,
+                          int64_t ldx, const int8_t* W, int64_t ldw, const float* sw,
+                          const sdca_adapters* adapters, void* S, int64_t lds, void* work,
+                          unsigned flags, hipStream_t stream) {
+  using namespace sdca_gpu;
+  int rc;
+  if ((rc = check_adapters("scores_adapted", data, adapters))) return rc;
+  if (!is_score_type(out))
+    return fail(SDCA_ERR_PRECISION, "scores_adapted gives F32, F16 or BF16 scores (got %d)", out);
+  if (d < 1 || m < 1 || n < 0 || m > INT32_MAX / 2 || n > INT32_MAX / 2)
+    return fail(SDCA_ERR_ARG_RANGE, "need d, m >= 1 and n >= 0 (got d %lld, m %lld, n %lld)",
+                (long long)d, (long long)m, (long long)n);
+  if (d > 131071)  // 2^14 d stays below 2^31
+    return fail(SDCA_ERR_ARG_RANGE, "d is at most 131071: the sums are 32-bit integers (got %lld)",
+                (long long)d);
+  if ((rc = check_matrix("X", d, ldx)) || (rc = check_matrix("W", d, ldw)) ||
+      (rc = check_matrix("S", m, lds)))
+    return rc;
+  if (n == 0) return SDCA_OK;
+  if (!X || !W || !sw || !S) return fail(SDCA_ERR_ARG_NULL, "X, W, sw and S must not be NULL");
+  const bool host = (flags & SDCA_HOST_PTR) != 0;
+  if ((rc = check_adapter_arrays(n, host, *adapters))) return rc;
+  if (host) work = nullptr;
+  DeviceBuffer dx, dw, dsw, dS;
+  StagedAdapters dad;
+  Adapters ad;
+  ScoresI8Launch a;
+  a.data = data;
+  a.out = out;
+  a.d = d;
+  a.m = m;
+  a.n = n;
+  a.ldx = ldx;
+  a.ldw = ldw;
+  a.lds = lds;
+  a.sx = nullptr;
+  a.stream = stream;
+  if ((rc = staged(X, span(d, n, ldx, element_size(data)), host, dx, stream, &a.X)) ||
+      (rc = staged(W, span(d, m, ldw, 1), host, dw, stream, &a.W)) ||
+      (rc = staged(sw, m * sizeof(float), host, dsw, stream, &a.sw)) ||
+      (rc = staged_out(S, span(m, n, lds, element_size(out)), host, dS, &a.S)) ||
+      (rc = dad.stage(data, d, m, n, *adapters, host, stream, &ad)))
+    return rc;
+  const AdaptedPlan p = plan_adapted(data, d, m, n, a.W, ldw, ad.rank);
+  if ((rc = scratch(work, p.end, stream, &work))) return rc;
+  char* at = static_cast<char*>(work);
+  TermsLaunch t;
+  t.data = data;
+  t.wide = d;
+  t.n = n;
+  t.X = a.X;
+  t.ldx = ldx;
+  t.adapters = &ad;
+  t.A = ad.A;
+  t.order = t.ordered = nullptr;
+  t.terms = reinterpret_cast<float*>(at + p.terms);
+  t.stream = stream;
+  SDCA_HIP_TRY(launch_terms(t), "adapter terms");
+  if (p.own_x) {
+    QuantLaunch q;
+    q.data = data;
+    q.d = d;
+    q.n = n;
+    q.X = a.X;
+    q.ldx = ldx;
+    q.Q = reinterpret_cast<int8_t*>(at);
+    q.ldq = q.pad = p.pad;
+    q.scales = reinterpret_cast<float*>(at + p.scales);
+    q.stream = stream;
+    SDCA_HIP_TRY(launch_quantize(q), "quantise kernel");
+    a.X = q.Q;
+    a.ldx = p.pad;
+    a.sx = q.scales;
+    a.data = SDCA_I8;
+  }
+  if (p.own_w) {
+    int8_t* ww = reinterpret_cast<int8_t*>(at + p.w);
+    SDCA_HIP_TRY(launch_repack_i8(a.W, ldw, d, m, ww, p.pad, p.pad, stream), "repack kernel");
+    a.W = ww;
+    a.ldw = p.pad;
+  }
+  SDCA_HIP_TRY(launch_scores_adapted(a, ad, t.terms), "adapted score kernel");
+  if (host) {
+    if ((rc = fetch_columns(S, a.S, m, n, lds, element_size(out), stream))) return rc;
+    SDCA_HIP_TRY(hipStreamSynchronize(stream), "hipStreamSynchronize");
+  }
+  return SDCA_OK;
+}
+
+int scores_adapted_grad_common(int data, int grad, int64_t d, int64_t m, int64_t n, const void* G,
+                               int64_t ldg, const void* X, int64_t ldx,
+                               const sdca_adapters* adapters, float* dA, float* dB, void* work,
+                               unsigned flags, hipStream_t stream) {
+  using namespace sdca_gpu;
+  int rc;
+  if ((rc = check_adapters("scores_adapted_grad", data, adapters))) return rc;
+  if (!is_score_type(grad))
+    return fail(SDCA_ERR_PRECISION, "scores_adapted_grad takes F32, F16 or BF16 gradients (got %d)", grad);
+  if (d < 1 || m < 1 || n < 0 || d > INT32_MAX / 2 || m > INT32_MAX / 2 || n > INT32_MAX / 2)
+    return fail(SDCA_ERR_ARG_RANGE, "need d, m >= 1 and n >= 0 (got d %lld, m %lld, n %lld)",
+                (long long)d, (long long)m, (long long)n);
+  if ((rc = check_matrix("G", m, ldg)) || (rc = check_matrix("X", d, ldx))) return rc;
+  if (!dA || !dB) return fail(SDCA_ERR_ARG_NULL, "dA and dB must not be NULL");
+  if (n && (!G || !X)) return fail(SDCA_ERR_ARG_NULL, "G and X must not be NULL");
+  const bool host = (flags & SDCA_HOST_PTR) != 0;
+  if ((rc = check_adapter_arrays(n, host, *adapters))) return rc;
+  if (host) work = nullptr;
+  DeviceBuffer dx, dg, dda, ddb;
+  StagedAdapters dad;
+  AdaptedGradLaunch a;
+  a.grad = grad;
+  a.d = d;
+  a.m = m;
+  a.n = n;
+  a.ldg = ldg;
+  a.ldx = ldx;
+  a.stream = stream;
+  const size_t rows = static_cast<size_t>(adapters->count) * adapters->rank;
+  if ((rc = staged(X, span(d, n, ldx, element_size(data)), host, dx, stream, &a.X)) ||
+      (rc = staged(G, span(m, n, ldg, element_size(grad)), host, dg, stream, &a.G)) ||
+      (rc = staged_out(dA, rows * d * sizeof(float), host, dda, &a.dA)) ||
+      (rc = staged_out(dB, rows * m * sizeof(float), host, ddb, &a.dB)) ||
+      (rc = dad.stage(data, d, m, n, *adapters, host, stream, &a.adapters)) ||
+      (rc = scratch(work, adapted_grad_work_bytes(grad, data, d, m, n, adapters->count, adapters->rank),
+                    stream, &a.work)))
+    return rc;
+  SDCA_HIP_TRY(launch_adapted_grad(a), "adapter gradient kernels");
+  if (host) {
+    if ((rc = fetch_columns(dA, a.dA, rows * d, 1, rows * d, sizeof(float), stream)) ||
+        (rc = fetch_columns(dB, a.dB, rows * m, 1, rows * m, sizeof(float), stream)))
+      return rc;
+    SDCA_HIP_TRY(hipStreamSynchronize(stream), "hipStreamSynchronize");
+  }
+  return SDCA_OK;
+}
+
 // Nothing is thrown through the C boundary (the workspace cache's map and
 // the messages can run out of memory).
 template <class F>
@@ -1642,6 +1848,38 @@ int sdca_log_probs_grad(sdca_dtype data, int64_t m, int64_t n, const void* S, in
   return guarded([&] {
     return log_probs_grad_common(data, m, n, S, lds, labels, g, h, stats, temperature, D, ldd,
                                  logp, work, flags, static_cast<hipStream_t>(stream));
+  });
+}
+
+size_t sdca_scores_adapted_work(sdca_dtype data, int64_t d, int64_t m, int64_t n,
+                                const int8_t* W, int64_t ldw, int64_t rank) {
+  if (d < 1 || m < 1 || n < 1 || rank < 1) return 0;
+  return plan_adapted(data, d, m, n, W, ldw, rank).end;
+}
+
+int sdca_scores_adapted(sdca_dtype data, sdca_dtype out, int64_t d, int64_t m, int64_t n,
+                        const void* X, int64_t ldx, const int8_t* W, int64_t ldw, const float* sw,
+                        const sdca_adapters* adapters, void* S, int64_t lds, void* work,
+                        unsigned flags, void* stream) {
+  return guarded([&] {
+    return scores_adapted_common(data, out, d, m, n, X, ldx, W, ldw, sw, adapters, S, lds, work,
+                                 flags, static_cast<hipStream_t>(stream));
+  });
+}
+
+size_t sdca_scores_adapted_grad_work(sdca_dtype data, sdca_dtype grad, int64_t d, int64_t m,
+                                     int64_t n, int64_t count, int64_t rank) {
+  if (d < 1 || m < 1 || n < 0 || count < 1 || rank < 1) return 0;
+  return sdca_gpu::adapted_grad_work_bytes(grad, data, d, m, n, count, rank);
+}
+
+int sdca_scores_adapted_grad(sdca_dtype data, sdca_dtype grad, int64_t d, int64_t m, int64_t n,
+                             const void* G, int64_t ldg, const void* X, int64_t ldx,
+                             const sdca_adapters* adapters, float* dA, float* dB, void* work,
+                             unsigned flags, void* stream) {
+  return guarded([&] {
+    return scores_adapted_grad_common(data, grad, d, m, n, G, ldg, X, ldx, adapters, dA, dB, work,
+                                      flags, static_cast<hipStream_t>(stream));
   });
 }
 
