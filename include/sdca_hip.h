@@ -589,7 +589,7 @@ typedef struct sdca_adapters {
  *      aligned, or NULL: the stream's scratch, as in sdca_log_probs.
  */
 size_t sdca_scores_adapted_work(sdca_dtype data, int64_t d, int64_t m, int64_t n,
-                                const int8_t* W, int64_t ldw, int64_t rank);
+                                const int8_t* W, int64_t ldw, int64_t count, int64_t rank);
 int sdca_scores_adapted(sdca_dtype data, sdca_dtype out, int64_t d, int64_t m, int64_t n,
                         const void* X, int64_t ldx, const int8_t* W, int64_t ldw, const float* sw,
                         const sdca_adapters* adapters, void* S, int64_t lds, void* work,

@@ -181,7 +181,7 @@ def library():
         lib.sdca_log_probs_grad.argtypes = [i32, i64, i64, ptr, i64, ptr, ptr, ptr, ptr, f64, ptr, i64,
                                             ptr, ptr, u32, ptr]
         ads = ctypes.POINTER(Adapters)
-        lib.sdca_scores_adapted_work.argtypes = [i32, i64, i64, i64, ptr, i64, i64]
+        lib.sdca_scores_adapted_work.argtypes = [i32, i64, i64, i64, ptr, i64, i64, i64]
         lib.sdca_scores_adapted_work.restype = size
         lib.sdca_scores_adapted.argtypes = [i32, i32, i64, i64, i64, ptr, i64, ptr, i64, ptr, ads, ptr, i64,
                                             ptr, u32, ptr]
@@ -1098,7 +1098,8 @@ def scores_adapted(X, W, w_scales, A, B, index, scale=1.0, out=None, dtype=None)
         raise SdcaError(3, f"scores cannot be {out.dtype}")
     lds = _pitch(out, "out", (n, m))
     _written(out, "out")
-    work = _scratch(X, lib.sdca_scores_adapted_work, data, d, m, n, _ptr(W), ldw, adapters.rank)
+    work = _scratch(X, lib.sdca_scores_adapted_work, data, d, m, n, _ptr(W), ldw,
+                    adapters.count, adapters.rank)
     _answer(X, "scores_adapted", lib.sdca_scores_adapted, data, code, d, m, n, _ptr(X), ldx, _ptr(W), ldw,
             _ptr(w_scales), adapters, _ptr(out), lds, _ptr(work))
     return out

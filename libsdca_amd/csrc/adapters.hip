@@ -8,6 +8,7 @@
 // sums over several segments are joined in the segments' order, so that
 // results do not change from run to run.
 #include <algorithm>
+#include <type_traits>
 
 #include "answer_launch.hpp"
 #include "answer_limits.hpp"
@@ -30,6 +31,9 @@ struct TermsArgs {
   float* terms;
 };
 
+// From so many examples on, 16 or 32 of them to a workgroup.
+constexpr int64_t kTileTerms = 128;
+
 // A workgroup takes eight of the adapter's rows for one example.
 template <class TX, class TA>
 __global__ __launch_bounds__(256) void terms_row_kernel(const TX* __restrict__ X,
@@ -39,20 +43,24 @@ __global__ __launch_bounds__(256) void terms_row_kernel(const TX* __restrict__ X
   const int64_t id = a.index[row];
   if (id < 0 || id >= a.count) return;
   const int k0 = blockIdx.y * 8;
+  if (k0 >= a.rank) {
+    if (threadIdx.x < 8) a.terms[row * a.pitch + k0 + threadIdx.x] = 0.f;
+    return;
+  }
   const TX* x = X + row * a.ldx;
   const TA* w = A + id * a.lda + static_cast<int64_t>(k0) * a.wide;
   float acc[8] = {};
   for (int at = threadIdx.x * 8; at < a.wide; at += 256 * 8) {
     float v[8];
     load_vec<8>(x, at, a.wide, v);
+    float u[8][8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (k0 + k >= a.rank) break;
-      float u[8];
-      load_vec<8>(w + static_cast<int64_t>(k) * a.wide, at, a.wide, u);
+    for (int k = 0; k < 8; ++k)  // (rows behind the rank: the last one again)
+      load_vec<8>(w + static_cast<int64_t>(min(k, a.rank - 1 - k0)) * a.wide, at, a.wide, u[k]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[k] = fmaf(v[e], u[e], acc[k]);
-    }
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[k] = fmaf(v[e], u[k][e], acc[k]);
   }
 #pragma unroll
   for (int k = 0; k < 8; ++k) acc[k] = wave_total(acc[k]);
@@ -69,6 +77,146 @@ __global__ __launch_bounds__(256) void terms_row_kernel(const TX* __restrict__ X
   }
 }
 
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+
+// Eight neighbouring values of a row from `at` on, zeros from `len` on.
+template <class T>
+__device__ inline void load_raw(const T* row, int64_t at, int64_t len, T (&v)[8]) {
+  if (at + 8 <= len) {
+    __builtin_memcpy(v, row + at, sizeof(v));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = at + e < len ? row[at + e] : from_float<T>(0.f);
+  }
+}
+
+// sum += a product of 16 rows by 16 columns over 32 values: a lane has eight
+// of row and of column lane % 16.  Two halves or two bfloat16 multiply as
+// they are, others in 32 bits; the sums are 32-bit either way.
+template <class TA, class TB>
+__device__ inline v4f multiply(const TA (&a)[8], const TB (&b)[8], v4f sum) {
+  if constexpr (std::is_same<TA, TB>::value && std::is_same<TA, __half>::value) {
+    v8h u, v;
+    __builtin_memcpy(&u, a, 16);
+    __builtin_memcpy(&v, b, 16);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(u, v, sum, 0, 0, 0);
+  } else if constexpr (std::is_same<TA, TB>::value && std::is_same<TA, __hip_bfloat16>::value) {
+    v8b u, v;
+    __builtin_memcpy(&u, a, 16);
+    __builtin_memcpy(&v, b, 16);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, v, sum, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      sum = __builtin_amdgcn_mfma_f32_16x16x4f32(to_float(a[e]), to_float(b[e]), sum, 0, 0, 0);
+    return sum;
+  }
+}
+
+// A workgroup takes 16 NE examples with all ranks (16 RF); its waves share the
+// wide axis, 32 values at a time, and add up through LDS.  Examples of
+// different adapters take turns; in the adapters' order that is rare.
+constexpr int kTermWaves = 8;
+template <class TX, class TA, int NE, int RF>
+__global__ __launch_bounds__(64 * kTermWaves) void terms_tile_kernel(
+    const TX* __restrict__ X, const TA* __restrict__ A, TermsArgs a, int64_t n,
+    const int* __restrict__ order, const int2* __restrict__ spans, int64_t first) {
+  constexpr int kAhead = RF > 4 ? 1 : std::is_same<TX, TA>::value && sizeof(TX) == 2 && RF < 4 ? 4 : 2;
+  constexpr int kFrags = NE * RF;
+  constexpr int kOnce = kFrags < 4 ? kFrags : 4;
+  __shared__ v4f part[kOnce][kTermWaves][64];
+  const int lane = threadIdx.x & 63, low = lane & 15, high = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t total = order ? spans[a.count].x : n;
+  const int64_t p0 = (first + blockIdx.x) * (16 * NE);
+  if (p0 >= total) return;
+  int64_t row[NE];
+  int id[NE];
+  unsigned long long left[NE];
+#pragma unroll
+  for (int j = 0; j < NE; ++j) {
+    const int64_t p = p0 + j * 16 + low;
+    row[j] = p < total ? (order ? order[p] : p) : -1;
+    const int64_t given = row[j] >= 0 ? a.index[row[j]] : -1;
+    id[j] = given >= 0 && given < a.count ? static_cast<int>(given) : -1;
+    left[j] = __ballot(id[j] >= 0);
+  }
+  while (true) {
+    int me = -1;
+#pragma unroll
+    for (int j = NE - 1; j >= 0; --j)
+      if (left[j]) me = __builtin_amdgcn_readlane(id[j], __builtin_ctzll(left[j]));
+    if (me < 0) break;
+    const TA* w[RF];
+    const TX* x[NE];
+    int of_w[RF], of_x[NE];
+#pragma unroll
+    for (int f = 0; f < RF; ++f) {
+      const int k = f * 16 + low;
+      of_w[f] = k < a.rank ? a.wide : 0;
+      w[f] = A + me * a.lda + static_cast<int64_t>(min(k, a.rank - 1)) * a.wide;
+    }
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+      left[j] &= ~__ballot(id[j] == me);
+      of_x[j] = id[j] == me ? a.wide : 0;
+      x[j] = X + max(row[j], int64_t(0)) * a.ldx;
+    }
+    v4f acc[NE][RF] = {};
+    for (int64_t at0 = wave * 32; at0 < a.wide; at0 += 32 * kTermWaves * kAhead) {
+      TX u[kAhead][NE][8];
+      TA v[kAhead][RF][8];
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        const int64_t at = at0 + s * (32 * kTermWaves) + high * 8;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) load_raw(x[j], at, of_x[j], u[s][j]);
+#pragma unroll
+        for (int f = 0; f < RF; ++f) load_raw(w[f], at, of_w[f], v[s][f]);
+      }
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s)
+#pragma unroll
+        for (int j = 0; j < NE; ++j)
+#pragma unroll
+          for (int f = 0; f < RF; ++f) acc[j][f] = multiply(v[s][f], u[s][j], acc[j][f]);
+    }
+    const float scale = a.scale.each ? a.scale.each[me] : a.scale.value;
+#pragma unroll
+    for (int g = 0; g < kFrags; g += kOnce) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kOnce; ++i) part[i][wave][lane] = acc[(g + i) / RF][(g + i) % RF];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kOnce; ++i) {
+        if (wave != i || id[(g + i) / RF] != me) continue;
+        v4f sum = part[i][0][lane];
+#pragma unroll
+        for (int q = 1; q < kTermWaves; ++q) sum += part[i][q][lane];
+        float* to = a.terms + row[(g + i) / RF] * a.pitch + (g + i) % RF * 16 + high * 4;
+        if ((g + i) % RF * 16 < a.pitch) *reinterpret_cast<v4f*>(to) = sum * scale;
+      }
+    }
+  }
+}
+
+template <class TX, class TA, int NE, int RF>
+void start_terms(const TermsLaunch& l, const TermsArgs& a) {
+  each_slice((l.n + 16 * NE - 1) / (16 * NE), 1, 64 * kTermWaves, [&](int64_t first, int64_t count) {
+    terms_tile_kernel<TX, TA, NE, RF><<<static_cast<unsigned>(count), 64 * kTermWaves, 0, l.stream>>>(
+        static_cast<const TX*>(l.X), static_cast<const TA*>(l.A), a, l.n, l.order, l.spans, first);
+  });
+}
+template <class TX, class TA, int NE>
+void start_terms(const TermsLaunch& l, const TermsArgs& a) {
+  if (a.rank <= 16) start_terms<TX, TA, NE, 1>(l, a);
+  else if (a.rank <= 32) start_terms<TX, TA, NE, 2>(l, a);
+  else if (a.rank <= 64) start_terms<TX, TA, NE, 4>(l, a);
+  else start_terms<TX, TA, 1, 8>(l, a);
+}
+
 template <class TX, class TA>
 hipError_t terms(const TermsLaunch& l) {
   const Adapters& ad = *l.adapters;
@@ -80,6 +228,13 @@ hipError_t terms(const TermsLaunch& l) {
   a.pitch = static_cast<int>(terms_pitch(ad.rank));
   a.count = static_cast<int>(ad.count);
   a.scale = ad.scale;
+  if (l.n >= kTileTerms) {
+    a.index = ad.index;
+    a.terms = l.terms;
+    if (l.n >= 4096) start_terms<TX, TA, 2>(l, a);
+    else start_terms<TX, TA, 1>(l, a);
+    return hipGetLastError();
+  }
   const int64_t groups = a.pitch / 8;
   each_slice(l.n, 1, 256 * groups, [&](int64_t first, int64_t count) {
     a.index = ad.index + first;
@@ -119,13 +274,14 @@ struct Segments {
 struct GroupArgs {
   const int64_t* index;
   int n, count;
-  int* order;    // rows by adapter, rising within each
-  int2* spans;   // an adapter's first place in `order`, and its number of rows
+  int* order;    // rows by adapter, rising within each, those without one last
+  int2* spans;   // an adapter's first place in `order`, and its number of rows; the others' last
   Segments by[2];
 };
 
-// A workgroup finds the places of one adapter's rows: its waves each count
-// their part of the index, then write.
+// A workgroup finds the places of one adapter's rows, or the last one those
+// of the rows without: its waves each count their part of the index, then
+// write.
 __global__ __launch_bounds__(1024) void group_kernel(GroupArgs a) {
   constexpr int kWaves = 16;
   __shared__ int less_of[kWaves], equal_of[kWaves];
@@ -135,12 +291,22 @@ __global__ __launch_bounds__(1024) void group_kernel(GroupArgs a) {
   const int64_t share = ((static_cast<int64_t>(a.n) + kWaves - 1) / kWaves + 63) / 64 * 64;
   const int64_t begin = min(static_cast<int64_t>(a.n), wave * share);
   const int64_t end = min(static_cast<int64_t>(a.n), begin + share);
+  constexpr int kBatch = 8;
+  const auto adapter = [&](int64_t i) {  // the rows without as `count`; none behind the end
+    if (i >= end) return int64_t(0x7fffffff);
+    const int64_t id = a.index[i];
+    return id >= 0 && id < a.count ? id : static_cast<int64_t>(a.count);
+  };
   int less = 0, equal = 0;
-#pragma unroll 4
-  for (int64_t i = begin + lane; i < end + lane; i += 64) {
-    const int64_t id = i < end ? a.index[i] : -1;
-    less += id >= 0 && id < me;
-    equal += id == me;
+  for (int64_t i = begin + lane; i < end + lane; i += 64 * kBatch) {
+    int64_t id[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) id[b] = adapter(i + b * 64);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      less += id[b] < me;
+      equal += id[b] == me;
+    }
   }
   less = wave_total(less);
   equal = wave_total(equal);
@@ -155,21 +321,29 @@ __global__ __launch_bounds__(1024) void group_kernel(GroupArgs a) {
   }
   place += before;
   if (equal) {
-    for (int64_t i = begin + lane; i < end + lane; i += 64) {
-      const bool mine = i < end && a.index[i] == me;
-      const unsigned long long mask = __ballot(mine);
-      if (mine)
-        a.order[place + __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask >> 32),
-                                                  __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask), 0))] =
-            static_cast<int>(i);
-      place += __popcll(mask);
+    for (int64_t i = begin + lane; i < end + lane; i += 64 * kBatch) {
+      int64_t id[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) id[b] = adapter(i + b * 64);
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const bool mine = id[b] == me;
+        const unsigned long long mask = __ballot(mine);
+        if (mine)
+          a.order[place + __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask >> 32),
+                                                    __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask), 0))] =
+              static_cast<int>(i + b * 64);
+        place += __popcll(mask);
+      }
     }
   }
   if (threadIdx.x == 0) a.spans[me] = make_int2(before, rows);
+  if (me == a.count) return;
   const bool last = me == a.count - 1;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const Segments& s = a.by[t];
+    if (!s.table) continue;
     const int64_t first = s.first(before, me);
     const int64_t behind = last ? s.first(a.n, a.count) : s.first(before + rows, me + 1);
     for (int64_t i = first + threadIdx.x; i < behind; i += 1024) {
@@ -234,28 +408,54 @@ __global__ __launch_bounds__(256) void sum_kernel(const T* __restrict__ Z, SumAr
   const int64_t c = c0 + low * V;
   const int* order = a.order + seg.first;
   v4f acc[V][RF] = {};
-  for (int p0 = 0; p0 < seg.rows; p0 += 4 * kSteps) {
-    float z[kSteps][V], t[kSteps][RF];
+  // The next rows' places, then the next rows, come while these multiply.
+  T z[kSteps][V];
+  float t[kSteps][RF];
+  int64_t row[kSteps];
+  const auto places = [&](int p0) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) row[s] = order[min(p0 + 4 * s + high, seg.rows - 1)];
+  };
+  const auto fetch = [&](int p0) {
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      const int p = p0 + 4 * s + high;
-      const bool in = p < seg.rows;
-      const int64_t row = order[in ? p : 0];
-      load_vec<V>(Z + row * a.ldz, c, in ? a.wide : 0, z[s]);
+      const bool in = p0 + 4 * s + high < seg.rows;
+      const T* from = Z + row[s] * a.ldz;
+      if (in && c + V <= a.wide) {
+        __builtin_memcpy(z[s], from + c, 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) z[s][e] = in && c + e < a.wide ? from[c + e] : from_float<T>(0.f);
+      }
 #pragma unroll
       for (int f = 0; f < RF; ++f) {
         const int k = rank0 + f * 16 + low;
-        t[s][f] = in && k < a.pitch ? a.terms[row * a.pitch + k] : 0.f;
+        t[s][f] = in && k < a.pitch ? a.terms[row[s] * a.pitch + k] : 0.f;
       }
+    }
+  };
+  places(0);
+  fetch(0);
+  places(4 * kSteps);
+  for (int p0 = 0; p0 < seg.rows; p0 += 4 * kSteps) {
+    T zn[kSteps][V];
+    float tn[kSteps][RF];
+    __builtin_memcpy(zn, z, sizeof(z));
+    __builtin_memcpy(tn, t, sizeof(t));
+    if (p0 + 4 * kSteps < seg.rows) {
+      fetch(p0 + 4 * kSteps);
+      places(p0 + 8 * kSteps);
     }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
 #pragma unroll
       for (int e = 0; e < V; ++e)
 #pragma unroll
-        for (int f = 0; f < RF; ++f)
-          acc[e][f] = RANKS_FIRST ? __builtin_amdgcn_mfma_f32_16x16x4f32(t[s][f], z[s][e], acc[e][f], 0, 0, 0)
-                                  : __builtin_amdgcn_mfma_f32_16x16x4f32(z[s][e], t[s][f], acc[e][f], 0, 0, 0);
+        for (int f = 0; f < RF; ++f) {
+          const float x = to_float(zn[s][e]);
+          acc[e][f] = RANKS_FIRST ? __builtin_amdgcn_mfma_f32_16x16x4f32(tn[s][f], x, acc[e][f], 0, 0, 0)
+                                  : __builtin_amdgcn_mfma_f32_16x16x4f32(x, tn[s][f], acc[e][f], 0, 0, 0);
+        }
   }
   const int64_t size = static_cast<int64_t>(a.rank) * a.wide;
   float* out = seg.slot < 0 ? a.out + seg.adapter * size : a.partial + seg.slot * size;
@@ -343,7 +543,7 @@ GradPlan plan_grad(int grad, int data, int64_t d, int64_t m, int64_t n, int64_t 
   p.length[0] = segment_length(es(grad), m, n);
   p.length[1] = segment_length(es(data), d, n);
   p.order = take(n * sizeof(int));
-  p.spans = take(count * sizeof(int2));
+  p.spans = take((count + 1) * sizeof(int2));
   size_t partial = 0;
   for (int t = 0; t < 2; ++t) {
     const Segments s = {p.length[t], nullptr};
@@ -418,6 +618,17 @@ hipError_t launch_terms(const TermsLaunch& l) {
   }
 }
 
+hipError_t launch_group(const Adapters& ad, int64_t n, int* order, int2* spans, hipStream_t stream) {
+  GroupArgs g = {};
+  g.index = ad.index;
+  g.n = static_cast<int>(n);
+  g.count = static_cast<int>(ad.count);
+  g.order = order;
+  g.spans = spans;
+  group_kernel<<<static_cast<unsigned>(ad.count + 1), 1024, 0, stream>>>(g);
+  return hipGetLastError();
+}
+
 size_t adapted_grad_work_bytes(int grad, int data, int64_t d, int64_t m, int64_t n, int64_t count,
                                int64_t rank) {
   return plan_grad(grad, data, d, m, n, count, rank).end;
@@ -434,7 +645,7 @@ hipError_t launch_adapted_grad(const AdaptedGradLaunch& l) {
   g.order = reinterpret_cast<int*>(work + p.order);
   g.spans = reinterpret_cast<int2*>(work + p.spans);
   for (int t = 0; t < 2; ++t) g.by[t] = Segments{p.length[t], reinterpret_cast<Segment*>(work + p.table[t])};
-  group_kernel<<<static_cast<unsigned>(ad.count), 1024, 0, l.stream>>>(g);
+  group_kernel<<<static_cast<unsigned>(ad.count + 1), 1024, 0, l.stream>>>(g);
   void* Bt = work + p.turned;
   if (ad.data == SDCA_F32) turn<float>(l, Bt);
   else turn<__half>(l, Bt);  // (two bytes either way)
@@ -443,7 +654,7 @@ hipError_t launch_adapted_grad(const AdaptedGradLaunch& l) {
   t.adapters = &ad;
   t.n = l.n;
   t.order = g.order;
-  t.ordered = nullptr;
+  t.spans = g.spans;
   t.stream = l.stream;
   t.data = ad.data;
   t.wide = l.d;

@@ -21,6 +21,8 @@ struct QuantLaunch {
   int8_t* Q;
   int64_t ldq, pad;
   float* scales;
+  // Column i of Q from column order[i] of X; NULL: from column i.
+  const int* order;
   hipStream_t stream;
 };
 hipError_t launch_quantize(const QuantLaunch& a);
@@ -146,19 +148,26 @@ struct TermsLaunch {
   int64_t ldx;
   const Adapters* adapters;
   const void* A;
-  // The rows in the order of their adapters, as `group` leaves it (NULL: as
-  // they come), and their number.
+  // The rows in the order of their adapters and each adapter's place and
+  // number in it, as launch_group leaves them; NULL: as they come.
   const int* order;
-  const int* ordered;
+  const int2* spans;
   float* terms;
   hipStream_t stream;
 };
 hipError_t launch_terms(const TermsLaunch& a);
 
+// The n rows in the order of their adapters, rising for each, those without
+// one last (`order`, n), and each adapter's first place and number of rows
+// (`spans`, count + 1: the last is of the rows without).
+hipError_t launch_group(const Adapters& adapters, int64_t n, int* order, int2* spans,
+                        hipStream_t stream);
+
 // launch_scores_i8 with adapters: terms are the examples' (of X_i itself, not
-// of its 8-bit form).
+// of its 8-bit form).  With an order, 8-bit example i of X is example order[i]
+// of the index, the terms and S.
 hipError_t launch_scores_adapted(const ScoresI8Launch& a, const Adapters& adapters,
-                                 const float* terms);
+                                 const float* terms, const int* order);
 
 struct AdaptedGradLaunch {
   int grad;  // G's type

@@ -1246,6 +1246,7 @@ int quantize_common(int data, int64_t d, int64_t n, const void* X, int64_t ldx, 
   a.ldx = ldx;
   a.ldq = ldq;
   a.pad = d;
+  a.order = nullptr;
   a.stream = stream;
   if ((rc = staged(X, span(d, n, ldx, element_size(data)), host, dx, stream, &a.X)) ||
       (rc = staged_out(Q, span(d, n, ldq, 1), host, dq, &a.Q)) ||
@@ -1333,6 +1334,7 @@ int scores_i8_common(int data, int out, int64_t d, int64_t m, int64_t n, const v
       q.Q = wx;
       q.ldq = q.pad = pad;
       q.scales = wsx;
+      q.order = nullptr;
       q.stream = stream;
       SDCA_HIP_TRY(launch_quantize(q), "quantise kernel");
       a.sx = wsx;
@@ -1616,11 +1618,11 @@ struct StagedAdapters {
 // it is not read in place, the examples' scales, their terms.
 struct AdaptedPlan {
   int64_t pad;
-  bool own_x, own_w;
-  size_t w, scales, terms, end;
+  bool own_x, own_w, grouped;
+  size_t w, scales, terms, order, spans, end;
 };
 AdaptedPlan plan_adapted(int data, int64_t d, int64_t m, int64_t n, const void* W, int64_t ldw,
-                         int64_t rank) {
+                         int64_t rank, int64_t count) {
   using namespace sdca_gpu;
   const auto whole = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
   AdaptedPlan p;
@@ -1630,7 +1632,12 @@ AdaptedPlan plan_adapted(int data, int64_t d, int64_t m, int64_t n, const void* 
   p.w = p.own_x ? whole(static_cast<size_t>(n) * p.pad) : 0;
   p.scales = p.w + (p.own_w ? whole(static_cast<size_t>(m) * p.pad) : 0);
   p.terms = p.scales + (p.own_x ? whole(n * sizeof(float)) : 0);
-  p.end = p.terms + whole(static_cast<size_t>(n) * terms_pitch(rank) * sizeof(float));
+  p.order = p.terms + whole(static_cast<size_t>(n) * terms_pitch(rank) * sizeof(float));
+  // Examples in the order of their adapters: a product of 16 of them then has
+  // one adapter, but for few.
+  p.grouped = p.own_x && count > 1 && n >= 256;
+  p.spans = p.order + (p.grouped ? whole(n * sizeof(int)) : 0);
+  p.end = p.spans + (p.grouped ? whole((count + 1) * sizeof(int2)) : 0);
   return p;
 }
 
@@ -1677,7 +1684,7 @@ int scores_adapted_common(int data, int out, int64_t d, int64_t m, int64_t n, co
       (rc = staged_out(S, span(m, n, lds, element_size(out)), host, dS, &a.S)) ||
       (rc = dad.stage(data, d, m, n, *adapters, host, stream, &ad)))
     return rc;
-  const AdaptedPlan p = plan_adapted(data, d, m, n, a.W, ldw, ad.rank);
+  const AdaptedPlan p = plan_adapted(data, d, m, n, a.W, ldw, ad.rank, ad.count);
   if ((rc = scratch(work, p.end, stream, &work))) return rc;
   char* at = static_cast<char*>(work);
   TermsLaunch t;
@@ -1688,7 +1695,15 @@ int scores_adapted_common(int data, int out, int64_t d, int64_t m, int64_t n, co
   t.ldx = ldx;
   t.adapters = &ad;
   t.A = ad.A;
-  t.order = t.ordered = nullptr;
+  t.order = nullptr;
+  t.spans = nullptr;
+  if (p.grouped) {
+    int* order = reinterpret_cast<int*>(at + p.order);
+    int2* spans = reinterpret_cast<int2*>(at + p.spans);
+    SDCA_HIP_TRY(launch_group(ad, n, order, spans, stream), "grouping kernel");
+    t.order = order;
+    t.spans = spans;
+  }
   t.terms = reinterpret_cast<float*>(at + p.terms);
   t.stream = stream;
   SDCA_HIP_TRY(launch_terms(t), "adapter terms");
@@ -1702,6 +1717,7 @@ int scores_adapted_common(int data, int out, int64_t d, int64_t m, int64_t n, co
     q.Q = reinterpret_cast<int8_t*>(at);
     q.ldq = q.pad = p.pad;
     q.scales = reinterpret_cast<float*>(at + p.scales);
+    q.order = t.order;
     q.stream = stream;
     SDCA_HIP_TRY(launch_quantize(q), "quantise kernel");
     a.X = q.Q;
@@ -1715,7 +1731,7 @@ int scores_adapted_common(int data, int out, int64_t d, int64_t m, int64_t n, co
     a.W = ww;
     a.ldw = p.pad;
   }
-  SDCA_HIP_TRY(launch_scores_adapted(a, ad, t.terms), "adapted score kernel");
+  SDCA_HIP_TRY(launch_scores_adapted(a, ad, t.terms, t.order), "adapted score kernel");
   if (host) {
     if ((rc = fetch_columns(S, a.S, m, n, lds, element_size(out), stream))) return rc;
     SDCA_HIP_TRY(hipStreamSynchronize(stream), "hipStreamSynchronize");
@@ -1852,9 +1868,9 @@ int sdca_log_probs_grad(sdca_dtype data, int64_t m, int64_t n, const void* S, in
 }
 
 size_t sdca_scores_adapted_work(sdca_dtype data, int64_t d, int64_t m, int64_t n,
-                                const int8_t* W, int64_t ldw, int64_t rank) {
-  if (d < 1 || m < 1 || n < 1 || rank < 1) return 0;
-  return plan_adapted(data, d, m, n, W, ldw, rank).end;
+                                const int8_t* W, int64_t ldw, int64_t count, int64_t rank) {
+  if (d < 1 || m < 1 || n < 1 || count < 1 || rank < 1) return 0;
+  return plan_adapted(data, d, m, n, W, ldw, rank, count).end;
 }
 
 int sdca_scores_adapted(sdca_dtype data, sdca_dtype out, int64_t d, int64_t m, int64_t n,

@@ -24,25 +24,32 @@ struct Adapted {
   const T* B;
   int64_t apart;  // from one adapter's B to the next one's
   int rank, count;
+  const int* order;  // or NULL
 
   Adapted from(int64_t n0, int64_t m0) const {
     Adapted a = *this;
-    a.terms += n0 * pitch;
-    a.index += n0;
+    if (order) {
+      a.order += n0;
+    } else {
+      a.terms += n0 * pitch;
+      a.index += n0;
+    }
     a.B += m0 * rank;
     return a;
   }
+  int64_t first_row(int64_t n0) const { return order ? 0 : n0; }
+  __device__ int64_t row(int64_t i) const { return order ? order[i] : i; }
 
   template <int FM, int Q>
   __device__ inline void operator()(v4f (&more)[FM], int64_t row0, int64_t n, int first, int m,
                                     int lane) const {
 #pragma unroll
     for (int i = 0; i < FM; ++i) more[i] = v4f{0.f, 0.f, 0.f, 0.f};
-    const int64_t row = row0 + (lane & 15);
-    const int64_t given = row < n ? index[row] : -1;
+    const int64_t i = row0 + (lane & 15), at_row = row(i < n ? i : n - 1);
+    const int64_t given = i < n ? index[at_row] : -1;
     const bool bad = given < -1 || given >= count;
     const int mine = bad ? -1 : static_cast<int>(given);
-    const float* t = terms + (row < n ? row : n - 1) * pitch;
+    const float* t = terms + at_row * pitch;
     int64_t at[FM];
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
@@ -89,31 +96,34 @@ struct Adapted {
 };
 
 template <class T, class Out>
-hipError_t scores(const ScoresI8Launch& a, const Adapters& ad, const float* terms) {
+hipError_t scores(const ScoresI8Launch& a, const Adapters& ad, const float* terms,
+                  const int* order) {
   const Adapted<T> extra = {terms, static_cast<int>(terms_pitch(ad.rank)), ad.index,
                             static_cast<const T*>(ad.B), a.m * ad.rank, static_cast<int>(ad.rank),
-                            static_cast<int>(ad.count)};
+                            static_cast<int>(ad.count), order};
   if (a.data == SDCA_I8) start_tiles<Out>(a, extra);
   else if (scores_i8_few(a.n, a.d)) start_few<T, Out>(a, extra);
   else start_strip<T, Out>(a, extra);
   return hipGetLastError();
 }
 template <class T>
-hipError_t scores(const ScoresI8Launch& a, const Adapters& ad, const float* terms) {
+hipError_t scores(const ScoresI8Launch& a, const Adapters& ad, const float* terms,
+                  const int* order) {
   switch (a.out) {
-    case SDCA_F32: return scores<T, float>(a, ad, terms);
-    case SDCA_F16: return scores<T, __half>(a, ad, terms);
-    default: return scores<T, __hip_bfloat16>(a, ad, terms);
+    case SDCA_F32: return scores<T, float>(a, ad, terms, order);
+    case SDCA_F16: return scores<T, __half>(a, ad, terms, order);
+    default: return scores<T, __hip_bfloat16>(a, ad, terms, order);
   }
 }
 
 }  // namespace
 
-hipError_t launch_scores_adapted(const ScoresI8Launch& a, const Adapters& ad, const float* terms) {
+hipError_t launch_scores_adapted(const ScoresI8Launch& a, const Adapters& ad, const float* terms,
+                                 const int* order) {
   switch (ad.data) {
-    case SDCA_F32: return scores<float>(a, ad, terms);
-    case SDCA_F16: return scores<__half>(a, ad, terms);
-    default: return scores<__hip_bfloat16>(a, ad, terms);
+    case SDCA_F32: return scores<float>(a, ad, terms, order);
+    case SDCA_F16: return scores<__half>(a, ad, terms, order);
+    default: return scores<__hip_bfloat16>(a, ad, terms, order);
   }
 }
 

@@ -58,10 +58,13 @@ __device__ inline TileAt tile_of(int id, int tiles_n, int tiles_m) {
 // What is added to a wave's scores before they are rounded.  operator() gives
 // it for 16 examples from `row` on by 16 FM classes from `first` on, in the
 // layout of Turned's acc; one() for one example and class, from a whole wave.
-// from() is the same for a slice that starts at that example and class.
+// from() is the same for a slice that starts at that example and class; the
+// slice's example i goes to row row(i) of S from its row first_row() on.
 struct Nothing {
   static constexpr bool some = false;
   Nothing from(int64_t, int64_t) const { return {}; }
+  int64_t first_row(int64_t n0) const { return n0; }
+  __device__ int64_t row(int64_t i) const { return i; }
 };
 
 // A wave's scores to memory: 16 examples at a time are turned round in LDS,
@@ -112,7 +115,7 @@ struct Turned {
         Out v[kUnit];
         __builtin_memcpy(v, __builtin_assume_aligned(turn + row * kPitch + along, 16), 16);
         if (rows + j * 16 + row >= n) continue;
-        Out* out = S + (rows + j * 16 + row) * lds + first + along;
+        Out* out = S + extra.row(rows + j * 16 + row) * lds + first + along;
         if (first + along + kUnit <= m) {
           __builtin_memcpy(out, v, 16);
         } else {
@@ -262,7 +265,7 @@ void start(const ScoresI8Launch& a, const Extra& extra) {
       scores_i8_kernel<Out, Extra, BN, BM, WN, WM, STAGES>
           <<<static_cast<unsigned>(tiles_n) * tiles_m, kThreads, 0, a.stream>>>(
               static_cast<const int8_t*>(a.X) + n0 * a.ldx, a.ldx, a.sx + n0, a.W + m0 * a.ldw, a.ldw,
-              a.sw + m0, static_cast<Out*>(a.S) + n0 * a.lds + m0, a.lds, static_cast<int>(a.d),
+              a.sw + m0, static_cast<Out*>(a.S) + extra.first_row(n0) * a.lds + m0, a.lds, static_cast<int>(a.d),
               static_cast<int>(m), static_cast<int>(n), tiles_n, tiles_m, extra.from(n0, m0));
     });
   });
@@ -602,7 +605,7 @@ void start_tiles(const ScoresI8Launch& a, const Extra& extra) {
       part.n = a.n - head;
       part.X = static_cast<const int8_t*>(a.X) + head * a.ldx;
       part.sx = a.sx + head;
-      part.S = static_cast<Out*>(a.S) + head * a.lds;
+      part.S = static_cast<Out*>(a.S) + extra.first_row(head) * a.lds;
       start_tile<Out>(part, extra.from(head, 0), rest.tile);
       return;
     }

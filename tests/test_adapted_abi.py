@@ -89,7 +89,7 @@ def test_c_entries_refuse():
         assert lib.sdca_scores_adapted(0, 0, 8, 5, 3, at, 8, at, 8, at, bad, at, 5, None, 1, None) == 2
     assert lib.sdca_scores_adapted_grad(0, 0, 8, 5, 3, at, 5, at, 8, ad, None, at, None, 1, None) == 1
     assert lib.sdca_scores_adapted_grad(0, 0, 8, 5, 3, at, 4, at, 8, ad, at, at, None, 1, None) == 2
-    assert lib.sdca_scores_adapted_work(0, 8, 5, 3, ctypes.c_void_p(at), 8, 4) > 0
+    assert lib.sdca_scores_adapted_work(0, 8, 5, 3, ctypes.c_void_p(at), 8, 2, 4) > 0
     assert lib.sdca_scores_adapted_grad_work(0, 0, 8, 5, 3, 2, 4) > 0
 
 

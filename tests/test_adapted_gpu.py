@@ -306,7 +306,7 @@ def test_a_training_step_and_an_answer(cuda, kind):
         full = base + torch.where(some[:, None], more, 0.0)
         want = torch.log_softmax(full, dim=1).gather(1, labels[:, None])[:, 0]
         (want * weight.double()).sum().backward()
-        assert float((logp.double() - want).abs().max()) < 1e-4
+        assert float((logp.double() - want.detach()).abs().max()) < 1e-4
         for got, w in ((dA, a.grad), (dB, b.grad)):
             assert float((got.double() - w).norm()) <= 1e-5 * float(w.norm()) + 1e-12
         A += 50 * dA
