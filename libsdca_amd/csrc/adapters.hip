@@ -148,39 +148,52 @@ __global__ __launch_bounds__(64 * kTermWaves) void terms_tile_kernel(
     for (int j = NE - 1; j >= 0; --j)
       if (left[j]) me = __builtin_amdgcn_readlane(id[j], __builtin_ctzll(left[j]));
     if (me < 0) break;
+    // (Rows behind the rank are the last one again, and examples of other
+    // adapters multiply like the rest: neither's sums are used.)
     const TA* w[RF];
     const TX* x[NE];
-    int of_w[RF], of_x[NE];
 #pragma unroll
-    for (int f = 0; f < RF; ++f) {
-      const int k = f * 16 + low;
-      of_w[f] = k < a.rank ? a.wide : 0;
-      w[f] = A + me * a.lda + static_cast<int64_t>(min(k, a.rank - 1)) * a.wide;
-    }
+    for (int f = 0; f < RF; ++f)
+      w[f] = A + me * a.lda + static_cast<int64_t>(min(f * 16 + low, a.rank - 1)) * a.wide;
 #pragma unroll
     for (int j = 0; j < NE; ++j) {
       left[j] &= ~__ballot(id[j] == me);
-      of_x[j] = id[j] == me ? a.wide : 0;
       x[j] = X + max(row[j], int64_t(0)) * a.ldx;
     }
     v4f acc[NE][RF] = {};
-    for (int64_t at0 = wave * 32; at0 < a.wide; at0 += 32 * kTermWaves * kAhead) {
-      TX u[kAhead][NE][8];
-      TA v[kAhead][RF][8];
-#pragma unroll
-      for (int s = 0; s < kAhead; ++s) {
-        const int64_t at = at0 + s * (32 * kTermWaves) + high * 8;
-#pragma unroll
-        for (int j = 0; j < NE; ++j) load_raw(x[j], at, of_x[j], u[s][j]);
-#pragma unroll
-        for (int f = 0; f < RF; ++f) load_raw(w[f], at, of_w[f], v[s][f]);
-      }
+    constexpr int kStep = 32 * kTermWaves;
+    TX u[kAhead][NE][8];
+    TA v[kAhead][RF][8];
+    const auto products = [&] {
 #pragma unroll
       for (int s = 0; s < kAhead; ++s)
 #pragma unroll
         for (int j = 0; j < NE; ++j)
 #pragma unroll
           for (int f = 0; f < RF; ++f) acc[j][f] = multiply(v[s][f], u[s][j], acc[j][f]);
+    };
+    int64_t at0 = wave * 32;
+    for (; at0 + (kAhead - 1) * kStep + 32 <= a.wide; at0 += kStep * kAhead) {
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        const int64_t at = at0 + s * kStep + high * 8;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) __builtin_memcpy(u[s][j], x[j] + at, sizeof(u[s][j]));
+#pragma unroll
+        for (int f = 0; f < RF; ++f) __builtin_memcpy(v[s][f], w[f] + at, sizeof(v[s][f]));
+      }
+      products();
+    }
+    if (at0 < a.wide) {
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        const int64_t at = at0 + s * kStep + high * 8;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) load_raw(x[j], at, a.wide, u[s][j]);
+#pragma unroll
+        for (int f = 0; f < RF; ++f) load_raw(w[f], at, a.wide, v[s][f]);
+      }
+      products();
     }
     const float scale = a.scale.each ? a.scale.each[me] : a.scale.value;
 #pragma unroll
@@ -195,8 +208,10 @@ __global__ __launch_bounds__(64 * kTermWaves) void terms_tile_kernel(
         v4f sum = part[i][0][lane];
 #pragma unroll
         for (int q = 1; q < kTermWaves; ++q) sum += part[i][q][lane];
-        float* to = a.terms + row[(g + i) / RF] * a.pitch + (g + i) % RF * 16 + high * 4;
-        if ((g + i) % RF * 16 < a.pitch) *reinterpret_cast<v4f*>(to) = sum * scale;
+        const int k = (g + i) % RF * 16 + high * 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = k + e < a.rank ? sum[e] * scale : 0.f;
+        if (k < a.pitch) *reinterpret_cast<v4f*>(a.terms + row[(g + i) / RF] * a.pitch + k) = sum;
       }
     }
   }
@@ -287,19 +302,18 @@ __global__ __launch_bounds__(1024) void group_kernel(GroupArgs a) {
   __shared__ int less_of[kWaves], equal_of[kWaves];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t me = blockIdx.x;
+  const int me = blockIdx.x;
   const int64_t share = ((static_cast<int64_t>(a.n) + kWaves - 1) / kWaves + 63) / 64 * 64;
   const int64_t begin = min(static_cast<int64_t>(a.n), wave * share);
   const int64_t end = min(static_cast<int64_t>(a.n), begin + share);
   constexpr int kBatch = 8;
   const auto adapter = [&](int64_t i) {  // the rows without as `count`; none behind the end
-    if (i >= end) return int64_t(0x7fffffff);
-    const int64_t id = a.index[i];
-    return id >= 0 && id < a.count ? id : static_cast<int64_t>(a.count);
+    const int64_t id = a.index[min(i, end - 1)];
+    return i >= end ? 0x7fffffff : id >= 0 && id < a.count ? static_cast<int>(id) : a.count;
   };
   int less = 0, equal = 0;
   for (int64_t i = begin + lane; i < end + lane; i += 64 * kBatch) {
-    int64_t id[kBatch];
+    int id[kBatch];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) id[b] = adapter(i + b * 64);
 #pragma unroll
@@ -322,7 +336,7 @@ __global__ __launch_bounds__(1024) void group_kernel(GroupArgs a) {
   place += before;
   if (equal) {
     for (int64_t i = begin + lane; i < end + lane; i += 64 * kBatch) {
-      int64_t id[kBatch];
+      int id[kBatch];
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) id[b] = adapter(i + b * 64);
 #pragma unroll
@@ -416,7 +430,17 @@ __global__ __launch_bounds__(256) void sum_kernel(const T* __restrict__ Z, SumAr
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) row[s] = order[min(p0 + 4 * s + high, seg.rows - 1)];
   };
+  const bool across = c0 + 16 * V <= a.wide && rank0 + 16 * RF <= a.pitch;
   const auto fetch = [&](int p0) {
+    if (across && p0 + 4 * kSteps <= seg.rows) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        __builtin_memcpy(z[s], Z + row[s] * a.ldz + c, 16);
+#pragma unroll
+        for (int f = 0; f < RF; ++f) t[s][f] = a.terms[row[s] * a.pitch + rank0 + f * 16 + low];
+      }
+      return;
+    }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const bool in = p0 + 4 * s + high < seg.rows;

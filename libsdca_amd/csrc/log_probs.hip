@@ -231,8 +231,18 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void log_probs_kerne
   bool started = false;
   for (int64_t at = first + (WAVES == 1 ? 0 : wave) * kStep; at < end; at += WAVES * kStep) {
     float v[kLoads][V];
+    if (at + kStep <= end) {
+      T raw[kLoads][V];
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u) load_vec<V>(row, at + (u * 64 + lane) * V, end, v[u], -INFINITY);
+      for (int u = 0; u < kLoads; ++u) __builtin_memcpy(raw[u], row + at + (u * 64 + lane) * V, 16);
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[u][e] = to_float(raw[u][e]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) load_vec<V>(row, at + (u * 64 + lane) * V, end, v[u], -INFINITY);
+    }
     float most = -INFINITY;
 #pragma unroll
     for (int u = 0; u < kLoads; ++u)

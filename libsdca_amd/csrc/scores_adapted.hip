@@ -9,12 +9,107 @@
 namespace sdca_gpu {
 namespace {
 
-// The adapters' part of 16 examples by 16 FM classes: 16 x 16 x 4 products in
-// 32 bits, classes by rank times rank by examples, whose layout is that of
-// the integer product's sums.  Examples of different adapters take turns: for
-// each adapter among the 16 the products are made for all, and each example
-// keeps those of its own, so that one adapter's infinities reach no other
-// example.
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+
+// Sixteen ranks of the terms (rows of 32-bit floats) and of B as the operands
+// of 16 x 16 products.  A lane has its example's, or its class's, part.
+//
+// 32 bits: four products of 16 x 16 x 4; lane group g holds ranks 4 g on.
+template <class T>
+struct Ranks {
+  static constexpr int kEach = 4;
+  static __device__ int from(int lane) { return lane / 16 * 4; }
+  float v[4];
+  int down = 0;
+  __device__ void take(const float* t, int lane) { __builtin_memcpy(v, t + from(lane), 16); }
+  __device__ v4f times(const T (&b)[4]) const {
+    v4f sum = {};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum = __builtin_amdgcn_mfma_f32_16x16x4f32(b[e], v[e], sum, 0, 0, 0);
+    return sum;
+  }
+};
+
+// A 32-bit float as the sum of PARTS 16-bit ones, each the rest's rounding (an
+// infinity is its first part alone).
+template <class H, int PARTS>
+__device__ inline void parts_of(float x, H (&p)[PARTS]) {
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    p[i] = static_cast<H>(x);
+    const float rest = x - static_cast<float>(p[i]);
+    x = fabsf(static_cast<float>(p[i])) < INFINITY ? rest : 0.f;
+  }
+}
+
+// 16 bits: products of 16 x 16 x 32 take the first 16 of their 32 places for
+// one part of the terms and the others for the next, with B's ranks in both:
+// lane groups 0 and 1 hold ranks 0 to 7 and 8 to 15, groups 2 and 3 again.
+//
+// Three bfloat16 make up the 24 bits of a term.
+template <>
+struct Ranks<__hip_bfloat16> {
+  static constexpr int kEach = 8;
+  static __device__ int from(int lane) { return lane / 16 % 2 * 8; }
+  v8b first, last;
+  int down = 0;
+  __device__ void take(const float* t, int lane) {
+    float v[8];
+    __builtin_memcpy(v, t + from(lane), 32);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      __bf16 p[3];
+      parts_of(v[e], p);
+      first[e] = lane < 32 ? p[0] : p[1];
+      last[e] = lane < 32 ? p[2] : static_cast<__bf16>(0.f);
+    }
+  }
+  __device__ v4f times(const __hip_bfloat16 (&b)[8]) const {
+    v8b u;
+    __builtin_memcpy(&u, b, 16);
+    const v4f sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, last, v4f{}, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, first, sum, 0, 0, 0);
+  }
+};
+
+// Two halves have 22 bits, a term's to 2^-23 of it: its 16 ranks are brought
+// to below 2^14 first, so that the second half of the largest is an ordinary
+// number, and their products back (`down`, a power of two).
+template <>
+struct Ranks<__half> {
+  static constexpr int kEach = 8;
+  static __device__ int from(int lane) { return lane / 16 % 2 * 8; }
+  v8h both;
+  int down;
+  __device__ void take(const float* t, int lane) {
+    float v[8], most = 0.f;
+    __builtin_memcpy(v, t + from(lane), 32);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
+    most = fmaxf(most, __shfl_xor(most, 16));
+    down = most < INFINITY ? __builtin_amdgcn_frexp_expf(most) - 14 : 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      _Float16 p[2];
+      parts_of(__builtin_amdgcn_ldexpf(v[e], -down), p);
+      both[e] = lane < 32 ? p[0] : p[1];
+    }
+  }
+  __device__ v4f times(const __half (&b)[8]) const {
+    v8h u;
+    __builtin_memcpy(&u, b, 16);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(u, both, v4f{}, 0, 0, 0);
+  }
+};
+
+// The adapters' part of a wave's scores: products of classes by ranks with
+// ranks by examples, whose layout is that of the integer product's sums.
+// Examples of different adapters take turns: for each adapter the products
+// are made for 16 examples at a time, and each example keeps those of its
+// own, so that one adapter's infinities reach no other example.  B is loaded
+// for some adapters at once: with an adapter for each example the loads'
+// latency is what this takes.
 template <class T>
 struct Adapted {
   static constexpr bool some = true;
@@ -40,47 +135,90 @@ struct Adapted {
   int64_t first_row(int64_t n0) const { return order ? 0 : n0; }
   __device__ int64_t row(int64_t i) const { return order ? order[i] : i; }
 
-  template <int FM, int Q>
-  __device__ inline void operator()(v4f (&more)[FM], int64_t row0, int64_t n, int first, int m,
-                                    int lane) const {
+  template <int FM, int FN, int Q>
+  __device__ inline void add(v4f (&scores)[FM][FN], int64_t row0, int64_t n, int first, int m,
+                             int lane) const {
+    using R = Ranks<T>;
+    constexpr int kOnce = FM > 2 ? 1 : FN > 2 ? 2 : 4;
+    int mine[FN];
+    const float* t[FN];
+    bool bad[FN];
 #pragma unroll
-    for (int i = 0; i < FM; ++i) more[i] = v4f{0.f, 0.f, 0.f, 0.f};
-    const int64_t i = row0 + (lane & 15), at_row = row(i < n ? i : n - 1);
-    const int64_t given = i < n ? index[at_row] : -1;
-    const bool bad = given < -1 || given >= count;
-    const int mine = bad ? -1 : static_cast<int>(given);
-    const float* t = terms + at_row * pitch;
+    for (int j = 0; j < FN; ++j) {
+      const int64_t i = row0 + j * 16 + (lane & 15), at_row = row(i < n ? i : n - 1);
+      const int64_t given = i < n ? index[at_row] : -1;
+      bad[j] = given < -1 || given >= count;
+      mine[j] = bad[j] ? -1 : static_cast<int>(given);
+      t[j] = terms + at_row * pitch;
+    }
     int64_t at[FM];
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int c = first + ((lane & 15) >> 2) * (4 * Q) + (lane & 3) + i / Q * 16 * Q + i % Q * 4;
       at[i] = static_cast<int64_t>(min(c, m - 1)) * rank;
     }
-    unsigned long long left = __ballot(mine >= 0);
-    while (left) {
-      const int a = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
-      const bool hit = mine == a;
-      left &= ~__ballot(hit);
-      const T* b = B + a * apart;
-      v4f sum[FM] = {};
-      for (int k0 = 0; k0 < rank; k0 += 4) {
-        const int k = k0 + lane / 16;
-        const float tk = t[k];  // (zeros behind the rank)
+    for (int k0 = 0; k0 < rank; k0 += 16) {
+      unsigned long long left[FN];
 #pragma unroll
-        for (int i = 0; i < FM; ++i) {
-          const float bk = k < rank ? to_float(b[at[i] + k]) : 0.f;
-          sum[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(bk, tk, sum[i], 0, 0, 0);
+      for (int j = 0; j < FN; ++j) left[j] = __ballot(mine[j] >= 0);
+      const auto next = [&] {
+        int a = -1;
+#pragma unroll
+        for (int j = FN - 1; j >= 0; --j)
+          if (left[j]) a = __builtin_amdgcn_readlane(mine[j], __builtin_ctzll(left[j]));
+#pragma unroll
+        for (int j = 0; j < FN; ++j) left[j] &= ~__ballot(mine[j] == a);
+        return a;
+      };
+      R terms_of[FN];
+#pragma unroll
+      for (int j = 0; j < FN; ++j) terms_of[j].take(t[j] + k0, lane);
+      const int k = k0 + R::from(lane);
+      int a[kOnce];
+      a[0] = next();
+      while (a[0] >= 0) {
+        T b[kOnce][FM][R::kEach];
+#pragma unroll
+        for (int q = 0; q < kOnce; ++q) {
+          if (q) a[q] = next();
+          const T* from = B + (a[q] < 0 ? a[0] : a[q]) * apart;
+#pragma unroll
+          for (int i = 0; i < FM; ++i) {
+            if (k0 + 16 <= rank) {
+              __builtin_memcpy(b[q][i], from + at[i] + k, sizeof(b[q][i]));
+            } else {
+#pragma unroll
+              for (int e = 0; e < R::kEach; ++e) b[q][i][e] = k + e < rank ? from[at[i] + k + e] : from_float<T>(0.f);
+            }
+          }
         }
+#pragma unroll
+        for (int q = 0; q < kOnce; ++q) {
+          if (a[q] < 0) break;
+#pragma unroll
+          for (int j = 0; j < FN; ++j) {
+            const bool hit = mine[j] == a[q];
+            if (!__ballot(hit)) continue;
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+              const v4f sum = terms_of[j].times(b[q][i]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float more = __builtin_amdgcn_ldexpf(sum[e], terms_of[j].down);
+                scores[i][j][e] = hit ? scores[i][j][e] + more : scores[i][j][e];
+              }
+            }
+          }
+        }
+        a[0] = next();
       }
+    }
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) more[i][e] = hit ? sum[i][e] : more[i][e];
-    }
-    if (bad) {
-#pragma unroll
-      for (int i = 0; i < FM; ++i) more[i] = v4f{NAN, NAN, NAN, NAN};
-    }
+        for (int e = 0; e < 4; ++e) scores[i][j][e] = bad[j] ? NAN : scores[i][j][e];
   }
 
   __device__ inline float one(int example, int c, int lane) const {

@@ -55,9 +55,9 @@ __device__ inline TileAt tile_of(int id, int tiles_n, int tiles_m) {
   return {group * kGroup + in % high, in / high};
 }
 
-// What is added to a wave's scores before they are rounded.  operator() gives
-// it for 16 examples from `row` on by 16 FM classes from `first` on, in the
-// layout of Turned's acc; one() for one example and class, from a whole wave.
+// What is added to a wave's scores before they are rounded: add() to 16 FN
+// examples by 16 FM classes in the layout of Turned's acc; one() is it for one
+// example and class, from a whole wave.
 // from() is the same for a slice that starts at that example and class; the
 // slice's example i goes to row row(i) of S from its row first_row() on.
 struct Nothing {
@@ -91,19 +91,32 @@ struct Turned {
     for (int g = 0; g < FM / Q; ++g)
 #pragma unroll
       for (int e = 0; e < kUnit; ++e) scale[g][e] = sw[min(first + g * 16 * Q + mine + e, m - 1)];
+    const auto score = [&](int i, int j, int e, float s) {
+      const int g = i / Q, at = i % Q * 4 + e;
+      return static_cast<float>(acc[i][j][e]) * s * scale[g][at];
+    };
+    v4f more[Extra::some ? FM : 1][Extra::some ? FN : 1];
+    if constexpr (Extra::some) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const float s = x_scale(j * 16 + (lane & 15));
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) more[i][j][e] = score(i, j, e, s);
+      }
+      extra.template add<FM, FN, Q>(more, rows, n, first, m, lane);
+    }
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-      const float s = x_scale(j * 16 + (lane & 15));
-      v4f more[FM];
-      if constexpr (Extra::some) extra.template operator()<FM, Q>(more, rows + j * 16, n, first, m, lane);
+      const float s = Extra::some ? 0.f : x_scale(j * 16 + (lane & 15));
 #pragma unroll
       for (int g = 0; g < FM / Q; ++g) {
         Out v[kUnit];
 #pragma unroll
         for (int e = 0; e < kUnit; ++e) {
-          float score = static_cast<float>(acc[g * Q + e / 4][j][e % 4]) * s * scale[g][e];
-          if constexpr (Extra::some) score += more[g * Q + e / 4][e % 4];
-          v[e] = from_float<Out>(score);
+          if constexpr (Extra::some) v[e] = from_float<Out>(more[g * Q + e / 4][j][e % 4]);
+          else v[e] = from_float<Out>(score(g * Q + e / 4, j, e % 4, s));
         }
         __builtin_memcpy(__builtin_assume_aligned(turn + (lane & 15) * kPitch + g * 16 * Q + mine, 16),
                          v, 16);
