@@ -45,6 +45,48 @@ __device__ inline float wave_largest(float v) {
   return fmaxf(v, other<32, VALU>(v));
 }
 
+// 16 bytes of a column as words, and as floats.  (Held as elements, 16-bit
+// scores take a register each.)
+template <class T>
+__device__ inline unsigned bits_of(T x) {
+  unsigned b = 0;
+  __builtin_memcpy(&b, &x, sizeof(T));
+  return b;
+}
+// The scores from `at` on, -infinity from `end` on.
+template <class T>
+__device__ inline void load_words(const T* row, int64_t at, int64_t end, unsigned (&w)[4]) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T)), kIn = V / 4;
+  if (at + V <= end) {
+    __builtin_memcpy(w, row + at, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = 0;
+#pragma unroll
+      for (int e = 0; e < kIn; ++e) {
+        const int64_t k = at + i * kIn + e;
+        w[i] |= bits_of(k < end ? row[k] : from_float<T>(-INFINITY)) << (16 * e);
+      }
+    }
+  }
+}
+template <class T, int V>
+__device__ inline void unpack(const unsigned (&w)[4], float (&v)[V]) {
+  static_assert(V * sizeof(T) == 16, "whole words");
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    if constexpr (sizeof(T) == 4) {
+      v[e] = __uint_as_float(w[e]);
+    } else {
+      const unsigned short b = static_cast<unsigned short>(w[e / 2] >> (16 * (e % 2)));
+      T x;
+      __builtin_memcpy(&x, &b, 2);
+      v[e] = to_float(x);
+    }
+  }
+}
+
 // The weights of some scores: their largest, and the sums of 2^e and e 2^e
 // with exponents relative to ref_of(max).  (A NaN among the scores makes the
 // sums NaN and leaves max.)
@@ -67,35 +109,45 @@ struct Mass {
 
 // ---------------------------------------------------------------------------
 // The best of a column: a wave's 64 entries (score, index) by lane, falling.
-// Candidates, which are scores of at least `bound`, gather in LDS; 64 of
-// them are sorted and merged into the list.
+// Candidates, which are entries of at least a bound, gather in LDS; 64 of
+// them are sorted and merged into the list.  The bound has an index too: of
+// very many equal scores (a mask of the lowest value) only those of low index
+// are candidates (64 rows of 128000, some so masked: 63 us with the score
+// alone, 18 with both).
 // ---------------------------------------------------------------------------
 struct Best {
   u64 list = 0;
   float bound = kLowest;  // a score below it, or -infinity or NaN, is none
+  int index = 0x7fffffff;  // the last index at which the bound itself is one
   int waiting = 0;
 
   __device__ void merge_sorted(u64 rising) {
     list = rising > list ? rising : list;
     list = sort_merge<32, true>(list, true);
   }
+  __device__ void at_least(u64 entry) {
+    if (!entry) return;
+    bound = score_of(static_cast<unsigned>(entry >> 32));
+    index = index_of(entry);
+  }
   __device__ void merge(u64 some, int top) {
     merge_sorted(sort_wave<true>(some, false));
-    const u64 last = read_lane64(list, top - 1);
-    if (last) bound = fmaxf(bound, score_of(static_cast<unsigned>(last >> 32)));
+    at_least(read_lane64(list, top - 1));
   }
-  __device__ void take(float s, int index, bool candidate, u64* room, int top) {
+  __device__ void take(float s, int at, u64* room, int top) {
+    if (!__ballot(s >= bound)) return;
+    const bool candidate = s > bound || (s == bound && at <= index);
     const u64 mask = __ballot(candidate);
     if (!mask) return;
     const int lane = threadIdx.x & 63;
     if (candidate) {
       const int before = __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask >> 32),
                                                    __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask), 0));
-      room[waiting + before] = entry_of(s, index);
+      room[waiting + before] = entry_of(s, at);
     }
     waiting += __popcll(mask);
-    wave_lds_sync();
     if (waiting < 64) return;
+    wave_lds_sync();
     const u64 first = room[lane], rest = room[64 + lane];
     wave_lds_sync();
     room[lane] = rest;
@@ -103,17 +155,10 @@ struct Best {
     waiting -= 64;
     merge(first, top);
   }
-  // Behind scores of lower index than all that follow: of those, ones equal
-  // to the last of a full list come after it.
-  __device__ void pass(int top) {
-    const u64 last = read_lane64(list, top - 1);
-    if (!last) return;
-    const unsigned key = static_cast<unsigned>(last >> 32);
-    if (score_of(key) == bound) bound = score_of(key + 1);
-  }
   __device__ void finish(u64* room, int top) {
     if (!waiting) return;
     const int lane = threadIdx.x & 63;
+    wave_lds_sync();
     merge(lane < waiting ? room[lane] : 0, top);
     waiting = 0;
   }
@@ -133,9 +178,21 @@ struct LogProbsArgs {
   u64* lists;
 };
 
+// A column's label and its score, read before the column goes by.
+struct Own {
+  int64_t label = -1;
+  float score = 0.f;
+  template <class T>
+  __device__ Own(const T* row, int64_t col, const LogProbsArgs& a) {
+    if (a.logp) label = a.labels[col];
+    if (label >= 0 && label < a.m) score = to_float(row[label]);
+  }
+};
+
 // A column's results, by one wave.
 template <class T>
-__device__ void finish(const T* row, int64_t col, Mass mass, u64 list, const LogProbsArgs& a) {
+__device__ void finish(const T* row, int64_t col, Mass mass, u64 list, const Own& own,
+                       const LogProbsArgs& a) {
   const int lane = threadIdx.x & 63;
   const float c = a.inv_t * kLog2e, max = mass.max, ref = ref_of(max, c);
   const bool near = fabsf(max * c) <= kFar;
@@ -158,10 +215,8 @@ __device__ void finish(const T* row, int64_t col, Mass mass, u64 list, const Log
   if (entropy < 0.f) entropy = 0.f;
   const auto logp = [&](float s) { return none ? -INFINITY : (exponent(s) - log_sum) * kLn2; };
   if (lane == 0) {
-    if (a.logp) {
-      const int64_t label = a.labels[col];
-      a.logp[col] = label == -1 ? 0.f : label < 0 || label >= a.m ? NAN : logp(to_float(row[label]));
-    }
+    if (a.logp)
+      a.logp[col] = own.label == -1 ? 0.f : own.label < 0 || own.label >= a.m ? NAN : logp(own.score);
     if (a.entropy) a.entropy[col] = entropy;
     if (a.stats) {
       float* out = a.stats + 3 * col;
@@ -225,24 +280,29 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void log_probs_kerne
   const T* row = S + col * a.lds;
   const float c = a.inv_t * kLog2e;
   const int first = blockIdx.y * a.length, end = min(a.m, first + a.length);
+  const Own own(row, col, a);
 
   Mass mass;
   Best best;
   bool started = false;
-  for (int64_t at = first + (WAVES == 1 ? 0 : wave) * kStep; at < end; at += WAVES * kStep) {
-    float v[kLoads][V];
+  // The next scores are on their way while these are worked on.
+  unsigned next[kLoads][4];
+  const auto fetch = [&](int64_t at) {
     if (at + kStep <= end) {
-      T raw[kLoads][V];
 #pragma unroll
-      for (int u = 0; u < kLoads; ++u) __builtin_memcpy(raw[u], row + at + (u * 64 + lane) * V, 16);
+      for (int u = 0; u < kLoads; ++u) __builtin_memcpy(next[u], row + at + (u * 64 + lane) * V, 16);
+    } else if (at < end) {
 #pragma unroll
-      for (int u = 0; u < kLoads; ++u)
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[u][e] = to_float(raw[u][e]);
-    } else {
-#pragma unroll
-      for (int u = 0; u < kLoads; ++u) load_vec<V>(row, at + (u * 64 + lane) * V, end, v[u], -INFINITY);
+      for (int u = 0; u < kLoads; ++u) load_words(row, at + (u * 64 + lane) * V, end, next[u]);
     }
+  };
+  int64_t at = first + (WAVES == 1 ? 0 : wave) * kStep;
+  fetch(at);
+  for (; at < end; at += WAVES * kStep) {
+    float v[kLoads][V];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) unpack<T>(next[u], v[u]);
+    fetch(at + WAVES * kStep);
     float most = -INFINITY;
 #pragma unroll
     for (int u = 0; u < kLoads; ++u)
@@ -272,9 +332,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void log_probs_kerne
         for (int u = 0; u < kLoads; ++u)
 #pragma unroll
           for (int e = 0; e < V; ++e)
-            best.take(v[u][e], static_cast<int>(at) + (u * 64 + lane) * V + e, v[u][e] >= best.bound,
-                      room[wave], a.top);
-        best.pass(a.top);
+            best.take(v[u][e], static_cast<int>(at) + (u * 64 + lane) * V + e, room[wave], a.top);
       }
     }
   }
@@ -285,7 +343,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void log_probs_kerne
     if (wave) return;
   }
   if (a.parts == 1) {
-    finish(row, col, mass, best.list, a);
+    finish(row, col, mass, best.list, own, a);
   } else {
     const int64_t part = col * a.parts + blockIdx.y;
     if (lane == 0) a.masses[part] = mass;
@@ -303,6 +361,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void log_probs_join_kernel(const T
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t col = blockIdx.x;
   const float c = a.inv_t * kLog2e;
+  const Own own(S + col * a.lds, col, a);
   Mass mass;
   const int mine = wave + lane * kJoinWaves;
   if (mine < a.parts) mass = a.masses[col * a.parts + mine];
@@ -313,7 +372,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void log_probs_join_kernel(const T
       best.merge_sorted(63 - lane < a.top ? a.lists[(col * a.parts + p) * a.top + 63 - lane] : 0);
   }
   join_waves<kJoinWaves, TOP>(mass, best.list, room, c, wave);
-  if (wave == 0) finish(S + col * a.lds, col, mass, best.list, a);
+  if (wave == 0) finish(S + col * a.lds, col, mass, best.list, own, a);
 }
 
 // How a launch takes the columns: waves to a part, parts to a column.
@@ -489,8 +548,20 @@ __global__ __launch_bounds__(256) void log_probs_grad_kernel(const T* S, T* D, G
 // The whole column in registers: its statistics and then its gradient from
 // one reading.  WAVES waves to a column (with one, four columns to a
 // workgroup), NV vectors to a lane.
+//
+// Scores stay as they came and are converted again for each use, one vector
+// after the other: as floats 16-bit ones take twice the registers, which
+// leaves one workgroup of 1024 to a compute unit, whose loads and exponentials
+// do not overlap.
+template <int NV>
+__device__ inline void keep_words(unsigned (&raw)[NV][4]) {
+#pragma unroll
+  for (int u = 0; u < NV; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(raw[u][i]));
+}
 template <class T, int WAVES, int NV>
-__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void log_probs_grad_whole_kernel(
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, NV > 8 ? 4 : WAVES == 16 ? 8 : 1) void log_probs_grad_whole_kernel(
     const T* S, T* D, GradArgs a) {
   constexpr int V = 16 / static_cast<int>(sizeof(T)), kLanes = 64 * WAVES;
   constexpr int kColumns = WAVES == 1 ? 4 : 1;
@@ -500,23 +571,18 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void log_probs_grad_
   const int64_t col = static_cast<int64_t>(blockIdx.x) * kColumns + threadIdx.x / kLanes;
   if (WAVES == 1 && col >= a.n) return;
   const T* s = S + col * a.lds;
-  T raw[NV][V];
+  unsigned raw[NV][4];
 #pragma unroll
-  for (int u = 0; u < NV; ++u) {
-    const int64_t at = static_cast<int64_t>(u * kLanes + lane) * V;
-    if (at + V <= a.m) {
-      __builtin_memcpy(raw[u], s + at, 16);
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e) raw[u][e] = at + e < a.m ? s[at + e] : from_float<T>(-INFINITY);
-    }
-  }
+  for (int u = 0; u < NV; ++u) load_words(s, static_cast<int64_t>(u * kLanes + lane) * V, a.m, raw[u]);
   GradColumn c(a, col);
   float max = -INFINITY;
 #pragma unroll
-  for (int u = 0; u < NV; ++u)
+  for (int u = 0; u < NV; ++u) {
+    float v[V];
+    unpack<T>(raw[u], v);
 #pragma unroll
-    for (int e = 0; e < V; ++e) max = fmaxf(max, to_float(raw[u][e]));
+    for (int e = 0; e < V; ++e) max = fmaxf(max, v[e]);
+  }
   max = wave_largest<true>(max);
   if constexpr (WAVES > 1) {
     if ((threadIdx.x & 63) == 0) part[0][wave] = max;
@@ -524,17 +590,22 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void log_probs_grad_
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) max = fmaxf(max, part[0][w]);
   }
+  keep_words(raw);
   const float by = a.inv_t * kLog2e, ref = ref_of(max, by);
   float sum = 0.f, weighted = 0.f;
   const auto add = [&](auto exponent) {
 #pragma unroll
-    for (int u = 0; u < NV; ++u)
+    for (int u = 0; u < NV; ++u) {
+      float v[V];
+      unpack<T>(raw[u], v);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float x = exponent(to_float(raw[u][e])), w = exp2_of(x);
+        const float x = exponent(v[e]), w = exp2_of(x);
         sum += w;
         weighted = fmaf(w, fmaxf(x, kGone), weighted);
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
   const bool near = fabsf(max * by) <= kFar || max == -INFINITY;
   if (near) {
@@ -552,6 +623,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void log_probs_grad_
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) sum += part[1][w], weighted += part[2][w];
   }
+  keep_words(raw);
   c.max = max;
   c.none = max == -INFINITY && sum == 0.f;
   c.log2_sum = log2f(sum);
@@ -564,11 +636,11 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void log_probs_grad_
       const int64_t at = static_cast<int64_t>(u * kLanes + lane) * V;
       if (at >= a.m) break;
       float v[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = to_float(raw[u][e]);
+      unpack<T>(raw[u], v);
       T out[V];
       grad_vec<T, V>(v, static_cast<int>(at), c, exponent, a.logp ? a.logp + col : nullptr, out);
       store_vec(d, at, a.m, out);
+      __builtin_amdgcn_sched_barrier(0);  // (all vectors' temporaries at once do not fit)
     }
   };
   if (near) write([&](float x) { return fmaf(x, by, -ref) - c.log2_sum; });
@@ -629,7 +701,7 @@ hipError_t log_probs_grad(LogProbsGradLaunch l) {
     if (l.m <= 256 * V * 4) return start_whole<T, 4, 4>(l), hipGetLastError();
     if (l.m <= 256 * V * 8) return start_whole<T, 4, 8>(l), hipGetLastError();
     if (l.m <= 1024 * V * 4) return start_whole<T, 16, 4>(l), hipGetLastError();
-    if (l.m <= whole_most<T>()) return start_whole<T, 16, 8>(l), hipGetLastError();
+    if (l.m <= whole_most<T>()) return start_whole<T, 8, 16>(l), hipGetLastError();
     LogProbsLaunch s = {};
     s.data = l.data;
     s.m = l.m;
