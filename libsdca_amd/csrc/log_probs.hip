@@ -53,11 +53,12 @@ __device__ inline unsigned bits_of(T x) {
   __builtin_memcpy(&b, &x, sizeof(T));
   return b;
 }
-// The scores from `at` on, -infinity from `end` on.
+// The scores from `at` on, -infinity before `begin` and from `end` on.
 template <class T>
-__device__ inline void load_words(const T* row, int64_t at, int64_t end, unsigned (&w)[4]) {
+__device__ inline void load_words(const T* row, int64_t at, int64_t begin, int64_t end,
+                                  unsigned (&w)[4]) {
   constexpr int V = 16 / static_cast<int>(sizeof(T)), kIn = V / 4;
-  if (at + V <= end) {
+  if (at >= begin && at + V <= end) {
     __builtin_memcpy(w, row + at, 16);
   } else {
 #pragma unroll
@@ -66,10 +67,17 @@ __device__ inline void load_words(const T* row, int64_t at, int64_t end, unsigne
 #pragma unroll
       for (int e = 0; e < kIn; ++e) {
         const int64_t k = at + i * kIn + e;
-        w[i] |= bits_of(k < end ? row[k] : from_float<T>(-INFINITY)) << (16 * e);
+        w[i] |= bits_of(k >= begin && k < end ? row[k] : from_float<T>(-INFINITY)) << (16 * e);
       }
     }
   }
+}
+// How many values a column's first value is behind a multiple of 16 bytes:
+// vectors are taken from there on (2048 columns of 100003 halves at 2 bytes'
+// alignment 91 us, of 100000 84).
+template <class T>
+__device__ inline int behind_16(const T* row) {
+  return static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T));
 }
 template <class T, int V>
 __device__ inline void unpack(const unsigned (&w)[4], float (&v)[V]) {
@@ -98,6 +106,32 @@ struct Mass {
     weighted = f * fmaf(fmaxf(by, kGone), sum, weighted);
     sum *= f;
     max = to;
+  }
+  // A lane's scores (as words); returns their largest.
+  template <class T, int N>
+  __device__ float add(const unsigned (&raw)[N][4], float c) {
+    constexpr int V = 16 / static_cast<int>(sizeof(T));
+    float v[N][V], most = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < N; ++u) unpack<T>(raw[u], v[u]);
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) most = fmaxf(most, v[u][e]);
+    if (most > max) rise(most, c);
+    const float ref = ref_of(max, c);
+    float s = 0.f, w_e = 0.f;
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float x = fmaf(v[u][e], c, -ref), w = exp2_of(x);
+        s += w;
+        w_e = fmaf(w, fmaxf(x, kGone), w_e);
+      }
+    sum += s;
+    weighted += w_e;
+    return most;
   }
   // All lanes' together, in every lane.
   __device__ void over_wave(float c) {
@@ -285,42 +319,17 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void log_probs_kerne
   Mass mass;
   Best best;
   bool started = false;
-  // The next scores are on their way while these are worked on.
-  unsigned next[kLoads][4];
-  const auto fetch = [&](int64_t at) {
-    if (at + kStep <= end) {
+  for (int64_t at = first - behind_16(row + first) + (WAVES == 1 ? 0 : wave) * kStep; at < end;
+       at += WAVES * kStep) {
+    unsigned raw[kLoads][4];
+    if (at >= first && at + kStep <= end) {
 #pragma unroll
-      for (int u = 0; u < kLoads; ++u) __builtin_memcpy(next[u], row + at + (u * 64 + lane) * V, 16);
-    } else if (at < end) {
+      for (int u = 0; u < kLoads; ++u) __builtin_memcpy(raw[u], row + at + (u * 64 + lane) * V, 16);
+    } else {
 #pragma unroll
-      for (int u = 0; u < kLoads; ++u) load_words(row, at + (u * 64 + lane) * V, end, next[u]);
+      for (int u = 0; u < kLoads; ++u) load_words(row, at + (u * 64 + lane) * V, first, end, raw[u]);
     }
-  };
-  int64_t at = first + (WAVES == 1 ? 0 : wave) * kStep;
-  fetch(at);
-  for (; at < end; at += WAVES * kStep) {
-    float v[kLoads][V];
-#pragma unroll
-    for (int u = 0; u < kLoads; ++u) unpack<T>(next[u], v[u]);
-    fetch(at + WAVES * kStep);
-    float most = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < kLoads; ++u)
-#pragma unroll
-      for (int e = 0; e < V; ++e) most = fmaxf(most, v[u][e]);
-    if (most > mass.max) mass.rise(most, c);
-    const float ref = ref_of(mass.max, c);
-    float sum = 0.f, weighted = 0.f;
-#pragma unroll
-    for (int u = 0; u < kLoads; ++u)
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float x = fmaf(v[u][e], c, -ref), w = exp2_of(x);
-        sum += w;
-        weighted = fmaf(w, fmaxf(x, kGone), weighted);
-      }
-    mass.sum += sum;
-    mass.weighted += weighted;
+    const float most = mass.add<T>(raw, c);
     if constexpr (TOP) {
       if (!started) {
         // `top` lanes have a score of at least this.
@@ -328,6 +337,9 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void log_probs_kerne
         started = true;
       }
       if (__ballot(most >= best.bound)) {
+        float v[kLoads][V];
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) unpack<T>(raw[u], v[u]);
 #pragma unroll
         for (int u = 0; u < kLoads; ++u)
 #pragma unroll
@@ -462,58 +474,68 @@ struct GradArgs {
   float* logp;
 };
 
-// A column's own numbers.  `g` and `h` are the gradients over T.
+// A column's own numbers.  With weights w = 2^e whose sum is 2^log2_sum, the
+// gradient of a score that is not the label's is w (c1 + c2 e).
 struct GradColumn {
-  float max, log2_sum, entropy, g, h;
+  float log2_sum, c1, c2, g;
   int label;
   bool none;
+
   __device__ GradColumn(const GradArgs& a, int64_t col) {
     const int64_t l = a.labels[col];
-    label = l >= 0 && l < a.m ? static_cast<int>(l) : -1;
+    // (Far below the first vector, which starts up to 15 before the column.)
+    label = l >= 0 && l < a.m ? static_cast<int>(l) : -0x7fffffff;
     g = l == -1 ? 0.f : label < 0 ? NAN : a.g[col] * a.inv_t;
-    h = a.h ? a.h[col] * a.inv_t : 0.f;
     if (a.logp && label < 0 && threadIdx.x % 64 == 0) a.logp[col] = l == -1 ? 0.f : NAN;
   }
-  // log2 p -> the gradient of a score that is not the label's.
+  __device__ void set(const GradArgs& a, int64_t col, float log_sum, float entropy, bool empty) {
+    log2_sum = log_sum;
+    none = empty;
+    const float h = a.h ? a.h[col] * a.inv_t : 0.f, one = exp2_of(-log2_sum);
+    c1 = none ? g * 0.f : -one * fmaf(h, fmaf(-log2_sum, kLn2, entropy), g);
+    c2 = none ? 0.f : -one * h * kLn2;
+  }
+  template <bool H>
   __device__ float of(float e) const {
-    const float p = exp2_of(e);
-    return none ? (g != g ? g : 0.f) : -p * fmaf(h, fmaf(fmaxf(e, kGone), kLn2, entropy), g);
+    const float w = exp2_of(e);
+    return H ? w * fmaf(c2, fmaxf(e, kGone), c1) : w * c1;
   }
 };
 
-template <class T, int V>
-__device__ inline void store_vec(T* row, int64_t at, int64_t len, const T (&v)[V]) {
-  if (at + V <= len) {
-    __builtin_memcpy(row + at, v, sizeof(v));
-  } else {
+// V scores of a column, from `at` on, to their gradients; the lane that has
+// the label's writes its log-probability.  (S and D may be one matrix: a lane
+// has read what it writes.)
+template <bool H, class T, int V, class Exponent>
+__device__ inline void grad_vec(const unsigned (&raw)[4], int at, int m, const GradColumn& c,
+                                Exponent exponent, float* logp, T* d) {
+  float s[V];
+  unpack<T>(raw, s);
+  T out[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e)
-      if (at + e < len) row[at + e] = v[e];
-  }
-}
-
-// V scores of a column to their gradients; the lane that has the label's
-// writes its log-probability.  (S and D may be one matrix: a lane has read
-// what it writes.)
-template <class T, int V, class Exponent>
-__device__ inline void grad_vec(const float (&s)[V], int at, const GradColumn& c, Exponent exponent,
-                                float* logp, T (&d)[V]) {
-#pragma unroll
-  for (int e = 0; e < V; ++e) d[e] = from_float<T>(c.of(exponent(s[e])));
+  for (int e = 0; e < V; ++e) out[e] = from_float<T>(c.of<H>(exponent(s[e])));
   if (c.label >= at && c.label < at + V) {
 #pragma unroll
     for (int e = 0; e < V; ++e)
       if (c.label == at + e) {
         const float x = exponent(s[e]);
-        if (!c.none) d[e] = from_float<T>(c.of(x) + c.g);
-        if (logp) *logp = c.none ? -INFINITY : x * kLn2;
+        if (!c.none) out[e] = from_float<T>(c.of<H>(x) + c.g);
+        if (logp) *logp = c.none ? -INFINITY : (x - c.log2_sum) * kLn2;
       }
+  }
+  if (at >= 0 && at + V <= m) {
+    unsigned words[4];  // (one store; of elements it would be four)
+    __builtin_memcpy(words, out, 16);
+    __builtin_memcpy(d + at, words, 16);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (at + e >= 0 && at + e < m) d[at + e] = out[e];
   }
 }
 
 // From the columns' statistics.  A workgroup takes 256 kLoads vectors of a
 // column (ROWS = 1), or each of its waves a column of its own.
-template <class T, int ROWS>
+template <class T, int ROWS, bool H>
 __global__ __launch_bounds__(256) void log_probs_grad_kernel(const T* S, T* D, GradArgs a) {
   constexpr int V = 16 / static_cast<int>(sizeof(T)), kLoads = 4, kLanes = 256 / ROWS;
   const int lane = threadIdx.x % kLanes;
@@ -521,26 +543,23 @@ __global__ __launch_bounds__(256) void log_probs_grad_kernel(const T* S, T* D, G
   if (col >= a.n) return;
   GradColumn c(a, col);
   const float* stats = a.stats + 3 * col;
-  c.max = stats[0];
-  c.log2_sum = stats[1] * kLog2e;
-  c.entropy = stats[2];
-  c.none = c.max == -INFINITY && c.log2_sum == -INFINITY;
-  const float by = a.inv_t * kLog2e;
-  const auto exponent = [&](float s) { return fmaf(fminf(s - c.max, 0.f), by, -c.log2_sum); };
+  const float max = stats[0], by = a.inv_t * kLog2e;
+  c.set(a, col, stats[1] * kLog2e, stats[2], max == -INFINITY && stats[1] == -INFINITY);
+  const auto exponent = [&](float s) { return fminf(s - max, 0.f) * by; };
   const T* s = S + col * a.lds;
   T* d = D + col * a.ldd;
-  for (int64_t at0 = static_cast<int64_t>(blockIdx.y) * kLanes * V * kLoads; at0 < a.m;
-       at0 += static_cast<int64_t>(gridDim.y) * kLanes * V * kLoads) {
-    float v[kLoads][V];
+  float* logp = a.logp ? a.logp + col : nullptr;
+  constexpr int kStep = kLanes * V * kLoads;
+  for (int64_t at0 = static_cast<int64_t>(blockIdx.y) * kStep - behind_16(s); at0 < a.m;
+       at0 += static_cast<int64_t>(gridDim.y) * kStep) {
+    unsigned raw[kLoads][4];
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u) load_vec<V>(s, at0 + (u * kLanes + lane) * V, a.m, v[u], -INFINITY);
+    for (int u = 0; u < kLoads; ++u) load_words(s, at0 + (u * kLanes + lane) * V, 0, a.m, raw[u]);
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
       const int64_t at = at0 + (u * kLanes + lane) * V;
       if (at >= a.m) break;
-      T out[V];
-      grad_vec<T, V>(v[u], static_cast<int>(at), c, exponent, a.logp ? a.logp + col : nullptr, out);
-      store_vec(d, at, a.m, out);
+      grad_vec<H, T, V>(raw[u], static_cast<int>(at), a.m, c, exponent, logp, d);
     }
   }
 }
@@ -560,8 +579,8 @@ __device__ inline void keep_words(unsigned (&raw)[NV][4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(raw[u][i]));
 }
-template <class T, int WAVES, int NV>
-__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, NV > 8 ? 4 : WAVES == 16 ? 8 : 1) void log_probs_grad_whole_kernel(
+template <class T, int WAVES, int NV, bool H>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, WAVES == 16 ? 8 : 1) void log_probs_grad_whole_kernel(
     const T* S, T* D, GradArgs a) {
   constexpr int V = 16 / static_cast<int>(sizeof(T)), kLanes = 64 * WAVES;
   constexpr int kColumns = WAVES == 1 ? 4 : 1;
@@ -571,9 +590,10 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, NV > 8 ? 4 : WAVES =
   const int64_t col = static_cast<int64_t>(blockIdx.x) * kColumns + threadIdx.x / kLanes;
   if (WAVES == 1 && col >= a.n) return;
   const T* s = S + col * a.lds;
+  const int at0 = lane * V - behind_16(s);
   unsigned raw[NV][4];
 #pragma unroll
-  for (int u = 0; u < NV; ++u) load_words(s, static_cast<int64_t>(u * kLanes + lane) * V, a.m, raw[u]);
+  for (int u = 0; u < NV; ++u) load_words(s, at0 + u * kLanes * V, 0, a.m, raw[u]);
   GradColumn c(a, col);
   float max = -INFINITY;
 #pragma unroll
@@ -624,32 +644,119 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, NV > 8 ? 4 : WAVES =
     for (int w = 0; w < WAVES; ++w) sum += part[1][w], weighted += part[2][w];
   }
   keep_words(raw);
-  c.max = max;
-  c.none = max == -INFINITY && sum == 0.f;
-  c.log2_sum = log2f(sum);
-  c.entropy = (c.log2_sum - weighted / sum) * kLn2;
-  if (c.entropy < 0.f) c.entropy = 0.f;
+  const float log2_sum = log2f(sum);
+  float entropy = (log2_sum - weighted / sum) * kLn2;
+  if (entropy < 0.f) entropy = 0.f;
+  c.set(a, col, log2_sum, entropy, max == -INFINITY && sum == 0.f);
   T* d = D + col * a.ldd;
+  float* logp = a.logp ? a.logp + col : nullptr;
   const auto write = [&](auto exponent) {
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      const int64_t at = static_cast<int64_t>(u * kLanes + lane) * V;
+      const int at = at0 + u * kLanes * V;
       if (at >= a.m) break;
-      float v[V];
-      unpack<T>(raw[u], v);
-      T out[V];
-      grad_vec<T, V>(v, static_cast<int>(at), c, exponent, a.logp ? a.logp + col : nullptr, out);
-      store_vec(d, at, a.m, out);
+      grad_vec<H, T, V>(raw[u], at, a.m, c, exponent, logp, d);
       __builtin_amdgcn_sched_barrier(0);  // (all vectors' temporaries at once do not fit)
     }
   };
-  if (near) write([&](float x) { return fmaf(x, by, -ref) - c.log2_sum; });
-  else write([&](float x) { return fmaf(fminf(x - max, 0.f), by, -c.log2_sum); });
+  if (near) write([&](float x) { return fmaf(x, by, -ref); });
+  else write([&](float x) { return fminf(x - max, 0.f) * by; });
 }
 
-// Columns that the whole-column kernel holds.
+// A longer column by one workgroup that goes through it twice: for the
+// statistics, and backwards for the gradient, which finds the column's end in
+// the L2 and the rest in the last-level cache.
+constexpr int kTwiceWaves = 16;
+template <class T, bool H>
+__global__ __launch_bounds__(64 * kTwiceWaves, 8) void log_probs_grad_twice_kernel(const T* S, T* D, GradArgs a) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T)), kLoads = 4, kLanes = 64 * kTwiceWaves;
+  constexpr int kStep = kLanes * V * kLoads;
+  __shared__ float part[3][kTwiceWaves];
+  __shared__ int odd;
+  const int lane = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(lane >> 6);
+  const int64_t col = blockIdx.x;
+  const T* s = S + col * a.lds;
+  T* d = D + col * a.ldd;
+  const float by = a.inv_t * kLog2e;
+  GradColumn c(a, col);
+  const int64_t begin = -static_cast<int64_t>(behind_16(s));
+  const int64_t steps = (a.m - begin + kStep - 1) / kStep;
+  const auto load = [&](int64_t step, unsigned (&raw)[kLoads][4]) {
+    const int64_t at0 = begin + step * kStep;
+    if (at0 >= 0 && at0 + kStep <= a.m) {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) __builtin_memcpy(raw[u], s + at0 + (u * kLanes + lane) * V, 16);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) load_words(s, at0 + (u * kLanes + lane) * V, 0, a.m, raw[u]);
+    }
+  };
+  Mass mass;
+  for (int64_t step = 0; step < steps; ++step) {
+    unsigned raw[kLoads][4];
+    load(step, raw);
+    mass.add<T>(raw, by);
+  }
+  mass.over_wave(by);
+  if ((lane & 63) == 0) part[0][wave] = mass.max, part[1][wave] = mass.sum, part[2][wave] = mass.weighted;
+  __syncthreads();
+  mass = Mass();
+  if ((lane & 63) < kTwiceWaves) {
+    mass.max = part[0][lane & 63];
+    mass.sum = part[1][lane & 63];
+    mass.weighted = part[2][lane & 63];
+  }
+  mass.over_wave(by);
+  const float max = mass.max, ref = ref_of(max, by);
+  const bool near = fabsf(max * by) <= kFar || max == -INFINITY;
+  if (!near) {
+    // Scores near the largest float, or infinite: once more, from s - max.
+    float sum = 0.f, weighted = 0.f;
+    bool bad = false;
+    for (int64_t i = lane; i < a.m; i += kLanes) {
+      const float x = to_float(s[i]), e = fminf(x - max, 0.f) * by, w = exp2_of(e);
+      bad |= x != x;
+      sum += w;
+      weighted = fmaf(w, fmaxf(e, kGone), weighted);
+    }
+    sum = wave_total(sum);
+    weighted = wave_total(weighted);
+    if (lane == 0) odd = 0;
+    __syncthreads();
+    if (bad) odd = 1;
+    if ((lane & 63) == 0) part[1][wave] = sum, part[2][wave] = weighted;
+    __syncthreads();
+    mass.sum = mass.weighted = 0.f;
+    for (int w = 0; w < kTwiceWaves; ++w) mass.sum += part[1][w], mass.weighted += part[2][w];
+    if (odd) mass.sum = NAN;
+  }
+  const float log2_sum = log2f(mass.sum);
+  float entropy = (log2_sum - mass.weighted / mass.sum) * kLn2;
+  if (entropy < 0.f) entropy = 0.f;
+  c.set(a, col, log2_sum, entropy, max == -INFINITY && mass.sum == 0.f);
+  float* logp = a.logp ? a.logp + col : nullptr;
+  for (int64_t step = steps - 1; step >= 0; --step) {
+    unsigned raw[kLoads][4];
+    load(step, raw);
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int64_t at = begin + step * kStep + (u * kLanes + lane) * V;
+      if (at >= a.m) break;
+      if (near) grad_vec<H, T, V>(raw[u], static_cast<int>(at), a.m, c, [&](float x) { return fmaf(x, by, -ref); }, logp, d);
+      else grad_vec<H, T, V>(raw[u], static_cast<int>(at), a.m, c, [&](float x) { return fminf(x - max, 0.f) * by; }, logp, d);
+    }
+  }
+}
+
+// From so many columns on they go to a workgroup each.
+constexpr int64_t kTwiceColumns = 256;
+
+// Columns that the whole-column kernel holds, wherever they start.
 template <class T>
-constexpr int64_t whole_most() { return 64 * 16 * 8 * 16 / static_cast<int64_t>(sizeof(T)); }
+constexpr int64_t whole_most(int vectors = 1024 * 4) {
+  return (vectors - 1) * int64_t(16) / static_cast<int64_t>(sizeof(T)) + 1;
+}
 
 template <class T>
 GradArgs args_of(const LogProbsGradLaunch& l, int64_t first, int64_t count) {
@@ -672,10 +779,21 @@ void start_whole(const LogProbsGradLaunch& l) {
   constexpr int64_t kColumns = WAVES == 1 ? 4 : 1;
   constexpr int kThreads = WAVES == 1 ? 256 : 64 * WAVES;
   each_slice(l.n, kColumns, kThreads, [&](int64_t first, int64_t count) {
-    log_probs_grad_whole_kernel<T, WAVES, NV>
-        <<<static_cast<unsigned>((count + kColumns - 1) / kColumns), kThreads, 0, l.stream>>>(
-            static_cast<const T*>(l.S) + first * l.lds, static_cast<T*>(l.D) + first * l.ldd,
-            args_of<T>(l, first, count));
+    const auto kernel = l.h ? log_probs_grad_whole_kernel<T, WAVES, NV, true>
+                            : log_probs_grad_whole_kernel<T, WAVES, NV, false>;
+    kernel<<<static_cast<unsigned>((count + kColumns - 1) / kColumns), kThreads, 0, l.stream>>>(
+        static_cast<const T*>(l.S) + first * l.lds, static_cast<T*>(l.D) + first * l.ldd,
+        args_of<T>(l, first, count));
+  });
+}
+
+template <class T>
+void start_twice(const LogProbsGradLaunch& l) {
+  each_slice(l.n, 1, 64 * kTwiceWaves, [&](int64_t first, int64_t count) {
+    const auto kernel = l.h ? log_probs_grad_twice_kernel<T, true> : log_probs_grad_twice_kernel<T, false>;
+    kernel<<<static_cast<unsigned>(count), 64 * kTwiceWaves, 0, l.stream>>>(
+        static_cast<const T*>(l.S) + first * l.lds, static_cast<T*>(l.D) + first * l.ldd,
+        args_of<T>(l, first, count));
   });
 }
 
@@ -685,10 +803,10 @@ void start_grad(const LogProbsGradLaunch& l) {
   const int64_t parts = ROWS > 1 ? 1 : (l.m + kEach - 1) / kEach;
   const unsigned across = static_cast<unsigned>(parts < 1024 ? parts : 1024);
   each_slice(l.n, ROWS, 256 * static_cast<int64_t>(across), [&](int64_t first, int64_t count) {
-    log_probs_grad_kernel<T, ROWS>
-        <<<dim3(static_cast<unsigned>((count + ROWS - 1) / ROWS), across), 256, 0, l.stream>>>(
-            static_cast<const T*>(l.S) + first * l.lds, static_cast<T*>(l.D) + first * l.ldd,
-            args_of<T>(l, first, count));
+    const auto kernel = l.h ? log_probs_grad_kernel<T, ROWS, true> : log_probs_grad_kernel<T, ROWS, false>;
+    kernel<<<dim3(static_cast<unsigned>((count + ROWS - 1) / ROWS), across), 256, 0, l.stream>>>(
+        static_cast<const T*>(l.S) + first * l.lds, static_cast<T*>(l.D) + first * l.ldd,
+        args_of<T>(l, first, count));
   });
 }
 
@@ -696,12 +814,18 @@ template <class T>
 hipError_t log_probs_grad(LogProbsGradLaunch l) {
   constexpr int64_t V = 16 / sizeof(T);
   if (!l.stats) {
-    if (l.m <= 64 * V) return start_whole<T, 1, 1>(l), hipGetLastError();
-    if (l.m <= 64 * V * 4) return start_whole<T, 1, 4>(l), hipGetLastError();
-    if (l.m <= 256 * V * 4) return start_whole<T, 4, 4>(l), hipGetLastError();
-    if (l.m <= 256 * V * 8) return start_whole<T, 4, 8>(l), hipGetLastError();
-    if (l.m <= 1024 * V * 4) return start_whole<T, 16, 4>(l), hipGetLastError();
-    if (l.m <= whole_most<T>()) return start_whole<T, 8, 16>(l), hipGetLastError();
+    const bool aligned = reinterpret_cast<uintptr_t>(l.S) % 16 == 0 && (l.n == 1 || l.lds % V == 0);
+    const auto holds = [&](int vectors) {
+      return l.m <= whole_most<T>(vectors) || (aligned && l.m <= vectors * V);
+    };
+    if (holds(64)) return start_whole<T, 1, 1>(l), hipGetLastError();
+    if (holds(64 * 4)) return start_whole<T, 1, 4>(l), hipGetLastError();
+    if (holds(256 * 4)) return start_whole<T, 4, 4>(l), hipGetLastError();
+    if (holds(256 * 8)) return start_whole<T, 4, 8>(l), hipGetLastError();
+    if (holds(1024 * 4)) return start_whole<T, 16, 4>(l), hipGetLastError();
+    // (4096 columns of 65536 bfloat16: 227 us, with the statistics in a launch
+    // of their own 302; but a few columns leave most of the device idle.)
+    if (l.n >= kTwiceColumns) return start_twice<T>(l), hipGetLastError();
     LogProbsLaunch s = {};
     s.data = l.data;
     s.m = l.m;
@@ -740,7 +864,7 @@ hipError_t launch_log_probs(const LogProbsLaunch& l) {
 }
 
 size_t log_probs_grad_work_bytes(int data, int64_t m, int64_t n, bool stats) {
-  if (stats || m <= (data == SDCA_F32 ? whole_most<float>() : whole_most<__half>())) return 0;
+  if (stats || n >= kTwiceColumns || m <= (data == SDCA_F32 ? whole_most<float>() : whole_most<__half>())) return 0;
   return (3 * static_cast<size_t>(n) * sizeof(float) + 15) / 16 * 16 + log_probs_work_bytes(data, m, n, 0);
 }
 
