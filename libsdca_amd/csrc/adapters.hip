@@ -21,46 +21,115 @@ namespace {
 typedef float v4f __attribute__((ext_vector_type(4)));
 
 // ---------------------------------------------------------------------------
-// Terms.
+// Terms, and with them the rows in 8 bits where Q is given.
 // ---------------------------------------------------------------------------
 struct TermsArgs {
   int64_t ldx, lda;  // lda: from one adapter's A to the next one's
   int wide, rank, pitch, count;
   const int64_t* index;
+  const int* order;  // or NULL
   PerColumn<float> scale;
   float* terms;
+  int8_t* Q;
+  int pad;
+  float* scales;
 };
 
 // From so many examples on, 16 or 32 of them to a workgroup.
 constexpr int64_t kTileTerms = 128;
 
-// A workgroup takes eight of the adapter's rows for one example.
+// Eight neighbouring values of a row from `at` on, zeros from `len` on.
+template <class T>
+__device__ inline void load_raw(const T* row, int64_t at, int64_t len, T (&v)[8]) {
+  if (at + 8 <= len) {
+    __builtin_memcpy(v, row + at, sizeof(v));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = at + e < len ? row[at + e] : from_float<T>(0.f);
+  }
+}
+
+// `lanes` lanes take the column x of d values to 8 bits with that scale, and
+// zeros up to pad.
+template <class T>
+__device__ inline void write_column(const T* x, int d, const ColumnScale& s, int8_t* q, int pad, int lane,
+                                    int lanes) {
+  constexpr int kOnce = sizeof(T) == 4 ? 2 : 4;
+  for (int at0 = lane * 8; at0 < pad; at0 += lanes * 8 * kOnce) {
+    T raw[kOnce][8];
+#pragma unroll
+    for (int i = 0; i < kOnce; ++i) load_column(x, at0 + i * lanes * 8, d, raw[i]);
+#pragma unroll
+    for (int i = 0; i < kOnce; ++i) {
+      const int at = at0 + i * lanes * 8;
+      if (at >= pad) break;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = to_float(raw[i][e]);
+      unsigned w[2];
+      quantize8(v, s, w);
+      end_column(at, d, w);
+      __builtin_memcpy(q + at, w, 8);  // (pad is whole tiles)
+    }
+  }
+}
+
+// A workgroup takes eight of the adapter's rows for one example; the last of
+// an example's workgroups its 8-bit form.
 template <class TX, class TA>
 __global__ __launch_bounds__(256) void terms_row_kernel(const TX* __restrict__ X,
                                                         const TA* __restrict__ A, TermsArgs a) {
   __shared__ float part[4][8];
-  const int64_t row = blockIdx.x;
+  __shared__ unsigned most_of[4];
+  const int64_t p = blockIdx.x, row = a.order ? a.order[p] : p;
+  const TX* x = X + row * a.ldx;
+  if (static_cast<int>(blockIdx.y) * 8 >= a.pitch) {
+    unsigned most = 0;
+    for (int at = threadIdx.x * 8; at < a.wide; at += 256 * 8) {
+      TX raw[8];
+      load_column(x, at, a.wide, raw);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = max(most, magnitude(to_float(raw[e])));
+    }
+#pragma unroll
+    for (int off = 32; off; off >>= 1) most = max(most, static_cast<unsigned>(__shfl_xor(most, off)));
+    if ((threadIdx.x & 63) == 0) most_of[threadIdx.x >> 6] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) most = max(most, most_of[w]);
+    const ColumnScale s(most);
+    if (threadIdx.x == 0) a.scales[p] = s.scale;
+    write_column(x, a.wide, s, a.Q + p * a.pad, a.pad, threadIdx.x, 256);
+    return;
+  }
   const int64_t id = a.index[row];
   if (id < 0 || id >= a.count) return;
   const int k0 = blockIdx.y * 8;
   if (k0 >= a.rank) {
-    if (threadIdx.x < 8) a.terms[row * a.pitch + k0 + threadIdx.x] = 0.f;
+    if (threadIdx.x < 8) a.terms[p * a.pitch + k0 + threadIdx.x] = 0.f;
     return;
   }
-  const TX* x = X + row * a.ldx;
   const TA* w = A + id * a.lda + static_cast<int64_t>(k0) * a.wide;
   float acc[8] = {};
-  for (int at = threadIdx.x * 8; at < a.wide; at += 256 * 8) {
-    float v[8];
-    load_vec<8>(x, at, a.wide, v);
-    float u[8][8];
+  const auto add = [&](int at, auto load) {
+    TX v[8];
+    TA u[8][8];
+    load(x, v);
 #pragma unroll
     for (int k = 0; k < 8; ++k)  // (rows behind the rank: the last one again)
-      load_vec<8>(w + static_cast<int64_t>(min(k, a.rank - 1 - k0)) * a.wide, at, a.wide, u[k]);
+      load(w + static_cast<int64_t>(min(k, a.rank - 1 - k0)) * a.wide, u[k]);
 #pragma unroll
     for (int k = 0; k < 8; ++k)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[k] = fmaf(v[e], u[k][e], acc[k]);
+      for (int e = 0; e < 8; ++e) acc[k] = fmaf(to_float(v[e]), to_float(u[k][e]), acc[k]);
+  };
+  for (int at0 = 0; at0 < a.wide; at0 += 256 * 8) {
+    const int at = at0 + threadIdx.x * 8;
+    if (at0 + 256 * 8 <= a.wide) {
+      add(at, [&](const auto* from, auto& v) { __builtin_memcpy(v, from + at, sizeof(v)); });
+    } else {
+      add(at, [&](const auto* from, auto& v) { load_raw(from, at, a.wide, v); });
+    }
   }
 #pragma unroll
   for (int k = 0; k < 8; ++k) acc[k] = wave_total(acc[k]);
@@ -73,23 +142,12 @@ __global__ __launch_bounds__(256) void terms_row_kernel(const TX* __restrict__ X
     const int k = threadIdx.x;
     const float sum = part[0][k] + part[1][k] + part[2][k] + part[3][k];
     const float scale = a.scale.each ? a.scale.each[id] : a.scale.value;
-    a.terms[row * a.pitch + k0 + k] = k0 + k < a.rank ? sum * scale : 0.f;
+    a.terms[p * a.pitch + k0 + k] = k0 + k < a.rank ? sum * scale : 0.f;
   }
 }
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
-
-// Eight neighbouring values of a row from `at` on, zeros from `len` on.
-template <class T>
-__device__ inline void load_raw(const T* row, int64_t at, int64_t len, T (&v)[8]) {
-  if (at + 8 <= len) {
-    __builtin_memcpy(v, row + at, sizeof(v));
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = at + e < len ? row[at + e] : from_float<T>(0.f);
-  }
-}
 
 // sum += a product of 16 rows by 16 columns over 32 values: a lane has eight
 // of row and of column lane % 16.  Two halves or two bfloat16 multiply as
@@ -116,45 +174,56 @@ __device__ inline v4f multiply(const TA (&a)[8], const TB (&b)[8], v4f sum) {
 
 // A workgroup takes 16 NE examples with all ranks (16 RF); its waves share the
 // wide axis, 32 values at a time, and add up through LDS.  Examples of
-// different adapters take turns; in the adapters' order that is rare.
+// different adapters take turns; in the adapters' order that is rare.  With
+// QUANT the largest magnitudes come with the first reading, and the rows are
+// read again for their 8-bit form, by then from the last-level cache (20000
+// rows of 4096 floats: XXX us, in two kernels 114 and 64).
 constexpr int kTermWaves = 8;
-template <class TX, class TA, int NE, int RF>
+constexpr int steps_ahead(int registers) {  // 72 registers of loads at most
+  return registers <= 9 ? 8 : registers <= 18 ? 4 : registers <= 36 ? 2 : 1;
+}
+template <class TX, class TA, int NE, int RF, bool QUANT>
 __global__ __launch_bounds__(64 * kTermWaves) void terms_tile_kernel(
     const TX* __restrict__ X, const TA* __restrict__ A, TermsArgs a, int64_t n,
-    const int* __restrict__ order, const int2* __restrict__ spans, int64_t first) {
-  constexpr int kAhead = RF > 4 ? 1 : std::is_same<TX, TA>::value && sizeof(TX) == 2 && RF < 4 ? 4 : 2;
+    const int2* __restrict__ spans, int64_t first) {
+  constexpr bool kOneType = std::is_same<TX, TA>::value;
+  constexpr int kAhead = steps_ahead(kOneType ? (NE + RF) * 2 * static_cast<int>(sizeof(TX)) : (NE + RF) * 8);
   constexpr int kFrags = NE * RF;
   constexpr int kOnce = kFrags < 4 ? kFrags : 4;
   __shared__ v4f part[kOnce][kTermWaves][64];
+  __shared__ unsigned most_of[kTermWaves][NE * 16];
   const int lane = threadIdx.x & 63, low = lane & 15, high = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t total = order ? spans[a.count].x : n;
+  const int64_t total = a.order && !QUANT ? spans[a.count].x : n;
   const int64_t p0 = (first + blockIdx.x) * (16 * NE);
   if (p0 >= total) return;
+  const auto row_of = [&](int64_t p) { return a.order ? static_cast<int64_t>(a.order[p]) : p; };
   int64_t row[NE];
   int id[NE];
   unsigned long long left[NE];
+  unsigned most[NE] = {};
 #pragma unroll
   for (int j = 0; j < NE; ++j) {
     const int64_t p = p0 + j * 16 + low;
-    row[j] = p < total ? (order ? order[p] : p) : -1;
+    row[j] = p < total ? row_of(p) : -1;
     const int64_t given = row[j] >= 0 ? a.index[row[j]] : -1;
     id[j] = given >= 0 && given < a.count ? static_cast<int>(given) : -1;
     left[j] = __ballot(id[j] >= 0);
   }
+  bool seen = !QUANT;
   while (true) {
     int me = -1;
 #pragma unroll
     for (int j = NE - 1; j >= 0; --j)
       if (left[j]) me = __builtin_amdgcn_readlane(id[j], __builtin_ctzll(left[j]));
-    if (me < 0) break;
+    if (me < 0 && seen) break;
     // (Rows behind the rank are the last one again, and examples of other
     // adapters multiply like the rest: neither's sums are used.)
     const TA* w[RF];
     const TX* x[NE];
 #pragma unroll
     for (int f = 0; f < RF; ++f)
-      w[f] = A + me * a.lda + static_cast<int64_t>(min(f * 16 + low, a.rank - 1)) * a.wide;
+      w[f] = A + max(me, 0) * a.lda + static_cast<int64_t>(min(f * 16 + low, a.rank - 1)) * a.wide;
 #pragma unroll
     for (int j = 0; j < NE; ++j) {
       left[j] &= ~__ballot(id[j] == me);
@@ -168,9 +237,14 @@ __global__ __launch_bounds__(64 * kTermWaves) void terms_tile_kernel(
 #pragma unroll
       for (int s = 0; s < kAhead; ++s)
 #pragma unroll
-        for (int j = 0; j < NE; ++j)
+        for (int j = 0; j < NE; ++j) {
 #pragma unroll
           for (int f = 0; f < RF; ++f) acc[j][f] = multiply(v[s][f], u[s][j], acc[j][f]);
+          if constexpr (QUANT) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most[j] = max(most[j], magnitude(to_float(u[s][j][e])));
+          }
+        }
     };
     int64_t at0 = wave * 32;
     for (; at0 + (kAhead - 1) * kStep + 32 <= a.wide; at0 += kStep * kAhead) {
@@ -182,7 +256,11 @@ __global__ __launch_bounds__(64 * kTermWaves) void terms_tile_kernel(
 #pragma unroll
         for (int f = 0; f < RF; ++f) __builtin_memcpy(v[s][f], w[f] + at, sizeof(v[s][f]));
       }
+      // (All loads first: in an order of its own choice the compiler has few on
+      // their way at a time.)
+      __builtin_amdgcn_sched_barrier(0);
       products();
+      __builtin_amdgcn_sched_barrier(0);
     }
     if (at0 < a.wide) {
 #pragma unroll
@@ -195,6 +273,8 @@ __global__ __launch_bounds__(64 * kTermWaves) void terms_tile_kernel(
       }
       products();
     }
+    seen = true;
+    if (me < 0) break;
     const float scale = a.scale.each ? a.scale.each[me] : a.scale.value;
 #pragma unroll
     for (int g = 0; g < kFrags; g += kOnce) {
@@ -204,31 +284,62 @@ __global__ __launch_bounds__(64 * kTermWaves) void terms_tile_kernel(
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < kOnce; ++i) {
-        if (wave != i || id[(g + i) / RF] != me) continue;
+        const int j = (g + i) / RF, k = (g + i) % RF * 16 + high * 4;
+        if (wave != i || id[j] != me) continue;
         v4f sum = part[i][0][lane];
 #pragma unroll
         for (int q = 1; q < kTermWaves; ++q) sum += part[i][q][lane];
-        const int k = (g + i) % RF * 16 + high * 4;
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum[e] = k + e < a.rank ? sum[e] * scale : 0.f;
-        if (k < a.pitch) *reinterpret_cast<v4f*>(a.terms + row[(g + i) / RF] * a.pitch + k) = sum;
+        if (k < a.pitch) *reinterpret_cast<v4f*>(a.terms + (p0 + j * 16 + low) * a.pitch + k) = sum;
       }
+    }
+  }
+  if constexpr (QUANT) {
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+      most[j] = max(most[j], static_cast<unsigned>(__shfl_xor(most[j], 16)));
+      most[j] = max(most[j], static_cast<unsigned>(__shfl_xor(most[j], 32)));
+      if (lane < 16) most_of[wave][j * 16 + lane] = most[j];
+    }
+    __syncthreads();
+    for (int r = wave; r < 16 * NE; r += kTermWaves) {
+      const int64_t p = p0 + r;
+      if (p >= total) break;
+      unsigned all = 0;
+#pragma unroll
+      for (int w = 0; w < kTermWaves; ++w) all = max(all, most_of[w][r]);
+      const ColumnScale s(all);
+      if (lane == 0) a.scales[p] = s.scale;
+      write_column(X + row_of(p) * a.ldx, a.wide, s, a.Q + p * a.pad, a.pad, lane, 64);
     }
   }
 }
 
-template <class TX, class TA, int NE, int RF>
+template <class TX, class TA, int NE, int RF, bool QUANT>
 void start_terms(const TermsLaunch& l, const TermsArgs& a) {
   each_slice((l.n + 16 * NE - 1) / (16 * NE), 1, 64 * kTermWaves, [&](int64_t first, int64_t count) {
-    terms_tile_kernel<TX, TA, NE, RF><<<static_cast<unsigned>(count), 64 * kTermWaves, 0, l.stream>>>(
-        static_cast<const TX*>(l.X), static_cast<const TA*>(l.A), a, l.n, l.order, l.spans, first);
+    terms_tile_kernel<TX, TA, NE, RF, QUANT><<<static_cast<unsigned>(count), 64 * kTermWaves, 0, l.stream>>>(
+        static_cast<const TX*>(l.X), static_cast<const TA*>(l.A), a, l.n, l.spans, first);
   });
 }
-template <class TX, class TA, int NE>
+template <class TX, class TA, int NE, int RF>
 void start_terms(const TermsLaunch& l, const TermsArgs& a) {
-  if (a.rank <= 16) start_terms<TX, TA, NE, 1>(l, a);
-  else if (a.rank <= 32) start_terms<TX, TA, NE, 2>(l, a);
-  else if (a.rank <= 64) start_terms<TX, TA, NE, 4>(l, a);
+  if constexpr (std::is_same<TX, TA>::value) {
+    if (l.Q) return start_terms<TX, TA, NE, RF, true>(l, a);
+  }
+  start_terms<TX, TA, NE, RF, false>(l, a);
+}
+// Of A there is as much to read as of 16 examples, or more for a rank above
+// 16: 32 share it.  (8192 rows of 14336 bfloat16, rank 16: 62 us, 16 at a time
+// 75; but 20000 rows of 4096 floats 84 and 71, with the registers of twice the
+// loads.)
+template <class TX, class TA>
+void start_terms(const TermsLaunch& l, const TermsArgs& a) {
+  const bool many = l.n >= 4096;
+  if (a.rank <= 16) many && sizeof(TX) == 2 ? start_terms<TX, TA, 2, 1>(l, a) : start_terms<TX, TA, 1, 1>(l, a);
+  else if (a.rank <= 32) many ? start_terms<TX, TA, 2, 2>(l, a) : start_terms<TX, TA, 1, 2>(l, a);
+  else if (a.rank <= 64) many ? start_terms<TX, TA, 2, 4>(l, a) : start_terms<TX, TA, 1, 4>(l, a);
   else start_terms<TX, TA, 1, 8>(l, a);
 }
 
@@ -243,20 +354,20 @@ hipError_t terms(const TermsLaunch& l) {
   a.pitch = static_cast<int>(terms_pitch(ad.rank));
   a.count = static_cast<int>(ad.count);
   a.scale = ad.scale;
+  a.index = ad.index;
+  a.order = l.order;
+  a.terms = l.terms;
+  a.Q = l.Q;
+  a.pad = static_cast<int>(l.pad);
+  a.scales = l.scales;
+  if (l.n == 0) return hipSuccess;
   if (l.n >= kTileTerms) {
-    a.index = ad.index;
-    a.terms = l.terms;
-    if (l.n >= 4096) start_terms<TX, TA, 2>(l, a);
-    else start_terms<TX, TA, 1>(l, a);
+    start_terms<TX, TA>(l, a);
     return hipGetLastError();
   }
-  const int64_t groups = a.pitch / 8;
-  each_slice(l.n, 1, 256 * groups, [&](int64_t first, int64_t count) {
-    a.index = ad.index + first;
-    a.terms = l.terms + first * a.pitch;
-    terms_row_kernel<TX, TA><<<dim3(static_cast<unsigned>(count), static_cast<unsigned>(groups)), 256, 0, l.stream>>>(
-        static_cast<const TX*>(l.X) + first * l.ldx, static_cast<const TA*>(l.A), a);
-  });
+  const unsigned groups = static_cast<unsigned>(a.pitch / 8 + (l.Q ? 1 : 0));
+  terms_row_kernel<TX, TA><<<dim3(static_cast<unsigned>(l.n), groups), 256, 0, l.stream>>>(
+      static_cast<const TX*>(l.X), static_cast<const TA*>(l.A), a);
   return hipGetLastError();
 }
 template <class TX>
@@ -291,6 +402,7 @@ struct GroupArgs {
   int n, count;
   int* order;    // rows by adapter, rising within each, those without one last
   int2* spans;   // an adapter's first place in `order`, and its number of rows; the others' last
+  int* ids;      // or NULL: the rows' adapters in their order, -1, or -2 for no adapter's number
   Segments by[2];
 };
 
@@ -298,7 +410,7 @@ struct GroupArgs {
 // of the rows without: its waves each count their part of the index, then
 // write.
 __global__ __launch_bounds__(1024) void group_kernel(GroupArgs a) {
-  constexpr int kWaves = 16;
+  constexpr int kWaves = 16, kBatch = 4;
   __shared__ int less_of[kWaves], equal_of[kWaves];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -306,16 +418,30 @@ __global__ __launch_bounds__(1024) void group_kernel(GroupArgs a) {
   const int64_t share = ((static_cast<int64_t>(a.n) + kWaves - 1) / kWaves + 63) / 64 * 64;
   const int64_t begin = min(static_cast<int64_t>(a.n), wave * share);
   const int64_t end = min(static_cast<int64_t>(a.n), begin + share);
-  constexpr int kBatch = 8;
-  const auto adapter = [&](int64_t i) {  // the rows without as `count`; none behind the end
-    const int64_t id = a.index[min(i, end - 1)];
-    return i >= end ? 0x7fffffff : id >= 0 && id < a.count ? static_cast<int>(id) : a.count;
+  // kBatch rows' adapters, the rows without as `count`, none behind the end.
+  // (A whole batch without conditions: its loads are then on their way
+  // together; 20000 rows took 18 us one load after the other.)
+  const auto adapters = [&](int64_t i0, int (&id)[kBatch]) {
+    int64_t raw[kBatch];
+    if (i0 + 64 * kBatch <= end) {
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) raw[b] = a.index[i0 + b * 64 + lane];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b)
+        id[b] = raw[b] >= 0 && raw[b] < a.count ? static_cast<int>(raw[b]) : a.count;
+    } else {
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int64_t i = i0 + b * 64 + lane;
+        raw[b] = i < end ? a.index[i] : 0;
+        id[b] = i >= end ? 0x7fffffff : raw[b] >= 0 && raw[b] < a.count ? static_cast<int>(raw[b]) : a.count;
+      }
+    }
   };
   int less = 0, equal = 0;
-  for (int64_t i = begin + lane; i < end + lane; i += 64 * kBatch) {
+  for (int64_t i0 = begin; i0 < end; i0 += 64 * kBatch) {
     int id[kBatch];
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) id[b] = adapter(i + b * 64);
+    adapters(i0, id);
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       less += id[b] < me;
@@ -335,18 +461,20 @@ __global__ __launch_bounds__(1024) void group_kernel(GroupArgs a) {
   }
   place += before;
   if (equal) {
-    for (int64_t i = begin + lane; i < end + lane; i += 64 * kBatch) {
+    for (int64_t i0 = begin; i0 < end; i0 += 64 * kBatch) {
       int id[kBatch];
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b) id[b] = adapter(i + b * 64);
+      adapters(i0, id);
+      const int64_t i = i0 + lane;
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
         const bool mine = id[b] == me;
         const unsigned long long mask = __ballot(mine);
-        if (mine)
-          a.order[place + __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask >> 32),
-                                                    __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask), 0))] =
-              static_cast<int>(i + b * 64);
+        if (mine) {
+          const int to = place + __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask >> 32),
+                                                           __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask), 0));
+          a.order[to] = static_cast<int>(i + b * 64);
+          if (a.ids) a.ids[to] = me < a.count ? me : a.index[i + b * 64] == -1 ? -1 : -2;
+        }
         place += __popcll(mask);
       }
     }
@@ -393,6 +521,27 @@ __global__ __launch_bounds__(256) void turn_kernel(const T* __restrict__ B, int 
 }
 
 // ---------------------------------------------------------------------------
+// 16 bytes of a row from `at` on as words, zeros from `len` on.
+template <class T>
+__device__ inline void load_some(const T* row, int64_t at, int64_t len, unsigned (&w)[4]) {
+  constexpr int kIn = 4 / static_cast<int>(sizeof(T));
+  if (at + 4 * kIn <= len) {
+    __builtin_memcpy(w, row + at, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = 0;
+#pragma unroll
+      for (int e = 0; e < kIn; ++e) {
+        const int64_t k = at + i * kIn + e;
+        unsigned b = 0;
+        if (k < len) __builtin_memcpy(&b, row + k, sizeof(T));
+        w[i] |= b << (16 * e);
+      }
+    }
+  }
+}
+
 // Sums over rows: out[c][k] or out[k][c] = sum_i Z_ic V_ik for the rows of a
 // segment, by 16 x 16 x 4 products in 32 bits.  A lane loads 16 bytes of a
 // row, V neighbouring values, four rows at a time; value e of all lanes makes
@@ -421,9 +570,10 @@ __global__ __launch_bounds__(256) void sum_kernel(const T* __restrict__ Z, SumAr
   const int rank0 = blockIdx.y * 16 * RF;
   const int64_t c = c0 + low * V;
   const int* order = a.order + seg.first;
+  const float* terms = a.terms + static_cast<int64_t>(seg.first) * a.pitch;
   v4f acc[V][RF] = {};
   // The next rows' places, then the next rows, come while these multiply.
-  T z[kSteps][V];
+  unsigned z[kSteps][4];
   float t[kSteps][RF];
   int64_t row[kSteps];
   const auto places = [&](int p0) {
@@ -437,24 +587,18 @@ __global__ __launch_bounds__(256) void sum_kernel(const T* __restrict__ Z, SumAr
       for (int s = 0; s < kSteps; ++s) {
         __builtin_memcpy(z[s], Z + row[s] * a.ldz + c, 16);
 #pragma unroll
-        for (int f = 0; f < RF; ++f) t[s][f] = a.terms[row[s] * a.pitch + rank0 + f * 16 + low];
+        for (int f = 0; f < RF; ++f) t[s][f] = terms[static_cast<int64_t>(p0 + 4 * s + high) * a.pitch + rank0 + f * 16 + low];
       }
       return;
     }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const bool in = p0 + 4 * s + high < seg.rows;
-      const T* from = Z + row[s] * a.ldz;
-      if (in && c + V <= a.wide) {
-        __builtin_memcpy(z[s], from + c, 16);
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) z[s][e] = in && c + e < a.wide ? from[c + e] : from_float<T>(0.f);
-      }
+      load_some(Z + row[s] * a.ldz, c, in ? a.wide : 0, z[s]);
 #pragma unroll
       for (int f = 0; f < RF; ++f) {
         const int k = rank0 + f * 16 + low;
-        t[s][f] = in && k < a.pitch ? a.terms[row[s] * a.pitch + k] : 0.f;
+        t[s][f] = in && k < a.pitch ? terms[static_cast<int64_t>(p0 + 4 * s + high) * a.pitch + k] : 0.f;
       }
     }
   };
@@ -462,24 +606,27 @@ __global__ __launch_bounds__(256) void sum_kernel(const T* __restrict__ Z, SumAr
   fetch(0);
   places(4 * kSteps);
   for (int p0 = 0; p0 < seg.rows; p0 += 4 * kSteps) {
-    T zn[kSteps][V];
+    unsigned zn[kSteps][4];
     float tn[kSteps][RF];
     __builtin_memcpy(zn, z, sizeof(z));
     __builtin_memcpy(tn, t, sizeof(t));
+    __builtin_amdgcn_sched_barrier(0);
     if (p0 + 4 * kSteps < seg.rows) {
       fetch(p0 + 4 * kSteps);
       places(p0 + 8 * kSteps);
     }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
+    for (int s = 0; s < kSteps; ++s) {
+      float x[V];
+      unpack<T>(zn[s], x);
 #pragma unroll
       for (int e = 0; e < V; ++e)
 #pragma unroll
-        for (int f = 0; f < RF; ++f) {
-          const float x = to_float(zn[s][e]);
-          acc[e][f] = RANKS_FIRST ? __builtin_amdgcn_mfma_f32_16x16x4f32(tn[s][f], x, acc[e][f], 0, 0, 0)
-                                  : __builtin_amdgcn_mfma_f32_16x16x4f32(x, tn[s][f], acc[e][f], 0, 0, 0);
-        }
+        for (int f = 0; f < RF; ++f)
+          acc[e][f] = RANKS_FIRST ? __builtin_amdgcn_mfma_f32_16x16x4f32(tn[s][f], x[e], acc[e][f], 0, 0, 0)
+                                  : __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], tn[s][f], acc[e][f], 0, 0, 0);
+    }
   }
   const int64_t size = static_cast<int64_t>(a.rank) * a.wide;
   float* out = seg.slot < 0 ? a.out + seg.adapter * size : a.partial + seg.slot * size;
@@ -642,13 +789,15 @@ hipError_t launch_terms(const TermsLaunch& l) {
   }
 }
 
-hipError_t launch_group(const Adapters& ad, int64_t n, int* order, int2* spans, hipStream_t stream) {
+hipError_t launch_group(const Adapters& ad, int64_t n, int* order, int2* spans, int* ids,
+                        hipStream_t stream) {
   GroupArgs g = {};
   g.index = ad.index;
   g.n = static_cast<int>(n);
   g.count = static_cast<int>(ad.count);
   g.order = order;
   g.spans = spans;
+  g.ids = ids;
   group_kernel<<<static_cast<unsigned>(ad.count + 1), 1024, 0, stream>>>(g);
   return hipGetLastError();
 }
@@ -662,7 +811,7 @@ hipError_t launch_adapted_grad(const AdaptedGradLaunch& l) {
   const Adapters& ad = l.adapters;
   const GradPlan p = plan_grad(l.grad, ad.data, l.d, l.m, l.n, ad.count, ad.rank);
   char* work = static_cast<char*>(l.work);
-  GroupArgs g;
+  GroupArgs g = {};
   g.index = ad.index;
   g.n = static_cast<int>(l.n);
   g.count = static_cast<int>(ad.count);
@@ -679,6 +828,9 @@ hipError_t launch_adapted_grad(const AdaptedGradLaunch& l) {
   t.n = l.n;
   t.order = g.order;
   t.spans = g.spans;
+  t.Q = nullptr;
+  t.pad = 0;
+  t.scales = nullptr;
   t.stream = l.stream;
   t.data = ad.data;
   t.wide = l.d;

@@ -21,8 +21,6 @@ struct QuantLaunch {
   int8_t* Q;
   int64_t ldq, pad;
   float* scales;
-  // Column i of Q from column order[i] of X; NULL: from column i.
-  const int* order;
   hipStream_t stream;
 };
 hipError_t launch_quantize(const QuantLaunch& a);
@@ -140,7 +138,7 @@ constexpr int64_t terms_pitch(int64_t rank) { return (rank + 15) / 16 * 16; }
 
 // terms[i] = scale_a X_i A_a' for the n rows of X (`wide` values of type
 // `data`, pitch ldx) with A_a's `rank` rows of `wide` values, adapters
-// count apart; rows without an adapter are left as they are.
+// count apart; rows without an adapter have none written.
 struct TermsLaunch {
   int data;
   int64_t wide, n;
@@ -149,25 +147,33 @@ struct TermsLaunch {
   const Adapters* adapters;
   const void* A;
   // The rows in the order of their adapters and each adapter's place and
-  // number in it, as launch_group leaves them; NULL: as they come.
+  // number in it, as launch_group leaves them: terms (and Q) are then in that
+  // order.  NULL: as they come.
   const int* order;
   const int2* spans;
   float* terms;
+  // NULL, or the rows in 8 bits besides, as launch_quantize gives them with
+  // ldq = pad.
+  int8_t* Q;
+  int64_t pad;
+  float* scales;
   hipStream_t stream;
 };
 hipError_t launch_terms(const TermsLaunch& a);
 
 // The n rows in the order of their adapters, rising for each, those without
-// one last (`order`, n), and each adapter's first place and number of rows
-// (`spans`, count + 1: the last is of the rows without).
-hipError_t launch_group(const Adapters& adapters, int64_t n, int* order, int2* spans,
+// one last (`order`, n), each adapter's first place and number of rows
+// (`spans`, count + 1: the last is of the rows without), and, or NULL, the
+// rows' adapters in that order (`ids`, n: -1 without, -2 where the index is
+// none of [-1, count)).
+hipError_t launch_group(const Adapters& adapters, int64_t n, int* order, int2* spans, int* ids,
                         hipStream_t stream);
 
 // launch_scores_i8 with adapters: terms are the examples' (of X_i itself, not
-// of its 8-bit form).  With an order, 8-bit example i of X is example order[i]
-// of the index, the terms and S.
+// of its 8-bit form).  With an order, 8-bit example i of X, its terms and
+// ids[i] are those of row order[i] of S.
 hipError_t launch_scores_adapted(const ScoresI8Launch& a, const Adapters& adapters,
-                                 const float* terms, const int* order);
+                                 const float* terms, const int* order, const int* ids);
 
 struct AdaptedGradLaunch {
   int grad;  // G's type

@@ -35,6 +35,23 @@ __device__ inline void load_vec(const T* row, int64_t at, int64_t len, float (&v
   }
 }
 
+// 16 bytes of a row, held as words, as floats.
+template <class T, int V>
+__device__ inline void unpack(const unsigned (&w)[4], float (&v)[V]) {
+  static_assert(V * sizeof(T) == 16, "whole words");
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    if constexpr (sizeof(T) == 4) {
+      v[e] = __uint_as_float(w[e]);
+    } else {
+      const unsigned short b = static_cast<unsigned short>(w[e / 2] >> (16 * (e % 2)));
+      T x;
+      __builtin_memcpy(&x, &b, 2);
+      v[e] = to_float(x);
+    }
+  }
+}
+
 // Eight values of a column of d for its quantiser: those from `at` on, or the
 // last eight where the column ends before at + 8: one load whatever d (20011
 // columns of 513 half-precision values 12 us, with a load for each value of

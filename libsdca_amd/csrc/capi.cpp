@@ -1246,7 +1246,6 @@ int quantize_common(int data, int64_t d, int64_t n, const void* X, int64_t ldx, 
   a.ldx = ldx;
   a.ldq = ldq;
   a.pad = d;
-  a.order = nullptr;
   a.stream = stream;
   if ((rc = staged(X, span(d, n, ldx, element_size(data)), host, dx, stream, &a.X)) ||
       (rc = staged_out(Q, span(d, n, ldq, 1), host, dq, &a.Q)) ||
@@ -1334,7 +1333,6 @@ int scores_i8_common(int data, int out, int64_t d, int64_t m, int64_t n, const v
       q.Q = wx;
       q.ldq = q.pad = pad;
       q.scales = wsx;
-      q.order = nullptr;
       q.stream = stream;
       SDCA_HIP_TRY(launch_quantize(q), "quantise kernel");
       a.sx = wsx;
@@ -1619,7 +1617,7 @@ struct StagedAdapters {
 struct AdaptedPlan {
   int64_t pad;
   bool own_x, own_w, grouped;
-  size_t w, scales, terms, order, spans, end;
+  size_t w, scales, terms, order, ids, spans, end;
 };
 AdaptedPlan plan_adapted(int data, int64_t d, int64_t m, int64_t n, const void* W, int64_t ldw,
                          int64_t rank, int64_t count) {
@@ -1636,7 +1634,8 @@ AdaptedPlan plan_adapted(int data, int64_t d, int64_t m, int64_t n, const void* 
   // Examples in the order of their adapters: a product of 16 of them then has
   // one adapter, but for few.
   p.grouped = p.own_x && count > 1 && n >= 256;
-  p.spans = p.order + (p.grouped ? whole(n * sizeof(int)) : 0);
+  p.ids = p.order + (p.grouped ? whole(n * sizeof(int)) : 0);
+  p.spans = p.ids + (p.grouped ? whole(n * sizeof(int)) : 0);
   p.end = p.spans + (p.grouped ? whole((count + 1) * sizeof(int2)) : 0);
   return p;
 }
@@ -1697,32 +1696,25 @@ int scores_adapted_common(int data, int out, int64_t d, int64_t m, int64_t n, co
   t.A = ad.A;
   t.order = nullptr;
   t.spans = nullptr;
+  int* ids = nullptr;
   if (p.grouped) {
     int* order = reinterpret_cast<int*>(at + p.order);
     int2* spans = reinterpret_cast<int2*>(at + p.spans);
-    SDCA_HIP_TRY(launch_group(ad, n, order, spans, stream), "grouping kernel");
+    ids = reinterpret_cast<int*>(at + p.ids);
+    SDCA_HIP_TRY(launch_group(ad, n, order, spans, ids, stream), "grouping kernel");
     t.order = order;
     t.spans = spans;
   }
   t.terms = reinterpret_cast<float*>(at + p.terms);
+  t.Q = p.own_x ? reinterpret_cast<int8_t*>(at) : nullptr;
+  t.pad = p.pad;
+  t.scales = reinterpret_cast<float*>(at + p.scales);
   t.stream = stream;
   SDCA_HIP_TRY(launch_terms(t), "adapter terms");
   if (p.own_x) {
-    QuantLaunch q;
-    q.data = data;
-    q.d = d;
-    q.n = n;
-    q.X = a.X;
-    q.ldx = ldx;
-    q.Q = reinterpret_cast<int8_t*>(at);
-    q.ldq = q.pad = p.pad;
-    q.scales = reinterpret_cast<float*>(at + p.scales);
-    q.order = t.order;
-    q.stream = stream;
-    SDCA_HIP_TRY(launch_quantize(q), "quantise kernel");
-    a.X = q.Q;
+    a.X = t.Q;
     a.ldx = p.pad;
-    a.sx = q.scales;
+    a.sx = t.scales;
     a.data = SDCA_I8;
   }
   if (p.own_w) {
@@ -1731,7 +1723,7 @@ int scores_adapted_common(int data, int out, int64_t d, int64_t m, int64_t n, co
     a.W = ww;
     a.ldw = p.pad;
   }
-  SDCA_HIP_TRY(launch_scores_adapted(a, ad, t.terms, t.order), "adapted score kernel");
+  SDCA_HIP_TRY(launch_scores_adapted(a, ad, t.terms, t.order, ids), "adapted score kernel");
   if (host) {
     if ((rc = fetch_columns(S, a.S, m, n, lds, element_size(out), stream))) return rc;
     SDCA_HIP_TRY(hipStreamSynchronize(stream), "hipStreamSynchronize");

@@ -79,22 +79,6 @@ template <class T>
 __device__ inline int behind_16(const T* row) {
   return static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T));
 }
-template <class T, int V>
-__device__ inline void unpack(const unsigned (&w)[4], float (&v)[V]) {
-  static_assert(V * sizeof(T) == 16, "whole words");
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    if constexpr (sizeof(T) == 4) {
-      v[e] = __uint_as_float(w[e]);
-    } else {
-      const unsigned short b = static_cast<unsigned short>(w[e / 2] >> (16 * (e % 2)));
-      T x;
-      __builtin_memcpy(&x, &b, 2);
-      v[e] = to_float(x);
-    }
-  }
-}
-
 // The weights of some scores: their largest, and the sums of 2^e and e 2^e
 // with exponents relative to ref_of(max).  (A NaN among the scores makes the
 // sums NaN and leaves max.)

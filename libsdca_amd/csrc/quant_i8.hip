@@ -25,14 +25,13 @@ template <class T, int TPC, int G, bool LOOP>
 __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ X, int64_t ldx,
                                                        int64_t d, int64_t n,
                                                        int8_t* __restrict__ Q, int64_t ldq,
-                                                       int64_t pad, float* __restrict__ scales,
-                                                       const int* __restrict__ order) {
+                                                       int64_t pad, float* __restrict__ scales) {
   constexpr int kColumns = 256 / TPC;
   __shared__ unsigned part[4];
   const int t = threadIdx.x % TPC;
   const int64_t col = static_cast<int64_t>(blockIdx.x) * kColumns + threadIdx.x / TPC;
   if (TPC <= 64 && col >= n) return;  // whole columns, and no barrier below
-  const T* x = X + (order ? order[col] : col) * ldx;
+  const T* x = X + col * ldx;
   int8_t* q = Q + col * ldq;
 
   float v[G][kVec];
@@ -88,8 +87,8 @@ void start(const QuantLaunch& a) {
   each_slice(a.n, kColumns, 256, [&](int64_t first, int64_t n) {
     quantize_kernel<T, TPC, G, LOOP>
         <<<static_cast<unsigned>((n + kColumns - 1) / kColumns), 256, 0, a.stream>>>(
-            static_cast<const T*>(a.X) + (a.order ? 0 : first) * a.ldx, a.ldx, a.d, n,
-            a.Q + first * a.ldq, a.ldq, a.pad, a.scales + first, a.order ? a.order + first : nullptr);
+            static_cast<const T*>(a.X) + first * a.ldx, a.ldx, a.d, n, a.Q + first * a.ldq, a.ldq,
+            a.pad, a.scales + first);
   });
 }
 

@@ -119,14 +119,15 @@ struct Adapted {
   const T* B;
   int64_t apart;  // from one adapter's B to the next one's
   int rank, count;
-  const int* order;  // or NULL
+  const int *order, *ids;  // or NULL
 
   Adapted from(int64_t n0, int64_t m0) const {
     Adapted a = *this;
+    a.terms += n0 * pitch;
     if (order) {
       a.order += n0;
+      a.ids += n0;
     } else {
-      a.terms += n0 * pitch;
       a.index += n0;
     }
     a.B += m0 * rank;
@@ -134,22 +135,37 @@ struct Adapted {
   }
   int64_t first_row(int64_t n0) const { return order ? 0 : n0; }
   __device__ int64_t row(int64_t i) const { return order ? order[i] : i; }
+  // -1: none, -2: no adapter's number
+  __device__ static int adapter(int64_t a, int count) {
+    return a >= -1 && a < count ? static_cast<int>(a) : -2;
+  }
 
   template <int FM, int FN, int Q>
   __device__ inline void add(v4f (&scores)[FM][FN], int64_t row0, int64_t n, int first, int m,
                              int lane) const {
     using R = Ranks<T>;
     constexpr int kOnce = FM > 2 ? 1 : FN > 2 ? 2 : 4;
-    int mine[FN];
+    int mine[FN], of[FN];
     const float* t[FN];
     bool bad[FN];
+    // (Without conditions, for the loads to be on their way together.)
+    if (ids) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) of[j] = ids[min(row0 + j * 16 + (lane & 15), n - 1)];
+    } else {
+      int64_t given[FN];
+#pragma unroll
+      for (int j = 0; j < FN; ++j) given[j] = index[min(row0 + j * 16 + (lane & 15), n - 1)];
+#pragma unroll
+      for (int j = 0; j < FN; ++j) of[j] = adapter(given[j], count);
+    }
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-      const int64_t i = row0 + j * 16 + (lane & 15), at_row = row(i < n ? i : n - 1);
-      const int64_t given = i < n ? index[at_row] : -1;
-      bad[j] = given < -1 || given >= count;
-      mine[j] = bad[j] ? -1 : static_cast<int>(given);
-      t[j] = terms + at_row * pitch;
+      const int64_t i = row0 + j * 16 + (lane & 15);
+      const int given = i < n ? of[j] : -1;
+      bad[j] = given < -1;
+      mine[j] = max(given, -1);
+      t[j] = terms + (i < n ? i : n - 1) * pitch;
     }
     int64_t at[FM];
 #pragma unroll
@@ -222,9 +238,8 @@ struct Adapted {
   }
 
   __device__ inline float one(int example, int c, int lane) const {
-    const int64_t a = index[example];
-    if (a == -1) return 0.f;
-    if (a < 0 || a >= count) return NAN;
+    const int a = adapter(index[example], count);
+    if (a < 0) return a == -1 ? 0.f : NAN;
     const float* t = terms + example * pitch;
     const T* b = B + a * apart + static_cast<int64_t>(c) * rank;
     float sum = 0.f;
@@ -235,10 +250,10 @@ struct Adapted {
 
 template <class T, class Out>
 hipError_t scores(const ScoresI8Launch& a, const Adapters& ad, const float* terms,
-                  const int* order) {
+                  const int* order, const int* ids) {
   const Adapted<T> extra = {terms, static_cast<int>(terms_pitch(ad.rank)), ad.index,
                             static_cast<const T*>(ad.B), a.m * ad.rank, static_cast<int>(ad.rank),
-                            static_cast<int>(ad.count), order};
+                            static_cast<int>(ad.count), order, ids};
   if (a.data == SDCA_I8) start_tiles<Out>(a, extra);
   else if (scores_i8_few(a.n, a.d)) start_few<T, Out>(a, extra);
   else start_strip<T, Out>(a, extra);
@@ -246,22 +261,22 @@ hipError_t scores(const ScoresI8Launch& a, const Adapters& ad, const float* term
 }
 template <class T>
 hipError_t scores(const ScoresI8Launch& a, const Adapters& ad, const float* terms,
-                  const int* order) {
+                  const int* order, const int* ids) {
   switch (a.out) {
-    case SDCA_F32: return scores<T, float>(a, ad, terms, order);
-    case SDCA_F16: return scores<T, __half>(a, ad, terms, order);
-    default: return scores<T, __hip_bfloat16>(a, ad, terms, order);
+    case SDCA_F32: return scores<T, float>(a, ad, terms, order, ids);
+    case SDCA_F16: return scores<T, __half>(a, ad, terms, order, ids);
+    default: return scores<T, __hip_bfloat16>(a, ad, terms, order, ids);
   }
 }
 
 }  // namespace
 
 hipError_t launch_scores_adapted(const ScoresI8Launch& a, const Adapters& ad, const float* terms,
-                                 const int* order) {
+                                 const int* order, const int* ids) {
   switch (ad.data) {
-    case SDCA_F32: return scores<float>(a, ad, terms, order);
-    case SDCA_F16: return scores<__half>(a, ad, terms, order);
-    default: return scores<__hip_bfloat16>(a, ad, terms, order);
+    case SDCA_F32: return scores<float>(a, ad, terms, order, ids);
+    case SDCA_F16: return scores<__half>(a, ad, terms, order, ids);
+    default: return scores<__hip_bfloat16>(a, ad, terms, order, ids);
   }
 }
 
