@@ -55,22 +55,28 @@ template <class T>
 __device__ inline void write_column(const T* x, int d, const ColumnScale& s, int8_t* q, int pad, int lane,
                                     int lanes) {
   constexpr int kOnce = sizeof(T) == 4 ? 2 : 4;
-  for (int at0 = lane * 8; at0 < pad; at0 += lanes * 8 * kOnce) {
+  const auto write = [&](const T (&raw)[8], int at, bool whole) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = to_float(raw[e]);
+    unsigned w[2];
+    quantize8(v, s, w);
+    if (!whole) end_column(at, d, w);
+    __builtin_memcpy(q + at, w, 8);  // (pad is whole tiles)
+  };
+  int first = 0;
+  for (; first + lanes * 8 * kOnce <= d; first += lanes * 8 * kOnce) {
     T raw[kOnce][8];
 #pragma unroll
-    for (int i = 0; i < kOnce; ++i) load_column(x, at0 + i * lanes * 8, d, raw[i]);
+    for (int i = 0; i < kOnce; ++i) __builtin_memcpy(raw[i], x + first + (i * lanes + lane) * 8, sizeof(raw[i]));
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < kOnce; ++i) {
-      const int at = at0 + i * lanes * 8;
-      if (at >= pad) break;
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = to_float(raw[i][e]);
-      unsigned w[2];
-      quantize8(v, s, w);
-      end_column(at, d, w);
-      __builtin_memcpy(q + at, w, 8);  // (pad is whole tiles)
-    }
+    for (int i = 0; i < kOnce; ++i) write(raw[i], first + (i * lanes + lane) * 8, true);
+  }
+  for (int at = first + lane * 8; at < pad; at += lanes * 8) {
+    T raw[8];
+    load_column(x, at, d, raw);
+    write(raw, at, false);
   }
 }
 
@@ -173,16 +179,15 @@ __device__ inline v4f multiply(const TA (&a)[8], const TB (&b)[8], v4f sum) {
 }
 
 // A workgroup takes 16 NE examples with all ranks (16 RF); its waves share the
-// wide axis, 32 values at a time, and add up through LDS.  Examples of
+// wide axis and add up through LDS.  Examples of
 // different adapters take turns; in the adapters' order that is rare.  With
 // QUANT the largest magnitudes come with the first reading, and the rows are
 // read again for their 8-bit form, by then from the last-level cache (20000
 // rows of 4096 floats: XXX us, in two kernels 114 and 64).
-constexpr int kTermWaves = 8;
 constexpr int steps_ahead(int registers) {  // 72 registers of loads at most
   return registers <= 9 ? 8 : registers <= 18 ? 4 : registers <= 36 ? 2 : 1;
 }
-template <class TX, class TA, int NE, int RF, bool QUANT>
+template <class TX, class TA, int NE, int RF, int kTermWaves, bool QUANT>
 __global__ __launch_bounds__(64 * kTermWaves) void terms_tile_kernel(
     const TX* __restrict__ X, const TA* __restrict__ A, TermsArgs a, int64_t n,
     const int2* __restrict__ spans, int64_t first) {
@@ -210,6 +215,11 @@ __global__ __launch_bounds__(64 * kTermWaves) void terms_tile_kernel(
     id[j] = given >= 0 && given < a.count ? static_cast<int>(given) : -1;
     left[j] = __ballot(id[j] >= 0);
   }
+  // A wave's part of the wide axis.  Rows of a width like 4096 begin on one
+  // channel of the L2, all sixteen, so waves work far from one another and
+  // workgroups begin at different places.
+  const int share = (a.wide + 32 * kTermWaves - 1) / (32 * kTermWaves) * 32;
+  const int begin = min(wave * share, a.wide), behind = min(begin + share, a.wide);
   bool seen = !QUANT;
   while (true) {
     int me = -1;
@@ -230,7 +240,6 @@ __global__ __launch_bounds__(64 * kTermWaves) void terms_tile_kernel(
       x[j] = X + max(row[j], int64_t(0)) * a.ldx;
     }
     v4f acc[NE][RF] = {};
-    constexpr int kStep = 32 * kTermWaves;
     TX u[kAhead][NE][8];
     TA v[kAhead][RF][8];
     const auto products = [&] {
@@ -246,32 +255,33 @@ __global__ __launch_bounds__(64 * kTermWaves) void terms_tile_kernel(
           }
         }
     };
-    int64_t at0 = wave * 32;
-    for (; at0 + (kAhead - 1) * kStep + 32 <= a.wide; at0 += kStep * kAhead) {
+    const int turns = (behind - begin + 32 * kAhead - 1) / (32 * kAhead);
+    for (int i = 0; i < turns; ++i) {
+      int turn = i + static_cast<int>(blockIdx.x % turns);
+      turn -= turn >= turns ? turns : 0;
+      const int at0 = begin + turn * 32 * kAhead + high * 8;
+      if (begin + (turn + 1) * 32 * kAhead <= behind) {
 #pragma unroll
-      for (int s = 0; s < kAhead; ++s) {
-        const int64_t at = at0 + s * kStep + high * 8;
+        for (int s = 0; s < kAhead; ++s) {
 #pragma unroll
-        for (int j = 0; j < NE; ++j) __builtin_memcpy(u[s][j], x[j] + at, sizeof(u[s][j]));
+          for (int j = 0; j < NE; ++j) __builtin_memcpy(u[s][j], x[j] + at0 + s * 32, sizeof(u[s][j]));
 #pragma unroll
-        for (int f = 0; f < RF; ++f) __builtin_memcpy(v[s][f], w[f] + at, sizeof(v[s][f]));
+          for (int f = 0; f < RF; ++f) __builtin_memcpy(v[s][f], w[f] + at0 + s * 32, sizeof(v[s][f]));
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < kAhead; ++s) {
+#pragma unroll
+          for (int j = 0; j < NE; ++j) load_raw(x[j], at0 + s * 32, behind, u[s][j]);
+#pragma unroll
+          for (int f = 0; f < RF; ++f) load_raw(w[f], at0 + s * 32, behind, v[s][f]);
+        }
       }
       // (All loads first: in an order of its own choice the compiler has few on
       // their way at a time.)
       __builtin_amdgcn_sched_barrier(0);
       products();
       __builtin_amdgcn_sched_barrier(0);
-    }
-    if (at0 < a.wide) {
-#pragma unroll
-      for (int s = 0; s < kAhead; ++s) {
-        const int64_t at = at0 + s * kStep + high * 8;
-#pragma unroll
-        for (int j = 0; j < NE; ++j) load_raw(x[j], at, a.wide, u[s][j]);
-#pragma unroll
-        for (int f = 0; f < RF; ++f) load_raw(w[f], at, a.wide, v[s][f]);
-      }
-      products();
     }
     seen = true;
     if (me < 0) break;
@@ -316,31 +326,38 @@ __global__ __launch_bounds__(64 * kTermWaves) void terms_tile_kernel(
   }
 }
 
-template <class TX, class TA, int NE, int RF, bool QUANT>
+template <class TX, class TA, int NE, int RF, int WAVES, bool QUANT>
 void start_terms(const TermsLaunch& l, const TermsArgs& a) {
-  each_slice((l.n + 16 * NE - 1) / (16 * NE), 1, 64 * kTermWaves, [&](int64_t first, int64_t count) {
-    terms_tile_kernel<TX, TA, NE, RF, QUANT><<<static_cast<unsigned>(count), 64 * kTermWaves, 0, l.stream>>>(
+  each_slice((l.n + 16 * NE - 1) / (16 * NE), 1, 64 * WAVES, [&](int64_t first, int64_t count) {
+    terms_tile_kernel<TX, TA, NE, RF, WAVES, QUANT><<<static_cast<unsigned>(count), 64 * WAVES, 0, l.stream>>>(
         static_cast<const TX*>(l.X), static_cast<const TA*>(l.A), a, l.n, l.spans, first);
   });
 }
-template <class TX, class TA, int NE, int RF>
+template <class TX, class TA, int NE, int RF, int WAVES>
 void start_terms(const TermsLaunch& l, const TermsArgs& a) {
   if constexpr (std::is_same<TX, TA>::value) {
-    if (l.Q) return start_terms<TX, TA, NE, RF, true>(l, a);
+    if (l.Q) return start_terms<TX, TA, NE, RF, WAVES, true>(l, a);
   }
-  start_terms<TX, TA, NE, RF, false>(l, a);
+  start_terms<TX, TA, NE, RF, WAVES, false>(l, a);
 }
 // Of A there is as much to read as of 16 examples, or more for a rank above
 // 16: 32 share it.  (8192 rows of 14336 bfloat16, rank 16: 62 us, 16 at a time
 // 75; but 20000 rows of 4096 floats 84 and 71, with the registers of twice the
-// loads.)
+// loads.)  Few workgroups have sixteen waves each.
 template <class TX, class TA>
 void start_terms(const TermsLaunch& l, const TermsArgs& a) {
   const bool many = l.n >= 4096;
-  if (a.rank <= 16) many && sizeof(TX) == 2 ? start_terms<TX, TA, 2, 1>(l, a) : start_terms<TX, TA, 1, 1>(l, a);
-  else if (a.rank <= 32) many ? start_terms<TX, TA, 2, 2>(l, a) : start_terms<TX, TA, 1, 2>(l, a);
-  else if (a.rank <= 64) many ? start_terms<TX, TA, 2, 4>(l, a) : start_terms<TX, TA, 1, 4>(l, a);
-  else start_terms<TX, TA, 1, 8>(l, a);
+  if (a.rank <= 16) {
+    if (!many) start_terms<TX, TA, 1, 1, 16>(l, a);
+    else if (sizeof(TX) == 2) start_terms<TX, TA, 2, 1, 8>(l, a);
+    else start_terms<TX, TA, 1, 1, 8>(l, a);
+  } else if (a.rank <= 32) {
+    many ? start_terms<TX, TA, 2, 2, 8>(l, a) : start_terms<TX, TA, 1, 2, 16>(l, a);
+  } else if (a.rank <= 64) {
+    many ? start_terms<TX, TA, 2, 4, 8>(l, a) : start_terms<TX, TA, 1, 4, 16>(l, a);
+  } else {
+    start_terms<TX, TA, 1, 8, 8>(l, a);
+  }
 }
 
 template <class TX, class TA>
