@@ -520,9 +520,9 @@ __global__ __launch_bounds__(1024) void group_kernel(GroupArgs a) {
 // ---------------------------------------------------------------------------
 // B (m x rank for each adapter) with its classes in a row.
 // ---------------------------------------------------------------------------
-template <class T>
+template <class T, class TO>
 __global__ __launch_bounds__(256) void turn_kernel(const T* __restrict__ B, int m, int rank,
-                                                   T* __restrict__ Bt, int64_t first) {
+                                                   TO* __restrict__ Bt, int64_t first) {
   constexpr int kClasses = 64;
   __shared__ T tile[kClasses * (kMostRank + 1)];
   const int64_t blocks = (m + kClasses - 1) / kClasses;
@@ -533,11 +533,14 @@ __global__ __launch_bounds__(256) void turn_kernel(const T* __restrict__ B, int 
   __syncthreads();
   const int c = threadIdx.x % kClasses;
   if (c >= classes) return;
-  for (int k = threadIdx.x / kClasses; k < rank; k += 256 / kClasses)
-    Bt[(a * rank + k) * m + c0 + c] = tile[c * (rank + 1) + k];
+  for (int k = threadIdx.x / kClasses; k < rank; k += 256 / kClasses) {
+    const T x = tile[c * (rank + 1) + k];
+    TO* to = Bt + (a * rank + k) * m + c0 + c;
+    if constexpr (std::is_same<T, TO>::value) *to = x;
+    else *to = to_float(x);
+  }
 }
 
-// ---------------------------------------------------------------------------
 // 16 bytes of a row from `at` on as words, zeros from `len` on.
 template <class T>
 __device__ inline void load_some(const T* row, int64_t at, int64_t len, unsigned (&w)[4]) {
@@ -564,6 +567,11 @@ __device__ inline void load_some(const T* row, int64_t at, int64_t len, unsigned
 // row, V neighbouring values, four rows at a time; value e of all lanes makes
 // an operand, 16 columns V apart by four rows, without a turn through LDS.
 // A wave has 16 V columns and 16 RF ranks.
+//
+// With TERMS the rows' own terms with Z, sum_c Z_ic Bt_kc, come from the same
+// reading: 16 rows go through LDS to lanes by row, the wave's part of Bt stays
+// in registers, the four waves' sums are added up in LDS, and the columns'
+// workgroups' by a kernel behind this one.
 // ---------------------------------------------------------------------------
 struct SumArgs {
   int64_t ldz;
@@ -573,18 +581,42 @@ struct SumArgs {
   const Segment* segments;
   int64_t blocks, first;  // of columns; the launch's first workgroup
   float *out, *partial;
+  // With TERMS: Bt of Z's type, rank rows of `wide` for each adapter; the
+  // columns' workgroups' terms, `rows` of them each.
+  const void* turned;
+  PerColumn<float> scale;
+  float* parts;
+  int64_t rows;
 };
 
-template <class T, int RF, bool RANKS_FIRST>
+template <class T, int RF, bool RANKS_FIRST, bool TERMS>
 __global__ __launch_bounds__(256) void sum_kernel(const T* __restrict__ Z, SumArgs a) {
   constexpr int V = 16 / static_cast<int>(sizeof(T)), kSteps = 4;
+  constexpr int kPitch = 16 * V + V;             // other banks for each row
+  constexpr int kChunks = TERMS ? 16 * V / 32 : 1;  // of 32 columns
+  static_assert(!(TERMS && RANKS_FIRST), "terms go with the columns' order");
+  __shared__ __align__(16) T turn[TERMS ? 4 : 1][TERMS ? 16 * kPitch : 1];
+  __shared__ v4f sums[TERMS ? 2 : 1][TERMS ? 4 : 1][TERMS ? RF : 1][TERMS ? 64 : 1];
   const int lane = threadIdx.x & 63, low = lane & 15, high = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t id = a.first + blockIdx.x;
   const Segment seg = a.segments[id / a.blocks];
   const int64_t c0 = (id % a.blocks * 4 + wave) * (16 * V);
-  if (!seg.rows || c0 >= a.wide) return;
+  if (!seg.rows || (!TERMS && c0 >= a.wide)) return;
   const int rank0 = blockIdx.y * 16 * RF;
+  T b[kChunks][TERMS ? RF : 1][8];
+  float scale = 0.f;
+  if constexpr (TERMS) {
+    scale = a.scale.each ? a.scale.each[seg.adapter] : a.scale.value;
+#pragma unroll
+    for (int f = 0; f < RF; ++f) {
+      // (Ranks behind the last are the last one again: their terms are not used.)
+      const int k = min(rank0 + f * 16 + low, a.rank - 1);
+      const T* from = static_cast<const T*>(a.turned) + (static_cast<int64_t>(seg.adapter) * a.rank + k) * a.wide;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) load_raw(from, c0 + i * 32 + high * 8, a.wide, b[i][f]);
+    }
+  }
   const int64_t c = c0 + low * V;
   const int* order = a.order + seg.first;
   const float* terms = a.terms + static_cast<int64_t>(seg.first) * a.pitch;
@@ -633,6 +665,36 @@ __global__ __launch_bounds__(256) void sum_kernel(const T* __restrict__ Z, SumAr
       places(p0 + 8 * kSteps);
     }
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (TERMS) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        __builtin_memcpy(__builtin_assume_aligned(&turn[wave][(4 * s + high) * kPitch + low * V], 16), zn[s], 16);
+      wave_lds_sync();
+      v4f own[RF] = {};
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        T u[8];
+        __builtin_memcpy(u, __builtin_assume_aligned(&turn[wave][low * kPitch + i * 32 + high * 8], 16), sizeof(u));
+#pragma unroll
+        for (int f = 0; f < RF; ++f) own[f] = multiply(b[i][f], u, own[f]);
+      }
+      wave_lds_sync();
+      const int turns = p0 / (4 * kSteps), which = turns & 1;
+#pragma unroll
+      for (int f = 0; f < RF; ++f) sums[which][wave][f][lane] = own[f];
+      // (The next turn's sums go to the other half, and those after them come
+      // behind the next barrier, when these have been read.)
+      __syncthreads();
+      if (wave == (turns & 3) && p0 + low < seg.rows) {
+        float* to = a.parts + (id % a.blocks * a.rows + seg.first + p0 + low) * a.pitch + rank0 + high * 4;
+#pragma unroll
+        for (int f = 0; f < RF; ++f) {
+          if (rank0 + f * 16 >= a.pitch) break;
+          const v4f all = ((sums[which][0][f][lane] + sums[which][1][f][lane]) + sums[which][2][f][lane]) + sums[which][3][f][lane];
+          *reinterpret_cast<v4f*>(to + f * 16) = all * scale;
+        }
+      }
+    }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       float x[V];
@@ -675,6 +737,22 @@ __global__ __launch_bounds__(256) void sum_kernel(const T* __restrict__ Z, SumAr
     }
 }
 
+// The rows' terms from those of the columns' workgroups.
+__global__ __launch_bounds__(256) void join_terms_kernel(const int2* __restrict__ spans, int count, int pitch,
+                                                         int64_t rows, int64_t blocks,
+                                                         const float* __restrict__ parts,
+                                                         float* __restrict__ terms) {
+  const int64_t size = static_cast<int64_t>(spans[count].x) * pitch / 4, apart = rows * pitch / 4;
+  const v4f* from = reinterpret_cast<const v4f*>(parts);
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < size;
+       i += static_cast<int64_t>(gridDim.x) * 256) {
+    v4f sum = {};
+#pragma unroll 4
+    for (int64_t b = 0; b < blocks; ++b) sum += from[b * apart + i];
+    reinterpret_cast<v4f*>(terms)[i] = sum;
+  }
+}
+
 // Adapters of several segments from their partial sums; zeros for those
 // without rows.
 __global__ __launch_bounds__(256) void join_kernel(const int2* __restrict__ spans, Segments s,
@@ -703,21 +781,35 @@ int segment_length(int es, int64_t wide, int64_t n) {
   return static_cast<int>(std::max<int64_t>(length, 64));
 }
 
-template <class T, int RF, bool RANKS_FIRST>
-void start_sums(const T* Z, SumArgs a, int64_t segments, hipStream_t stream) {
+template <class T>
+int64_t column_blocks(int64_t wide) {
   constexpr int64_t kColumns = 4 * 16 * (16 / sizeof(T));
-  a.blocks = (a.wide + kColumns - 1) / kColumns;
+  return (wide + kColumns - 1) / kColumns;
+}
+
+template <class T, int RF, bool RANKS_FIRST, bool TERMS>
+void start_sums(const T* Z, SumArgs a, int64_t segments, hipStream_t stream) {
+  a.blocks = column_blocks<T>(a.wide);
   const unsigned ranks = (a.rank + 16 * RF - 1) / (16 * RF);
   each_slice(segments * a.blocks, 1, 256 * static_cast<int64_t>(ranks), [&](int64_t first, int64_t count) {
     a.first = first;
-    sum_kernel<T, RF, RANKS_FIRST><<<dim3(static_cast<unsigned>(count), ranks), 256, 0, stream>>>(Z, a);
+    sum_kernel<T, RF, RANKS_FIRST, TERMS><<<dim3(static_cast<unsigned>(count), ranks), 256, 0, stream>>>(Z, a);
   });
 }
+template <class T, bool RANKS_FIRST, bool TERMS>
+void start_sums(const T* Z, const SumArgs& a, int64_t segments, hipStream_t stream) {
+  if (a.rank <= 16) start_sums<T, 1, RANKS_FIRST, TERMS>(Z, a, segments, stream);
+  else if (a.rank <= 32) start_sums<T, 2, RANKS_FIRST, TERMS>(Z, a, segments, stream);
+  else start_sums<T, 4, RANKS_FIRST, TERMS>(Z, a, segments, stream);
+}
+
+// Whether G's terms come with dB's sums: Bt is then of G's type.
+bool terms_with_sums(int grad, int data) { return grad == data || grad == SDCA_F32; }
 
 struct GradPlan {
   int length[2];  // of segments: dB's, dA's
   int64_t segments[2];
-  size_t order, spans, table[2], turned, terms[2], partial, end;
+  size_t order, spans, table[2], turned, terms[2], parts, partial, end;
 };
 GradPlan plan_grad(int grad, int data, int64_t d, int64_t m, int64_t n, int64_t count, int64_t rank) {
   GradPlan p;
@@ -741,17 +833,21 @@ GradPlan plan_grad(int grad, int data, int64_t d, int64_t m, int64_t n, int64_t 
       partial = std::max(partial, static_cast<size_t>(s.slot(n) + 1) * rank * (t ? d : m) * sizeof(float));
     p.terms[t] = take(static_cast<size_t>(n) * terms_pitch(rank) * sizeof(float));
   }
-  p.turned = take(static_cast<size_t>(count) * m * rank * es(data));
+  const bool with = terms_with_sums(grad, data);
+  p.turned = take(static_cast<size_t>(count) * m * rank * es(with ? grad : data));
+  const int64_t blocks = grad == SDCA_F32 ? column_blocks<float>(m) : column_blocks<__half>(m);
+  p.parts = take(with ? static_cast<size_t>(blocks) * n * terms_pitch(rank) * sizeof(float) : 0);
   p.partial = take(partial);
   p.end = at;
   return p;
 }
 
-template <class T>
-void sums(const void* Z, int64_t ldz, int64_t wide, bool ranks_first, const GradPlan& p, int t,
-          const float* terms, float* out, const AdaptedGradLaunch& l) {
+template <class T, bool RANKS_FIRST, bool TERMS>
+void sums(const void* Z, int64_t ldz, int64_t wide, const GradPlan& p, const float* terms, float* out,
+          const AdaptedGradLaunch& l) {
+  constexpr int t = RANKS_FIRST ? 1 : 0;
   char* work = static_cast<char*>(l.work);
-  SumArgs a;
+  SumArgs a = {};
   a.ldz = ldz;
   a.wide = static_cast<int>(wide);
   a.rank = static_cast<int>(l.adapters.rank);
@@ -761,39 +857,39 @@ void sums(const void* Z, int64_t ldz, int64_t wide, bool ranks_first, const Grad
   a.segments = reinterpret_cast<const Segment*>(work + p.table[t]);
   a.out = out;
   a.partial = reinterpret_cast<float*>(work + p.partial);
-  const T* z = static_cast<const T*>(Z);
-  const int frags = a.rank <= 16 ? 1 : a.rank <= 32 ? 2 : 4;
-  if (ranks_first) {
-    if (frags == 1) start_sums<T, 1, true>(z, a, p.segments[t], l.stream);
-    else if (frags == 2) start_sums<T, 2, true>(z, a, p.segments[t], l.stream);
-    else start_sums<T, 4, true>(z, a, p.segments[t], l.stream);
-  } else {
-    if (frags == 1) start_sums<T, 1, false>(z, a, p.segments[t], l.stream);
-    else if (frags == 2) start_sums<T, 2, false>(z, a, p.segments[t], l.stream);
-    else start_sums<T, 4, false>(z, a, p.segments[t], l.stream);
+  a.turned = work + p.turned;
+  a.scale = l.adapters.scale;
+  a.parts = reinterpret_cast<float*>(work + p.parts);
+  a.rows = l.n;
+  start_sums<T, RANKS_FIRST, TERMS>(static_cast<const T*>(Z), a, p.segments[t], l.stream);
+  const int2* spans = reinterpret_cast<const int2*>(work + p.spans);
+  if (TERMS && l.n) {
+    const int64_t some = (l.n * a.pitch / 4 + 255) / 256;
+    join_terms_kernel<<<static_cast<unsigned>(std::min<int64_t>(some, 8192)), 256, 0, l.stream>>>(
+        spans, static_cast<int>(l.adapters.count), a.pitch, l.n, column_blocks<T>(wide), a.parts,
+        reinterpret_cast<float*>(work + p.terms[1]));
   }
   const int64_t size = wide * a.rank, blocks = std::min<int64_t>((size + 255) / 256, 4096);
   const Segments s = {p.length[t], nullptr};
   join_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(l.adapters.count)), 256, 0, l.stream>>>(
-      reinterpret_cast<const int2*>(work + p.spans), s, size, a.partial, out);
-}
-void sums(int type, const void* Z, int64_t ldz, int64_t wide, bool ranks_first, const GradPlan& p,
-          int t, const float* terms, float* out, const AdaptedGradLaunch& l) {
-  switch (type) {
-    case SDCA_F32: return sums<float>(Z, ldz, wide, ranks_first, p, t, terms, out, l);
-    case SDCA_F16: return sums<__half>(Z, ldz, wide, ranks_first, p, t, terms, out, l);
-    default: return sums<__hip_bfloat16>(Z, ldz, wide, ranks_first, p, t, terms, out, l);
-  }
+      spans, s, size, a.partial, out);
 }
 
-template <class T>
+template <class T, class TO>
 void turn(const AdaptedGradLaunch& l, void* Bt) {
   const int64_t blocks = (l.m + 63) / 64;
   each_slice(blocks * l.adapters.count, 1, 256, [&](int64_t first, int64_t count) {
-    turn_kernel<T><<<static_cast<unsigned>(count), 256, 0, l.stream>>>(
+    turn_kernel<T, TO><<<static_cast<unsigned>(count), 256, 0, l.stream>>>(
         static_cast<const T*>(l.adapters.B), static_cast<int>(l.m), static_cast<int>(l.adapters.rank),
-        static_cast<T*>(Bt), first);
+        static_cast<TO*>(Bt), first);
   });
+}
+template <class T>
+void turn(const AdaptedGradLaunch& l, void* Bt) {
+  if constexpr (!std::is_same<T, float>::value) {
+    if (l.grad == SDCA_F32) return turn<T, float>(l, Bt);
+  }
+  turn<T, T>(l, Bt);
 }
 
 }  // namespace
@@ -837,8 +933,11 @@ hipError_t launch_adapted_grad(const AdaptedGradLaunch& l) {
   for (int t = 0; t < 2; ++t) g.by[t] = Segments{p.length[t], reinterpret_cast<Segment*>(work + p.table[t])};
   group_kernel<<<static_cast<unsigned>(ad.count + 1), 1024, 0, l.stream>>>(g);
   void* Bt = work + p.turned;
-  if (ad.data == SDCA_F32) turn<float>(l, Bt);
-  else turn<__half>(l, Bt);  // (two bytes either way)
+  switch (ad.data) {
+    case SDCA_F32: turn<float>(l, Bt); break;
+    case SDCA_F16: turn<__half>(l, Bt); break;
+    default: turn<__hip_bfloat16>(l, Bt);
+  }
   float *T = reinterpret_cast<float*>(work + p.terms[0]), *U = reinterpret_cast<float*>(work + p.terms[1]);
   TermsLaunch t;
   t.adapters = &ad;
@@ -857,15 +956,31 @@ hipError_t launch_adapted_grad(const AdaptedGradLaunch& l) {
   t.terms = T;
   hipError_t e = launch_terms(t);
   if (e != hipSuccess) return e;
-  t.data = l.grad;
-  t.wide = l.m;
-  t.X = l.G;
-  t.ldx = l.ldg;
-  t.A = Bt;
-  t.terms = U;
-  if ((e = launch_terms(t)) != hipSuccess) return e;
-  sums(l.grad, l.G, l.ldg, l.m, false, p, 0, T, l.dB, l);
-  sums(ad.data, l.X, l.ldx, l.d, true, p, 1, U, l.dA, l);
+  const bool with = terms_with_sums(l.grad, ad.data);
+  if (!with) {
+    t.data = l.grad;
+    t.wide = l.m;
+    t.X = l.G;
+    t.ldx = l.ldg;
+    t.A = Bt;
+    t.terms = U;
+    if ((e = launch_terms(t)) != hipSuccess) return e;
+  }
+  switch (l.grad) {
+    case SDCA_F32: sums<float, false, true>(l.G, l.ldg, l.m, p, T, l.dB, l); break;
+    case SDCA_F16:
+      with ? sums<__half, false, true>(l.G, l.ldg, l.m, p, T, l.dB, l)
+           : sums<__half, false, false>(l.G, l.ldg, l.m, p, T, l.dB, l);
+      break;
+    default:
+      with ? sums<__hip_bfloat16, false, true>(l.G, l.ldg, l.m, p, T, l.dB, l)
+           : sums<__hip_bfloat16, false, false>(l.G, l.ldg, l.m, p, T, l.dB, l);
+  }
+  switch (ad.data) {
+    case SDCA_F32: sums<float, true, false>(l.X, l.ldx, l.d, p, U, l.dA, l); break;
+    case SDCA_F16: sums<__half, true, false>(l.X, l.ldx, l.d, p, U, l.dA, l); break;
+    default: sums<__hip_bfloat16, true, false>(l.X, l.ldx, l.d, p, U, l.dA, l);
+  }
   return hipGetLastError();
 }
 
