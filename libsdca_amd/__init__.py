@@ -201,8 +201,15 @@ def check(rc):
         raise SdcaError(rc, msg)
 
 
+_torch_types = {}  # a small call asks some forty times
+
+
 def _is_torch(x):
-    return type(x).__module__.startswith("torch")
+    t = type(x)
+    known = _torch_types.get(t)
+    if known is None:
+        known = _torch_types[t] = t.__module__.startswith("torch")
+    return known
 
 
 def _dtype_code(x):
@@ -910,7 +917,9 @@ def _setting(v, name, n, kind, like):
         return None
     if _is_torch(like):
         torch = sys.modules["torch"]
-        v = torch.as_tensor(v, dtype=getattr(torch, kind), device=like.device).contiguous()
+        dtype = getattr(torch, kind)
+        if not (_is_torch(v) and v.dtype == dtype and v.device == like.device and v.is_contiguous()):
+            v = torch.as_tensor(v, dtype=dtype, device=like.device).contiguous()
     elif _is_torch(v):
         raise SdcaError(2, f"{name}: numpy arrays and torch tensors cannot be mixed in one call")
     else:

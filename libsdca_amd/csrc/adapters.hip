@@ -426,34 +426,27 @@ struct GroupArgs {
 // A workgroup finds the places of one adapter's rows, or the last one those
 // of the rows without: its waves each count their part of the index, then
 // write.
-__global__ __launch_bounds__(1024) void group_kernel(GroupArgs a) {
-  constexpr int kWaves = 16, kBatch = 4;
+__device__ void group(const GroupArgs& a, int me) {
+  constexpr int kWaves = 16, kBatch = 10;
   __shared__ int less_of[kWaves], equal_of[kWaves];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int me = blockIdx.x;
   const int64_t share = ((static_cast<int64_t>(a.n) + kWaves - 1) / kWaves + 63) / 64 * 64;
   const int64_t begin = min(static_cast<int64_t>(a.n), wave * share);
   const int64_t end = min(static_cast<int64_t>(a.n), begin + share);
   // kBatch rows' adapters, the rows without as `count`, none behind the end.
-  // (A whole batch without conditions: its loads are then on their way
-  // together; 20000 rows took 18 us one load after the other.)
+  // (All loaded, and held to be used, so that the loads are on their way
+  // together: left to itself the compiler makes each wait for the one before,
+  // and 20000 rows took 18 us.)
+  int64_t raw[kBatch];
   const auto adapters = [&](int64_t i0, int (&id)[kBatch]) {
-    int64_t raw[kBatch];
-    if (i0 + 64 * kBatch <= end) {
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) raw[b] = a.index[i0 + b * 64 + lane];
+    for (int b = 0; b < kBatch; ++b) raw[b] = a.index[min(i0 + b * 64 + lane, end - 1)];
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b)
-        id[b] = raw[b] >= 0 && raw[b] < a.count ? static_cast<int>(raw[b]) : a.count;
-    } else {
+    for (int b = 0; b < kBatch; ++b) asm volatile("" : "+v"(raw[b]));
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        const int64_t i = i0 + b * 64 + lane;
-        raw[b] = i < end ? a.index[i] : 0;
-        id[b] = i >= end ? 0x7fffffff : raw[b] >= 0 && raw[b] < a.count ? static_cast<int>(raw[b]) : a.count;
-      }
-    }
+    for (int b = 0; b < kBatch; ++b)
+      id[b] = i0 + b * 64 + lane >= end ? 0x7fffffff : raw[b] >= 0 && raw[b] < a.count ? static_cast<int>(raw[b]) : a.count;
   };
   int less = 0, equal = 0;
   for (int64_t i0 = begin; i0 < end; i0 += 64 * kBatch) {
@@ -490,7 +483,7 @@ __global__ __launch_bounds__(1024) void group_kernel(GroupArgs a) {
           const int to = place + __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask >> 32),
                                                            __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask), 0));
           a.order[to] = static_cast<int>(i + b * 64);
-          if (a.ids) a.ids[to] = me < a.count ? me : a.index[i + b * 64] == -1 ? -1 : -2;
+          if (a.ids) a.ids[to] = me < a.count ? me : raw[b] == -1 ? -1 : -2;
         }
         place += __popcll(mask);
       }
@@ -520,25 +513,40 @@ __global__ __launch_bounds__(1024) void group_kernel(GroupArgs a) {
 // ---------------------------------------------------------------------------
 // B (m x rank for each adapter) with its classes in a row.
 // ---------------------------------------------------------------------------
+struct TurnArgs {
+  const void* B;
+  int64_t m;
+  int rank;
+  void* to;
+};
 template <class T, class TO>
-__global__ __launch_bounds__(256) void turn_kernel(const T* __restrict__ B, int m, int rank,
-                                                   TO* __restrict__ Bt, int64_t first) {
+__device__ void turn(const TurnArgs& a, int64_t id) {
   constexpr int kClasses = 64;
   __shared__ T tile[kClasses * (kMostRank + 1)];
-  const int64_t blocks = (m + kClasses - 1) / kClasses;
-  const int64_t id = first + blockIdx.x, a = id / blocks, c0 = id % blocks * kClasses;
-  const int classes = static_cast<int>(min(static_cast<int64_t>(kClasses), m - c0));
-  const T* b = B + (a * m + c0) * rank;
-  for (int i = threadIdx.x; i < classes * rank; i += 256) tile[i / rank * (rank + 1) + i % rank] = b[i];
+  const int64_t blocks = (a.m + kClasses - 1) / kClasses;
+  const int64_t which = id / blocks, c0 = id % blocks * kClasses;
+  const int classes = static_cast<int>(min(static_cast<int64_t>(kClasses), a.m - c0)), rank = a.rank;
+  const T* b = static_cast<const T*>(a.B) + (which * a.m + c0) * rank;
+  for (int i = threadIdx.x; i < classes * rank; i += 1024) tile[i / rank * (rank + 1) + i % rank] = b[i];
   __syncthreads();
   const int c = threadIdx.x % kClasses;
   if (c >= classes) return;
-  for (int k = threadIdx.x / kClasses; k < rank; k += 256 / kClasses) {
+  for (int k = threadIdx.x / kClasses; k < rank; k += 1024 / kClasses) {
     const T x = tile[c * (rank + 1) + k];
-    TO* to = Bt + (a * rank + k) * m + c0 + c;
+    TO* to = static_cast<TO*>(a.to) + (which * rank + k) * a.m + c0 + c;
     if constexpr (std::is_same<T, TO>::value) *to = x;
     else *to = to_float(x);
   }
+}
+
+__global__ __launch_bounds__(1024) void group_kernel(GroupArgs a) { group(a, blockIdx.x); }
+
+// Both in one launch: the first workgroups group, the others turn.
+template <class T, class TO>
+__global__ __launch_bounds__(1024) void group_turn_kernel(GroupArgs g, TurnArgs t, int64_t first) {
+  const int64_t id = first + blockIdx.x;
+  if (id <= g.count) group(g, static_cast<int>(id));
+  else turn<T, TO>(t, id - g.count - 1);
 }
 
 // 16 bytes of a row from `at` on as words, zeros from `len` on.
@@ -591,6 +599,8 @@ struct SumArgs {
 
 template <class T, int RF, bool RANKS_FIRST, bool TERMS>
 __global__ __launch_bounds__(256) void sum_kernel(const T* __restrict__ Z, SumArgs a) {
+  // (kSteps loads of a lane ahead of its products: with eight 8192 x 14336
+  // bfloat16 with terms take the same 78 us.)
   constexpr int V = 16 / static_cast<int>(sizeof(T)), kSteps = 4;
   constexpr int kPitch = 16 * V + V;             // other banks for each row
   constexpr int kChunks = TERMS ? 16 * V / 32 : 1;  // of 32 columns
@@ -667,31 +677,34 @@ __global__ __launch_bounds__(256) void sum_kernel(const T* __restrict__ Z, SumAr
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (TERMS) {
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-        __builtin_memcpy(__builtin_assume_aligned(&turn[wave][(4 * s + high) * kPitch + low * V], 16), zn[s], 16);
-      wave_lds_sync();
-      v4f own[RF] = {};
+      for (int h = 0; h < kSteps / 4; ++h) {  // sixteen rows
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        T u[8];
-        __builtin_memcpy(u, __builtin_assume_aligned(&turn[wave][low * kPitch + i * 32 + high * 8], 16), sizeof(u));
+        for (int s = 0; s < 4; ++s)
+          __builtin_memcpy(__builtin_assume_aligned(&turn[wave][(4 * s + high) * kPitch + low * V], 16), zn[4 * h + s], 16);
+        wave_lds_sync();
+        v4f own[RF] = {};
 #pragma unroll
-        for (int f = 0; f < RF; ++f) own[f] = multiply(b[i][f], u, own[f]);
-      }
-      wave_lds_sync();
-      const int turns = p0 / (4 * kSteps), which = turns & 1;
+        for (int i = 0; i < kChunks; ++i) {
+          T u[8];
+          __builtin_memcpy(u, __builtin_assume_aligned(&turn[wave][low * kPitch + i * 32 + high * 8], 16), sizeof(u));
 #pragma unroll
-      for (int f = 0; f < RF; ++f) sums[which][wave][f][lane] = own[f];
-      // (The next turn's sums go to the other half, and those after them come
-      // behind the next barrier, when these have been read.)
-      __syncthreads();
-      if (wave == (turns & 3) && p0 + low < seg.rows) {
-        float* to = a.parts + (id % a.blocks * a.rows + seg.first + p0 + low) * a.pitch + rank0 + high * 4;
+          for (int f = 0; f < RF; ++f) own[f] = multiply(b[i][f], u, own[f]);
+        }
+        wave_lds_sync();
+        const int p = p0 + 16 * h, turns = p / 16, which = turns & 1;
 #pragma unroll
-        for (int f = 0; f < RF; ++f) {
-          if (rank0 + f * 16 >= a.pitch) break;
-          const v4f all = ((sums[which][0][f][lane] + sums[which][1][f][lane]) + sums[which][2][f][lane]) + sums[which][3][f][lane];
-          *reinterpret_cast<v4f*>(to + f * 16) = all * scale;
+        for (int f = 0; f < RF; ++f) sums[which][wave][f][lane] = own[f];
+        // (The next turn's sums go to the other half, and those after them come
+        // behind the next barrier, when these have been read.)
+        __syncthreads();
+        if (wave == (turns & 3) && p + low < seg.rows) {
+          float* to = a.parts + (id % a.blocks * a.rows + seg.first + p + low) * a.pitch + rank0 + high * 4;
+#pragma unroll
+          for (int f = 0; f < RF; ++f) {
+            if (rank0 + f * 16 >= a.pitch) break;
+            const v4f all = ((sums[which][0][f][lane] + sums[which][1][f][lane]) + sums[which][2][f][lane]) + sums[which][3][f][lane];
+            *reinterpret_cast<v4f*>(to + f * 16) = all * scale;
+          }
         }
       }
     }
@@ -737,38 +750,44 @@ __global__ __launch_bounds__(256) void sum_kernel(const T* __restrict__ Z, SumAr
     }
 }
 
-// The rows' terms from those of the columns' workgroups.
-__global__ __launch_bounds__(256) void join_terms_kernel(const int2* __restrict__ spans, int count, int pitch,
-                                                         int64_t rows, int64_t blocks,
-                                                         const float* __restrict__ parts,
-                                                         float* __restrict__ terms) {
-  const int64_t size = static_cast<int64_t>(spans[count].x) * pitch / 4, apart = rows * pitch / 4;
-  const v4f* from = reinterpret_cast<const v4f*>(parts);
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < size;
-       i += static_cast<int64_t>(gridDim.x) * 256) {
-    v4f sum = {};
+// What is left of sums in parts: the rows' terms from those of the columns'
+// workgroups (by the first `terms_blocks` workgroups), and the adapters of
+// several segments from their partial sums, zeros for those without rows (by
+// `each` for each adapter).
+struct JoinArgs {
+  const int2* spans;
+  int count, pitch;
+  int64_t terms_blocks, rows, parts;
+  const float* part_terms;
+  float* terms;
+  Segments segments;
+  int64_t each, size;
+  const float* partial;
+  float* out;
+};
+__global__ __launch_bounds__(256) void join_kernel(JoinArgs j, int64_t first) {
+  const int64_t id = first + blockIdx.x;
+  if (id < j.terms_blocks) {
+    const int64_t size = static_cast<int64_t>(j.spans[j.count].x) * j.pitch / 4, apart = j.rows * j.pitch / 4;
+    const v4f* from = reinterpret_cast<const v4f*>(j.part_terms);
+    for (int64_t i = id * 256 + threadIdx.x; i < size; i += j.terms_blocks * 256) {
+      v4f sum = {};
 #pragma unroll 4
-    for (int64_t b = 0; b < blocks; ++b) sum += from[b * apart + i];
-    reinterpret_cast<v4f*>(terms)[i] = sum;
+      for (int64_t b = 0; b < j.parts; ++b) sum += from[b * apart + i];
+      reinterpret_cast<v4f*>(j.terms)[i] = sum;
+    }
+    return;
   }
-}
-
-// Adapters of several segments from their partial sums; zeros for those
-// without rows.
-__global__ __launch_bounds__(256) void join_kernel(const int2* __restrict__ spans, Segments s,
-                                                   int64_t size, const float* __restrict__ partial,
-                                                   float* __restrict__ out) {
-  const int64_t a = blockIdx.y;
-  const int2 span = spans[a];
-  if (span.y && span.y <= s.length) return;
-  const int parts = (span.y + s.length - 1) / s.length;
-  const float* from = partial + s.slot(span.x) * size;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < size;
-       i += static_cast<int64_t>(gridDim.x) * 256) {
+  const int64_t a = (id - j.terms_blocks) / j.each, block = (id - j.terms_blocks) % j.each;
+  const int2 span = j.spans[a];
+  if (span.y && span.y <= j.segments.length) return;
+  const int parts = (span.y + j.segments.length - 1) / j.segments.length;
+  const float* from = j.partial + j.segments.slot(span.x) * j.size;
+  for (int64_t i = block * 256 + threadIdx.x; i < j.size; i += j.each * 256) {
     float sum = 0.f;
 #pragma unroll 4
-    for (int p = 0; p < parts; ++p) sum += from[p * size + i];
-    out[a * size + i] = sum;
+    for (int p = 0; p < parts; ++p) sum += from[p * j.size + i];
+    j.out[a * j.size + i] = sum;
   }
 }
 
@@ -777,7 +796,7 @@ __global__ __launch_bounds__(256) void join_kernel(const int2* __restrict__ span
 int segment_length(int es, int64_t wide, int64_t n) {
   const int64_t columns = 4 * 16 * (16 / es), blocks = (wide + columns - 1) / columns;
   const int64_t parts = std::max<int64_t>(1, 512 / blocks);
-  const int64_t length = ((n + parts - 1) / parts + 15) / 16 * 16;
+  const int64_t length = ((n + parts - 1) / parts + 31) / 32 * 32;
   return static_cast<int>(std::max<int64_t>(length, 64));
 }
 
@@ -862,34 +881,37 @@ void sums(const void* Z, int64_t ldz, int64_t wide, const GradPlan& p, const flo
   a.parts = reinterpret_cast<float*>(work + p.parts);
   a.rows = l.n;
   start_sums<T, RANKS_FIRST, TERMS>(static_cast<const T*>(Z), a, p.segments[t], l.stream);
-  const int2* spans = reinterpret_cast<const int2*>(work + p.spans);
-  if (TERMS && l.n) {
-    const int64_t some = (l.n * a.pitch / 4 + 255) / 256;
-    join_terms_kernel<<<static_cast<unsigned>(std::min<int64_t>(some, 8192)), 256, 0, l.stream>>>(
-        spans, static_cast<int>(l.adapters.count), a.pitch, l.n, column_blocks<T>(wide), a.parts,
-        reinterpret_cast<float*>(work + p.terms[1]));
-  }
-  const int64_t size = wide * a.rank, blocks = std::min<int64_t>((size + 255) / 256, 4096);
-  const Segments s = {p.length[t], nullptr};
-  join_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(l.adapters.count)), 256, 0, l.stream>>>(
-      spans, s, size, a.partial, out);
+  JoinArgs j = {};
+  j.spans = reinterpret_cast<const int2*>(work + p.spans);
+  j.count = static_cast<int>(l.adapters.count);
+  j.pitch = a.pitch;
+  j.terms_blocks = TERMS ? std::min<int64_t>((l.n * a.pitch / 4 + 255) / 256, 8192) : 0;
+  j.rows = l.n;
+  j.parts = column_blocks<T>(wide);
+  j.part_terms = a.parts;
+  j.terms = reinterpret_cast<float*>(work + p.terms[1]);
+  j.segments = Segments{p.length[t], nullptr};
+  j.size = wide * a.rank;
+  j.each = std::min<int64_t>((j.size + 255) / 256, std::max<int64_t>(1, 16384 / j.count));
+  j.partial = a.partial;
+  j.out = out;
+  each_slice(j.terms_blocks + j.each * j.count, 1, 256, [&](int64_t first, int64_t count) {
+    join_kernel<<<static_cast<unsigned>(count), 256, 0, l.stream>>>(j, first);
+  });
 }
 
 template <class T, class TO>
-void turn(const AdaptedGradLaunch& l, void* Bt) {
-  const int64_t blocks = (l.m + 63) / 64;
-  each_slice(blocks * l.adapters.count, 1, 256, [&](int64_t first, int64_t count) {
-    turn_kernel<T, TO><<<static_cast<unsigned>(count), 256, 0, l.stream>>>(
-        static_cast<const T*>(l.adapters.B), static_cast<int>(l.m), static_cast<int>(l.adapters.rank),
-        static_cast<TO*>(Bt), first);
+void group_turn(const GroupArgs& g, const TurnArgs& t, hipStream_t stream) {
+  each_slice((t.m + 63) / 64 * g.count + g.count + 1, 1, 1024, [&](int64_t first, int64_t count) {
+    group_turn_kernel<T, TO><<<static_cast<unsigned>(count), 1024, 0, stream>>>(g, t, first);
   });
 }
 template <class T>
-void turn(const AdaptedGradLaunch& l, void* Bt) {
+void group_turn(const GroupArgs& g, const TurnArgs& t, int grad, hipStream_t stream) {
   if constexpr (!std::is_same<T, float>::value) {
-    if (l.grad == SDCA_F32) return turn<T, float>(l, Bt);
+    if (grad == SDCA_F32) return group_turn<T, float>(g, t, stream);
   }
-  turn<T, T>(l, Bt);
+  group_turn<T, T>(g, t, stream);
 }
 
 }  // namespace
@@ -931,12 +953,12 @@ hipError_t launch_adapted_grad(const AdaptedGradLaunch& l) {
   g.order = reinterpret_cast<int*>(work + p.order);
   g.spans = reinterpret_cast<int2*>(work + p.spans);
   for (int t = 0; t < 2; ++t) g.by[t] = Segments{p.length[t], reinterpret_cast<Segment*>(work + p.table[t])};
-  group_kernel<<<static_cast<unsigned>(ad.count + 1), 1024, 0, l.stream>>>(g);
   void* Bt = work + p.turned;
+  const TurnArgs turned = {ad.B, l.m, static_cast<int>(ad.rank), Bt};
   switch (ad.data) {
-    case SDCA_F32: turn<float>(l, Bt); break;
-    case SDCA_F16: turn<__half>(l, Bt); break;
-    default: turn<__hip_bfloat16>(l, Bt);
+    case SDCA_F32: group_turn<float>(g, turned, l.grad, l.stream); break;
+    case SDCA_F16: group_turn<__half>(g, turned, l.grad, l.stream); break;
+    default: group_turn<__hip_bfloat16>(g, turned, l.grad, l.stream);
   }
   float *T = reinterpret_cast<float*>(work + p.terms[0]), *U = reinterpret_cast<float*>(work + p.terms[1]);
   TermsLaunch t;
