@@ -30,6 +30,8 @@ struct TermsArgs {
   const int* order;  // or NULL
   PerColumn<float> scale;
   float* terms;
+  int parts;      // of the wide axis, and from one's terms to the next one's
+  int64_t apart;
   int8_t* Q;
   int pad;
   float* scales;
@@ -81,7 +83,8 @@ __device__ inline void write_column(const T* x, int d, const ColumnScale& s, int
 }
 
 // A workgroup takes eight of the adapter's rows for one example; the last of
-// an example's workgroups its 8-bit form.
+// an example's workgroups its 8-bit form.  With parts the terms are there
+// already, and only that last one runs, which adds them up.
 template <class TX, class TA>
 __global__ __launch_bounds__(256) void terms_row_kernel(const TX* __restrict__ X,
                                                         const TA* __restrict__ A, TermsArgs a) {
@@ -89,7 +92,14 @@ __global__ __launch_bounds__(256) void terms_row_kernel(const TX* __restrict__ X
   __shared__ unsigned most_of[4];
   const int64_t p = blockIdx.x, row = a.order ? a.order[p] : p;
   const TX* x = X + row * a.ldx;
-  if (static_cast<int>(blockIdx.y) * 8 >= a.pitch) {
+  if (a.parts > 1 || static_cast<int>(blockIdx.y) * 8 >= a.pitch) {
+    if (a.parts > 1 && static_cast<int>(threadIdx.x) < a.pitch) {
+      float* t = a.terms + p * a.pitch + threadIdx.x;
+      float sum = t[0];
+#pragma unroll 4
+      for (int i = 1; i < a.parts; ++i) sum += t[i * a.apart];
+      t[0] = sum;
+    }
     unsigned most = 0;
     for (int at = threadIdx.x * 8; at < a.wide; at += 256 * 8) {
       TX raw[8];
@@ -218,8 +228,9 @@ __global__ __launch_bounds__(64 * kTermWaves) void terms_tile_kernel(
   // A wave's part of the wide axis.  Rows of a width like 4096 begin on one
   // channel of the L2, all sixteen, so waves work far from one another and
   // workgroups begin at different places.
-  const int share = (a.wide + 32 * kTermWaves - 1) / (32 * kTermWaves) * 32;
-  const int begin = min(wave * share, a.wide), behind = min(begin + share, a.wide);
+  const int waves = kTermWaves * gridDim.y, share = (a.wide + 32 * waves - 1) / (32 * waves) * 32;
+  const int begin = min((static_cast<int>(blockIdx.y) * kTermWaves + wave) * share, a.wide);
+  const int behind = min(begin + share, a.wide);
   bool seen = !QUANT;
   while (true) {
     int me = -1;
@@ -257,7 +268,7 @@ __global__ __launch_bounds__(64 * kTermWaves) void terms_tile_kernel(
     };
     const int turns = (behind - begin + 32 * kAhead - 1) / (32 * kAhead);
     for (int i = 0; i < turns; ++i) {
-      int turn = i + static_cast<int>(blockIdx.x % turns);
+      int turn = i + static_cast<int>(blockIdx.x % turns);  // (turns is 0 for a wave without a part)
       turn -= turn >= turns ? turns : 0;
       const int at0 = begin + turn * 32 * kAhead + high * 8;
       if (begin + (turn + 1) * 32 * kAhead <= behind) {
@@ -301,7 +312,8 @@ __global__ __launch_bounds__(64 * kTermWaves) void terms_tile_kernel(
         for (int q = 1; q < kTermWaves; ++q) sum += part[i][q][lane];
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum[e] = k + e < a.rank ? sum[e] * scale : 0.f;
-        if (k < a.pitch) *reinterpret_cast<v4f*>(a.terms + (p0 + j * 16 + low) * a.pitch + k) = sum;
+        if (k < a.pitch)
+          *reinterpret_cast<v4f*>(a.terms + blockIdx.y * a.apart + (p0 + j * 16 + low) * a.pitch + k) = sum;
       }
     }
   }
@@ -328,15 +340,16 @@ __global__ __launch_bounds__(64 * kTermWaves) void terms_tile_kernel(
 
 template <class TX, class TA, int NE, int RF, int WAVES, bool QUANT>
 void start_terms(const TermsLaunch& l, const TermsArgs& a) {
-  each_slice((l.n + 16 * NE - 1) / (16 * NE), 1, 64 * WAVES, [&](int64_t first, int64_t count) {
-    terms_tile_kernel<TX, TA, NE, RF, WAVES, QUANT><<<static_cast<unsigned>(count), 64 * WAVES, 0, l.stream>>>(
+  each_slice((l.n + 16 * NE - 1) / (16 * NE), 1, 64 * WAVES * l.parts, [&](int64_t first, int64_t count) {
+    terms_tile_kernel<TX, TA, NE, RF, WAVES, QUANT>
+        <<<dim3(static_cast<unsigned>(count), l.parts), 64 * WAVES, 0, l.stream>>>(
         static_cast<const TX*>(l.X), static_cast<const TA*>(l.A), a, l.n, l.spans, first);
   });
 }
 template <class TX, class TA, int NE, int RF, int WAVES>
 void start_terms(const TermsLaunch& l, const TermsArgs& a) {
   if constexpr (std::is_same<TX, TA>::value) {
-    if (l.Q) return start_terms<TX, TA, NE, RF, WAVES, true>(l, a);
+    if (l.Q && l.parts == 1) return start_terms<TX, TA, NE, RF, WAVES, true>(l, a);
   }
   start_terms<TX, TA, NE, RF, WAVES, false>(l, a);
 }
@@ -377,9 +390,15 @@ hipError_t terms(const TermsLaunch& l) {
   a.Q = l.Q;
   a.pad = static_cast<int>(l.pad);
   a.scales = l.scales;
+  a.parts = l.parts;
+  a.apart = l.n * a.pitch;
   if (l.n == 0) return hipSuccess;
   if (l.n >= kTileTerms) {
     start_terms<TX, TA>(l, a);
+    if (l.parts > 1) {
+      terms_row_kernel<TX, TA><<<static_cast<unsigned>(l.n), 256, 0, l.stream>>>(
+          static_cast<const TX*>(l.X), static_cast<const TA*>(l.A), a);
+    }
     return hipGetLastError();
   }
   const unsigned groups = static_cast<unsigned>(a.pitch / 8 + (l.Q ? 1 : 0));
@@ -916,6 +935,15 @@ void group_turn(const GroupArgs& g, const TurnArgs& t, int grad, hipStream_t str
 
 }  // namespace
 
+// Few workgroups of 16 examples read at some 60 GB/s each: the wide axis is
+// shared by more of them until they come to one for each compute unit (1024
+// rows of 4096 halves, rank 32, and their 8-bit form: 31 us in one part, XX in
+// four with the sums and the 8-bit form in a launch behind).
+int terms_parts(int64_t n) {
+  const int64_t tiles = (n + 15) / 16;
+  return n < kTileTerms || tiles > 128 ? 1 : static_cast<int>(std::min<int64_t>(8, 256 / tiles));
+}
+
 hipError_t launch_terms(const TermsLaunch& l) {
   switch (l.data) {
     case SDCA_F32: return terms<float>(l);
@@ -966,6 +994,7 @@ hipError_t launch_adapted_grad(const AdaptedGradLaunch& l) {
   t.n = l.n;
   t.order = g.order;
   t.spans = g.spans;
+  t.parts = 1;
   t.Q = nullptr;
   t.pad = 0;
   t.scales = nullptr;

@@ -152,6 +152,9 @@ struct TermsLaunch {
   const int* order;
   const int2* spans;
   float* terms;
+  // 1, or with Q terms_parts(n): the wide axis in so many parts, for which
+  // `terms` has room n rows apart; the terms are the first part's in the end.
+  int parts;
   // NULL, or the rows in 8 bits besides, as launch_quantize gives them with
   // ldq = pad.
   int8_t* Q;
@@ -159,6 +162,7 @@ struct TermsLaunch {
   float* scales;
   hipStream_t stream;
 };
+int terms_parts(int64_t n);
 hipError_t launch_terms(const TermsLaunch& a);
 
 // The n rows in the order of their adapters, rising for each, those without

@@ -1617,6 +1617,7 @@ struct StagedAdapters {
 struct AdaptedPlan {
   int64_t pad;
   bool own_x, own_w, grouped;
+  int parts;  // of the terms
   size_t w, scales, terms, order, ids, spans, end;
 };
 AdaptedPlan plan_adapted(int data, int64_t d, int64_t m, int64_t n, const void* W, int64_t ldw,
@@ -1630,7 +1631,8 @@ AdaptedPlan plan_adapted(int data, int64_t d, int64_t m, int64_t n, const void* 
   p.w = p.own_x ? whole(static_cast<size_t>(n) * p.pad) : 0;
   p.scales = p.w + (p.own_w ? whole(static_cast<size_t>(m) * p.pad) : 0);
   p.terms = p.scales + (p.own_x ? whole(n * sizeof(float)) : 0);
-  p.order = p.terms + whole(static_cast<size_t>(n) * terms_pitch(rank) * sizeof(float));
+  p.parts = p.own_x ? terms_parts(n) : 1;
+  p.order = p.terms + whole(static_cast<size_t>(p.parts) * n * terms_pitch(rank) * sizeof(float));
   // Examples in the order of their adapters: a product of 16 of them then has
   // one adapter, but for few.
   p.grouped = p.own_x && count > 1 && n >= 256;
@@ -1706,6 +1708,7 @@ int scores_adapted_common(int data, int out, int64_t d, int64_t m, int64_t n, co
     t.spans = spans;
   }
   t.terms = reinterpret_cast<float*>(at + p.terms);
+  t.parts = p.parts;
   t.Q = p.own_x ? reinterpret_cast<int8_t*>(at) : nullptr;
   t.pad = p.pad;
   t.scales = reinterpret_cast<float*>(at + p.scales);
