@@ -523,7 +523,8 @@ int sdca_sample(sdca_dtype data, int64_t m, int64_t n, const void* S, int64_t ld
  *              largest scores' log-probabilities and places, falling, ties by
  *              rising index; -infinity and -1 beyond the scores above
  *              -infinity.  top is at most 64; 0 for none.
- * All in 32 bits.  A column whose scores are all -infinity has log-
+ * All in 32 bits; the last bits depend on m, n and a column's address modulo
+ * 16.  A column whose scores are all -infinity has log-
  * probabilities of -infinity, log Z = -infinity and entropy 0; one that holds
  * a NaN has NaN for all of them.  A label that is none of [-1, m) is
  * SDCA_ERR_LABELS in host arrays; in device memory its logp is NaN.
@@ -561,7 +562,8 @@ int sdca_log_probs_grad(sdca_dtype data, int64_t m, int64_t n, const void* S, in
 /*
  * Low-rank adapters of one weight matrix: example i's scores get
  * scale_a B_a (A_a x_i), a = index[i].
- *   count (1..65535) adapters of `rank` (1..128);
+ *   count (1..65535) adapters of `rank` (1..128); calls of 256 examples or
+ *      more read the index once for each adapter;
  *   A: count times a d x rank matrix, B: count times a rank x m one, column-
  *      major, contiguous and one behind the other, in the examples' type;
  *   index: n adapters in [0, count), or -1 for an example without one.
@@ -584,7 +586,9 @@ typedef struct sdca_adapters {
  * the second part of x_i itself, not of its 8-bit form, in 32 bits; the two
  * are added in 32 bits and rounded to `out` once.  data, and the adapters'
  * type: SDCA_F32, SDCA_F16 or SDCA_BF16; the other arguments and their limits
- * as in sdca_scores_i8.  An example's scores depend on its own adapter alone.
+ * as in sdca_scores_i8.  What other examples' adapters hold, infinities and
+ * NaN among it, does not reach an example's scores; their last bits depend on
+ * the sizes and on the example's place among those of its adapter.
  *   work: device memory of at least sdca_scores_adapted_work bytes, 256-byte
  *      aligned, or NULL: the stream's scratch, as in sdca_log_probs.
  */

@@ -1003,7 +1003,7 @@ def log_probs(S, labels, temperature=1.0, top=0, entropy=False, stats=False):
     best = _empty((n, max(top, 0)), "float32", S) if top else None
     at = _empty((n, max(top, 0)), "int64", S) if top else None
     work = _scratch(S, lib.sdca_log_probs_work, data, m, n, top)
-    _answer(S, "log_probs", lib.sdca_log_probs, data, m, n, _ptr(S), lds, _ptr(labels), temperature, top,
+    _answer(S, "log_probs", lib.sdca_log_probs, data, m, n, _ptr(S), lds, _ptr(labels), float(temperature), top,
             _ptr(logp), _ptr(ent), _ptr(st), _ptr(best), _ptr(at), _ptr(work))
     res = (logp,) + ((ent,) if entropy else ()) + ((st,) if stats else ()) + ((best, at) if top else ())
     return res if len(res) > 1 else logp
@@ -1044,7 +1044,7 @@ def log_probs_grad(S, labels, g, g_entropy=None, stats=None, temperature=1.0, ou
     lp = _empty((n,), "float32", S) if logp else None
     work = _scratch(S, lib.sdca_log_probs_grad_work, data, m, n, _ptr(stats))
     _answer(S, "log_probs_grad", lib.sdca_log_probs_grad, data, m, n, _ptr(S), lds, _ptr(labels), _ptr(g),
-            _ptr(g_entropy), _ptr(stats), temperature, _ptr(out), ldd, _ptr(lp), _ptr(work))
+            _ptr(g_entropy), _ptr(stats), float(temperature), _ptr(out), ldd, _ptr(lp), _ptr(work))
     return (out, lp) if logp else out
 
 
@@ -1072,7 +1072,7 @@ def _adapters(X, A, B, index, scale, m):
     _values(index, "index", n, sys.modules["torch"].int64 if _is_torch(X) else np.int64, X)
     each = _setting(scale, "scale", count, "float32", X)
     return Adapters(count, rank, _ptr(A), _ptr(B), _ptr(index), _ptr(each),
-                    1.0 if each is not None else scale), each
+                    1.0 if each is not None else float(scale)), each
 
 
 def scores_adapted(X, W, w_scales, A, B, index, scale=1.0, out=None, dtype=None):

@@ -189,11 +189,12 @@ __device__ inline v4f multiply(const TA (&a)[8], const TB (&b)[8], v4f sum) {
 }
 
 // A workgroup takes 16 NE examples with all ranks (16 RF); its waves share the
-// wide axis and add up through LDS.  Examples of
-// different adapters take turns; in the adapters' order that is rare.  With
-// QUANT the largest magnitudes come with the first reading, and the rows are
-// read again for their 8-bit form, by then from the last-level cache (20000
-// rows of 4096 floats: XXX us, in two kernels 114 and 64).
+// wide axis and add up through LDS.  Examples of different adapters take
+// turns; in the adapters' order that is rare.  With QUANT the largest
+// magnitudes come with the first reading, and the rows are read again for
+// their 8-bit form, by then mostly from the last-level cache (20000 rows of
+// 4096 floats, rank 16: 147 us, in two kernels 97 and 76).  A compute unit
+// takes some 60 GB/s here, half of it A's rows from the L2.
 constexpr int steps_ahead(int registers) {  // 72 registers of loads at most
   return registers <= 9 ? 8 : registers <= 18 ? 4 : registers <= 36 ? 2 : 1;
 }
@@ -354,9 +355,9 @@ void start_terms(const TermsLaunch& l, const TermsArgs& a) {
   start_terms<TX, TA, NE, RF, WAVES, false>(l, a);
 }
 // Of A there is as much to read as of 16 examples, or more for a rank above
-// 16: 32 share it.  (8192 rows of 14336 bfloat16, rank 16: 62 us, 16 at a time
-// 75; but 20000 rows of 4096 floats 84 and 71, with the registers of twice the
-// loads.)  Few workgroups have sixteen waves each.
+// 16: 32 share it.  (8192 rows of 14336 bfloat16, rank 16: 49 us, 16 at a time
+// 59; 20000 rows of 4096 floats take 88 either way, with twice the registers
+// for the same loads.)  Few workgroups have sixteen waves each.
 template <class TX, class TA>
 void start_terms(const TermsLaunch& l, const TermsArgs& a) {
   const bool many = l.n >= 4096;
@@ -937,7 +938,7 @@ void group_turn(const GroupArgs& g, const TurnArgs& t, int grad, hipStream_t str
 
 // Few workgroups of 16 examples read at some 60 GB/s each: the wide axis is
 // shared by more of them until they come to one for each compute unit (1024
-// rows of 4096 halves, rank 32, and their 8-bit form: 31 us in one part, XX in
+// rows of 4096 halves, rank 32, and their 8-bit form: 31 us in one part, 20 in
 // four with the sums and the 8-bit form in a launch behind).
 int terms_parts(int64_t n) {
   const int64_t tiles = (n + 15) / 16;

@@ -155,6 +155,30 @@ def test_gradients(cuda, n, d, m, r, count, kind):
             assert all(torch.equal(x, y) for x, y in zip(got, far))
 
 
+@pytest.mark.parametrize("kind", ["float16", "bfloat16"])
+@pytest.mark.parametrize("n", [5, 200])
+def test_small_values(cuda, kind, n):
+    """Gradients, examples and adapters among the type's subnormal numbers,
+    as probabilities far from the label's are, and terms far apart."""
+    import torch
+    import libsdca_amd as sd
+    d, m, r = 300, 200, 20
+    X, W, sw, A, B, index, scale = _operands(cuda, n, d, m, r, 3, kind, "mixed", n)
+    dt = X.dtype
+    small = 2.0 ** (-20 if kind == "float16" else -126)
+    G = (torch.randn((n, m), generator=_gen(cuda, 1), device=cuda) * small).to(dt)
+    assert bool((G != 0).any())
+    got = sd.scores_adapted_grad(G, X, A, B, index, scale=scale)
+    if kind == "float16":  # (the sums of the others are no ordinary floats themselves)
+        ref.check_grads([_np(v) for v in got], _np(G), _np(X), _np(A), _np(B), _np(index), _np(scale))
+    A2 = (A.float() * torch.logspace(-6, 2, r, device=cuda)[None, :, None]).to(dt)
+    for X2, B2 in ((X, B), ((X.float() * 2.0 ** -14).to(dt), B), (X, (B.float() * 2.0 ** -18).to(dt))):
+        S = sd.scores_adapted(X2, W, sw, A2, B2, index, scale=scale)
+        _check(S, X2, W, sw, A2, B2, index, scale, "float32")
+        ref.check_grads([_np(v) for v in sd.scores_adapted_grad(G.float(), X2, A2, B2, index, scale=scale)],
+                        _np(G.float()), _np(X2), _np(A2), _np(B2), _np(index), _np(scale))
+
+
 def test_offsets_beyond_32_bits(cuda):
     import torch
     import libsdca_amd as sd
