@@ -562,8 +562,8 @@ int sdca_log_probs_grad(sdca_dtype data, int64_t m, int64_t n, const void* S, in
 /*
  * Low-rank adapters of one weight matrix: example i's scores get
  * scale_a B_a (A_a x_i), a = index[i].
- *   count (1..65535) adapters of `rank` (1..128); calls of 256 examples or
- *      more read the index once for each adapter;
+ *   count (1..65535) adapters of `rank` (1..128); calls of thousands of examples
+ *      read the index once for each adapter;
  *   A: count times a d x rank matrix, B: count times a rank x m one, column-
  *      major, contiguous and one behind the other, in the examples' type;
  *   index: n adapters in [0, count), or -1 for an example without one.

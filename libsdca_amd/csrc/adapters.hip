@@ -37,9 +37,6 @@ struct TermsArgs {
   float* scales;
 };
 
-// From so many examples on, 16 or 32 of them to a workgroup.
-constexpr int64_t kTileTerms = 128;
-
 // Eight neighbouring values of a row from `at` on, zeros from `len` on.
 template <class T>
 __device__ inline void load_raw(const T* row, int64_t at, int64_t len, T (&v)[8]) {
@@ -394,7 +391,7 @@ hipError_t terms(const TermsLaunch& l) {
   a.parts = l.parts;
   a.apart = l.n * a.pitch;
   if (l.n == 0) return hipSuccess;
-  if (l.n >= kTileTerms) {
+  if (!terms_by_rows(l.n, ad.rank)) {
     start_terms<TX, TA>(l, a);
     if (l.parts > 1) {
       terms_row_kernel<TX, TA><<<static_cast<unsigned>(l.n), 256, 0, l.stream>>>(
@@ -812,7 +809,8 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs j, int64_t first) {
 }
 
 // Rows of a segment, so that the columns' workgroups times the segments come
-// to about 512, two waves to a SIMD: more parts cost the joining of their sums.
+// to about 512, two waves to a SIMD (8192 x 14336 bfloat16 with terms: 78 us;
+// 256 of them 112; 1024 83, and 6 more for the joining of their sums).
 int segment_length(int es, int64_t wide, int64_t n) {
   const int64_t columns = 4 * 16 * (16 / es), blocks = (wide + columns - 1) / columns;
   const int64_t parts = std::max<int64_t>(1, 512 / blocks);
@@ -940,9 +938,9 @@ void group_turn(const GroupArgs& g, const TurnArgs& t, int grad, hipStream_t str
 // shared by more of them until they come to one for each compute unit (1024
 // rows of 4096 halves, rank 32, and their 8-bit form: 31 us in one part, 20 in
 // four with the sums and the 8-bit form in a launch behind).
-int terms_parts(int64_t n) {
+int terms_parts(int64_t n, int64_t rank) {
   const int64_t tiles = (n + 15) / 16;
-  return n < kTileTerms || tiles > 128 ? 1 : static_cast<int>(std::min<int64_t>(8, 256 / tiles));
+  return terms_by_rows(n, rank) || tiles > 128 ? 1 : static_cast<int>(std::min<int64_t>(8, 256 / tiles));
 }
 
 hipError_t launch_terms(const TermsLaunch& l) {

@@ -162,7 +162,13 @@ struct TermsLaunch {
   float* scales;
   hipStream_t stream;
 };
-int terms_parts(int64_t n);
+// Whether an example has workgroups of its own, or 16 and more share one: then
+// the adapters' order is worth finding first.  (us with and without, order and
+// product included, m = d = 4096, fp16: rank 16, 8 adapters, n = 1024: 46, 56;
+// 2048: 68, 75; 3000: 101, 98; rank 32, 4 adapters, 1024: 52, 58; 2048: 79, 79;
+// rank 64, 512: 50, 50; 1024: 81, 66.)
+constexpr bool terms_by_rows(int64_t n, int64_t rank) { return n * terms_pitch(rank) <= 32768; }
+int terms_parts(int64_t n, int64_t rank);
 hipError_t launch_terms(const TermsLaunch& a);
 
 // The n rows in the order of their adapters, rising for each, those without

@@ -1631,11 +1631,11 @@ AdaptedPlan plan_adapted(int data, int64_t d, int64_t m, int64_t n, const void* 
   p.w = p.own_x ? whole(static_cast<size_t>(n) * p.pad) : 0;
   p.scales = p.w + (p.own_w ? whole(static_cast<size_t>(m) * p.pad) : 0);
   p.terms = p.scales + (p.own_x ? whole(n * sizeof(float)) : 0);
-  p.parts = p.own_x ? terms_parts(n) : 1;
+  p.parts = p.own_x ? terms_parts(n, rank) : 1;
   p.order = p.terms + whole(static_cast<size_t>(p.parts) * n * terms_pitch(rank) * sizeof(float));
   // Examples in the order of their adapters: a product of 16 of them then has
   // one adapter, but for few.
-  p.grouped = p.own_x && count > 1 && n >= 256;
+  p.grouped = p.own_x && count > 1 && !terms_by_rows(n, rank);
   p.ids = p.order + (p.grouped ? whole(n * sizeof(int)) : 0);
   p.spans = p.ids + (p.grouped ? whole(n * sizeof(int)) : 0);
   p.end = p.spans + (p.grouped ? whole((count + 1) * sizeof(int2)) : 0);

@@ -131,7 +131,7 @@ struct Mass {
 // them are sorted and merged into the list.  The bound has an index too: of
 // very many equal scores (a mask of the lowest value) only those of low index
 // are candidates (64 rows of 128000, some so masked: 63 us with the score
-// alone, 18 with both).
+// alone, 16 with both).
 // ---------------------------------------------------------------------------
 struct Best {
   u64 list = 0;
@@ -380,12 +380,19 @@ LogProbsPlan plan_log_probs(int64_t m, int64_t n) {
     const int64_t length = ((m + parts - 1) / parts + 2047) / 2048 * 2048;
     return LogProbsPlan{4, static_cast<int>((m + length - 1) / length), static_cast<int>(length)};
   };
-  if (m <= 2048) return {1, 1, static_cast<int>(m)};
-  if (n < 256 && m > 32768) {
+  // us without and with 10 alternatives: 500 x 2000 floats 7.2, 9.1 by one wave
+  // to a column, 7.4, 13.9 by sixteen; 5000 x 4000 16, 22 by one, 16, 31 by
+  // four, but 4 x 4000 4.8, 11.5 and by sixteen 4.0, 7.9.
+  if (m <= 2048 || (m <= 8192 && n >= 2048)) return {1, 1, static_cast<int>(m)};
+  // 300 x 64000 bfloat16 14.4, 22.3 in parts, 13.7, 29.3 by four waves; 600 x
+  // 64000 20.4, 32.0 and 18.2, 33.1.
+  if (n < 512 && m > 32768) {
     const int64_t parts = (1024 + n - 1) / n, most = (m + 8191) / 8192;
     return split(parts < most ? (parts < 64 ? parts : 64) : (most < 64 ? most : 64));
   }
-  if (n < 512) return {16, 1, static_cast<int>(m)};
+  // 1 x 16000 floats 4.3, 9.1 by sixteen waves, 4.9, 12.0 by four; 300 x 16000
+  // bfloat16 7.3, 16.6 and 6.4, 12.2.
+  if (n < 256) return {16, 1, static_cast<int>(m)};
   return {4, 1, static_cast<int>(m)};
 }
 
@@ -807,7 +814,7 @@ hipError_t log_probs_grad(LogProbsGradLaunch l) {
     if (holds(256 * 4)) return start_whole<T, 4, 4>(l), hipGetLastError();
     if (holds(256 * 8)) return start_whole<T, 4, 8>(l), hipGetLastError();
     if (holds(1024 * 4)) return start_whole<T, 16, 4>(l), hipGetLastError();
-    // (4096 columns of 65536 bfloat16: 227 us, with the statistics in a launch
+    // (4096 columns of 65536 bfloat16: 231 us, with the statistics in a launch
     // of their own 302; but a few columns leave most of the device idle.)
     if (l.n >= kTwiceColumns) return start_twice<T>(l), hipGetLastError();
     LogProbsLaunch s = {};

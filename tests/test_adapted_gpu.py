@@ -14,7 +14,10 @@ HALF_STEP = {"float32": (2.0 ** -24, 2.0 ** -149), "float16": (2.0 ** -11, 2.0 *
 SHAPES = [(1, 1, 1, 1, 1), (1, 4096, 1000, 8, 4), (2, 513, 70, 5, 3), (2, 1024, 9000, 16, 2), (3, 100, 300, 3, 2),
           (5, 17, 137, 128, 2), (31, 513, 137, 10, 3), (33, 64, 256, 16, 40), (48, 600, 513, 17, 5),
           (64, 128, 1024, 33, 3), (65, 4100, 65, 64, 2), (130, 1030, 1001, 65, 4), (200, 256, 700, 31, 1),
-          (257, 300, 515, 100, 7), (700, 2048, 600, 16, 3), (1111, 130, 2050, 8, 20), (3000, 72, 1030, 4, 2)]
+          (257, 300, 515, 100, 7), (700, 2048, 600, 16, 3), (1111, 130, 2050, 8, 20), (3000, 72, 1030, 4, 2),
+          # terms of many examples together: each number of ranks, in parts and not, 16 and 32 to a workgroup
+          (600, 301, 270, 100, 7), (1111, 130, 300, 32, 20), (700, 521, 300, 61, 3), (2200, 300, 280, 16, 5),
+          (4100, 200, 300, 32, 4), (4300, 77, 270, 64, 2), (4099, 64, 260, 128, 3)]
 
 
 def _gen(cuda, seed):
