@@ -934,10 +934,10 @@ void group_turn(const GroupArgs& g, const TurnArgs& t, int grad, hipStream_t str
 
 }  // namespace
 
-// Few workgroups of 16 examples read at some 60 GB/s each: the wide axis is
+// A few workgroups of 16 examples read at some 60 GB/s each: the wide axis is
 // shared by more of them until they come to one for each compute unit (1024
-// rows of 4096 halves, rank 32, and their 8-bit form: 31 us in one part, 20 in
-// four with the sums and the 8-bit form in a launch behind).
+// rows of 4096 halves, rank 32, and their 8-bit form, all in tiles: 31 us in one
+// part, 20 in four with the sums and the 8-bit form in a launch behind).
 int terms_parts(int64_t n, int64_t rank) {
   const int64_t tiles = (n + 15) / 16;
   return terms_by_rows(n, rank) || tiles > 128 ? 1 : static_cast<int>(std::min<int64_t>(8, 256 / tiles));
