@@ -11,12 +11,14 @@
 // sum w log w relative to it, and brings them to a larger maximum when one
 // comes.  Exponents are in base 2, relative to a reference rather than to
 // the maximum itself: with c = log2(e) / T and ref = M c rounded and held
-// within +-1e30, e_j = fma(s_j, c, -ref) is one instruction, and the same
+// within +-2^24, e_j = fma(s_j, c, -ref) is one instruction, and the same
 // reference in every term cancels in the differences that are the results.
-// Masked scores at the type's lowest value or -infinity then have weight 0
-// beside any ordinary score.  A column whose M c is beyond 1e30 (scores near
-// the largest float, +infinity, or nothing but lowest values) is gone through
-// a second time with exponents from s_j - M.
+// Up to 2^24 the rounding is half a unit at most: the weights' largest is
+// between 2^-1/2 and 2^1/2.  (At 2^32 it is 2^7 or more, and the weights
+// infinite or 0.)  Scores masked at -1e9, at the type's lowest value or at
+// -infinity then have weight 0 beside any ordinary score.  A column whose M c
+// is beyond 2^24 (large scores, a temperature near nothing, +infinity, or
+// nothing but masks) is gone through a second time with exponents from s_j - M.
 #include "answer_launch.hpp"
 #include "answer_limits.hpp"
 #include "answer_types.hpp"
@@ -27,7 +29,7 @@ namespace sdca_gpu {
 namespace {
 
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
-constexpr float kFar = 1e30f;
+constexpr float kFar = 16777216.f;
 constexpr float kLowest = -3.402823466e38f;
 // Exponents below this have weight 0, and 0 times this is 0.
 constexpr float kGone = -200.f;

@@ -1,0 +1,97 @@
+"""sdca_log_probs and sdca_log_probs_grad where scores over the temperature
+pass what 32 bits hold to a unit: finite masks, large scores, temperatures near
+nothing.  Against the plain forms in 64 bits (tests/log_probs_oracle.py)."""
+import numpy as np
+import pytest
+
+from tests import log_probs_oracle as ref
+
+pytestmark = pytest.mark.gpu
+
+KINDS = ["float32", "float16", "bfloat16"]
+HALF_STEP = {"float32": (2.0 ** -24, 2.0 ** -149), "float16": (2.0 ** -11, 2.0 ** -25), "bfloat16": (2.0 ** -8, 2.0 ** -134)}
+MASKS = {"float16": [-3e4, -6e4, -65504.0],
+         "float32": [-1e8, -1e9, -5e9, -1e10, -1e12, -1e18, -1e20, -1e25]}
+MASKS["bfloat16"] = MASKS["float32"]
+# Where M log2(e) / T is 2^24.
+EDGE = 2.0 ** 24 * np.log(2)
+
+
+def _gen(cuda, seed):
+    import torch
+    g = torch.Generator(device=cuda)
+    g.manual_seed(seed)
+    return g
+
+
+def _np(t):
+    import torch
+    return (t.float() if t.dtype == torch.bfloat16 else t).cpu().numpy()
+
+
+def _rows(cuda, n, m, kind, T):
+    """(S, labels, number of special rows, the first ones)."""
+    import torch
+    g = _gen(cuda, n + m)
+    S = torch.randn((n, m), generator=g, device=cuda) * 4
+    labels = torch.randint(0, m, (n,), generator=g, device=cuda)
+    most = torch.finfo(getattr(torch, kind)).max
+    i = 0
+    for v in MASKS[kind]:
+        S[i, : m - m // 8 - 1] = v   # whole lanes and waves see masks alone
+        labels[i] = m - 1
+        S[i + 1, m // 8 + 1:] = v    # masks behind the others
+        labels[i + 1] = 0
+        S[i + 2] = v                 # nothing but masks
+        i += 3
+    S[i] = min(1e10, most / 2)
+    S[i + 1, m // 3] = min(1e10, most / 2)
+    S[i + 2] = (S[i + 2] * 1e9).clamp(-most, most)
+    edge = min(EDGE * T, most / 2)
+    apart = torch.randint(-20, 21, (2, m), generator=g, device=cuda) * T
+    S[i + 3], S[i + 4] = edge + apart[0], -edge + apart[1]
+    S[i + 5, ::3] = -2 * edge        # near and far in turn
+    S[i + 6] = torch.linspace(-2 * edge, 2 * edge, m, device=cuda)
+    S[i + 7] = torch.linspace(2 * edge, -2 * edge, m, device=cuda)
+    labels[i + 7] = 0
+    return S.to(getattr(torch, kind)), labels, i + 8
+
+
+def _check(cuda, n, m, kind, T):
+    import torch
+    import libsdca_amd as sd
+    print(n, m, kind, T, flush=True)
+    S, labels, some = _rows(cuda, n, m, kind, T)
+    few = slice(0, some)
+    hS, hl = _np(S[few]), _np(labels[few])
+    stats = None
+    for top in (0, 3):
+        res = sd.log_probs(S, labels, temperature=T, top=top, entropy=True, stats=True)
+        stats = res[2]
+        host = [_np(v[few]) for v in res]
+        ref.check(hS, hl, T, host[0], host[1], host[2], tuple(host[3:]) or None)
+    # gradients of the loss in its units: their size does not go with 1 / T
+    unit = min(1.0, 1024 * T)
+    g = torch.randn(n, generator=_gen(cuda, 3), device=cuda) * unit
+    h = torch.randn(n, generator=_gen(cuda, 4), device=cuda) * unit
+    for hh, st in ((None, None), (h, None), (h, stats)):
+        D, lp = sd.log_probs_grad(S, labels, g, g_entropy=hh, stats=st, temperature=T, logp=True)
+        ref.check_grad(_np(D[few]), hS, hl, _np(g[few]).astype(np.float64), None if hh is None else _np(hh[few]), T,
+                       *HALF_STEP[kind])
+        ref.check(hS, hl, T, _np(lp[few]))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T", [30.0, 1.0, 0.1, 1e-4, 1e-8, 1e-9, 1e-12, 2.0 ** -126])
+# a wave to a column, in one vector or four; 4, 16 waves; parts
+@pytest.mark.parametrize("m", [60, 900, 3000, 9000, 40_000])
+def test_far_scores(cuda, m, T, kind):
+    _check(cuda, 32, m, kind, T)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T", [1.0, 1e-9])
+# a wave to a longer column; four waves to one, short and long, and the gradient in two passes
+@pytest.mark.parametrize("n,m", [(2100, 4000), (300, 5000), (300, 33_000), (520, 40_000)])
+def test_far_scores_of_many_columns(cuda, n, m, T, kind):
+    _check(cuda, n, m, kind, T)
