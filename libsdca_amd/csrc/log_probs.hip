@@ -16,9 +16,15 @@
 // Up to 2^24 the rounding is half a unit at most: the weights' largest is
 // between 2^-1/2 and 2^1/2.  (At 2^32 it is 2^7 or more, and the weights
 // infinite or 0.)  Scores masked at -1e9, at the type's lowest value or at
-// -infinity then have weight 0 beside any ordinary score.  A column whose M c
-// is beyond 2^24 (large scores, a temperature near nothing, +infinity, or
-// nothing but masks) is gone through a second time with exponents from s_j - M.
+// -infinity then have weight 0 beside any ordinary score.  Where a maximum is
+// far, M c beyond 2^24 (large scores, a temperature near nothing, +infinity, or
+// nothing but masks), exponents are (s_j - M) c instead.  Log-probabilities
+// then take a second pass, over the column or a workgroup's part of it, from
+// the caches; the gradient's kernels have them in the pass that they make.
+// (64 columns of 128000 bfloat16, top 20, us: ordinary 17.4, one all masks
+// 22.9, all such 23.7, all but 100 scores of each at -1e9 23.4.  With such
+// exponents in the first pass 17.6, 20.9, 21.6 and 21.8, but 600 x 64000 19.2
+// where it is 18.2, and 64 x 128000 with masks in some columns 21.7, not 20.9.)
 #include "answer_launch.hpp"
 #include "answer_limits.hpp"
 #include "answer_types.hpp"
@@ -36,16 +42,9 @@ constexpr float kGone = -200.f;
 
 __device__ inline float exp2_of(float e) { return __builtin_amdgcn_exp2f(e); }
 __device__ inline float ref_of(float max, float c) { return fminf(fmaxf(max * c, -kFar), kFar); }
-
-template <bool VALU>
-__device__ inline float wave_largest(float v) {
-  v = fmaxf(v, other<1, VALU>(v));
-  v = fmaxf(v, other<2, VALU>(v));
-  v = fmaxf(v, other<4, VALU>(v));
-  v = fmaxf(v, other<8, VALU>(v));
-  v = fmaxf(v, other<16, VALU>(v));
-  return fmaxf(v, other<32, VALU>(v));
-}
+__device__ inline bool is_far(float max, float c) { return fabsf(max * c) > kFar && max > -INFINITY; }
+// s - max where infinities are equal, and NaN stays.
+__device__ inline float below(float s, float max) { return s == max ? 0.f : s - max; }
 
 // 16 bytes of a column as words, and as floats.  (Held as elements, 16-bit
 // scores take a register each.)
@@ -81,20 +80,44 @@ template <class T>
 __device__ inline int behind_16(const T* row) {
   return static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T));
 }
+// What exponents are relative to: the maximum itself where it is far, or a
+// reference.
+struct Origin {
+  float from, ref;
+  __device__ Origin(float max, float c) {
+    const bool far = is_far(max, c);
+    from = far ? max : 0.f;
+    ref = far ? 0.f : ref_of(max, c);
+  }
+  __device__ float exponent(float s, float c) const { return fmaf(below(s, from), c, -ref); }
+};
 // The weights of some scores: their largest, and the sums of 2^e and e 2^e
-// with exponents relative to ref_of(max).  (A NaN among the scores makes the
+// with exponents relative to its origin.  (A NaN among the scores makes the
 // sums NaN and leaves max.)
 struct Mass {
   float max = -INFINITY, sum = 0.f, weighted = 0.f;
 
-  __device__ void rise(float to, float c) {  // to a larger or equal maximum
-    const float by = ref_of(max, c) - ref_of(to, c), f = exp2_of(by);
+  __device__ void shift(float by) {
+    const float f = exp2_of(by);
     weighted = f * fmaf(fmaxf(by, kGone), sum, weighted);
     sum *= f;
+  }
+  // To a larger or equal maximum.
+  template <bool ANY>
+  __device__ void rise(float to, float c) {
+    if constexpr (ANY) {
+      const Origin old(max, c), now(to, c);
+      // (By 1/2 at most where there is a weight; without one it can be large.)
+      shift(fminf(fmaf(below(old.from, now.from), c, old.ref - now.ref), 1.f));
+    } else {
+      shift(ref_of(max, c) - ref_of(to, c));
+    }
     max = to;
   }
-  // A lane's scores (as words); returns their largest.
-  template <class T, int N>
+  // A lane's scores (as words); returns their largest.  Without ANY as if no
+  // maximum were far: a negative one's weights are then too small, and a
+  // positive one's mean nothing.
+  template <class T, bool ANY, int N>
   __device__ float add(const unsigned (&raw)[N][4], float c) {
     constexpr int V = 16 / static_cast<int>(sizeof(T));
     float v[N][V], most = -INFINITY;
@@ -104,26 +127,45 @@ struct Mass {
     for (int u = 0; u < N; ++u)
 #pragma unroll
       for (int e = 0; e < V; ++e) most = fmaxf(most, v[u][e]);
-    if (most > max) rise(most, c);
-    const float ref = ref_of(max, c);
+    if (most > max) rise<ANY>(most, c);
+    const Origin origin(max, c);
+    if (!ANY || !__ballot(origin.from != 0.f)) {
+      const float ref = ref_of(max, c);
+      weigh(v, [&](float x) { return fmaf(x, c, -ref); });
+    } else {
+      weigh(v, [&](float x) { return origin.exponent(x, c); });
+    }
+    return most;
+  }
+  // A vector of a lane's scores beside a far maximum that is not below them.
+  template <class T>
+  __device__ void add_below(const unsigned (&raw)[4], float c) {
+    float v[1][16 / sizeof(T)];
+    unpack<T>(raw, v[0]);
+    weigh(v, [&](float x) { return below(x, max) * c; });
+  }
+  // All lanes' together, in every lane.
+  template <bool ANY>
+  __device__ void over_wave(float c) {
+    rise<ANY>(wave_max<true>(max), c);
+    sum = wave_total(sum);
+    weighted = wave_total(weighted);
+  }
+
+ private:
+  template <int N, int V, class Exponent>
+  __device__ void weigh(const float (&v)[N][V], Exponent exponent) {
     float s = 0.f, w_e = 0.f;
 #pragma unroll
     for (int u = 0; u < N; ++u)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float x = fmaf(v[u][e], c, -ref), w = exp2_of(x);
+        const float x = exponent(v[u][e]), w = exp2_of(x);
         s += w;
         w_e = fmaf(w, fmaxf(x, kGone), w_e);
       }
     sum += s;
     weighted += w_e;
-    return most;
-  }
-  // All lanes' together, in every lane.
-  __device__ void over_wave(float c) {
-    rise(wave_largest<true>(max), c);
-    sum = wave_total(sum);
-    weighted = wave_total(weighted);
   }
 };
 
@@ -210,25 +252,11 @@ struct Own {
 };
 
 // A column's results, by one wave.
-template <class T>
-__device__ void finish(const T* row, int64_t col, Mass mass, u64 list, const Own& own,
-                       const LogProbsArgs& a) {
+__device__ inline void finish(int64_t col, const Mass& mass, u64 list, const Own& own, const LogProbsArgs& a) {
   const int lane = threadIdx.x & 63;
-  const float c = a.inv_t * kLog2e, max = mass.max, ref = ref_of(max, c);
-  const bool near = fabsf(max * c) <= kFar;
-  const auto exponent = [&](float s) { return near ? fmaf(s, c, -ref) : fminf(s - max, 0.f) * c; };
-  if (!near && max > -INFINITY) {
-    float sum = 0.f, weighted = 0.f;
-    bool bad = false;
-    for (int64_t i = lane; i < a.m; i += 64) {
-      const float s = to_float(row[i]), e = exponent(s), w = exp2_of(e);
-      bad |= s != s;
-      sum += w;
-      weighted = fmaf(w, fmaxf(e, kGone), weighted);
-    }
-    mass.sum = __ballot(bad) ? NAN : wave_total(sum);
-    mass.weighted = wave_total(weighted);
-  }
+  const float c = a.inv_t * kLog2e, max = mass.max;
+  const Origin origin(max, c);
+  const auto exponent = [&](float s) { return origin.exponent(s, c); };
   const bool none = max == -INFINITY && mass.sum == 0.f;
   const float log_sum = log2f(mass.sum);
   float entropy = none ? 0.f : (log_sum - mass.weighted / mass.sum) * kLn2;
@@ -253,20 +281,34 @@ __device__ void finish(const T* row, int64_t col, Mass mass, u64 list, const Own
   }
 }
 
-// The masses of WAVES waves, and their best, in the first.
-template <int WAVES, bool TOP>
-__device__ inline void join_waves(Mass& mass, u64& list, u64 (*room)[128], float c, int wave) {
+// The masses of WAVES waves, and their best, in the first.  again(max) sees the
+// largest of all, and returns in all waves whether it has changed the masses.
+template <int WAVES, bool TOP, class Again>
+__device__ inline void join_waves(Mass& mass, u64& list, u64 (*room)[128], float c, int wave, Again again) {
   __shared__ float of_wave[WAVES][3];
   const int lane = threadIdx.x & 63;
-  if (lane == 0) {
-    of_wave[wave][0] = mass.max;
-    of_wave[wave][1] = mass.sum;
-    of_wave[wave][2] = mass.weighted;
-  }
+  const auto give = [&] {
+    if (lane == 0) {
+      of_wave[wave][0] = mass.max;
+      of_wave[wave][1] = mass.sum;
+      of_wave[wave][2] = mass.weighted;
+    }
+  };
+  give();
 #pragma unroll
   for (int s = 1; s < WAVES; s *= 2) {
     if (TOP && (wave & (2 * s - 1)) == s) room[wave][lane] = list;
     if (TOP || s == 1) __syncthreads();
+    if (s == 1) {
+      float most = of_wave[0][0];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) most = fmaxf(most, of_wave[w][0]);
+      if (again(most)) {
+        __syncthreads();
+        give();
+        __syncthreads();
+      }
+    }
     if (TOP && (wave & (2 * s - 1)) == 0) {
       Best b;
       b.list = list;
@@ -281,7 +323,7 @@ __device__ inline void join_waves(Mass& mass, u64& list, u64 (*room)[128], float
       mass.sum = of_wave[lane][1];
       mass.weighted = of_wave[lane][2];
     }
-    mass.over_wave(c);
+    mass.over_wave<true>(c);
   }
 }
 
@@ -305,8 +347,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void log_probs_kerne
   Mass mass;
   Best best;
   bool started = false;
-  for (int64_t at = first - behind_16(row + first) + (WAVES == 1 ? 0 : wave) * kStep; at < end;
-       at += WAVES * kStep) {
+  const int64_t begin = first - behind_16(row + first) + (WAVES == 1 ? 0 : wave) * kStep;
+  for (int64_t at = begin; at < end; at += WAVES * kStep) {
     unsigned raw[kLoads][4];
     if (at >= first && at + kStep <= end) {
 #pragma unroll
@@ -315,7 +357,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void log_probs_kerne
 #pragma unroll
       for (int u = 0; u < kLoads; ++u) load_words(row, at + (u * 64 + lane) * V, first, end, raw[u]);
     }
-    const float most = mass.add<T>(raw, c);
+    const float most = mass.add<T, false>(raw, c);
     if constexpr (TOP) {
       if (!started) {
         // `top` lanes have a score of at least this.
@@ -335,13 +377,32 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void log_probs_kerne
     }
   }
   if constexpr (TOP) best.finish(room[wave], a.top);
-  mass.over_wave(c);
-  if constexpr (WAVES > 1) {
-    join_waves<WAVES, TOP>(mass, best.list, room, c, wave);
+  mass.over_wave<false>(c);
+  // Where the largest of the column, or of the workgroup's part, is far: the
+  // weights once more, from differences.
+  const auto again = [&](float most) {
+    if (!__builtin_amdgcn_readfirstlane(is_far(most, c))) return false;
+    mass.max = most;
+    mass.sum = mass.weighted = 0.f;
+    for (int64_t at = begin; at < end; at += WAVES * kStep) {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        unsigned raw[4];
+        load_words(row, at + (u * 64 + lane) * V, first, end, raw);
+        mass.add_below<T>(raw, c);
+      }
+    }
+    mass.over_wave<true>(c);
+    return true;
+  };
+  if constexpr (WAVES == 1) {
+    again(mass.max);
+  } else {
+    join_waves<WAVES, TOP>(mass, best.list, room, c, wave, again);
     if (wave) return;
   }
   if (a.parts == 1) {
-    finish(row, col, mass, best.list, own, a);
+    finish(col, mass, best.list, own, a);
   } else {
     const int64_t part = col * a.parts + blockIdx.y;
     if (lane == 0) a.masses[part] = mass;
@@ -363,14 +424,14 @@ __global__ __launch_bounds__(64 * kJoinWaves) void log_probs_join_kernel(const T
   Mass mass;
   const int mine = wave + lane * kJoinWaves;
   if (mine < a.parts) mass = a.masses[col * a.parts + mine];
-  mass.over_wave(c);
+  mass.over_wave<true>(c);
   Best best;
   if constexpr (TOP) {
     for (int p = wave; p < a.parts; p += kJoinWaves)
       best.merge_sorted(63 - lane < a.top ? a.lists[(col * a.parts + p) * a.top + 63 - lane] : 0);
   }
-  join_waves<kJoinWaves, TOP>(mass, best.list, room, c, wave);
-  if (wave == 0) finish(S + col * a.lds, col, mass, best.list, own, a);
+  join_waves<kJoinWaves, TOP>(mass, best.list, room, c, wave, [](float) { return false; });
+  if (wave == 0) finish(col, mass, best.list, own, a);
 }
 
 // How a launch takes the columns: waves to a part, parts to a column.
@@ -596,7 +657,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, WAVES == 16 ? 8 : 1)
 #pragma unroll
     for (int e = 0; e < V; ++e) max = fmaxf(max, v[e]);
   }
-  max = wave_largest<true>(max);
+  max = wave_max<true>(max);
   if constexpr (WAVES > 1) {
     if ((threadIdx.x & 63) == 0) part[0][wave] = max;
     __syncthreads();
@@ -620,13 +681,9 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, WAVES == 16 ? 8 : 1)
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  const bool near = fabsf(max * by) <= kFar || max == -INFINITY;
-  if (near) {
-    add([&](float x) { return fmaf(x, by, -ref); });
-  } else {
-    // (NaN keeps its NaN: the smaller of it and 0 would be 0.)
-    add([&](float x) { return x != x ? x : fminf(x - max, 0.f) * by; });
-  }
+  const bool far = is_far(max, by);
+  if (far) add([&](float x) { return below(x, max) * by; });
+  else add([&](float x) { return fmaf(x, by, -ref); });
   sum = wave_total(sum);
   weighted = wave_total(weighted);
   if constexpr (WAVES > 1) {
@@ -652,8 +709,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, WAVES == 16 ? 8 : 1)
       __builtin_amdgcn_sched_barrier(0);  // (all vectors' temporaries at once do not fit)
     }
   };
-  if (near) write([&](float x) { return fmaf(x, by, -ref); });
-  else write([&](float x) { return fminf(x - max, 0.f) * by; });
+  if (far) write([&](float x) { return below(x, max) * by; });
+  else write([&](float x) { return fmaf(x, by, -ref); });
 }
 
 // A longer column by one workgroup that goes through it twice: for the
@@ -665,7 +722,6 @@ __global__ __launch_bounds__(64 * kTwiceWaves, 8) void log_probs_grad_twice_kern
   constexpr int V = 16 / static_cast<int>(sizeof(T)), kLoads = 4, kLanes = 64 * kTwiceWaves;
   constexpr int kStep = kLanes * V * kLoads;
   __shared__ float part[3][kTwiceWaves];
-  __shared__ int odd;
   const int lane = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(lane >> 6);
   const int64_t col = blockIdx.x;
@@ -689,9 +745,9 @@ __global__ __launch_bounds__(64 * kTwiceWaves, 8) void log_probs_grad_twice_kern
   for (int64_t step = 0; step < steps; ++step) {
     unsigned raw[kLoads][4];
     load(step, raw);
-    mass.add<T>(raw, by);
+    mass.add<T, true>(raw, by);
   }
-  mass.over_wave(by);
+  mass.over_wave<true>(by);
   if ((lane & 63) == 0) part[0][wave] = mass.max, part[1][wave] = mass.sum, part[2][wave] = mass.weighted;
   __syncthreads();
   mass = Mass();
@@ -700,30 +756,9 @@ __global__ __launch_bounds__(64 * kTwiceWaves, 8) void log_probs_grad_twice_kern
     mass.sum = part[1][lane & 63];
     mass.weighted = part[2][lane & 63];
   }
-  mass.over_wave(by);
+  mass.over_wave<true>(by);
   const float max = mass.max, ref = ref_of(max, by);
-  const bool near = fabsf(max * by) <= kFar || max == -INFINITY;
-  if (!near) {
-    // Scores near the largest float, or infinite: once more, from s - max.
-    float sum = 0.f, weighted = 0.f;
-    bool bad = false;
-    for (int64_t i = lane; i < a.m; i += kLanes) {
-      const float x = to_float(s[i]), e = fminf(x - max, 0.f) * by, w = exp2_of(e);
-      bad |= x != x;
-      sum += w;
-      weighted = fmaf(w, fmaxf(e, kGone), weighted);
-    }
-    sum = wave_total(sum);
-    weighted = wave_total(weighted);
-    if (lane == 0) odd = 0;
-    __syncthreads();
-    if (bad) odd = 1;
-    if ((lane & 63) == 0) part[1][wave] = sum, part[2][wave] = weighted;
-    __syncthreads();
-    mass.sum = mass.weighted = 0.f;
-    for (int w = 0; w < kTwiceWaves; ++w) mass.sum += part[1][w], mass.weighted += part[2][w];
-    if (odd) mass.sum = NAN;
-  }
+  const bool far = is_far(max, by);
   const float log2_sum = log2f(mass.sum);
   float entropy = (log2_sum - mass.weighted / mass.sum) * kLn2;
   if (entropy < 0.f) entropy = 0.f;
@@ -736,8 +771,8 @@ __global__ __launch_bounds__(64 * kTwiceWaves, 8) void log_probs_grad_twice_kern
     for (int u = 0; u < kLoads; ++u) {
       const int64_t at = begin + step * kStep + (u * kLanes + lane) * V;
       if (at >= a.m) break;
-      if (near) grad_vec<H, T, V>(raw[u], static_cast<int>(at), a.m, c, [&](float x) { return fmaf(x, by, -ref); }, logp, d);
-      else grad_vec<H, T, V>(raw[u], static_cast<int>(at), a.m, c, [&](float x) { return fminf(x - max, 0.f) * by; }, logp, d);
+      if (far) grad_vec<H, T, V>(raw[u], static_cast<int>(at), a.m, c, [&](float x) { return below(x, max) * by; }, logp, d);
+      else grad_vec<H, T, V>(raw[u], static_cast<int>(at), a.m, c, [&](float x) { return fmaf(x, by, -ref); }, logp, d);
     }
   }
 }

@@ -95,3 +95,16 @@ def test_far_scores(cuda, m, T, kind):
 @pytest.mark.parametrize("n,m", [(2100, 4000), (300, 5000), (300, 33_000), (520, 40_000)])
 def test_far_scores_of_many_columns(cuda, n, m, T, kind):
     _check(cuda, n, m, kind, T)
+
+
+@pytest.mark.parametrize("n,m", [(1, 2 ** 22), (2, 2 ** 21 + 5)])
+def test_sums_of_far_columns_keep_their_digits(cuda, n, m):
+    """A long column whose weights come from differences: as few additions
+    behind one another as elsewhere (one wave alone would make 2^16)."""
+    import torch
+    import libsdca_amd as sd
+    steps = torch.rand((n, m), generator=_gen(cuda, m), device=cuda)
+    S = 3e10 - 2048 * (4 * steps).floor()   # 1e10 is beyond 2^24 at T = 1000
+    labels = torch.randint(0, m, (n,), generator=_gen(cuda, 1), device=cuda)
+    res = [_np(v) for v in sd.log_probs(S, labels, temperature=1000.0, entropy=True, stats=True)]
+    ref.check(_np(S), _np(labels), 1000.0, *res)
