@@ -25,6 +25,8 @@
 // 22.9, all such 23.7, all but 100 scores of each at -1e9 23.4.  With such
 // exponents in the first pass 17.6, 20.9, 21.6 and 21.8, but 600 x 64000 19.2
 // where it is 18.2, and 64 x 128000 with masks in some columns 21.7, not 20.9.)
+#include <type_traits>
+
 #include "answer_launch.hpp"
 #include "answer_limits.hpp"
 #include "answer_types.hpp"
@@ -529,23 +531,29 @@ struct GradArgs {
 };
 
 // A column's own numbers.  With weights w = 2^e whose sum is 2^log2_sum, the
-// gradient of a score that is not the label's is w (c1 + c2 e).
+// gradient of a score that is not the label's is w (c1 + c2 e).  The constants
+// have 1 / T in them, or where they could then pass the largest float
+// (`apart`: of a weight of 0 they would make NaN) it is multiplied last.
 struct GradColumn {
-  float log2_sum, c1, c2, g;
+  float log2_sum, c1, c2, g, h;
   int label;
-  bool none;
+  bool none, apart;
 
   __device__ GradColumn(const GradArgs& a, int64_t col) {
     const int64_t l = a.labels[col];
     // (Far below the first vector, which starts up to 15 before the column.)
     label = l >= 0 && l < a.m ? static_cast<int>(l) : -0x7fffffff;
-    g = l == -1 ? 0.f : label < 0 ? NAN : a.g[col] * a.inv_t;
+    g = l == -1 ? 0.f : label < 0 ? NAN : a.g[col];
+    h = a.h ? a.h[col] : 0.f;
+    // (log p and e are below 256 in size where there is a weight.)
+    apart = !((fabsf(g) + 512.f * fabsf(h)) * a.inv_t < 1e38f);
+    if (!apart) g *= a.inv_t, h *= a.inv_t;
     if (a.logp && label < 0 && threadIdx.x % 64 == 0) a.logp[col] = l == -1 ? 0.f : NAN;
   }
-  __device__ void set(const GradArgs& a, int64_t col, float log_sum, float entropy, bool empty) {
+  __device__ void set(float log_sum, float entropy, bool empty) {
     log2_sum = log_sum;
     none = empty;
-    const float h = a.h ? a.h[col] * a.inv_t : 0.f, one = exp2_of(-log2_sum);
+    const float one = exp2_of(-log2_sum);
     c1 = none ? g * 0.f : -one * fmaf(h, fmaf(-log2_sum, kLn2, entropy), g);
     c2 = none ? 0.f : -one * h * kLn2;
   }
@@ -559,20 +567,21 @@ struct GradColumn {
 // V scores of a column, from `at` on, to their gradients; the lane that has
 // the label's writes its log-probability.  (S and D may be one matrix: a lane
 // has read what it writes.)
-template <bool H, class T, int V, class Exponent>
-__device__ inline void grad_vec(const unsigned (&raw)[4], int at, int m, const GradColumn& c,
+template <bool H, bool APART, class T, int V, class Exponent>
+__device__ inline void grad_vec(const unsigned (&raw)[4], int at, int m, const GradColumn& c, float last,
                                 Exponent exponent, float* logp, T* d) {
+  const auto result = [&](float x) { return from_float<T>(APART ? x * last : x); };
   float s[V];
   unpack<T>(raw, s);
   T out[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) out[e] = from_float<T>(c.of<H>(exponent(s[e])));
+  for (int e = 0; e < V; ++e) out[e] = result(c.of<H>(exponent(s[e])));
   if (c.label >= at && c.label < at + V) {
 #pragma unroll
     for (int e = 0; e < V; ++e)
       if (c.label == at + e) {
         const float x = exponent(s[e]);
-        if (!c.none) out[e] = from_float<T>(c.of<H>(x) + c.g);
+        if (!c.none) out[e] = result(c.of<H>(x) + c.g);
         if (logp) *logp = c.none ? -INFINITY : (x - c.log2_sum) * kLn2;
       }
   }
@@ -598,12 +607,13 @@ __global__ __launch_bounds__(256) void log_probs_grad_kernel(const T* S, T* D, G
   GradColumn c(a, col);
   const float* stats = a.stats + 3 * col;
   const float max = stats[0], by = a.inv_t * kLog2e;
-  c.set(a, col, stats[1] * kLog2e, stats[2], max == -INFINITY && stats[1] == -INFINITY);
+  c.set(stats[1] * kLog2e, stats[2], max == -INFINITY && stats[1] == -INFINITY);
   const auto exponent = [&](float s) { return fminf(s - max, 0.f) * by; };
   const T* s = S + col * a.lds;
   T* d = D + col * a.ldd;
   float* logp = a.logp ? a.logp + col : nullptr;
   constexpr int kStep = kLanes * V * kLoads;
+  const float last = c.apart ? a.inv_t : 1.f;
   for (int64_t at0 = static_cast<int64_t>(blockIdx.y) * kStep - behind_16(s); at0 < a.m;
        at0 += static_cast<int64_t>(gridDim.y) * kStep) {
     unsigned raw[kLoads][4];
@@ -613,7 +623,7 @@ __global__ __launch_bounds__(256) void log_probs_grad_kernel(const T* S, T* D, G
     for (int u = 0; u < kLoads; ++u) {
       const int64_t at = at0 + (u * kLanes + lane) * V;
       if (at >= a.m) break;
-      grad_vec<H, T, V>(raw[u], static_cast<int>(at), a.m, c, exponent, logp, d);
+      grad_vec<H, true, T, V>(raw[u], static_cast<int>(at), a.m, c, last, exponent, logp, d);
     }
   }
 }
@@ -666,6 +676,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, WAVES == 16 ? 8 : 1)
   }
   keep_words(raw);
   const float by = a.inv_t * kLog2e, ref = ref_of(max, by);
+  const Origin origin(max, by);
+  const bool odd = is_far(max, by) || c.apart;
   float sum = 0.f, weighted = 0.f;
   const auto add = [&](auto exponent) {
 #pragma unroll
@@ -681,8 +693,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, WAVES == 16 ? 8 : 1)
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  const bool far = is_far(max, by);
-  if (far) add([&](float x) { return below(x, max) * by; });
+  if (odd) add([&](float x) { return origin.exponent(x, by); });
   else add([&](float x) { return fmaf(x, by, -ref); });
   sum = wave_total(sum);
   weighted = wave_total(weighted);
@@ -697,20 +708,20 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, WAVES == 16 ? 8 : 1)
   const float log2_sum = log2f(sum);
   float entropy = (log2_sum - weighted / sum) * kLn2;
   if (entropy < 0.f) entropy = 0.f;
-  c.set(a, col, log2_sum, entropy, max == -INFINITY && sum == 0.f);
+  c.set(log2_sum, entropy, max == -INFINITY && sum == 0.f);
   T* d = D + col * a.ldd;
   float* logp = a.logp ? a.logp + col : nullptr;
-  const auto write = [&](auto exponent) {
+  const auto write = [&](auto apart, auto exponent) {
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       const int at = at0 + u * kLanes * V;
       if (at >= a.m) break;
-      grad_vec<H, T, V>(raw[u], at, a.m, c, exponent, logp, d);
+      grad_vec<H, apart, T, V>(raw[u], at, a.m, c, c.apart ? a.inv_t : 1.f, exponent, logp, d);
       __builtin_amdgcn_sched_barrier(0);  // (all vectors' temporaries at once do not fit)
     }
   };
-  if (far) write([&](float x) { return below(x, max) * by; });
-  else write([&](float x) { return fmaf(x, by, -ref); });
+  if (odd) write(std::true_type(), [&](float x) { return origin.exponent(x, by); });
+  else write(std::false_type(), [&](float x) { return fmaf(x, by, -ref); });
 }
 
 // A longer column by one workgroup that goes through it twice: for the
@@ -758,11 +769,12 @@ __global__ __launch_bounds__(64 * kTwiceWaves, 8) void log_probs_grad_twice_kern
   }
   mass.over_wave<true>(by);
   const float max = mass.max, ref = ref_of(max, by);
-  const bool far = is_far(max, by);
+  const Origin origin(max, by);
+  const bool odd = is_far(max, by) || c.apart;
   const float log2_sum = log2f(mass.sum);
   float entropy = (log2_sum - mass.weighted / mass.sum) * kLn2;
   if (entropy < 0.f) entropy = 0.f;
-  c.set(a, col, log2_sum, entropy, max == -INFINITY && mass.sum == 0.f);
+  c.set(log2_sum, entropy, max == -INFINITY && mass.sum == 0.f);
   float* logp = a.logp ? a.logp + col : nullptr;
   for (int64_t step = steps - 1; step >= 0; --step) {
     unsigned raw[kLoads][4];
@@ -771,8 +783,13 @@ __global__ __launch_bounds__(64 * kTwiceWaves, 8) void log_probs_grad_twice_kern
     for (int u = 0; u < kLoads; ++u) {
       const int64_t at = begin + step * kStep + (u * kLanes + lane) * V;
       if (at >= a.m) break;
-      if (far) grad_vec<H, T, V>(raw[u], static_cast<int>(at), a.m, c, [&](float x) { return below(x, max) * by; }, logp, d);
-      else grad_vec<H, T, V>(raw[u], static_cast<int>(at), a.m, c, [&](float x) { return fmaf(x, by, -ref); }, logp, d);
+      if (odd) {
+        grad_vec<H, true, T, V>(raw[u], static_cast<int>(at), a.m, c, c.apart ? a.inv_t : 1.f,
+                                [&](float x) { return origin.exponent(x, by); }, logp, d);
+      } else {
+        grad_vec<H, false, T, V>(raw[u], static_cast<int>(at), a.m, c, 1.f,
+                                 [&](float x) { return fmaf(x, by, -ref); }, logp, d);
+      }
     }
   }
 }

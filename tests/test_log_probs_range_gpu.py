@@ -108,3 +108,41 @@ def test_sums_of_far_columns_keep_their_digits(cuda, n, m):
     labels = torch.randint(0, m, (n,), generator=_gen(cuda, 1), device=cuda)
     res = [_np(v) for v in sd.log_probs(S, labels, temperature=1000.0, entropy=True, stats=True)]
     ref.check(_np(S), _np(labels), 1000.0, *res)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T", [2.0 ** -126, 1e-37, 1e-36, 1e-30])
+@pytest.mark.parametrize("n,m", [(12, 40), (12, 900), (12, 3000), (12, 30_000), (12, 70_000), (260, 70_000)])
+def test_gradient_of_weights_beyond_the_temperature(cuda, n, m, T, kind):
+    """g / T and h / T pass the largest float: labels without weight, and with
+    all of it, still have no gradient."""
+    import torch
+    import libsdca_amd as sd
+    print(n, m, kind, T, flush=True)
+    S = torch.randint(-30, 30, (n, m), generator=_gen(cuda, m), device=cuda).to(getattr(torch, kind))
+    labels = torch.randint(0, m, (n,), generator=_gen(cuda, 1), device=cuda)
+    S[torch.arange(n, device=cuda), labels] = 40
+    labels[3] = -1
+    S[4] *= 1e-38   # (an ordinary column of the smallest numbers, or zeros)
+    g = torch.full((n,), 9.0, device=cuda)
+    h = torch.full((n,), -3.0, device=cuda)
+    g[4] = h[4] = T
+    if kind != "float16":   # another label than the largest: a gradient of its size
+        labels[5] = (labels[5] + 1) % m
+        g[5] = 0.25
+    few = slice(0, 12)
+    hS, hl = _np(S[few]), _np(labels[few])
+    stats = sd.log_probs(S, labels, temperature=T, stats=True)[1]
+    for hh, st in ((None, None), (h, None), (None, stats), (h, stats)):
+        D, lp = sd.log_probs_grad(S, labels, g, g_entropy=hh, stats=st, temperature=T, logp=True)
+        ref.check_grad(_np(D[few]), hS, hl, _np(g[few]).astype(np.float64), None if hh is None else _np(hh[few]), T,
+                       *HALF_STEP[kind])
+        ref.check(hS, hl, T, _np(lp[few]))
+    # a gradient that has no 32-bit value is infinite, the others stay
+    g[6], labels[6] = 1e38, (labels[6] + 1) % m
+    for st in (None, stats):
+        D = sd.log_probs_grad(S, labels, g, stats=st, temperature=T).float()
+        top = int(S[6].float().argmax())
+        assert D[6, labels[6]] == float("inf") and D[6, top] == -float("inf")
+        D[6, labels[6]] = D[6, top] = 0
+        assert not bool(D[6].any())
