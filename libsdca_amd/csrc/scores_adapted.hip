@@ -18,6 +18,7 @@ typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 // 32 bits: four products of 16 x 16 x 4; lane group g holds ranks 4 g on.
 template <class T>
 struct Ranks {
+  static constexpr unsigned kInfinite = 0;  // (no parts)
   static constexpr int kEach = 4;
   static __device__ int from(int lane) { return lane / 16 * 4; }
   float v[4];
@@ -42,6 +43,17 @@ __device__ inline void parts_of(float x, H (&p)[PARTS]) {
     x = fabsf(static_cast<float>(p[i])) < INFINITY ? rest : 0.f;
   }
 }
+// Into bfloat16 by their bits, eight and eight: no part is beyond the term.
+template <int PARTS>
+__device__ inline void parts_of(float x, __bf16 (&p)[PARTS]) {
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    const unsigned high = __float_as_uint(x) & 0xffff0000u;
+    const unsigned short bits = static_cast<unsigned short>(high >> 16);
+    __builtin_memcpy(&p[i], &bits, 2);
+    x = fabsf(x) < INFINITY ? x - __uint_as_float(high) : 0.f;
+  }
+}
 
 // 16 bits: products of 16 x 16 x 32 take the first 16 of their 32 places for
 // one part of the terms and the others for the next, with B's ranks in both:
@@ -50,6 +62,7 @@ __device__ inline void parts_of(float x, H (&p)[PARTS]) {
 // Three bfloat16 make up the 24 bits of a term.
 template <>
 struct Ranks<__hip_bfloat16> {
+  static constexpr unsigned kInfinite = 0x7f80;
   static constexpr int kEach = 8;
   static __device__ int from(int lane) { return lane / 16 % 2 * 8; }
   v8b first, last;
@@ -64,6 +77,8 @@ struct Ranks<__hip_bfloat16> {
       first[e] = lane < 32 ? p[0] : p[1];
       last[e] = lane < 32 ? p[2] : static_cast<__bf16>(0.f);
     }
+    // (Made here: the compiler would keep the terms and split them at each use.)
+    asm volatile("" : "+v"(first), "+v"(last));
   }
   __device__ v4f times(const __hip_bfloat16 (&b)[8]) const {
     v8b u;
@@ -78,6 +93,7 @@ struct Ranks<__hip_bfloat16> {
 // number, and their products back (`down`, a power of two).
 template <>
 struct Ranks<__half> {
+  static constexpr unsigned kInfinite = 0x7c00;
   static constexpr int kEach = 8;
   static __device__ int from(int lane) { return lane / 16 % 2 * 8; }
   v8h both;
@@ -88,7 +104,8 @@ struct Ranks<__half> {
 #pragma unroll
     for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
     most = fmaxf(most, __shfl_xor(most, 16));
-    down = most < INFINITY ? __builtin_amdgcn_frexp_expf(most) - 14 : 0;
+    // (Beside an infinite term the largest finite one must not become another.)
+    down = (most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 128) - 14;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       _Float16 p[2];
@@ -103,6 +120,25 @@ struct Ranks<__half> {
   }
 };
 
+// The adapters that 16 FN examples have, one after the other, and -1.
+template <int FN>
+struct Turns {
+  unsigned long long left[FN];
+  __device__ explicit Turns(const int (&mine)[FN]) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j) left[j] = __ballot(mine[j] >= 0);
+  }
+  __device__ int next(const int (&mine)[FN]) {
+    int a = -1;
+#pragma unroll
+    for (int j = FN - 1; j >= 0; --j)
+      if (left[j]) a = __builtin_amdgcn_readlane(mine[j], __builtin_ctzll(left[j]));
+#pragma unroll
+    for (int j = 0; j < FN; ++j) left[j] &= ~__ballot(mine[j] == a);
+    return a;
+  }
+};
+
 // The adapters' part of a wave's scores: products of classes by ranks with
 // ranks by examples, whose layout is that of the integer product's sums.
 // Examples of different adapters take turns: for each adapter the products
@@ -110,6 +146,10 @@ struct Ranks<__half> {
 // own, so that one adapter's infinities reach no other example.  B is loaded
 // for some adapters at once: with an adapter for each example the loads'
 // latency is what this takes.
+//
+// A term's parts can be 0 where the term is not, and times an infinity of B
+// that is NaN: where a wave's B holds one, its products are left out, and made
+// from the terms themselves at the end.
 template <class T>
 struct Adapted {
   static constexpr bool some = true;
@@ -140,14 +180,18 @@ struct Adapted {
     return a >= -1 && a < count ? static_cast<int>(a) : -2;
   }
 
-  template <int FM, int FN, int Q>
-  __device__ inline void add(v4f (&scores)[FM][FN], int64_t row0, int64_t n, int first, int m,
-                             int lane) const {
-    using R = Ranks<T>;
-    constexpr int kOnce = FM > 2 ? 1 : FN > 2 ? 2 : 4;
-    int mine[FN], of[FN];
+  // Where a lane's examples and classes are.
+  template <int FM, int FN>
+  struct Place {
+    int mine[FN];       // its examples' adapters, -1: none
     const float* t[FN];
-    bool bad[FN];
+    bool bad[FN];       // no adapter's number
+    int64_t at[FM];
+  };
+  template <int FM, int FN, int Q>
+  __device__ inline void find(Place<FM, FN>& place, int64_t row0, int64_t n, int first, int m, int lane) const {
+    int of[FN];
+    auto& [mine, t, bad, at] = place;
     // (Without conditions, for the loads to be on their way together.)
     if (ids) {
 #pragma unroll
@@ -167,50 +211,45 @@ struct Adapted {
       mine[j] = max(given, -1);
       t[j] = terms + (i < n ? i : n - 1) * pitch;
     }
-    int64_t at[FM];
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int c = first + ((lane & 15) >> 2) * (4 * Q) + (lane & 3) + i / Q * 16 * Q + i % Q * 4;
       at[i] = static_cast<int64_t>(min(c, m - 1)) * rank;
     }
+  }
+
+  template <int FM, int FN, int Q>
+  __device__ inline void add(v4f (&scores)[FM][FN], int64_t row0, int64_t n, int first, int m,
+                             int lane) const {
+    using R = Ranks<T>;
+    constexpr int kOnce = FM > 2 ? 1 : FN > 2 ? 2 : 4;
+    Place<FM, FN> place;
+    find<FM, FN, Q>(place, row0, n, first, m, lane);
+    auto& [mine, t, bad, at] = place;
+    bool again = false;
     for (int k0 = 0; k0 < rank; k0 += 16) {
-      unsigned long long left[FN];
-#pragma unroll
-      for (int j = 0; j < FN; ++j) left[j] = __ballot(mine[j] >= 0);
-      const auto next = [&] {
-        int a = -1;
-#pragma unroll
-        for (int j = FN - 1; j >= 0; --j)
-          if (left[j]) a = __builtin_amdgcn_readlane(mine[j], __builtin_ctzll(left[j]));
-#pragma unroll
-        for (int j = 0; j < FN; ++j) left[j] &= ~__ballot(mine[j] == a);
-        return a;
-      };
+      Turns<FN> turns(mine);
       R terms_of[FN];
 #pragma unroll
       for (int j = 0; j < FN; ++j) terms_of[j].take(t[j] + k0, lane);
       const int k = k0 + R::from(lane);
       int a[kOnce];
-      a[0] = next();
+      a[0] = turns.next(mine);
       while (a[0] >= 0) {
         T b[kOnce][FM][R::kEach];
 #pragma unroll
         for (int q = 0; q < kOnce; ++q) {
-          if (q) a[q] = next();
+          if (q) a[q] = turns.next(mine);
           const T* from = B + (a[q] < 0 ? a[0] : a[q]) * apart;
 #pragma unroll
-          for (int i = 0; i < FM; ++i) {
-            if (k0 + 16 <= rank) {
-              __builtin_memcpy(b[q][i], from + at[i] + k, sizeof(b[q][i]));
-            } else {
-#pragma unroll
-              for (int e = 0; e < R::kEach; ++e) b[q][i][e] = k + e < rank ? from[at[i] + k + e] : from_float<T>(0.f);
-            }
-          }
+          for (int i = 0; i < FM; ++i) load(from + at[i], k0, k, b[q][i]);
         }
 #pragma unroll
         for (int q = 0; q < kOnce; ++q) {
           if (a[q] < 0) break;
+          // (No branch: the products need not wait for this.)
+          const bool out = R::kInfinite != 0 && __ballot(infinite(b[q], R::kInfinite));
+          again |= out;
 #pragma unroll
           for (int j = 0; j < FN; ++j) {
             const bool hit = mine[j] == a[q];
@@ -221,12 +260,12 @@ struct Adapted {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float more = __builtin_amdgcn_ldexpf(sum[e], terms_of[j].down);
-                scores[i][j][e] = hit ? scores[i][j][e] + more : scores[i][j][e];
+                scores[i][j][e] = hit && !out ? scores[i][j][e] + more : scores[i][j][e];
               }
             }
           }
         }
-        a[0] = next();
+        a[0] = turns.next(mine);
       }
     }
 #pragma unroll
@@ -235,6 +274,79 @@ struct Adapted {
       for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) scores[i][j][e] = bad[j] ? NAN : scores[i][j][e];
+    if constexpr (R::kInfinite != 0) {
+      if (again) add_whole<FM, FN, Q>(scores, row0, n, first, m, lane);
+    }
+  }
+
+  // A lane's ranks of a class, from k of the 16 that begin at k0.
+  template <int EACH>
+  __device__ inline void load(const T* row, int k0, int k, T (&b)[EACH]) const {
+    if (k0 + 16 <= rank) {
+      __builtin_memcpy(b, row + k, sizeof(b));
+    } else {
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) b[e] = k + e < rank ? row[k + e] : from_float<T>(0.f);
+    }
+  }
+
+  // Whether one of these is an infinity or NaN: by the largest of their bits.
+  template <class Some>
+  __device__ static inline bool infinite(const Some& b, unsigned limit) {
+    typedef unsigned short v2u __attribute__((ext_vector_type(2)));
+    unsigned w[sizeof(b) / 4];
+    __builtin_memcpy(w, &b, sizeof(w));
+    v2u most = {};
+#pragma unroll
+    for (unsigned word : w) {
+      const unsigned size = word & 0x7fff7fffu;
+      v2u two;
+      __builtin_memcpy(&two, &size, 4);
+      most = __builtin_elementwise_max(most, two);
+    }
+    return max(static_cast<unsigned>(most[0]), static_cast<unsigned>(most[1])) >= limit;
+  }
+
+  // The products that were left out, in 32 bits.
+  template <int FM, int FN, int Q>
+  __device__ inline void add_whole(v4f (&scores)[FM][FN], int64_t row0, int64_t n, int first, int m, int lane) const {
+    using Whole = Ranks<float>;
+    // (Found again, so that nothing is kept for this.)
+    asm volatile("" : "+v"(lane));
+    Place<FM, FN> place;
+    find<FM, FN, Q>(place, row0, n, first, m, lane);
+    auto& [mine, t, bad, at] = place;
+    for (int k0 = 0; k0 < rank; k0 += 16) {
+      Turns<FN> turns(mine);
+      for (int a = turns.next(mine); a >= 0; a = turns.next(mine)) {
+        const T* from = B + a * apart;
+        T b[FM][Ranks<T>::kEach];
+#pragma unroll
+        for (int i = 0; i < FM; ++i) load(from + at[i], k0, k0 + Ranks<T>::from(lane), b[i]);
+        if (!__ballot(infinite(b, Ranks<T>::kInfinite))) continue;
+        float whole[FM][Whole::kEach];
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+          T some[Whole::kEach];
+          load(from + at[i], k0, k0 + Whole::from(lane), some);
+#pragma unroll
+          for (int e = 0; e < Whole::kEach; ++e) whole[i][e] = to_float(some[e]);
+        }
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          const bool hit = mine[j] == a;
+          if (!__ballot(hit)) continue;
+          Whole terms_of;
+          terms_of.take(t[j] + k0, lane);
+#pragma unroll
+          for (int i = 0; i < FM; ++i) {
+            const v4f sum = terms_of.times(whole[i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) scores[i][j][e] = hit ? scores[i][j][e] + sum[e] : scores[i][j][e];
+          }
+        }
+      }
+    }
   }
 
   __device__ inline float one(int example, int c, int lane) const {
