@@ -22,7 +22,7 @@ struct Ranks {
   static constexpr int kEach = 4;
   static __device__ int from(int lane) { return lane / 16 * 4; }
   float v[4];
-  int down = 0;
+  static constexpr float back = 1.f;
   __device__ void take(const float* t, int lane) { __builtin_memcpy(v, t + from(lane), 16); }
   __device__ v4f times(const T (&b)[4]) const {
     v4f sum = {};
@@ -32,93 +32,98 @@ struct Ranks {
   }
 };
 
-// A 32-bit float as the sum of PARTS 16-bit ones, each the rest's rounding (an
-// infinity is its first part alone).
-template <class H, int PARTS>
-__device__ inline void parts_of(float x, H (&p)[PARTS]) {
-#pragma unroll
-  for (int i = 0; i < PARTS; ++i) {
-    p[i] = static_cast<H>(x);
-    const float rest = x - static_cast<float>(p[i]);
-    x = fabsf(static_cast<float>(p[i])) < INFINITY ? rest : 0.f;
-  }
+// Two 32-bit floats' first digits as 16-bit ones, in a word, and what is left
+// of them.  Cut off rather than rounded: a part beyond its term would be an
+// infinity where the term is the largest, and would cost the instruction's sum,
+// which cuts as well, a digit.
+__device__ inline unsigned cut(__half, float& x, float& y) {
+  const auto both = __builtin_amdgcn_cvt_pkrtz(x, y);
+  x = fmaf(static_cast<float>(both[0]), -1.f, x);
+  y = fmaf(static_cast<float>(both[1]), -1.f, y);
+  return __builtin_bit_cast(unsigned, both);
 }
-// Into bfloat16 by their bits, eight and eight: no part is beyond the term.
-template <int PARTS>
-__device__ inline void parts_of(float x, __bf16 (&p)[PARTS]) {
-#pragma unroll
-  for (int i = 0; i < PARTS; ++i) {
-    const unsigned high = __float_as_uint(x) & 0xffff0000u;
-    const unsigned short bits = static_cast<unsigned short>(high >> 16);
-    __builtin_memcpy(&p[i], &bits, 2);
-    x = fabsf(x) < INFINITY ? x - __uint_as_float(high) : 0.f;
-  }
+__device__ inline unsigned cut(__hip_bfloat16, float& x, float& y) {
+  const unsigned u = __float_as_uint(x), v = __float_as_uint(y);
+  x -= __uint_as_float(u & 0xffff0000u);
+  y -= __uint_as_float(v & 0xffff0000u);
+  return __builtin_amdgcn_perm(v, u, 0x07060302);
 }
 
-// 16 bits: products of 16 x 16 x 32 take the first 16 of their 32 places for
-// one part of the terms and the others for the next, with B's ranks in both:
-// lane groups 0 and 1 hold ranks 0 to 7 and 8 to 15, groups 2 and 3 again.
+__device__ inline v4f multiply(__half, const unsigned (&a)[4], const unsigned (&b)[4], const v4f& sum) {
+  v8h u, v;
+  __builtin_memcpy(&u, a, 16);
+  __builtin_memcpy(&v, b, 16);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(u, v, sum, 0, 0, 0);
+}
+__device__ inline v4f multiply(__hip_bfloat16, const unsigned (&a)[4], const unsigned (&b)[4], const v4f& sum) {
+  v8b u, v;
+  __builtin_memcpy(&u, a, 16);
+  __builtin_memcpy(&v, b, 16);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, v, sum, 0, 0, 0);
+}
+
+// 16 bits: a term is the sum of three parts, which hold its 24 digits, eight and
+// more at a time.  Products of 16 x 16 x 32 take the first 16 of their 32 places
+// for one part and the others for the next, with B's ranks in both: lane groups
+// 0 and 1 hold ranks 0 to 7 and 8 to 15, groups 2 and 3 again.
 //
-// Three bfloat16 make up the 24 bits of a term.
-template <>
-struct Ranks<__hip_bfloat16> {
-  static constexpr unsigned kInfinite = 0x7f80;
+// Halves have few exponents: the 16 ranks are brought to below 2^14 first, so
+// that the parts of the largest are ordinary numbers (what is below 2^-24 then,
+// 2^-37 of the largest, is lost), and their products back (by the power of two
+// `back`, itself at least 2^-126).  (Two halves, in one instruction, held 23
+// digits and took as long: 1024 x 14336, rank 32, 95 us and 94.)
+template <class T>
+struct RanksInParts {
+  static constexpr bool kHalf = std::is_same<T, __half>::value;
+  static constexpr unsigned kInfinite = kHalf ? 0x7c00 : 0x7f80;
   static constexpr int kEach = 8;
   static __device__ int from(int lane) { return lane / 16 % 2 * 8; }
-  v8b first, last;
-  int down = 0;
-  __device__ void take(const float* t, int lane) {
-    float v[8];
-    __builtin_memcpy(v, t + from(lane), 32);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      __bf16 p[3];
-      parts_of(v[e], p);
-      first[e] = lane < 32 ? p[0] : p[1];
-      last[e] = lane < 32 ? p[2] : static_cast<__bf16>(0.f);
-    }
-    // (Made here: the compiler would keep the terms and split them at each use.)
-    asm volatile("" : "+v"(first), "+v"(last));
-  }
-  __device__ v4f times(const __hip_bfloat16 (&b)[8]) const {
-    v8b u;
-    __builtin_memcpy(&u, b, 16);
-    const v4f sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, last, v4f{}, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, first, sum, 0, 0, 0);
-  }
-};
+  unsigned first[4], last[4];
+  float back = 1.f;
 
-// Two halves have 22 bits, a term's to 2^-23 of it: its 16 ranks are brought
-// to below 2^14 first, so that the second half of the largest is an ordinary
-// number, and their products back (`down`, a power of two).
-template <>
-struct Ranks<__half> {
-  static constexpr unsigned kInfinite = 0x7c00;
-  static constexpr int kEach = 8;
-  static __device__ int from(int lane) { return lane / 16 % 2 * 8; }
-  v8h both;
-  int down;
   __device__ void take(const float* t, int lane) {
     float v[8], most = 0.f;
     __builtin_memcpy(v, t + from(lane), 32);
 #pragma unroll
     for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
-    most = fmaxf(most, __shfl_xor(most, 16));
-    // (Beside an infinite term the largest finite one must not become another.)
-    down = (most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 128) - 14;
+    if constexpr (kHalf) {
+      most = fmaxf(most, __shfl_xor(most, 16));
+      // (Beside an infinite term the largest finite one must not become another.)
+      const int down = max((most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 128) - 14, -126);
+      back = __builtin_amdgcn_ldexpf(1.f, down);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      _Float16 p[2];
-      parts_of(__builtin_amdgcn_ldexpf(v[e], -down), p);
-      both[e] = lane < 32 ? p[0] : p[1];
+      for (int e = 0; e < 8; ++e) v[e] = __builtin_amdgcn_ldexpf(v[e], -down);
+    }
+    if (__ballot(most == INFINITY)) split<true>(v, lane);
+    else split<false>(v, lane);
+    // (Made here: the compiler would keep the terms and split them at each use.)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(first[i]), "+v"(last[i]));
+  }
+  // An infinity is its first part alone.
+  template <bool INFINITE>
+  __device__ void split(const float (&v)[8], int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x = v[2 * i], y = v[2 * i + 1];
+      const unsigned one = cut(T(), x, y);
+      if (INFINITE && fabsf(v[2 * i]) == INFINITY) x = 0.f;
+      if (INFINITE && fabsf(v[2 * i + 1]) == INFINITY) y = 0.f;
+      const unsigned two = cut(T(), x, y), three = cut(T(), x, y);
+      first[i] = lane < 32 ? one : two;
+      last[i] = lane < 32 ? three : 0;
     }
   }
-  __device__ v4f times(const __half (&b)[8]) const {
-    v8h u;
-    __builtin_memcpy(&u, b, 16);
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(u, both, v4f{}, 0, 0, 0);
+  __device__ v4f times(const T (&b)[8]) const {
+    unsigned u[4];
+    __builtin_memcpy(u, b, 16);
+    return multiply(T(), u, first, multiply(T(), u, last, v4f{}));
   }
 };
+template <>
+struct Ranks<__half> : RanksInParts<__half> {};
+template <>
+struct Ranks<__hip_bfloat16> : RanksInParts<__hip_bfloat16> {};
 
 // The adapters that 16 FN examples have, one after the other, and -1.
 template <int FN>
@@ -184,14 +189,14 @@ struct Adapted {
   template <int FM, int FN>
   struct Place {
     int mine[FN];       // its examples' adapters, -1: none
-    const float* t[FN];
+    int row[FN];        // of terms
     bool bad[FN];       // no adapter's number
     int64_t at[FM];
   };
   template <int FM, int FN, int Q>
   __device__ inline void find(Place<FM, FN>& place, int64_t row0, int64_t n, int first, int m, int lane) const {
     int of[FN];
-    auto& [mine, t, bad, at] = place;
+    auto& [mine, row, bad, at] = place;
     // (Without conditions, for the loads to be on their way together.)
     if (ids) {
 #pragma unroll
@@ -209,7 +214,7 @@ struct Adapted {
       const int given = i < n ? of[j] : -1;
       bad[j] = given < -1;
       mine[j] = max(given, -1);
-      t[j] = terms + (i < n ? i : n - 1) * pitch;
+      row[j] = static_cast<int>(i < n ? i : n - 1);
     }
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
@@ -225,47 +230,58 @@ struct Adapted {
     constexpr int kOnce = FM > 2 ? 1 : FN > 2 ? 2 : 4;
     Place<FM, FN> place;
     find<FM, FN, Q>(place, row0, n, first, m, lane);
-    auto& [mine, t, bad, at] = place;
+    auto& [mine, row, bad, at] = place;
     bool again = false;
-    for (int k0 = 0; k0 < rank; k0 += 16) {
-      Turns<FN> turns(mine);
-      R terms_of[FN];
+    // Terms of 64 examples at most in registers, and B for each such part of the
+    // examples.  (128 do not fit beside the scores: 1024 x 14336 halves, rank 32, 99
+    // us, so 95.)
+    constexpr int kExamples = FN > 4 ? FN / 2 : FN;
 #pragma unroll
-      for (int j = 0; j < FN; ++j) terms_of[j].take(t[j] + k0, lane);
-      const int k = k0 + R::from(lane);
-      int a[kOnce];
-      a[0] = turns.next(mine);
-      while (a[0] >= 0) {
-        T b[kOnce][FM][R::kEach];
+    for (int j0 = 0; j0 < FN; j0 += kExamples) {
+      for (int k0 = 0; k0 < rank; k0 += 16) {
+        int these[kExamples];
 #pragma unroll
-        for (int q = 0; q < kOnce; ++q) {
-          if (q) a[q] = turns.next(mine);
-          const T* from = B + (a[q] < 0 ? a[0] : a[q]) * apart;
+        for (int j = 0; j < kExamples; ++j) these[j] = mine[j0 + j];
+        Turns<kExamples> turns(these);
+        R terms_of[kExamples];
 #pragma unroll
-          for (int i = 0; i < FM; ++i) load(from + at[i], k0, k, b[q][i]);
-        }
+        for (int j = 0; j < kExamples; ++j)
+          terms_of[j].take(terms + static_cast<int64_t>(row[j0 + j]) * pitch + k0, lane);
+        const int k = k0 + R::from(lane);
+        int a[kOnce];
+        a[0] = turns.next(these);
+        while (a[0] >= 0) {
+          T b[kOnce][FM][R::kEach];
 #pragma unroll
-        for (int q = 0; q < kOnce; ++q) {
-          if (a[q] < 0) break;
-          // (No branch: the products need not wait for this.)
-          const bool out = R::kInfinite != 0 && __ballot(infinite(b[q], R::kInfinite));
-          again |= out;
+          for (int q = 0; q < kOnce; ++q) {
+            if (q) a[q] = turns.next(these);
+            const T* from = B + (a[q] < 0 ? a[0] : a[q]) * apart;
 #pragma unroll
-          for (int j = 0; j < FN; ++j) {
-            const bool hit = mine[j] == a[q];
-            if (!__ballot(hit)) continue;
+            for (int i = 0; i < FM; ++i) load(from + at[i], k0, k, b[q][i]);
+          }
 #pragma unroll
-            for (int i = 0; i < FM; ++i) {
-              const v4f sum = terms_of[j].times(b[q][i]);
+          for (int q = 0; q < kOnce; ++q) {
+            if (a[q] < 0) break;
+            // (No branch: the products need not wait for this.)
+            const bool out = R::kInfinite != 0 && __ballot(infinite(b[q], R::kInfinite));
+            again |= out;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float more = __builtin_amdgcn_ldexpf(sum[e], terms_of[j].down);
-                scores[i][j][e] = hit && !out ? scores[i][j][e] + more : scores[i][j][e];
+            for (int j = 0; j < kExamples; ++j) {
+              const bool hit = these[j] == a[q];
+              if (!__ballot(hit)) continue;
+#pragma unroll
+              for (int i = 0; i < FM; ++i) {
+                const v4f sum = terms_of[j].times(b[q][i]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float more = fmaf(sum[e], terms_of[j].back, scores[i][j0 + j][e]);
+                  scores[i][j0 + j][e] = hit && !out ? more : scores[i][j0 + j][e];
+                }
               }
             }
           }
+          a[0] = turns.next(these);
         }
-        a[0] = turns.next(mine);
       }
     }
 #pragma unroll
@@ -315,7 +331,7 @@ struct Adapted {
     asm volatile("" : "+v"(lane));
     Place<FM, FN> place;
     find<FM, FN, Q>(place, row0, n, first, m, lane);
-    auto& [mine, t, bad, at] = place;
+    auto& [mine, row, bad, at] = place;
     for (int k0 = 0; k0 < rank; k0 += 16) {
       Turns<FN> turns(mine);
       for (int a = turns.next(mine); a >= 0; a = turns.next(mine)) {
@@ -337,7 +353,7 @@ struct Adapted {
           const bool hit = mine[j] == a;
           if (!__ballot(hit)) continue;
           Whole terms_of;
-          terms_of.take(t[j] + k0, lane);
+          terms_of.take(terms + static_cast<int64_t>(row[j]) * pitch + k0, lane);
 #pragma unroll
           for (int i = 0; i < FM; ++i) {
             const v4f sum = terms_of.times(whole[i]);

@@ -1,5 +1,5 @@
 """sdca_scores_adapted with adapters and terms at the ends of their types'
-ranges."""
+ranges, and the digits that terms are held in."""
 import numpy as np
 import pytest
 
@@ -126,3 +126,32 @@ def test_infinite_and_largest_terms(cuda, n, d, m, kind):
     got = _np(sd.scores_adapted(X, W, sw, A, B, index, scale=scale))
     # (the terms' zeros of X times infinity are NaN in both: row 0 of adapter 1 alone)
     _check(got, want, 2.0 ** -24 * 64 * size)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,d,m", SHAPES)
+def test_terms_have_32_bits(cuda, n, d, m, kind):
+    """One term of 24 digits times 1 is the score."""
+    import torch
+    import libsdca_amd as sd
+    dt = getattr(torch, kind)
+    g = _gen(cuda, n)
+    X = torch.zeros((n, d), device=cuda)
+    A = torch.zeros((2, 2, d), device=cuda)
+    # eight digits at a time: 1.xxxxxxx + 2^-8 xxxxxxxx + 2^-16 xxxxxxxx
+    digits = torch.randint(0, 128, (n, 3), generator=g, device=cuda)
+    X[:, 0] = 1 + digits[:, 0] / 128
+    X[:, 1], X[:, 2] = digits[:, 1], digits[:, 2] * 2 + 1
+    A[:, 0, 0], A[:, 0, 1], A[:, 0, 2] = 1, 2.0 ** -14, 2.0 ** -23
+    A[:, 0, 1:3] *= 2.0 ** 9   # (ordinary halves)
+    X[:, 1:3] *= 2.0 ** -9
+    W = torch.zeros((m, -(-d // 16) * 16), dtype=torch.int8, device=cuda)[:, :d]
+    sw = torch.ones(m, device=cuda)
+    B = torch.zeros((2, m, 2), device=cuda)
+    B[:, :, 0] = 1
+    index = torch.arange(n, device=cuda) % 2
+    X, A, B = X.to(dt), A.to(dt), B.to(dt)
+    T = (X.double() * A[0, 0].double()).sum(dim=1)
+    assert torch.equal(T.float().double(), T)
+    got = sd.scores_adapted(X, W, sw, A, B, index)
+    assert torch.equal(got, T.float()[:, None].expand(n, m))
