@@ -608,7 +608,8 @@ int sdca_scores_adapted(sdca_dtype data, sdca_dtype out, int64_t d, int64_t m, i
  * adapter without examples).  The sums' order depends on the sizes and the
  * index alone.  The examples are data and the weights fixed: neither has a
  * gradient.  d and m are at most 2^30 - 1.
- *   work: as above, sdca_scores_adapted_grad_work bytes.
+ *   work: as above, sdca_scores_adapted_grad_work bytes: for large G and few
+ *      adapters some rank / 256 of G's own (rank in whole 16).
  */
 size_t sdca_scores_adapted_grad_work(sdca_dtype data, sdca_dtype grad, int64_t d, int64_t m,
                                      int64_t n, int64_t count, int64_t rank);
