@@ -12,6 +12,7 @@ def test_its_share_of_a_large_gradient(data, grad, rank):
     work = sd.library().sdca_scores_adapted_grad_work(data, grad, d, m, n, 1, rank)
     pitch = (rank + 15) // 16 * 16
     turned = m * rank * 4
-    partial = 129 * rank * d * 4   # dA's sums: 64 segments at most, two places for each
+    # sums in parts, two places for each segment: dA's of 64 segments at most, dB's of two
+    partial = rank * 4 * max(129 * d, 5 * m)
     rows = 2 * n * pitch * 4 + 64 * n
     assert work <= n * m * (4 if grad == F32 else 2) * pitch // 256 + turned + partial + rows
