@@ -18,8 +18,6 @@
 namespace sdca_gpu {
 namespace {
 
-typedef float v4f __attribute__((ext_vector_type(4)));
-
 // ---------------------------------------------------------------------------
 // Terms, and with them the rows in 8 bits where Q is given.
 // ---------------------------------------------------------------------------
@@ -159,24 +157,13 @@ __global__ __launch_bounds__(256) void terms_row_kernel(const TX* __restrict__ X
   }
 }
 
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef __bf16 v8b __attribute__((ext_vector_type(8)));
-
 // sum += a product of 16 rows by 16 columns over 32 values: a lane has eight
 // of row and of column lane % 16.  Two halves or two bfloat16 multiply as
 // they are, others in 32 bits; the sums are 32-bit either way.
 template <class TA, class TB>
 __device__ inline v4f multiply(const TA (&a)[8], const TB (&b)[8], v4f sum) {
-  if constexpr (std::is_same<TA, TB>::value && std::is_same<TA, __half>::value) {
-    v8h u, v;
-    __builtin_memcpy(&u, a, 16);
-    __builtin_memcpy(&v, b, 16);
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(u, v, sum, 0, 0, 0);
-  } else if constexpr (std::is_same<TA, TB>::value && std::is_same<TA, __hip_bfloat16>::value) {
-    v8b u, v;
-    __builtin_memcpy(&u, a, 16);
-    __builtin_memcpy(&v, b, 16);
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, v, sum, 0, 0, 0);
+  if constexpr (std::is_same<TA, TB>::value && sizeof(TA) == 2) {
+    return multiply_16<TA>(a, b, sum);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)

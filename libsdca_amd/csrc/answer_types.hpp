@@ -7,6 +7,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace sdca_gpu {
 
 __device__ inline float to_float(float x) { return x; }
@@ -129,6 +131,27 @@ __device__ inline void quantize8(const float (&v)[8], const ColumnScale& s, unsi
     const unsigned low = __builtin_amdgcn_perm(b[4 * h + 1], b[4 * h], 0x0c0c0400);
     const unsigned high = __builtin_amdgcn_perm(b[4 * h + 3], b[4 * h + 2], 0x04000c0c);
     w[h] = low | high;
+  }
+}
+
+// sum += a product of 16 rows by 16 columns over 32 values of 16 bits: a lane
+// has eight of row and of column lane % 16, those from lane / 16 * 8 on.
+typedef float v4f __attribute__((ext_vector_type(4)));
+template <class T>
+__device__ inline v4f multiply_16(const void* a, const void* b, const v4f& sum) {
+  if constexpr (std::is_same<T, __half>::value) {
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    v8 u, v;
+    __builtin_memcpy(&u, a, 16);
+    __builtin_memcpy(&v, b, 16);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(u, v, sum, 0, 0, 0);
+  } else {
+    static_assert(std::is_same<T, __hip_bfloat16>::value, "16 bits");
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    v8 u, v;
+    __builtin_memcpy(&u, a, 16);
+    __builtin_memcpy(&v, b, 16);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, v, sum, 0, 0, 0);
   }
 }
 

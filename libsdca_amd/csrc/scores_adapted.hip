@@ -9,9 +9,6 @@
 namespace sdca_gpu {
 namespace {
 
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef __bf16 v8b __attribute__((ext_vector_type(8)));
-
 // Sixteen ranks of the terms (rows of 32-bit floats) and of B as the operands
 // of 16 x 16 products.  A lane has its example's, or its class's, part.
 //
@@ -47,19 +44,6 @@ __device__ inline unsigned cut(__hip_bfloat16, float& x, float& y) {
   x -= __uint_as_float(u & 0xffff0000u);
   y -= __uint_as_float(v & 0xffff0000u);
   return __builtin_amdgcn_perm(v, u, 0x07060302);
-}
-
-__device__ inline v4f multiply(__half, const unsigned (&a)[4], const unsigned (&b)[4], const v4f& sum) {
-  v8h u, v;
-  __builtin_memcpy(&u, a, 16);
-  __builtin_memcpy(&v, b, 16);
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(u, v, sum, 0, 0, 0);
-}
-__device__ inline v4f multiply(__hip_bfloat16, const unsigned (&a)[4], const unsigned (&b)[4], const v4f& sum) {
-  v8b u, v;
-  __builtin_memcpy(&u, a, 16);
-  __builtin_memcpy(&v, b, 16);
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, v, sum, 0, 0, 0);
 }
 
 // 16 bits: a term is the sum of three parts, which hold its 24 digits, eight and
@@ -115,9 +99,7 @@ struct RanksInParts {
     }
   }
   __device__ v4f times(const T (&b)[8]) const {
-    unsigned u[4];
-    __builtin_memcpy(u, b, 16);
-    return multiply(T(), u, first, multiply(T(), u, last, v4f{}));
+    return multiply_16<T>(b, first, multiply_16<T>(b, last, v4f{}));
   }
 };
 template <>

@@ -14,7 +14,6 @@ namespace sdca_gpu {
 namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
-typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr int kTileK = static_cast<int>(kI8TileK);
 
