@@ -146,10 +146,12 @@ struct Mass {
     unpack<T>(raw, v[0]);
     weigh(v, [&](float x) { return below(x, max) * c; });
   }
-  // All lanes' together, in every lane.
+  // All lanes' together, in every lane; `most` is their largest.
   template <bool ANY>
-  __device__ void over_wave(float c) {
-    rise<ANY>(wave_max<true>(max), c);
+  __device__ void over_wave(float c) { over_wave<ANY>(wave_max<true>(max), c); }
+  template <bool ANY>
+  __device__ void over_wave(float most, float c) {
+    rise<ANY>(most, c);
     sum = wave_total(sum);
     weighted = wave_total(weighted);
   }
@@ -296,19 +298,34 @@ __device__ inline void join_waves(Mass& mass, u64& list, u64 (*room)[128], float
       of_wave[wave][2] = mass.weighted;
     }
   };
+  Mass all;  // a wave's by lane
+  const auto take = [&] {
+    if (lane < WAVES) {
+      all.max = of_wave[lane][0];
+      all.sum = of_wave[lane][1];
+      all.weighted = of_wave[lane][2];
+    }
+  };
+  float most = 0.f;
   give();
 #pragma unroll
   for (int s = 1; s < WAVES; s *= 2) {
     if (TOP && (wave & (2 * s - 1)) == s) room[wave][lane] = list;
     if (TOP || s == 1) __syncthreads();
     if (s == 1) {
-      float most = of_wave[0][0];
+      if constexpr (TOP) {  // (few registers beside the lists: 20 x 166617 halves 17.6 us, 18.2 as below)
+        most = of_wave[0][0];
 #pragma unroll
-      for (int w = 1; w < WAVES; ++w) most = fmaxf(most, of_wave[w][0]);
+        for (int w = 1; w < WAVES; ++w) most = fmaxf(most, of_wave[w][0]);
+      } else {
+        take();
+        most = wave_max<true>(all.max);
+      }
       if (again(most)) {
         __syncthreads();
         give();
         __syncthreads();
+        take();
       }
     }
     if (TOP && (wave & (2 * s - 1)) == 0) {
@@ -319,13 +336,9 @@ __device__ inline void join_waves(Mass& mass, u64& list, u64 (*room)[128], float
     }
   }
   if (wave == 0) {
-    mass = Mass();
-    if (lane < WAVES) {
-      mass.max = of_wave[lane][0];
-      mass.sum = of_wave[lane][1];
-      mass.weighted = of_wave[lane][2];
-    }
-    mass.over_wave<true>(c);
+    if (TOP) take();
+    mass = all;
+    mass.over_wave<true>(most, c);
   }
 }
 
@@ -386,8 +399,11 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void log_probs_kerne
     if (!__builtin_amdgcn_readfirstlane(is_far(most, c))) return false;
     mass.max = most;
     mass.sum = mass.weighted = 0.f;
+    // (A loop keeps the kernels with alternatives short: 20 x 166617 halves 17.6 us,
+    // 18.3 with it unrolled; 2048 x 100003 halves without 82.5, unrolled 81.1.)
+    constexpr int kInLine = TOP || WAVES == 1 ? 1 : kLoads;
     for (int64_t at = begin; at < end; at += WAVES * kStep) {
-#pragma unroll
+#pragma unroll kInLine
       for (int u = 0; u < kLoads; ++u) {
         unsigned raw[4];
         load_words(row, at + (u * 64 + lane) * V, first, end, raw);
